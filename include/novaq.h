@@ -54,7 +54,8 @@ enum novaq_dtype {
   NOVAQ_BF16 = 2,
   NOVAQ_E4M3 = 3,
   NOVAQ_E5M2 = 4,
-  NOVAQ_E2M1 = 5
+  NOVAQ_E2M1 = 5,
+  NOVAQ_F64 = 6 /* IEEE binary64: novaq_clip_grad_norm only */
 };
 
 /* Padding modes of NovaNN's conv2d (novann/functional.py:325-344): numpy.pad's
@@ -410,6 +411,105 @@ int novaq_conv2d_backward_noalloc(const float *grad, const float *x, int64_t N, 
                                   const float *w_scale, int64_t C_out, int KH, int KW, int sh,
                                   int sw, int ph, int pw, int pad_mode, float *grad_input,
                                   float *grad_weight, float *grad_bias, void *stream);
+
+/* out (N, D) = dec(table[ids[i]]) * (s * factor) for N token ids of id_bits (32
+ * or 64) bits; the (V, D) table in w_dtype (F32, F16, BF16, E4M3, E5M2, or E2M1
+ * packed along D, rows of whole bytes), w_scale its s (NULL = 1; only with a
+ * quantized type); out in out_dtype (F32, F16, BF16), rounded once to nearest
+ * even.  The two factors are multiplied first, then each element once, in fp32.
+ * An id outside 0 .. V - 1 gives a row of NaN.  ids element-aligned.
+ * No reference counterpart (the reference has no token layers). */
+int novaq_embedding(const void *ids, int id_bits, int64_t N, const void *table, int w_dtype,
+                    const float *w_scale, int64_t V, int64_t D, float factor, void *out,
+                    int out_dtype, void *stream);
+
+/* Bytes of device workspace novaq_embedding_backward needs for these shapes. */
+size_t novaq_embedding_backward_workspace(int64_t N, int64_t V, int64_t D);
+
+/* grad_table (V, D) = factor * (for each row v the sum of grad[i] over the i
+ * with ids[i] = v), the gradient of the dequantized table; rows without a token
+ * are 0.  With accumulate != 0 it is added to what grad_table holds, and rows
+ * without a token are not touched (a table shared with the output layer).  grad
+ * (N, D) and grad_table in F32, F16 or BF16.  Sums are fp32 in an order that
+ * depends on the ids alone, so results repeat bit for bit; one rounding to
+ * grad_table's type.  Ids outside 0 .. V - 1 add nothing.  N, V below 2^31.
+ * workspace: novaq_embedding_backward_workspace() bytes, 16-byte aligned, not
+ * used after the call's kernels complete. */
+int novaq_embedding_backward(const void *grad, int grad_dtype, const void *ids, int id_bits,
+                             int64_t N, int64_t V, int64_t D, float factor, int accumulate,
+                             void *grad_table, int out_dtype, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+enum novaq_reduction {
+  NOVAQ_REDUCE_NONE = 0, /* one loss a row */
+  NOVAQ_REDUCE_MEAN = 1, /* over the rows that have a loss; 0 if none has */
+  NOVAQ_REDUCE_SUM = 2
+};
+
+/* Bytes of device workspace of the two calls below. */
+size_t novaq_linear_cross_entropy_workspace(int64_t N, int64_t D, int64_t V, int x_dtype,
+                                            int w_dtype);
+size_t novaq_linear_cross_entropy_backward_workspace(int64_t N, int64_t D, int64_t V, int x_dtype,
+                                                     int w_dtype);
+
+/* Softmax cross entropy of logits l = x @ (s * dec(w_q))^T over V classes, the
+ * logits never stored:
+ *   lse[n]  = log(sum over v of exp(l[n, v]))
+ *   loss[n] = lse[n] - l[n, t[n]],   0 where t[n] == ignore_index
+ * x (N, D) in F32, F16 or BF16, w_q (V, D) as novaq_linear_forward's; targets
+ * of target_bits (32 or 64) bits, element-aligned.  The products run in f16
+ * where x is F16, else in bf16, on operands rounded to that type (FP8 / FP4
+ * codes are exact in both), with fp32 sums, maxima and exponentials.  A target
+ * outside 0 .. V - 1 that is not ignore_index gives a NaN loss.  loss: N values
+ * (NOVAQ_REDUCE_NONE) or one; lse: N values, for the backward.
+ * No reference counterpart as one call: it stands for F.linear followed by
+ * CrossEntropyLoss (novann/losses/loss_functions.py:8-167), on logits instead
+ * of probabilities. */
+int novaq_linear_cross_entropy(const void *x, int x_dtype, int64_t N, int64_t D, const void *w_q,
+                               int w_dtype, const float *w_scale, int64_t V, const void *targets,
+                               int target_bits, int64_t ignore_index, int reduction, float *loss,
+                               float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Its gradients with respect to x (grad_input (N, D), in x_dtype) and to the
+ * dequantized weight (grad_weight (V, D), in gw_dtype F32, F16 or BF16), either
+ * may be NULL.  lse as the forward left it; grad: the loss's own gradient on
+ * the device, one value, or N with NOVAQ_REDUCE_NONE, or NULL for 1.  The
+ * softmax is computed again from lse, a piece of the vocabulary at a time, and
+ * rounded to the products' 16-bit type before its two products (fp32 sums);
+ * each output is rounded once.  Rows that are ignored get a zero gradient and
+ * add nothing, whatever x holds there; a target outside the vocabulary makes
+ * its gradients NaN. */
+int novaq_linear_cross_entropy_backward(const void *x, int x_dtype, int64_t N, int64_t D,
+                                        const void *w_q, int w_dtype, const float *w_scale,
+                                        int64_t V, const void *targets, int target_bits,
+                                        int64_t ignore_index, int reduction, const float *grad,
+                                        const float *lse, void *grad_input, void *grad_weight,
+                                        int gw_dtype, void *workspace, size_t workspace_bytes,
+                                        void *stream);
+
+/* One gradient of novaq_clip_grad_norm: n elements at grad, and where the
+ * clipped ones go: out (grad itself to clip in place, NULL for none).  Types:
+ * F32, F16, BF16 or NOVAQ_F64, element-aligned. */
+typedef struct novaq_gradient {
+  const void *grad;
+  void *out;
+  int64_t n;
+  int grad_dtype;
+  int out_dtype;
+} novaq_gradient;
+
+/* Bytes of device workspace novaq_clip_grad_norm needs for count gradients. */
+size_t novaq_clip_grad_norm_workspace(int64_t count);
+
+/* *norm = sqrt(sum of g^2 over all elements of all gradients), summed in fp64,
+ * and out = g * min(1, max_norm / (norm + eps)) (one fp32 multiply, fp64 for
+ * F64 gradients, rounded to out's type) for each gradient that has an out.  The list is host memory, read
+ * before the call returns.  A NaN norm makes every output NaN; an infinite one
+ * makes finite gradients 0.
+ * Stands for the clipping inside SGD.step (novann/optim/sgd.py:37-82), for any
+ * optimizer. */
+int novaq_clip_grad_norm(const novaq_gradient *list, int64_t count, float max_norm, float eps,
+                         float *norm, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

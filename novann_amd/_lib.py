@@ -12,8 +12,10 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libnovaq.so")
 
 F32, F16, BF16, E4M3, E5M2, E2M1 = range(6)
+F64 = 6  # gradients to be clipped only
 DTYPES = {"f32": F32, "f16": F16, "bf16": BF16, "e4m3": E4M3, "e5m2": E5M2, "e2m1": E2M1}
 DTYPE_NAMES = {v: k for k, v in DTYPES.items()}
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 PAD_MODES = {"zeros": 0, "reflect": 1, "replicate": 2, "circular": 3}
 
 OK, EINVAL, EDTYPE, ESHAPE, EPADMODE, EALIGN, EHIP, ENOTSUP, ESCRATCH = (
@@ -85,6 +87,23 @@ SIGNATURES = {
     "novaq_conv2d_backward_noalloc": (_i32, [_f32p, _f32p, _i64, _i64, _i64, _i64, _vp, _i32,
                                              _f32p, _i64, _i32, _i32, _i32, _i32, _i32, _i32,
                                              _i32, _f32p, _f32p, _f32p, _vp]),
+    "novaq_embedding": (_i32, [_vp, _i32, _i64, _vp, _i32, _f32p, _i64, _i64, ctypes.c_float, _vp,
+                               _i32, _vp]),
+    "novaq_embedding_backward_workspace": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "novaq_embedding_backward": (_i32, [_vp, _i32, _vp, _i32, _i64, _i64, _i64, ctypes.c_float,
+                                        _i32, _vp, _i32, _vp, ctypes.c_size_t, _vp]),
+    "novaq_linear_cross_entropy_workspace": (ctypes.c_size_t, [_i64, _i64, _i64, _i32, _i32]),
+    "novaq_linear_cross_entropy_backward_workspace": (ctypes.c_size_t,
+                                                      [_i64, _i64, _i64, _i32, _i32]),
+    "novaq_linear_cross_entropy": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _f32p, _i64, _vp,
+                                          _i32, _i64, _i32, _f32p, _f32p, _vp, ctypes.c_size_t,
+                                          _vp]),
+    "novaq_linear_cross_entropy_backward": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _f32p, _i64,
+                                                   _vp, _i32, _i64, _i32, _f32p, _f32p, _vp, _vp,
+                                                   _i32, _vp, ctypes.c_size_t, _vp]),
+    "novaq_clip_grad_norm_workspace": (ctypes.c_size_t, [_i64]),
+    "novaq_clip_grad_norm": (_i32, [_vp, _i64, ctypes.c_float, ctypes.c_float, _f32p, _vp,
+                                    ctypes.c_size_t, _vp]),
 }
 
 _lib = None

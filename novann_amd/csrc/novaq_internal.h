@@ -211,4 +211,27 @@ int conv2d_backward_launch(const float* grad, const float* x, int64_t N, int64_t
 int colsum_launch(const float* x, int64_t rows, int64_t cols, float* out, hipStream_t stream,
                   int pt = 0, int pco = 0, int pc = 0);
 
+// Token kernels (novaq.h has their semantics; arguments are validated by the C
+// ABI).  bits: 32 or 64, the ids' width.
+int embedding_launch(const void* ids, int bits, int64_t N, const void* table, int w_dtype,
+                     const float* scale, int64_t V, int64_t D, float factor, void* out,
+                     int out_dtype, hipStream_t stream);
+size_t embedding_backward_workspace(int64_t N, int64_t V, int64_t D);
+int embedding_backward_launch(const void* grad, int g_dtype, const void* ids, int bits, int64_t N,
+                              int64_t V, int64_t D, float factor, int accumulate, void* out,
+                              int o_dtype, void* workspace, hipStream_t stream);
+size_t vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype,
+                            bool backward);
+int vocab_loss_launch(const void* x, int x_dtype, int64_t N, int64_t D, const void* w, int w_dtype,
+                      const float* w_scale, int64_t V, const void* ids, int bits, int64_t ignore,
+                      int reduction, float* loss, float* lse, void* ws, hipStream_t stream);
+int vocab_loss_backward_launch(const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
+                               int w_dtype, const float* w_scale, int64_t V, const void* ids,
+                               int bits, int64_t ignore, int reduction, const float* grad,
+                               const float* lse, void* gx, void* gw, int gw_dtype, void* ws,
+                               hipStream_t stream);
+size_t clip_grad_norm_workspace(int64_t count);
+int clip_grad_norm_launch(const novaq_gradient* list, int64_t count, float max_norm, float eps,
+                          float* norm, void* workspace, hipStream_t stream);
+
 }  // namespace novaq

@@ -1,0 +1,219 @@
+// Matrix products of 16-bit operands (bf16 or f16) with fp32 sums for the
+// vocabulary loss:
+//
+//   C[M, N] = sum over k of A(m, k) * B(n, k)
+//
+// Each operand lies either K-contiguous (element (r, k) at r * ld + k) or
+// K-strided (at k * ld + r), ld a multiple of 8 elements and 16-byte aligned.
+// Tiles go from memory straight into LDS (buffer_load ... lds, 16 bytes a
+// lane) through a ring of NS stages of 64 K; a K-contiguous tile is read into
+// MFMA fragments with 16-byte reads, a K-strided one with gfx950's transposing
+// read (ds_read_b64_tr_b16; its lane order is in TokenTile::read), so no operand
+// needs a transposed copy.  What lies past a matrix's last row reads as zeros
+// through the buffer descriptor, whose base moves with the K block, so no
+// offset outgrows 32 bits however long an operand is.  A K-contiguous operand's
+// rows are whole multiples of 64 K (the callers keep padded copies); K-strided
+// rows past K read as zeros; their columns past the matrix read what follows
+// them and go into sums that are not stored.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "novaq_convert.h"
+#include "novaq_internal.h"
+
+namespace novaq {
+namespace {
+
+typedef float tg_f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t tg_u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t tg_u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 tg_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 tg_f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 tg_bf16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) tg_bf16x4 tg_lds_bf16x4;
+typedef __attribute__((address_space(3))) void tg_lds_void;
+
+// One 32 x 32 x 16 MFMA on fragments held as raw words (CT: BF16 or F16).
+template <int CT>
+__device__ __forceinline__ tg_f32x16 tg_mfma(const tg_u32x4& a, const tg_u32x4& b,
+                                             const tg_f32x16& c) {
+  if constexpr (CT == BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(tg_bf16x8, a),
+                                                   __builtin_bit_cast(tg_bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(tg_f16x8, a),
+                                                  __builtin_bit_cast(tg_f16x8, b), c, 0, 0, 0);
+}
+
+// fp32 -> the compute type's 16-bit code, nearest even.
+template <int CT>
+__device__ __forceinline__ uint32_t tg_pack2(float lo, float hi) {
+  if constexpr (CT == BF16) {
+    return pack_bf16x2(f2u(lo), f2u(hi));
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 h = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, h);
+  }
+}
+
+// One operand of a product: rows (M or N) of K elements.
+struct TokenOp {
+  const uint16_t* p;
+  int64_t rows;  // M (or N)
+  int64_t ld;    // elements between rows (K-contiguous) or between K (K-strided)
+};
+
+// The LDS tile of one operand: R rows (or columns) of 64 K, 128 R bytes.
+//   K-contiguous: row r holds 8 chunks of 16 bytes, chunk c at slot
+//     c ^ ((r >> 1) & 7): the 16 rows that one 16-byte read touches at a time
+//     fall in distinct banks.
+//   K-strided: K row k holds R / 8 chunks, chunk c at slot c ^ (4 (k & 3)):
+//     the four K rows that a transposing read touches lie in distinct 64-byte
+//     bank ranges.
+template <bool KS, int R, int NTH>
+struct TokenTile {
+  static constexpr int bytes = R * 128;
+  static constexpr int loads = R * 8 / NTH;  // 16-byte loads a lane a stage
+  static constexpr int cpr = KS ? R / 8 : 8;  // chunks a row
+  static_assert(R % 32 == 0 && (R * 8) % NTH == 0 && NTH % cpr == 0, "tile shape");
+
+  // byte offsets of this lane's loads from the tile's base in memory
+  struct Src {
+    const uint16_t* base;
+    int64_t left;     // bytes from base to the operand's end
+    uint32_t voff[loads];
+  };
+
+  __device__ static __forceinline__ Src source(const TokenOp& op, int64_t r0, int64_t K, int tid) {
+    Src s;
+    const int row0 = tid / cpr;  // tile row (or K row) of load 0
+    constexpr int step = NTH / cpr;
+    if constexpr (KS) {
+      s.base = op.p + r0;
+      s.left = (K * op.ld - r0) * 2;
+    } else {
+      s.base = op.p + r0 * op.ld;
+      s.left = (op.rows - r0) * op.ld * 2;
+    }
+#pragma unroll
+    for (int i = 0; i < loads; ++i) {
+      const int r = row0 + i * step;
+      const int c = (tid % cpr) ^ (KS ? 4 * (r & 3) : ((r >> 1) & 7));
+      s.voff[i] = (uint32_t)r * (uint32_t)(op.ld * 2) + c * 16;
+    }
+    return s;
+  }
+
+  // Copies stage kb (64 K) to lds (this wave's part of every load).
+  __device__ static __forceinline__ void load(const Src& s, const TokenOp& op, int kb,
+                                              uint8_t* lds, int wave) {
+    const int64_t at = KS ? (int64_t)kb * 64 * op.ld * 2 : (int64_t)kb * 128;
+    int64_t left = s.left - at;
+    left = left < 0 ? 0 : left > 0x7FFFFFFF ? 0x7FFFFFFF : left;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(s.base) + at), (short)0, (int)left,
+        0x00020000);
+#pragma unroll
+    for (int i = 0; i < loads; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (tg_lds_void*)(lds + (i * NTH + wave * 64) * 16), 16, s.voff[i], 0, 0, 0);
+  }
+
+  // Lane's byte offset of fragment (32 rows from w0 + 32 i, K 16 s .. + 15):
+  //   K-contiguous: lane l reads row l % 32, K 8 (l / 32) .. + 7.
+  //   K-strided: in each group of 16 lanes lane p names 8 bytes (K row p / 4,
+  //     columns 4 (p % 4) .. + 3 of a 4 x 16 block) and receives column p of
+  //     the block; the second read is 4 K rows further.
+  __device__ static __forceinline__ tg_u32x4 read(const uint8_t* lds, int w0, int i, int s,
+                                                  int lane) {
+    if constexpr (KS) {
+      const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
+      const int byte = ((w0 + i * 32) * 2 ^ ((k & 3) * 64)) +
+                       (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+      const uint8_t* p = lds + (16 * s + k) * (R * 2) + byte;
+      const tg_u32x2 lo = __builtin_bit_cast(
+          tg_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((tg_lds_bf16x4*)p));
+      const tg_u32x2 hi = __builtin_bit_cast(
+          tg_u32x2,
+          __builtin_amdgcn_ds_read_tr16_b64_v4bf16((tg_lds_bf16x4*)(p + 4 * (R * 2))));
+      return tg_u32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+      const int r = lane & 31, h = lane >> 5;
+      return *reinterpret_cast<const tg_u32x4*>(lds + (w0 + i * 32 + r) * 128 +
+                                                (((2 * s + h) ^ ((r >> 1) & 7)) << 4));
+    }
+  }
+};
+
+// The product of one BM x BN tile by 4 waves (2 x 2) of WM x WN: K blocks kb0
+// to kb1 of 64.  acc[i][j]: rows wm + 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4,
+// column wn + 32 j + lane % 32.  After it returns every wave is done with LDS.
+template <int CT, bool AKS, bool BKS, int WM_, int WN_>
+struct TokenGemm {
+  static constexpr int WM = WM_, WN = WN_, BM = 2 * WM, BN = 2 * WN, NTH = 256;
+  static constexpr int MT = WM / 32, NT = WN / 32;
+  using A = TokenTile<AKS, BM, NTH>;
+  using B = TokenTile<BKS, BN, NTH>;
+  static constexpr int stage = A::bytes + B::bytes;
+  static constexpr int NS = 2;
+  static constexpr int lds_bytes = NS * stage;
+  typedef tg_f32x16 Acc[MT][NT];
+
+  struct Frags {
+    tg_u32x4 a[MT];
+    tg_u32x4 b[NT];
+  };
+
+  __device__ static __forceinline__ void run(Acc& acc, const TokenOp& oa, const TokenOp& ob,
+                                             int64_t m0, int64_t n0, int64_t K, int kb0, int kb1,
+                                             uint8_t* lds) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = (wave & 1) * WM, wn = (wave >> 1) * WN;
+    const typename A::Src sa = A::source(oa, m0, K, tid);
+    const typename B::Src sb = B::source(ob, n0, K, tid);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+    auto issue = [&](int kb) {
+      uint8_t* at = lds + (kb & 1) * stage;
+      A::load(sa, oa, kb, at, wave);
+      B::load(sb, ob, kb, at + A::bytes, wave);
+    };
+    auto read = [&](Frags& f, int kb, const int s) {
+      const uint8_t* at = lds + (kb & 1) * stage;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) f.a[i] = A::read(at, wm, i, s, lane);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) f.b[j] = B::read(at + A::bytes, wn, j, s, lane);
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = tg_mfma<CT>(f.a[i], f.b[j], acc[i][j]);
+    };
+    for (int kb = kb0; kb < kb1; ++kb) {
+      issue(kb);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      Frags f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        read(f, kb, s);
+        multiply(f);
+      }
+      __syncthreads();
+    }
+  }
+};
+
+}  // namespace
+}  // namespace novaq

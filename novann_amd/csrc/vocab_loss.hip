@@ -1,0 +1,683 @@
+// Softmax cross entropy of a linear head over a large vocabulary, and its
+// gradients, without keeping the logits.  With x (N, D), a table W (V, D) of
+// codes and its scale s:
+//
+//   l[n, v]  = s * sum_d x[n, d] dec(W[v, d])
+//   lse[n]   = log sum_v exp(l[n, v])
+//   loss[n]  = lse[n] - l[n, t[n]]             (0 where t[n] is ignore_index)
+//   P[n, v]  = f[n] (exp(l[n, v] - lse[n]) - [v = t[n]])
+//   grad_x   = g s P dec(W),  grad_W = g P^T x
+//
+// f[n] is 0 for ignored rows and else 1 (reduction mean: g = upstream / count,
+// sum: g = upstream) or, with a gradient for each row, that gradient over the
+// largest of them in magnitude (which is g).
+//
+// The vocabulary is walked in pieces.  The forward multiplies a piece's rows
+// with x and reduces each tile of logits to one (maximum, sum of 2^(l2 -
+// maximum)) a row, l2 = l log2(e); a last kernel joins a row's tiles.  The
+// backward computes a piece's logits again, stores P of that piece in 16 bits
+// and multiplies it with the piece (grad_x, summed over the pieces in fp32)
+// and with x (grad_W's rows of the piece): 8 N V D operations for both, 6 of
+// them needed by any method.
+//
+// Types: the products run in 16 bits, f16 where x is f16 and bf16 otherwise;
+// FP8 and FP4 codes are exact in both, fp32 x or W and 16-bit W of the other
+// type are rounded to nearest even.  P is rounded to the same type before its
+// products (half an ulp of 2^-8 or 2^-11: the size of the gradients' own
+// rounding where they are stored in 16 bits); in f16 it carries a factor of
+// 2^14, which keeps probabilities down to 2^-28 in its normal range.  Logits,
+// maxima, sums, lse and all accumulation are fp32; the loss over the rows is
+// summed in fp64.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "novaq_internal.h"
+#include "token_gemm.h"
+#include "token_io.h"
+
+namespace novaq {
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int T_NONE = -1, T_BAD = -2;  // no loss; an id outside the vocabulary
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// dst (rows x dp, 16 bits, dp % 64 == 0) = src (rows x D, ST) as CT, zeros past
+// D; rows whose target is T_NONE become zeros (targets may be null).
+template <int ST, int CT, bool VEC>
+__global__ __launch_bounds__(256) void loss_copy_kernel(const uint8_t* __restrict__ src,
+                                                        int64_t rows, int64_t D, int64_t dp,
+                                                        const int* __restrict__ targets,
+                                                        uint16_t* __restrict__ dst) {
+  const int64_t per = dp / 8, total = rows * per, rb = row_bytes(ST, D);
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
+       q += (int64_t)gridDim.x * 256) {
+    const int64_t row = q / per, c = (q - row * per) * 8;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (c < D && !(targets && targets[row] == T_NONE))
+      load8<ST, VEC>(src + row * rb, c, D, v);
+    ti_u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<ti_u32x4*>(dst + row * dp + c) = o;
+  }
+}
+
+template <int CT>
+int copy_launch(const void* src, int st, int64_t rows, int64_t D, int64_t dp, const int* targets,
+                uint16_t* dst, hipStream_t stream) {
+  if (rows == 0) return NOVAQ_OK;
+  const int64_t units = rows * (dp / 8);
+  const dim3 grid((unsigned)std::min<int64_t>((units + 255) / 256, 16384));
+  const uint8_t* s = static_cast<const uint8_t*>(src);
+#define NOVAQ_COPY(ST)                                                                        \
+  case ST:                                                                                    \
+    if (D % 8 == 0)                                                                           \
+      hipLaunchKernelGGL((loss_copy_kernel<ST, CT, true>), grid, dim3(256), 0, stream, s,     \
+                         rows, D, dp, targets, dst);                                          \
+    else                                                                                      \
+      hipLaunchKernelGGL((loss_copy_kernel<ST, CT, false>), grid, dim3(256), 0, stream, s,    \
+                         rows, D, dp, targets, dst);                                          \
+    break;
+  switch (st) {
+    NOVAQ_COPY(F32)
+    NOVAQ_COPY(F16)
+    NOVAQ_COPY(BF16)
+    NOVAQ_COPY(E4M3)
+    NOVAQ_COPY(E5M2)
+    NOVAQ_COPY(E2M1)
+    default: return NOVAQ_EDTYPE;
+  }
+#undef NOVAQ_COPY
+  return check_launch();
+}
+
+// Per-row state, by one workgroup: targets as int32 (T_NONE, T_BAD), the row
+// factors f (NaN for T_BAD, so its gradients show) and scal[0] = g, scal[1] =
+// the number of rows with a loss.  grad: one value, or one a row
+// (per_row), or null (1).
+__global__ __launch_bounds__(1024) void loss_rows_kernel(const void* __restrict__ ids, int bits,
+                                                         int64_t ignore, int64_t N, int64_t V,
+                                                         const float* __restrict__ grad,
+                                                         int per_row, int mean,
+                                                         int* __restrict__ targets,
+                                                         float* __restrict__ f,
+                                                         float* __restrict__ scal) {
+  __shared__ int cnt[16];
+  __shared__ float top[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int c = 0;
+  float m = 0.0f;
+  bool nan = false;
+  for (int64_t n = tid; n < N; n += 1024) {
+    const int64_t t = token_at(ids, bits, n);
+    const int k = t == ignore ? T_NONE : t < 0 || t >= V ? T_BAD : (int)t;
+    targets[n] = k;
+    c += k != T_NONE;
+    if (per_row && k != T_NONE) {
+      const float a = fabsf(grad[n]);
+      nan |= a != a;
+      m = fmaxf(m, a);
+    }
+  }
+  if (nan) m = u2f(0x7FC00000u);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    c += __shfl_xor(c, d);
+    const float o = __shfl_xor(m, d);
+    m = m != m || o != o ? u2f(0x7FC00000u) : fmaxf(m, o);
+  }
+  if (lane == 0) cnt[wave] = c, top[wave] = m;
+  __syncthreads();
+  c = 0, m = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    c += cnt[w];
+    m = m != m || top[w] != top[w] ? u2f(0x7FC00000u) : fmaxf(m, top[w]);
+  }
+  if (tid == 0 && scal) {
+    float g = per_row ? m : grad ? *grad : 1.0f;
+    if (mean) g = c > 0 ? g / (float)c : 0.0f;
+    scal[0] = g;
+    scal[1] = (float)c;
+  }
+  if (f)
+    for (int64_t n = tid; n < N; n += 1024) {
+      const int k = targets[n];
+      float v = k == T_NONE ? 0.0f : 1.0f;
+      if (per_row && k != T_NONE) v = m > 0.0f ? grad[n] / m : m;  // (all zero: 0; NaN: NaN)
+      f[n] = k == T_BAD ? u2f(0x7FC00000u) : v;
+    }
+}
+
+// 8 workgroups in a row go to the 8 XCDs: those of one XCD take a compact
+// group of tiles, 4 along M.
+__device__ __forceinline__ void tile_of(int t, int tm, int tn, int& m, int& n) {
+  const int T = tm * tn;
+  if ((T & 7) == 0) t = (t & 7) * (T >> 3) + (t >> 3);
+  constexpr int GM = 4;
+  const int group = t / (GM * tn), first = group * GM, gm = min(tm - first, GM);
+  const int rem = t - group * GM * tn;
+  m = first + rem % gm;
+  n = rem / gm;
+}
+
+// The forward's tile: BM vocabulary rows (from v0 + m0) x BN tokens.  A lane
+// holds one token's logits of a column, so a row's maximum and sum stay in
+// registers but for one exchange between the lane halves and one between the
+// two waves that share the tokens.
+template <int CT, class G>
+__global__ __launch_bounds__(G::NTH, 1) void loss_stats_kernel(
+    TokenOp w, TokenOp x, int64_t dp, const float* __restrict__ w_scale, int64_t v0, int64_t N,
+    const int* __restrict__ targets, float2* __restrict__ stats, int64_t vtiles,
+    float* __restrict__ tlogit, int tm, int tn) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int mi, ni;
+  tile_of(blockIdx.x, tm, tn, mi, ni);
+  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN;
+  typename G::Acc acc;
+  G::run(acc, w, x, m0, n0, dp, 0, (int)(dp / 64), lds);
+
+  const float c2 = (w_scale ? *w_scale : 1.0f) * LOG2E;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
+  const int rows = (int)min((int64_t)G::BM, w.rows - m0) - wm - 4 * half;  // of this lane
+  float2* part = reinterpret_cast<float2*>(lds);  // [BN]
+  float2 st[G::NT];
+#pragma unroll
+  for (int j = 0; j < G::NT; ++j) {
+    const int64_t n = n0 + wn + 32 * j + (lane & 31);
+    const int t = n < N ? targets[n] : T_NONE;
+    const int at = t < 0 ? -1 : (int)(t - v0 - m0 < 0 || t - v0 - m0 >= G::BM ? -1 : t - v0 - m0);
+    const int mine = at < 0 ? -1 : at - wm - 4 * half;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at_row = 32 * i + 8 * (r >> 2) + (r & 3);
+        const float l = acc[i][j][r] * c2;
+        acc[i][j][r] = l;
+        m = at_row < rows ? fmaxf(m, l) : m;
+        if (at_row == mine) tlogit[n] = l;
+      }
+    const float z = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at_row = 32 * i + 8 * (r >> 2) + (r & 3);
+        s += at_row < rows ? __builtin_amdgcn_exp2f(acc[i][j][r] - z) : 0.0f;
+      }
+    const float om = __shfl_xor(m, 32), os = __shfl_xor(s, 32), t2 = fmaxf(m, om);
+    const float tz = t2 == -INFINITY ? 0.0f : t2;
+    s = s * __builtin_amdgcn_exp2f(m - tz) + os * __builtin_amdgcn_exp2f(om - tz);
+    st[j] = float2{t2, s};
+    if ((wave & 1) && half == 0) part[wn + 32 * j + (lane & 31)] = st[j];
+  }
+  __syncthreads();
+  if ((wave & 1) == 0 && half == 0) {
+#pragma unroll
+    for (int j = 0; j < G::NT; ++j) {
+      const int64_t n = n0 + wn + 32 * j + (lane & 31);
+      const float2 o = part[wn + 32 * j + (lane & 31)];
+      const float m = fmaxf(st[j].x, o.x), z = m == -INFINITY ? 0.0f : m;
+      const float s = st[j].y * __builtin_amdgcn_exp2f(st[j].x - z) +
+                      o.y * __builtin_amdgcn_exp2f(o.x - z);
+      if (n < N) stats[n * vtiles + (v0 + m0) / G::BM] = float2{m, s};
+    }
+  }
+}
+
+// One wave a row joins the tiles' (maximum, sum) pairs: lse and the loss.
+__global__ __launch_bounds__(256) void loss_join_kernel(const float2* __restrict__ stats,
+                                                        int64_t vtiles, int64_t N,
+                                                        const int* __restrict__ targets,
+                                                        const float* __restrict__ tlogit,
+                                                        float* __restrict__ lse,
+                                                        float* __restrict__ loss) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N) return;
+  float m = -INFINITY, s = 0.0f;
+  for (int64_t i = lane; i < vtiles; i += 64) {
+    const float2 o = stats[n * vtiles + i];
+    const float t = fmaxf(m, o.x), z = t == -INFINITY ? 0.0f : t;
+    s = s * __builtin_amdgcn_exp2f(m - z) + o.y * __builtin_amdgcn_exp2f(o.x - z);
+    m = t;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const float om = __shfl_xor(m, d), os = __shfl_xor(s, d);
+    const float t = fmaxf(m, om), z = t == -INFINITY ? 0.0f : t;
+    s = s * __builtin_amdgcn_exp2f(m - z) + os * __builtin_amdgcn_exp2f(om - z);
+    m = t;
+  }
+  if (lane == 0) {
+    const float l2 = m + log2f(s);
+    const int t = targets[n];
+    lse[n] = l2 * LN2;
+    // (the difference in base 2: the factor's rounding falls on the loss alone)
+    loss[n] = t == T_NONE ? 0.0f : t == T_BAD ? u2f(0x7FC00000u) : (l2 - tlogit[n]) * LN2;
+  }
+}
+
+// The rows' losses summed in fp64 in a fixed order, over the count for mean
+// (0 where no row has a loss).
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict__ each, int64_t N,
+                                                        int mean, const float* __restrict__ scal,
+                                                        float* __restrict__ out) {
+  __shared__ double part[16];
+  double s = 0.0;
+  for (int64_t n = threadIdx.x; n < N; n += 1024) s += (double)each[n];
+#pragma unroll
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int w = 0; w < 16; ++w) s += part[w];
+    if (mean) s = scal[1] > 0.0f ? s / (double)scal[1] : 0.0;
+    *out = (float)s;
+  }
+}
+
+// The backward's P of one piece: the forward's tile, then f (2^(l2 - lse2) -
+// [v = t]) in 16 bits at P[n][v] (pitch vp; the piece's columns past the
+// vocabulary are zeros), through LDS so that rows leave in whole lines.
+template <int CT, class G>
+__global__ __launch_bounds__(G::NTH, 1) void loss_prob_kernel(
+    TokenOp w, TokenOp x, int64_t dp, const float* __restrict__ w_scale, int64_t v0, int64_t N,
+    const int* __restrict__ targets, const float* __restrict__ f, const float* __restrict__ lse,
+    float pscale, uint16_t* __restrict__ P, int64_t vp, int tm, int tn) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int mi, ni;
+  tile_of(blockIdx.x, tm, tn, mi, ni);
+  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN;
+  typename G::Acc acc;
+  G::run(acc, w, x, m0, n0, dp, 0, (int)(dp / 64), lds);
+
+  const float c2 = (w_scale ? *w_scale : 1.0f) * LOG2E;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
+  const int rows = (int)min((int64_t)G::BM, w.rows - m0) - wm - 4 * half;
+  // token rows of BM 16-bit values and 16 bytes more, so that the rows that a
+  // store touches start in different banks
+  constexpr int PITCH = G::BM * 2 + 16;
+#pragma unroll
+  for (int j = 0; j < G::NT; ++j) {
+    const int col = wn + 32 * j + (lane & 31);
+    const int64_t n = n0 + col;
+    const bool in = n < N;
+    const int t = in ? targets[n] : T_NONE;
+    const int64_t d = (int64_t)t - v0 - m0 - wm - 4 * half;
+    const int mine = t < 0 || d < 0 || d >= G::BM ? -1 : (int)d;
+    const float fn = in ? f[n] * pscale : 0.0f, l2 = in ? lse[n] * LOG2E : 0.0f;
+    const bool none = t == T_NONE;
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at_row = 32 * i + 8 * q + e;
+          const float p = __builtin_amdgcn_exp2f(acc[i][j][4 * q + e] * c2 - l2);
+          const float y = fn * (at_row == mine ? p - 1.0f : p);
+          v[e] = none || at_row >= rows ? 0.0f : y;
+        }
+        *reinterpret_cast<tg_u32x2*>(lds + col * PITCH + (wm + 4 * half + 32 * i + 8 * q) * 2) =
+            tg_u32x2{tg_pack2<CT>(v[0], v[1]), tg_pack2<CT>(v[2], v[3])};
+      }
+  }
+  __syncthreads();
+  constexpr int CPR = G::BM / 8;  // 16-byte chunks a token row
+  for (int q = threadIdx.x; q < G::BN * CPR; q += G::NTH) {
+    const int r = q / CPR, c = q % CPR;
+    if (n0 + r < N)
+      *reinterpret_cast<tg_u32x4*>(P + (n0 + r) * vp + m0 + c * 8) =
+          *reinterpret_cast<const tg_u32x4*>(lds + r * PITCH + c * 16);
+  }
+}
+
+// grad_x's share of one piece: P (N x K) times the piece's rows (K x D), K
+// blocks of this split, added to (or, first, stored in) the split's fp32 sums.
+template <int CT, class G>
+__global__ __launch_bounds__(G::NTH, 1) void loss_dx_kernel(TokenOp p, TokenOp w, int64_t K,
+                                                            int64_t kblocks, int splits,
+                                                            float* __restrict__ sums, int64_t N,
+                                                            int64_t dp, int64_t D, int first,
+                                                            int tm, int tn) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int mi, ni;
+  const int split = blockIdx.x / (tm * tn);
+  tile_of(blockIdx.x % (tm * tn), tm, tn, mi, ni);
+  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN;
+  typename G::Acc acc;
+  G::run(acc, p, w, m0, n0, K, (int)(kblocks * split / splits),
+         (int)(kblocks * (split + 1) / splits), lds);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
+  float* out = sums + (int64_t)split * N * dp;
+#pragma unroll
+  for (int j = 0; j < G::NT; ++j) {
+    const int64_t d = n0 + wn + 32 * j + (lane & 31);
+    if (d >= D) continue;
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int64_t n = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+        if (n >= N) continue;
+        float* q = out + n * dp + d;
+        *q = first ? acc[i][j][r] : *q + acc[i][j][r];
+      }
+  }
+}
+
+// grad_x = the splits' sums, in order, times g s / pscale, as OT.
+template <int OT>
+__global__ __launch_bounds__(256) void loss_dx_store_kernel(const float* __restrict__ sums,
+                                                            int splits, int64_t N, int64_t dp,
+                                                            int64_t D,
+                                                            const float* __restrict__ scal,
+                                                            const float* __restrict__ w_scale,
+                                                            float inv_pscale,
+                                                            const int* __restrict__ targets,
+                                                            void* __restrict__ out) {
+  const float a = scal[0] * (w_scale ? *w_scale : 1.0f) * inv_pscale;
+  const int64_t per = dp / 8, total = N * per;
+  const bool vec = D % 8 == 0;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
+       q += (int64_t)gridDim.x * 256) {
+    const int64_t n = q / per, c = (q - n * per) * 8;
+    if (c >= D) continue;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = 0; s < splits; ++s) {
+      const float4* p = reinterpret_cast<const float4*>(sums + ((int64_t)s * N + n) * dp + c);
+      const float4 lo = p[0], hi = p[1];
+      v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+      v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+    }
+    const bool none = targets[n] == T_NONE;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = none ? 0.0f : v[i] * a;
+    if (vec) store8<OT, true>(out, n * D + c, 8, v);
+    else store8<OT, false>(out, n * D + c, D - c, v);
+  }
+}
+
+// grad_W's rows of one piece: P^T (vc x N) times x (N x D), times g / pscale.
+template <int CT, int OT, class G>
+__global__ __launch_bounds__(G::NTH, 1) void loss_dw_kernel(TokenOp p, TokenOp x, int64_t N,
+                                                            int64_t kblocks, int64_t vc,
+                                                            int64_t D,
+                                                            const float* __restrict__ scal,
+                                                            float inv_pscale,
+                                                            uint8_t* __restrict__ out, int tm,
+                                                            int tn) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int mi, ni;
+  tile_of(blockIdx.x, tm, tn, mi, ni);
+  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN;
+  typename G::Acc acc;
+  G::run(acc, p, x, m0, n0, N, 0, (int)kblocks, lds);
+  const float a = scal[0] * inv_pscale;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
+#pragma unroll
+  for (int j = 0; j < G::NT; ++j) {
+    const int64_t d = n0 + wn + 32 * j + (lane & 31);
+    if (d >= D) continue;
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int64_t v = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+        if (v >= vc) continue;
+        const float y = acc[i][j][r] * a;
+        if constexpr (OT == F32) reinterpret_cast<float*>(out)[v * D + d] = y;
+        else reinterpret_cast<uint16_t*>(out)[v * D + d] = (uint16_t)encode<OT>(f2u(y));
+      }
+  }
+}
+
+// --------------------------------------------------------------------------
+// the plan of a call: what its shapes and types make of the workspace
+
+struct LossPlan {
+  int ct;            // the products' type
+  int64_t dp;        // row pitch of the 16-bit copies
+  bool copy_x, copy_w;
+  int64_t piece;     // vocabulary rows a piece (a multiple of 256)
+  int64_t vtiles;    // tiles of the vocabulary
+  int splits;        // of grad_x's K
+  size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, total;
+};
+
+constexpr int64_t TILE = 128;
+
+LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bool backward) {
+  LossPlan p{};
+  p.ct = x_dtype == F16 ? F16 : BF16;
+  p.dp = (D + 63) / 64 * 64;
+  // x is copied in the backward (ignored rows become zeros, which its product
+  // over the rows needs) and where it is not in the products' type and whole
+  // blocks of 64
+  p.copy_x = backward || x_dtype != p.ct || D % 64 != 0;
+  p.copy_w = w_dtype != p.ct || D % 64 != 0;
+  const int64_t vr = (V + 255) / 256 * 256;
+  p.piece = std::min<int64_t>(vr, 8192);
+  if (backward)
+    p.piece = std::min(p.piece, std::max<int64_t>(1024, ((int64_t)1 << 29) / std::max<int64_t>(
+                                                                    2 * N, 1) / 256 * 256));
+  p.vtiles = (V + TILE - 1) / TILE;
+  const int64_t tiles = ((N + TILE - 1) / TILE) * ((D + TILE - 1) / TILE);
+  p.splits = 1;
+  while (p.splits < 16 && tiles * p.splits * 2 <= device_cu_count() &&
+         p.piece / 64 / (p.splits * 2) >= 4)
+    p.splits *= 2;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t b = at;
+    at += align256(bytes);
+    return b;
+  };
+  p.targets = take((size_t)N * 4);
+  p.scal = take(16);
+  p.xc = take(p.copy_x ? (size_t)N * p.dp * 2 : 0);
+  p.wc = take(p.copy_w ? (size_t)p.piece * p.dp * 2 : 0);
+  if (backward) {
+    p.f = take((size_t)N * 4);
+    p.P = take((size_t)N * p.piece * 2);
+    p.sums = take((size_t)p.splits * N * p.dp * 4);
+  } else {
+    p.stats = take((size_t)N * p.vtiles * 8);
+    p.tlogit = take((size_t)N * 4);
+    p.each = take((size_t)N * 4);
+  }
+  p.total = at;
+  return p;
+}
+
+template <class G>
+int raise_lds(const void* kern, DeviceFlags& raised) {
+  return allow_lds(raised, kern, G::lds_bytes, G::lds_bytes);
+}
+
+#define NOVAQ_LAUNCH(KERN, GRID, G, STREAM, ...)                                          \
+  do {                                                                                    \
+    static DeviceFlags raised;                                                            \
+    const int rc_ = raise_lds<G>(reinterpret_cast<const void*>(&KERN), raised);           \
+    if (rc_ != NOVAQ_OK) return rc_;                                                      \
+    hipLaunchKernelGGL(KERN, dim3((unsigned)(GRID)), dim3(G::NTH), G::lds_bytes, STREAM,  \
+                       __VA_ARGS__);                                                      \
+    const int rl_ = check_launch();                                                       \
+    if (rl_ != NOVAQ_OK) return rl_;                                                      \
+  } while (0)
+
+template <int CT>
+int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
+            int w_dtype, const float* w_scale, int64_t V, const void* ids, int bits,
+            int64_t ignore, int reduction, float* loss, float* lse, uint8_t* ws, hipStream_t st) {
+  using G = TokenGemm<CT, false, false, 64, 64>;
+  int* targets = reinterpret_cast<int*>(ws + p.targets);
+  float* scal = reinterpret_cast<float*>(ws + p.scal);
+  float2* stats = reinterpret_cast<float2*>(ws + p.stats);
+  float* tl = reinterpret_cast<float*>(ws + p.tlogit);
+  float* each = reduction == NOVAQ_REDUCE_NONE ? loss : reinterpret_cast<float*>(ws + p.each);
+  hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, st, ids, bits, ignore, N, V,
+                     (const float*)nullptr, 0, 0, targets, (float*)nullptr, scal);
+  int rc = check_launch();
+  if (rc != NOVAQ_OK) return rc;
+  const uint16_t* xc = reinterpret_cast<const uint16_t*>(x);
+  if (p.copy_x) {
+    uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.xc);
+    rc = copy_launch<CT>(x, x_dtype, N, D, p.dp, nullptr, d, st);
+    if (rc != NOVAQ_OK) return rc;
+    xc = d;
+  }
+  const TokenOp ox{xc, N, p.dp};
+  for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+    const int64_t vc = std::min(p.piece, V - v0);
+    const uint16_t* wc = reinterpret_cast<const uint16_t*>(w) + v0 * D;
+    if (p.copy_w) {
+      uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.wc);
+      rc = copy_launch<CT>(static_cast<const uint8_t*>(w) + v0 * row_bytes(w_dtype, D), w_dtype,
+                           vc, D, p.dp, nullptr, d, st);
+      if (rc != NOVAQ_OK) return rc;
+      wc = d;
+    }
+    const TokenOp ow{wc, vc, p.dp};
+    const int tm = (int)((vc + G::BM - 1) / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
+    NOVAQ_LAUNCH((loss_stats_kernel<CT, G>), (int64_t)tm * tn, G, st, ow, ox, p.dp, w_scale, v0,
+                 N, targets, stats, p.vtiles, tl, tm, tn);
+  }
+  hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, st, stats,
+                     p.vtiles, N, targets, tl, lse, each);
+  rc = check_launch();
+  if (rc != NOVAQ_OK || reduction == NOVAQ_REDUCE_NONE) return rc;
+  hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, each, N,
+                     reduction == NOVAQ_REDUCE_MEAN, scal, loss);
+  return check_launch();
+}
+
+template <int CT>
+int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
+             int w_dtype, const float* w_scale, int64_t V, const void* ids, int bits,
+             int64_t ignore, int reduction, const float* grad, const float* lse, void* gx,
+             void* gw, int gw_dtype, uint8_t* ws, hipStream_t st) {
+  using GL = TokenGemm<CT, false, false, 64, 64>;
+  using GX = TokenGemm<CT, false, true, 64, 64>;
+  using GW = TokenGemm<CT, true, true, 64, 64>;
+  int* targets = reinterpret_cast<int*>(ws + p.targets);
+  float* scal = reinterpret_cast<float*>(ws + p.scal);
+  float* f = reinterpret_cast<float*>(ws + p.f);
+  uint16_t* P = reinterpret_cast<uint16_t*>(ws + p.P);
+  float* sums = reinterpret_cast<float*>(ws + p.sums);
+  uint16_t* xc = reinterpret_cast<uint16_t*>(ws + p.xc);
+  const float pscale = CT == F16 ? 0x1p14f : 1.0f, inv = 1.0f / pscale;
+  hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, st, ids, bits, ignore, N, V, grad,
+                     reduction == NOVAQ_REDUCE_NONE && grad ? 1 : 0,
+                     reduction == NOVAQ_REDUCE_MEAN, targets, f, scal);
+  int rc = check_launch();
+  if (rc != NOVAQ_OK) return rc;
+  rc = copy_launch<CT>(x, x_dtype, N, D, p.dp, targets, xc, st);
+  if (rc != NOVAQ_OK) return rc;
+  const TokenOp ox{xc, N, p.dp};
+  for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+    const int64_t vc = std::min(p.piece, V - v0), vp = (vc + 255) / 256 * 256;
+    const uint16_t* wc = reinterpret_cast<const uint16_t*>(w) + v0 * D;
+    if (p.copy_w) {
+      uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.wc);
+      rc = copy_launch<CT>(static_cast<const uint8_t*>(w) + v0 * row_bytes(w_dtype, D), w_dtype,
+                           vc, D, p.dp, nullptr, d, st);
+      if (rc != NOVAQ_OK) return rc;
+      wc = d;
+    }
+    const TokenOp ow{wc, vc, p.dp}, op{P, N, vp}, opt{P, vp, vp};
+    {
+      const int tm = (int)(vp / GL::BM), tn = (int)((N + GL::BN - 1) / GL::BN);
+      NOVAQ_LAUNCH((loss_prob_kernel<CT, GL>), (int64_t)tm * tn, GL, st, ow, ox, p.dp, w_scale,
+                   v0, N, targets, f, lse, pscale, P, vp, tm, tn);
+    }
+    if (gx) {
+      const int tm = (int)((N + GX::BM - 1) / GX::BM), tn = (int)((D + GX::BN - 1) / GX::BN);
+      NOVAQ_LAUNCH((loss_dx_kernel<CT, GX>), (int64_t)tm * tn * p.splits, GX, st, op, ow, vc,
+                   vp / 64, p.splits, sums, N, p.dp, D, v0 == 0 ? 1 : 0, tm, tn);
+    }
+    if (gw) {
+      const int tm = (int)((vc + GW::BM - 1) / GW::BM), tn = (int)((D + GW::BN - 1) / GW::BN);
+      uint8_t* out = static_cast<uint8_t*>(gw) + v0 * D * (gw_dtype == F32 ? 4 : 2);
+      switch (gw_dtype) {
+        case F32:
+          NOVAQ_LAUNCH((loss_dw_kernel<CT, F32, GW>), (int64_t)tm * tn, GW, st, opt, ox, N,
+                       (N + 63) / 64, vc, D, scal, inv, out, tm, tn);
+          break;
+        case F16:
+          NOVAQ_LAUNCH((loss_dw_kernel<CT, F16, GW>), (int64_t)tm * tn, GW, st, opt, ox, N,
+                       (N + 63) / 64, vc, D, scal, inv, out, tm, tn);
+          break;
+        default:
+          NOVAQ_LAUNCH((loss_dw_kernel<CT, BF16, GW>), (int64_t)tm * tn, GW, st, opt, ox, N,
+                       (N + 63) / 64, vc, D, scal, inv, out, tm, tn);
+      }
+    }
+  }
+  if (gx) {
+    const dim3 grid((unsigned)std::min<int64_t>((N * (p.dp / 8) + 255) / 256, 4096));
+    switch (x_dtype) {
+      case F32:
+        hipLaunchKernelGGL(loss_dx_store_kernel<F32>, grid, dim3(256), 0, st, sums, p.splits, N,
+                           p.dp, D, scal, w_scale, inv, targets, gx);
+        break;
+      case F16:
+        hipLaunchKernelGGL(loss_dx_store_kernel<F16>, grid, dim3(256), 0, st, sums, p.splits, N,
+                           p.dp, D, scal, w_scale, inv, targets, gx);
+        break;
+      default:
+        hipLaunchKernelGGL(loss_dx_store_kernel<BF16>, grid, dim3(256), 0, st, sums, p.splits, N,
+                           p.dp, D, scal, w_scale, inv, targets, gx);
+    }
+    rc = check_launch();
+  }
+  return rc;
+}
+
+#undef NOVAQ_LAUNCH
+
+}  // namespace
+
+size_t vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype,
+                            bool backward) {
+  return loss_plan(N, D, V, x_dtype, w_dtype, backward).total;
+}
+
+int vocab_loss_launch(const void* x, int x_dtype, int64_t N, int64_t D, const void* w, int w_dtype,
+                      const float* w_scale, int64_t V, const void* ids, int bits, int64_t ignore,
+                      int reduction, float* loss, float* lse, void* ws, hipStream_t stream) {
+  const LossPlan p = loss_plan(N, D, V, x_dtype, w_dtype, false);
+  uint8_t* b = static_cast<uint8_t*>(ws);
+  return p.ct == F16 ? forward<F16>(p, x, x_dtype, N, D, w, w_dtype, w_scale, V, ids, bits, ignore,
+                                    reduction, loss, lse, b, stream)
+                     : forward<BF16>(p, x, x_dtype, N, D, w, w_dtype, w_scale, V, ids, bits,
+                                     ignore, reduction, loss, lse, b, stream);
+}
+
+int vocab_loss_backward_launch(const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
+                               int w_dtype, const float* w_scale, int64_t V, const void* ids,
+                               int bits, int64_t ignore, int reduction, const float* grad,
+                               const float* lse, void* gx, void* gw, int gw_dtype, void* ws,
+                               hipStream_t stream) {
+  const LossPlan p = loss_plan(N, D, V, x_dtype, w_dtype, true);
+  uint8_t* b = static_cast<uint8_t*>(ws);
+  return p.ct == F16
+             ? backward<F16>(p, x, x_dtype, N, D, w, w_dtype, w_scale, V, ids, bits, ignore,
+                             reduction, grad, lse, gx, gw, gw_dtype, b, stream)
+             : backward<BF16>(p, x, x_dtype, N, D, w, w_dtype, w_scale, V, ids, bits, ignore,
+                              reduction, grad, lse, gx, gw, gw_dtype, b, stream);
+}
+
+}  // namespace novaq

@@ -579,3 +579,237 @@ def avg_pool2d(input):
                                               None if xs is None else xs.data_ptr(), N, C, H, W,
                                               y.data_ptr(), _stream(x.device)), "avg_pool2d")
     return y.cpu().numpy() if was_numpy else y
+
+
+# --------------------------------------------------------------------------
+# token operators: the lookup in a table, the loss over a vocabulary
+
+_TOKEN_FLOATS = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}
+
+
+def _ids_arg(ids, limit: Optional[int], what: str, ignore: Optional[int] = None):
+    """(contiguous int32 or int64 device tensor, its bits).  Ids that are on the
+    host are checked against 0 .. limit - 1 (ValueError); what a kernel does
+    with an id on the device that lies outside is said by each operator."""
+    if isinstance(ids, torch.Tensor):
+        if not ids.is_cuda:
+            ids = ids.detach().numpy()
+    elif not isinstance(ids, np.ndarray):
+        ids = np.asarray(ids)
+    if isinstance(ids, np.ndarray):
+        if ids.dtype.kind not in "iu" and ids.size:
+            raise TypeError(f"{what} must be integers, got {ids.dtype}")
+        ids = ids.astype(np.int64)
+        bad = (ids < 0) | (ids >= limit)
+        if ignore is not None:
+            bad &= ids != ignore
+        if bad.any():
+            raise ValueError(f"{what}: id {ids[bad].flat[0]} is not in 0..{limit - 1}")
+        return torch.from_numpy(np.ascontiguousarray(ids)).to(_device()), 64
+    if ids.dtype is torch.int64:
+        return ids.contiguous(), 64
+    if ids.dtype is torch.int32:
+        return ids.contiguous(), 32
+    if ids.dtype in (torch.int16, torch.int8, torch.uint8):
+        return ids.to(torch.int32).contiguous(), 32
+    raise TypeError(f"{what} must be integers, got {ids.dtype}")
+
+
+def _table_arg(weight, dev: torch.device):
+    """(codes, dtype code, scale or None, (V, D)) of a 2-D table: quantized
+    codes, or fp32 / bf16 / f16 data as stored (other types become fp32)."""
+    if isinstance(weight, QuantizedParameters):
+        w, dt, scale = _weight_args(weight, dev)
+        shape = weight.shape
+    else:
+        data = weight.data if isinstance(weight, Parameters) else weight
+        if isinstance(data, torch.Tensor) and data.is_cuda and data.dtype in _TOKEN_FLOATS:
+            w, dt, scale = _aligned(data.contiguous()), DTYPES[_TOKEN_FLOATS[data.dtype]], None
+        else:
+            w, dt, scale = _to_device_f32(data, "weight")[0], DTYPES["f32"], None
+        shape = tuple(w.shape)
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"weight must be a (rows, columns) table, got shape {tuple(shape)}")
+    return w, dt, scale, shape
+
+
+def _float_arg(a, what: str):
+    """(contiguous fp32 / bf16 / f16 device tensor, dtype code, was numpy)."""
+    if isinstance(a, torch.Tensor) and a.is_cuda and a.dtype in _TOKEN_FLOATS:
+        return _aligned(a.contiguous()), DTYPES[_TOKEN_FLOATS[a.dtype]], False
+    t, was_numpy = _to_device_f32(a, what)
+    return t, DTYPES["f32"], was_numpy
+
+
+def _out_dtype(name: str):
+    if name not in ("f32", "bf16", "f16"):
+        raise TypeError(f"out_dtype must be 'f32', 'bf16' or 'f16', got {name!r}")
+    return OUT_STORAGE[name]
+
+
+def _workspace(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def embedding(tokens, weight, *, factor: float = 1.0, out_dtype: str = "f32"):
+    """Rows of a table: out[..., :] = factor * weight[tokens[...], :].
+
+    tokens: integers of any shape (device tensor or host array); weight (V, D):
+    Parameters (fp32, or a bf16 / f16 device tensor), QuantizedParameters
+    (E4M3 / E5M2 / E2M1 codes and scale) or a tensor.  Returns tokens.shape +
+    (D,) in ``out_dtype`` ('f32', 'bf16' or 'f16'), each element scaled by one
+    fp32 multiply and rounded once; an ndarray for tokens that were one (f32,
+    f16).  Tokens on the host are checked (ValueError); one on the device that
+    is outside the table gives a row of NaN.  No counterpart in the reference,
+    which has no token layers."""
+    was_numpy = isinstance(tokens, np.ndarray)
+    w, wdt, ws, (V, D) = _table_arg(weight, tokens.device if isinstance(tokens, torch.Tensor)
+                                    and tokens.is_cuda else _device())
+    ids, bits = _ids_arg(tokens, V, "tokens")
+    store = _out_dtype(out_dtype)
+    out = torch.empty((*ids.shape, D), dtype=store, device=w.device)
+    check(_lib.load().novaq_embedding(
+        ids.data_ptr(), bits, ids.numel(), w.data_ptr(), wdt,
+        None if ws is None else ws.data_ptr(), V, D, factor, out.data_ptr(), DTYPES[out_dtype],
+        _stream(w.device)), "embedding")
+    return out.cpu().numpy() if was_numpy and store != torch.bfloat16 else out
+
+
+def embedding_backward(grad, tokens, weight, *, factor: float = 1.0, out=None,
+                       accumulate: bool = False):
+    """Gradient of ``embedding(tokens, weight, factor=factor)`` with respect to
+    the (dequantized) table, for grad = dL/dout, tokens.shape + (D,) in fp32,
+    bf16 or f16.
+
+    Returns (V, D): factor times, for each row, the sum of the gradients of the
+    positions that hold its token, 0 for rows without one; fp32, or in ``out``'s
+    type (fp32, bf16 or f16, contiguous, 16-byte aligned) when that is given.
+    ``accumulate`` adds it to what ``out`` holds: the other gradient of a table
+    that is the output layer's too.  Sums are fp32 in an order that depends on the
+    tokens alone: equal calls give equal bits.  Tokens outside the table add
+    nothing.  weight: as in ``embedding``, or its (V, D) shape."""
+    if isinstance(weight, tuple):
+        shape = weight
+    else:
+        shape = weight.shape if isinstance(weight, QuantizedParameters) else tuple(
+            (weight.data if isinstance(weight, Parameters) else weight).shape)
+    if len(shape) != 2:
+        raise ValueError(f"weight must be a (rows, columns) table, got shape {tuple(shape)}")
+    V, D = shape
+    g, gdt, was_numpy = _float_arg(grad, "grad")
+    ids, bits = _ids_arg(tokens, V, "tokens")
+    if tuple(g.shape) != (*ids.shape, D):
+        raise ValueError(f"grad {tuple(g.shape)} does not match tokens {tuple(ids.shape)} and "
+                         f"{D} columns")
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate adds to out: none was given")
+        out = torch.empty((V, D), dtype=torch.float32, device=g.device)
+    else:
+        if not isinstance(out, torch.Tensor) or not out.is_cuda or out.dtype not in _TOKEN_FLOATS:
+            raise TypeError("out must be an fp32, bf16 or f16 device tensor")
+        if tuple(out.shape) != (V, D) or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {(V, D)} tensor")
+        was_numpy = False
+    lib = _lib.load()
+    N = ids.numel()
+    nbytes = lib.novaq_embedding_backward_workspace(N, V, D)
+    work = _workspace(nbytes, g.device)
+    check(lib.novaq_embedding_backward(
+        g.data_ptr() if N else None, gdt, ids.data_ptr() if N else None, bits, N, V, D, factor,
+        1 if accumulate else 0, out.data_ptr(), DTYPES[_TOKEN_FLOATS[out.dtype]],
+        None if work is None else work.data_ptr(), nbytes, _stream(g.device)),
+        "embedding backward")
+    return out.cpu().numpy() if was_numpy else out
+
+
+def _loss_args(input, weight, targets, ignore_index, reduction):
+    if reduction not in _lib.REDUCTIONS:
+        raise ValueError(f"reduction must be one of {tuple(_lib.REDUCTIONS)}, got {reduction!r}")
+    x, xdt, was_numpy = _float_arg(input, "input")
+    if x.dim() != 2:
+        raise ValueError(f"linear_cross_entropy expects a 2-D input, got shape {tuple(x.shape)}")
+    w, wdt, ws, (V, D) = _table_arg(weight, x.device)
+    if x.shape[1] != D:
+        raise ValueError(f"matmul: input {tuple(x.shape)} does not match weight {(V, D)}")
+    ids, bits = _ids_arg(targets, V, "targets", ignore_index)
+    if tuple(ids.shape) != (x.shape[0],):
+        raise ValueError(f"targets {tuple(ids.shape)} do not match {x.shape[0]} rows")
+    return x, xdt, was_numpy, w, wdt, ws, V, D, ids, bits
+
+
+def linear_cross_entropy(input, weight, targets, *, ignore_index: int = -100,
+                         reduction: str = "mean", extras: bool = False):
+    """Softmax cross entropy of the logits input @ weight^T, which are never
+    stored: loss[n] = log(sum_v exp(l[n, v])) - l[n, targets[n]].
+
+    input (N, D) fp32, bf16 or f16; weight (V, D) as in ``embedding``; targets
+    (N,) integers, rows with ``ignore_index`` have no loss.  reduction 'mean'
+    (over the rows that have a loss; 0 when none has), 'sum' or 'none'.  Returns
+    a 0-d fp32 tensor ((N,) for 'none'), numpy values for numpy input;
+    ``extras=True`` returns (loss, lse) with the rows' log-sum-exp (N,) for the
+    backward.  The products run in f16 for f16 input and in bf16 otherwise (fp32
+    operands are rounded, as in ``linear``), with fp32 sums.  Targets on the host
+    are checked (ValueError); one on the device outside the vocabulary gives a NaN
+    loss.  Stands for F.linear with CrossEntropyLoss
+    (novann/losses/loss_functions.py:8-167), on logits."""
+    x, xdt, was_numpy, w, wdt, ws, V, D, ids, bits = _loss_args(input, weight, targets,
+                                                                ignore_index, reduction)
+    N = x.shape[0]
+    lib = _lib.load()
+    loss = torch.empty((N,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
+    lse = torch.empty(N, dtype=torch.float32, device=x.device)
+    nbytes = lib.novaq_linear_cross_entropy_workspace(N, D, V, xdt, wdt)
+    work = _workspace(nbytes, x.device)
+    check(lib.novaq_linear_cross_entropy(
+        x.data_ptr(), xdt, N, D, w.data_ptr(), wdt, None if ws is None else ws.data_ptr(), V,
+        ids.data_ptr(), bits, ignore_index, _lib.REDUCTIONS[reduction], loss.data_ptr(),
+        lse.data_ptr(), work.data_ptr(), nbytes, _stream(x.device)), "linear cross entropy")
+    if was_numpy:
+        loss, lse = loss.cpu().numpy()[()], lse.cpu().numpy()
+    return (loss, lse) if extras else loss
+
+
+def linear_cross_entropy_backward(input, weight, targets, lse, *, grad=None,
+                                  ignore_index: int = -100, reduction: str = "mean",
+                                  weight_grad_dtype: Optional[str] = None):
+    """Gradients of ``linear_cross_entropy`` (same arguments; lse as it returned
+    it): (grad_input (N, D) in input's type, grad_weight (V, D) in
+    ``weight_grad_dtype``, input's type by default).
+
+    grad: the loss's own gradient, a number or fp32 tensor (one value, or (N,)
+    with reduction 'none'; default 1).  grad_weight is the gradient of the
+    dequantized table.  The softmax is rounded to the products' 16-bit type
+    before it is multiplied, sums are fp32.  Ignored rows get and give no
+    gradient, whatever they hold.  ndarrays in -> ndarrays out (fp32, f16)."""
+    x, xdt, was_numpy, w, wdt, ws, V, D, ids, bits = _loss_args(input, weight, targets,
+                                                                ignore_index, reduction)
+    N = x.shape[0]
+    name = weight_grad_dtype or _TOKEN_FLOATS[x.dtype]
+    store = _out_dtype(name)
+    l, _ = _to_device_f32(lse, "lse")
+    if tuple(l.shape) != (N,):
+        raise ValueError(f"lse {tuple(l.shape)} does not match {N} rows")
+    g = None
+    if grad is not None:
+        if isinstance(grad, (int, float)):
+            g = torch.full((N,) if reduction == "none" else (1,), float(grad), device=x.device)
+        else:
+            g, _ = _to_device_f32(grad, "grad")
+        if g.numel() != (N if reduction == "none" else 1):
+            raise ValueError(f"grad has {g.numel()} values, the loss "
+                             f"{N if reduction == 'none' else 1}")
+    lib = _lib.load()
+    gx = torch.empty((N, D), dtype=x.dtype, device=x.device)
+    gw = torch.empty((V, D), dtype=store, device=x.device)
+    nbytes = lib.novaq_linear_cross_entropy_backward_workspace(N, D, V, xdt, wdt)
+    work = _workspace(nbytes, x.device)
+    check(lib.novaq_linear_cross_entropy_backward(
+        x.data_ptr(), xdt, N, D, w.data_ptr(), wdt, None if ws is None else ws.data_ptr(), V,
+        ids.data_ptr(), bits, ignore_index, _lib.REDUCTIONS[reduction],
+        None if g is None else g.data_ptr(), l.data_ptr(), gx.data_ptr(), gw.data_ptr(),
+        DTYPES[name], work.data_ptr(), nbytes, _stream(x.device)),
+        "linear cross entropy backward")
+    if was_numpy:
+        return gx.cpu().numpy(), (gw.cpu().numpy() if store != torch.bfloat16 else gw)
+    return gx, gw

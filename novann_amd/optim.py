@@ -16,6 +16,7 @@ array steps in float32 (the reference's float32 parameters).
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Iterable, List, Optional
 
 import numpy as np
@@ -142,3 +143,103 @@ class AdamW:
         """Clears the gradients of all optimized parameters (adamw.py:67-70)."""
         for p in self.params:
             p.zero_grad(set_to_none=set_to_none)
+
+
+_GRAD_TYPES = {torch.float32: DTYPES["f32"], torch.float16: DTYPES["f16"],
+               torch.bfloat16: DTYPES["bf16"], torch.float64: _lib.F64}
+
+
+def _clip(grads, outs, max_norm: float, eps: float, dev) -> torch.Tensor:
+    """The C call: device gradients and, when clipped ones are asked for, where
+    they go (both contiguous)."""
+    types = _GRAD_TYPES
+    if outs is None:
+        rows = [(g.data_ptr(), 0, g.numel(), types[g.dtype]) for g in grads]
+    else:
+        rows = [(g.data_ptr(), o.data_ptr(), g.numel(), types[g.dtype] | types[o.dtype] << 32)
+                for g, o in zip(grads, outs)]
+    # the rows of novaq_gradient (address, address, count, the two types)
+    table = array("q", [v for row in rows for v in row])
+    lib = _lib.load()
+    nbytes = lib.novaq_clip_grad_norm_workspace(len(rows))
+    work = torch.empty(nbytes + 16, dtype=torch.uint8, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    check(lib.novaq_clip_grad_norm(table.buffer_info()[0] if rows else None, len(rows), max_norm,
+                                   eps, norm.data_ptr(), work.data_ptr(), nbytes,
+                                   torch._C._cuda_getCurrentRawStream(dev.index)),
+          "clip_grad_norm")
+    return norm
+
+
+def _check_device_grad(g, what: str) -> None:
+    if g.dtype not in _GRAD_TYPES:
+        raise TypeError(f"{what} must be fp32, f16, bf16 or float64, got {g.dtype}")
+    if not g.is_cuda:
+        raise ValueError(f"{what} must be CUDA (HIP) device tensors, got one on {g.device}")
+
+
+def _gradients(items):
+    """[(holder or None, gradient)] of tensors, arrays or parameters with one."""
+    found = []
+    for p in items:
+        if isinstance(p, (torch.Tensor, np.ndarray)):
+            found.append((None, p))
+        elif p.grad is not None:
+            found.append((p, p.grad))
+    return found
+
+
+def _upload(g) -> torch.Tensor:
+    if isinstance(g, np.ndarray):
+        if g.dtype not in (np.float32, np.float64, np.float16):
+            raise TypeError(f"gradients must be float arrays, got {g.dtype}")
+        return torch.from_numpy(np.ascontiguousarray(g)).to(_device())
+    _check_device_grad(g, "gradients")
+    return g if g.is_contiguous() else g.contiguous()
+
+
+def grad_norm(gradients: Iterable) -> torch.Tensor:
+    """The 2-norm over all elements of all gradients (device tensors, numpy
+    arrays, or parameters, whose ``grad`` counts), a 0-d fp32 device tensor.
+    Squares are summed in fp64."""
+    dev_grads = [_upload(g) for _, g in _gradients(gradients)]
+    dev = dev_grads[0].device if dev_grads else _device()
+    return _clip(dev_grads, None, 0.0, 0.0, dev)
+
+
+def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
+                   out: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
+    """Scales gradients by min(1, max_norm / (norm + eps)), norm being their
+    common 2-norm, and returns that norm (a 0-d fp32 device tensor; nothing waits
+    for the device unless a gradient is a numpy array).
+
+    gradients: device tensors (fp32, f16, bf16, float64, mixed), numpy arrays, or
+    parameters, whose ``grad`` is taken; those without one are passed over.  They
+    are clipped in place, or, with ``out`` (a device tensor of the same shape for
+    each, contiguous, of any of these types), written there: bf16 gradients to the
+    fp32 ones an optimizer steps with in the same pass.  A NaN norm makes every
+    gradient NaN.  Stands for the clipping of the reference's SGD
+    (novann/optim/sgd.py:37-82), before any optimizer's step."""
+    max_norm, eps = float(max_norm), float(eps)
+    if not max_norm >= 0.0 or not eps >= 0.0:
+        raise ValueError(f"max_norm and eps must not be negative, got {max_norm} and {eps}")
+    found = _gradients(gradients)
+    dev_grads = [_upload(g) for _, g in found]
+    dev = dev_grads[0].device if dev_grads else _device()
+    if out is not None:
+        outs = list(out)
+        if len(outs) != len(dev_grads):
+            raise ValueError(f"{len(outs)} outputs for {len(dev_grads)} gradients")
+        for g, o in zip(dev_grads, outs):
+            _check_device_grad(o, "out")
+            if o.shape != g.shape or not o.is_contiguous():
+                raise ValueError(f"out must be contiguous with the gradient's shape "
+                                 f"{tuple(g.shape)}, got {tuple(o.shape)}")
+        return _clip(dev_grads, outs, max_norm, eps, dev)
+    norm = _clip(dev_grads, dev_grads, max_norm, eps, dev)
+    for (_, g), d in zip(found, dev_grads):
+        if isinstance(g, np.ndarray):
+            g[...] = d.cpu().numpy()
+        elif d is not g:
+            g.copy_(d)
+    return norm
