@@ -16,14 +16,14 @@ bool plain_float(int dt) { return dt == F32 || dt == F16 || dt == BF16; }
 bool any_weight(int dt) { return dt >= F32 && dt <= E2M1; }
 constexpr int64_t INT = 0x7FFFFFFF;
 
-// A (V, D) table: its type and whether it may have a scale, its sizes (row
-// pitches stay within 32 bits).
+// A (V, D) table: its type and whether it may have a scale, its sizes (256 fp32
+// rows stay within a buffer's 2 GiB).
 int check_table(int w_dtype, const float* w_scale, int64_t V, int64_t D) {
   if (!any_weight(w_dtype)) return NOVAQ_EDTYPE;
   if (w_scale && !is_quant(w_dtype)) return NOVAQ_EINVAL;
   if (V < 0 || D < 0) return NOVAQ_EINVAL;
   if (V == 0 || D == 0) return NOVAQ_ESHAPE;
-  if (V >= INT || D > (1 << 22)) return NOVAQ_ENOTSUP;
+  if (V >= INT || D > (1 << 20)) return NOVAQ_ENOTSUP;
   return NOVAQ_OK;
 }
 
@@ -68,7 +68,7 @@ int novaq_embedding(const void* ids, int id_bits, int64_t N, const void* table, 
 }
 
 size_t novaq_embedding_backward_workspace(int64_t N, int64_t V, int64_t D) {
-  if (N <= 0 || N >= INT - 1024 || V <= 0 || V >= INT || D <= 0 || D > (1 << 22)) return 0;
+  if (N <= 0 || N >= INT - 1024 || V <= 0 || V >= INT || D <= 0 || D > (1 << 20)) return 0;
   return embedding_backward_workspace(N, V, D);
 }
 

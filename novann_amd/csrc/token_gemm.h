@@ -6,7 +6,7 @@
 // Each operand lies either K-contiguous (element (r, k) at r * ld + k) or
 // K-strided (at k * ld + r), ld a multiple of 8 elements and 16-byte aligned.
 // Tiles go from memory straight into LDS (buffer_load ... lds, 16 bytes a
-// lane) through a ring of NS stages of 64 K; a K-contiguous tile is read into
+// lane) through two stages of 64 K; a K-contiguous tile is read into
 // MFMA fragments with 16-byte reads, a K-strided one with gfx950's transposing
 // read (ds_read_b64_tr_b16; its lane order is in TokenTile::read), so no operand
 // needs a transposed copy.  What lies past a matrix's last row reads as zeros
@@ -148,6 +148,18 @@ struct TokenTile {
   }
 };
 
+// Spreads a step's R LDS reads over its M MFMAs, reads first: in a burst they
+// would hold the matrix cores at each step's start.
+template <int R, int M, int I = 0>
+__device__ __forceinline__ void tg_mix() {
+  if constexpr (I < R) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    if constexpr ((I + 1) * M / R > I * M / R)
+      __builtin_amdgcn_sched_group_barrier(0x008, (I + 1) * M / R - I * M / R, 0);
+    tg_mix<R, M, I + 1>();
+  }
+}
+
 // The product of one BM x BN tile by 4 waves (2 x 2) of WM x WN: K blocks kb0
 // to kb1 of 64.  acc[i][j]: rows wm + 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4,
 // column wn + 32 j + lane % 32.  After it returns every wave is done with LDS.
@@ -158,8 +170,10 @@ struct TokenGemm {
   using A = TokenTile<AKS, BM, NTH>;
   using B = TokenTile<BKS, BN, NTH>;
   static constexpr int stage = A::bytes + B::bytes;
-  static constexpr int NS = 2;
-  static constexpr int lds_bytes = NS * stage;
+  // (the epilogue that stores P passes its tile through LDS, rows padded)
+  static constexpr int out_bytes = BN * (BM * 2 + 16);
+  static constexpr int lds_bytes = 2 * stage > out_bytes ? 2 * stage : out_bytes;
+  static constexpr int R = MT * (AKS ? 2 : 1) + NT * (BKS ? 2 : 1);  // LDS reads a step
   typedef tg_f32x16 Acc[MT][NT];
 
   struct Frags {
@@ -182,13 +196,13 @@ struct TokenGemm {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-    auto issue = [&](int kb) {
-      uint8_t* at = lds + (kb & 1) * stage;
+    auto issue = [&](int kb, int slot) {
+      uint8_t* at = lds + slot * stage;
       A::load(sa, oa, kb, at, wave);
       B::load(sb, ob, kb, at + A::bytes, wave);
     };
-    auto read = [&](Frags& f, int kb, const int s) {
-      const uint8_t* at = lds + (kb & 1) * stage;
+    auto read = [&](Frags& f, int slot, const int s) {
+      const uint8_t* at = lds + slot * stage;
 #pragma unroll
       for (int i = 0; i < MT; ++i) f.a[i] = A::read(at, wm, i, s, lane);
 #pragma unroll
@@ -200,18 +214,52 @@ struct TokenGemm {
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = tg_mfma<CT>(f.a[i], f.b[j], acc[i][j]);
     };
-    for (int kb = kb0; kb < kb1; ++kb) {
-      issue(kb);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      Frags f;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        read(f, kb, s);
-        multiply(f);
-      }
-      __syncthreads();
+    // Stage kb in four steps of 16 K, each step's fragments read while the one
+    // before is multiplied.  Before the last step: every wave's reads of stage kb
+    // and its copies of stage kb + 1 are done (counters, then the barrier), so
+    // stage kb + 2 may overwrite kb's slot, and step 0 of kb + 1 be read.
+    const int nb = kb1 - kb0;
+    if (nb <= 0) return;
+    auto wait_all = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    Frags f0, f1;
+    issue(kb0, 0);
+    if (nb > 1) {
+      issue(kb0 + 1, 1);
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(A::loads + B::loads) : "memory");
+    } else {
+      wait_all();
     }
+    read(f0, 0, 0);
+    for (int i = 0; i + 1 < nb; ++i) {
+      const int slot = i & 1;
+      read(f1, slot, 1);
+      multiply(f0);
+      tg_mix<R, MT * NT>();
+      read(f0, slot, 2);
+      multiply(f1);
+      tg_mix<R, MT * NT>();
+      read(f1, slot, 3);
+      multiply(f0);
+      tg_mix<R, MT * NT>();
+      wait_all();
+      if (i + 2 < nb) issue(kb0 + i + 2, slot);
+      read(f0, slot ^ 1, 0);
+      multiply(f1);
+      tg_mix<R, MT * NT>();
+    }
+    const int slot = (nb - 1) & 1;
+    read(f1, slot, 1);
+    multiply(f0);
+    read(f0, slot, 2);
+    multiply(f1);
+    read(f1, slot, 3);
+    multiply(f0);
+    multiply(f1);
+    wait_all();
   }
 };
 

@@ -31,6 +31,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "novaq_internal.h"
 #include "token_gemm.h"
 #include "token_io.h"
@@ -40,6 +43,11 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int T_NONE = -1, T_BAD = -2;  // no loss; an id outside the vocabulary
+
+// P's row pitch: its width and 128 elements more, so that rows of a power of two
+// do not fall on the same memory channels (grad_x's product of 4096 x 4096 x
+// 131072 reads 256 rows of it at a time).
+__host__ __device__ constexpr int64_t p_pitch(int64_t vp) { return vp + 128; }
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
@@ -360,20 +368,31 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_dx_kernel(TokenOp p, TokenOp w
          (int)(kblocks * (split + 1) / splits), lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
-  float* out = sums + (int64_t)split * N * dp;
+  // what lies past N or D is left out by the descriptor (offsets past it)
+  const int rows = (int)min((int64_t)G::BM, N - m0);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      sums + ((int64_t)split * N + m0) * dp, (short)0, rows * (int)dp * 4, 0x00020000);
+  const uint32_t pitch = (uint32_t)dp * 4;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
     const int64_t d = n0 + wn + 32 * j + (lane & 31);
-    if (d >= D) continue;
+    const uint32_t at = d < D ? (uint32_t)(wm + 4 * half) * pitch + (uint32_t)d * 4 : 0x80000000u;
 #pragma unroll
-    for (int i = 0; i < G::MT; ++i)
+    for (int i = 0; i < G::MT; ++i) {
+      float old[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t n = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (n >= N) continue;
-        float* q = out + n * dp + d;
-        *q = first ? acc[i][j][r] : *q + acc[i][j][r];
-      }
+      for (int r = 0; r < 16; ++r)
+        old[r] = first ? 0.0f
+                       : u2f(__builtin_amdgcn_raw_buffer_load_b32(
+                             rs, at + (32 * i + 8 * (r >> 2) + (r & 3)) * pitch, 0, 0));
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        __builtin_amdgcn_raw_buffer_store_b32(f2u(old[r] + acc[i][j][r]), rs,
+                                              at + (32 * i + 8 * (r >> 2) + (r & 3)) * pitch, 0,
+                                              0);
+      // (16 loads in flight at a time: all of a tile's would not fit the registers)
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 }
 
@@ -427,20 +446,27 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_dw_kernel(TokenOp p, TokenOp x
   const float a = scal[0] * inv_pscale;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
+  constexpr int OB = OT == F32 ? 4 : 2;
+  const int rows = (int)min((int64_t)G::BM, vc - m0);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      out + m0 * D * OB, (short)0, rows * (int)D * OB, 0x00020000);
+  const uint32_t pitch = (uint32_t)D * OB;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
     const int64_t d = n0 + wn + 32 * j + (lane & 31);
-    if (d >= D) continue;
+    const uint32_t at = d < D ? (uint32_t)(wm + 4 * half) * pitch + (uint32_t)d * OB : 0x80000000u;
 #pragma unroll
-    for (int i = 0; i < G::MT; ++i)
+    for (int i = 0; i < G::MT; ++i) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int64_t v = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (v >= vc) continue;
+        const uint32_t o = at + (32 * i + 8 * (r >> 2) + (r & 3)) * pitch;
         const float y = acc[i][j][r] * a;
-        if constexpr (OT == F32) reinterpret_cast<float*>(out)[v * D + d] = y;
-        else reinterpret_cast<uint16_t*>(out)[v * D + d] = (uint16_t)encode<OT>(f2u(y));
+        if constexpr (OT == F32) __builtin_amdgcn_raw_buffer_store_b32(f2u(y), rs, o, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)tg_pack2<OT>(y, 0.0f), rs, o, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 }
 
@@ -453,11 +479,16 @@ struct LossPlan {
   bool copy_x, copy_w;
   int64_t piece;     // vocabulary rows a piece (a multiple of 256)
   int64_t vtiles;    // tiles of the vocabulary
+  bool big_l, big_x, big_w;  // 256 x 256 tiles for the logits, grad_x, grad_W
   int splits;        // of grad_x's K
   size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, total;
 };
 
-constexpr int64_t TILE = 128;
+// Tiles of 256 x 256 (one workgroup a CU, 25% less LDS traffic an operation than
+// 128 x 128) where they make at least half a workgroup a CU, else 128 x 128.
+bool large_tiles(int64_t M, int64_t N) {
+  return ((M + 255) / 256) * ((N + 255) / 256) >= device_cu_count() / 2;
+}
 
 LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bool backward) {
   LossPlan p{};
@@ -473,8 +504,12 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   if (backward)
     p.piece = std::min(p.piece, std::max<int64_t>(1024, ((int64_t)1 << 29) / std::max<int64_t>(
                                                                     2 * N, 1) / 256 * 256));
-  p.vtiles = (V + TILE - 1) / TILE;
-  const int64_t tiles = ((N + TILE - 1) / TILE) * ((D + TILE - 1) / TILE);
+  p.big_l = large_tiles(p.piece, N);
+  p.big_x = large_tiles(N, D);
+  p.big_w = large_tiles(p.piece, D);
+  p.vtiles = (V + (p.big_l ? 255 : 127)) / (p.big_l ? 256 : 128);
+  const int64_t tx = p.big_x ? 256 : 128;
+  const int64_t tiles = ((N + tx - 1) / tx) * ((D + tx - 1) / tx);
   p.splits = 1;
   while (p.splits < 16 && tiles * p.splits * 2 <= device_cu_count() &&
          p.piece / 64 / (p.splits * 2) >= 4)
@@ -491,7 +526,7 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   p.wc = take(p.copy_w ? (size_t)p.piece * p.dp * 2 : 0);
   if (backward) {
     p.f = take((size_t)N * 4);
-    p.P = take((size_t)N * p.piece * 2);
+    p.P = take((size_t)N * p_pitch(p.piece) * 2);
     p.sums = take((size_t)p.splits * N * p.dp * 4);
   } else {
     p.stats = take((size_t)N * p.vtiles * 8);
@@ -522,7 +557,6 @@ template <int CT>
 int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
             int w_dtype, const float* w_scale, int64_t V, const void* ids, int bits,
             int64_t ignore, int reduction, float* loss, float* lse, uint8_t* ws, hipStream_t st) {
-  using G = TokenGemm<CT, false, false, 64, 64>;
   int* targets = reinterpret_cast<int*>(ws + p.targets);
   float* scal = reinterpret_cast<float*>(ws + p.scal);
   float2* stats = reinterpret_cast<float2*>(ws + p.stats);
@@ -551,9 +585,16 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
       wc = d;
     }
     const TokenOp ow{wc, vc, p.dp};
-    const int tm = (int)((vc + G::BM - 1) / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
-    NOVAQ_LAUNCH((loss_stats_kernel<CT, G>), (int64_t)tm * tn, G, st, ow, ox, p.dp, w_scale, v0,
-                 N, targets, stats, p.vtiles, tl, tm, tn);
+    auto stats_of = [&](auto g) -> int {
+      using G = decltype(g);
+      const int tm = (int)((vc + G::BM - 1) / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
+      NOVAQ_LAUNCH((loss_stats_kernel<CT, G>), (int64_t)tm * tn, G, st, ow, ox, p.dp, w_scale,
+                   v0, N, targets, stats, p.vtiles, tl, tm, tn);
+      return NOVAQ_OK;
+    };
+    rc = p.big_l ? stats_of(TokenGemm<CT, false, false, 128, 128>{})
+                 : stats_of(TokenGemm<CT, false, false, 64, 64>{});
+    if (rc != NOVAQ_OK) return rc;
   }
   hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, st, stats,
                      p.vtiles, N, targets, tl, lse, each);
@@ -569,9 +610,6 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
              int w_dtype, const float* w_scale, int64_t V, const void* ids, int bits,
              int64_t ignore, int reduction, const float* grad, const float* lse, void* gx,
              void* gw, int gw_dtype, uint8_t* ws, hipStream_t st) {
-  using GL = TokenGemm<CT, false, false, 64, 64>;
-  using GX = TokenGemm<CT, false, true, 64, 64>;
-  using GW = TokenGemm<CT, true, true, 64, 64>;
   int* targets = reinterpret_cast<int*>(ws + p.targets);
   float* scal = reinterpret_cast<float*>(ws + p.scal);
   float* f = reinterpret_cast<float*>(ws + p.f);
@@ -597,33 +635,48 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
       if (rc != NOVAQ_OK) return rc;
       wc = d;
     }
-    const TokenOp ow{wc, vc, p.dp}, op{P, N, vp}, opt{P, vp, vp};
-    {
-      const int tm = (int)(vp / GL::BM), tn = (int)((N + GL::BN - 1) / GL::BN);
-      NOVAQ_LAUNCH((loss_prob_kernel<CT, GL>), (int64_t)tm * tn, GL, st, ow, ox, p.dp, w_scale,
-                   v0, N, targets, f, lse, pscale, P, vp, tm, tn);
-    }
-    if (gx) {
-      const int tm = (int)((N + GX::BM - 1) / GX::BM), tn = (int)((D + GX::BN - 1) / GX::BN);
-      NOVAQ_LAUNCH((loss_dx_kernel<CT, GX>), (int64_t)tm * tn * p.splits, GX, st, op, ow, vc,
+    const int64_t pp = p_pitch(vp);
+    const TokenOp ow{wc, vc, p.dp}, op{P, N, pp}, opt{P, vp, pp};
+    auto prob = [&](auto g) -> int {
+      using G = decltype(g);
+      const int tm = (int)(vp / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
+      NOVAQ_LAUNCH((loss_prob_kernel<CT, G>), (int64_t)tm * tn, G, st, ow, ox, p.dp, w_scale, v0,
+                   N, targets, f, lse, pscale, P, pp, tm, tn);
+      return NOVAQ_OK;
+    };
+    rc = p.big_l ? prob(TokenGemm<CT, false, false, 128, 128>{})
+                 : prob(TokenGemm<CT, false, false, 64, 64>{});
+    if (rc != NOVAQ_OK) return rc;
+    auto dx = [&](auto g) -> int {
+      using G = decltype(g);
+      const int tm = (int)((N + G::BM - 1) / G::BM), tn = (int)((D + G::BN - 1) / G::BN);
+      NOVAQ_LAUNCH((loss_dx_kernel<CT, G>), (int64_t)tm * tn * p.splits, G, st, op, ow, vc,
                    vp / 64, p.splits, sums, N, p.dp, D, v0 == 0 ? 1 : 0, tm, tn);
+      return NOVAQ_OK;
+    };
+    if (gx) {
+      rc = p.big_x ? dx(TokenGemm<CT, false, true, 128, 128>{})
+                   : dx(TokenGemm<CT, false, true, 64, 64>{});
+      if (rc != NOVAQ_OK) return rc;
     }
+    auto dw = [&](auto g, auto ot) -> int {
+      using G = decltype(g);
+      constexpr int OT = decltype(ot)::value;
+      const int tm = (int)((vc + G::BM - 1) / G::BM), tn = (int)((D + G::BN - 1) / G::BN);
+      uint8_t* out = static_cast<uint8_t*>(gw) + v0 * D * (OT == F32 ? 4 : 2);
+      NOVAQ_LAUNCH((loss_dw_kernel<CT, OT, G>), (int64_t)tm * tn, G, st, opt, ox, N,
+                   (N + 63) / 64, vc, D, scal, inv, out, tm, tn);
+      return NOVAQ_OK;
+    };
+    auto dw_to = [&](auto ot) -> int {
+      return p.big_w ? dw(TokenGemm<CT, true, true, 128, 128>{}, ot)
+                     : dw(TokenGemm<CT, true, true, 64, 64>{}, ot);
+    };
     if (gw) {
-      const int tm = (int)((vc + GW::BM - 1) / GW::BM), tn = (int)((D + GW::BN - 1) / GW::BN);
-      uint8_t* out = static_cast<uint8_t*>(gw) + v0 * D * (gw_dtype == F32 ? 4 : 2);
-      switch (gw_dtype) {
-        case F32:
-          NOVAQ_LAUNCH((loss_dw_kernel<CT, F32, GW>), (int64_t)tm * tn, GW, st, opt, ox, N,
-                       (N + 63) / 64, vc, D, scal, inv, out, tm, tn);
-          break;
-        case F16:
-          NOVAQ_LAUNCH((loss_dw_kernel<CT, F16, GW>), (int64_t)tm * tn, GW, st, opt, ox, N,
-                       (N + 63) / 64, vc, D, scal, inv, out, tm, tn);
-          break;
-        default:
-          NOVAQ_LAUNCH((loss_dw_kernel<CT, BF16, GW>), (int64_t)tm * tn, GW, st, opt, ox, N,
-                       (N + 63) / 64, vc, D, scal, inv, out, tm, tn);
-      }
+      rc = gw_dtype == F32   ? dw_to(std::integral_constant<int, F32>{})
+           : gw_dtype == F16 ? dw_to(std::integral_constant<int, F16>{})
+                             : dw_to(std::integral_constant<int, BF16>{});
+      if (rc != NOVAQ_OK) return rc;
     }
   }
   if (gx) {
