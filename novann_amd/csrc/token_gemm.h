@@ -160,12 +160,13 @@ __device__ __forceinline__ void tg_mix() {
   }
 }
 
-// The product of one BM x BN tile by 4 waves (2 x 2) of WM x WN: K blocks kb0
+// The product of one BM x BN tile by WGM x WGN waves of WM x WN: K blocks kb0
 // to kb1 of 64.  acc[i][j]: rows wm + 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4,
 // column wn + 32 j + lane % 32.  After it returns every wave is done with LDS.
-template <int CT, bool AKS, bool BKS, int WM_, int WN_>
+template <int CT, bool AKS, bool BKS, int WM_, int WN_, int WGN_>
 struct TokenGemm {
-  static constexpr int WM = WM_, WN = WN_, BM = 2 * WM, BN = 2 * WN, NTH = 256;
+  static constexpr int WM = WM_, WN = WN_, WGM = 2, WGN = WGN_;
+  static constexpr int BM = WGM * WM, BN = WGN * WN, NTH = 64 * WGM * WGN;
   static constexpr int MT = WM / 32, NT = WN / 32;
   using A = TokenTile<AKS, BM, NTH>;
   using B = TokenTile<BKS, BN, NTH>;
@@ -186,7 +187,7 @@ struct TokenGemm {
                                              uint8_t* lds) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = (wave & 1) * WM, wn = (wave >> 1) * WN;
+    const int wm = (wave % WGM) * WM, wn = (wave / WGM) * WN;
     const typename A::Src sa = A::source(oa, m0, K, tid);
     const typename B::Src sb = B::source(ob, n0, K, tid);
 #pragma unroll

@@ -189,41 +189,63 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_stats_kernel(
 
   const float c2 = (w_scale ? *w_scale : 1.0f) * LOG2E;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
+  const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   const int rows = (int)min((int64_t)G::BM, w.rows - m0) - wm - 4 * half;  // of this lane
+  const bool ragged = w.rows - m0 < G::BM;
   float2* part = reinterpret_cast<float2*>(lds);  // [BN]
   float2 st[G::NT];
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
     const int64_t n = n0 + wn + 32 * j + (lane & 31);
     const int t = n < N ? targets[n] : T_NONE;
-    const int at = t < 0 ? -1 : (int)(t - v0 - m0 < 0 || t - v0 - m0 >= G::BM ? -1 : t - v0 - m0);
-    const int mine = at < 0 ? -1 : at - wm - 4 * half;
-    float m = -INFINITY;
+    const int64_t d = (int64_t)t - v0 - m0 - wm - 4 * half;
+    const int mine = t < 0 || d < 0 || d >= G::WM ? -1 : (int)d;
+    if (__ballot(mine >= 0)) {  // (few tiles hold a target of their tokens)
+      float l = 0.0f;
+      bool here = false;
 #pragma unroll
-    for (int i = 0; i < G::MT; ++i)
+      for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int at_row = 32 * i + 8 * (r >> 2) + (r & 3);
-        const float l = acc[i][j][r] * c2;
-        acc[i][j][r] = l;
-        m = at_row < rows ? fmaxf(m, l) : m;
-        if (at_row == mine) tlogit[n] = l;
-      }
-    const float z = m == -INFINITY ? 0.0f : m;
+        for (int r = 0; r < 16; ++r) {
+          const bool hit = 32 * i + 8 * (r >> 2) + (r & 3) == mine;
+          l = hit ? acc[i][j][r] : l;
+          here |= hit;
+        }
+      if (here) tlogit[n] = l * c2;
+    }
+    // rows past the vocabulary: below every logit (acc's sign makes it so in
+    // either sign of the scale)
+    if (ragged) {
+#pragma unroll
+      for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * i + 8 * (r >> 2) + (r & 3) >= rows) acc[i][j][r] = c2 < 0.0f ? INFINITY : -INFINITY;
+    }
+    float top = acc[0][j][0];
+    if (c2 < 0.0f) {
+#pragma unroll
+      for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fminf(top, acc[i][j][r]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+    }
+    const float m = top * c2, z = m == -INFINITY ? 0.0f : m;
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int at_row = 32 * i + 8 * (r >> 2) + (r & 3);
-        s += at_row < rows ? __builtin_amdgcn_exp2f(acc[i][j][r] - z) : 0.0f;
-      }
+      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c2, -z));
     const float om = __shfl_xor(m, 32), os = __shfl_xor(s, 32), t2 = fmaxf(m, om);
     const float tz = t2 == -INFINITY ? 0.0f : t2;
     s = s * __builtin_amdgcn_exp2f(m - tz) + os * __builtin_amdgcn_exp2f(om - tz);
     st[j] = float2{t2, s};
     if ((wave & 1) && half == 0) part[wn + 32 * j + (lane & 31)] = st[j];
+    __builtin_amdgcn_sched_barrier(0);  // (a column's values at a time in registers)
   }
   __syncthreads();
   if ((wave & 1) == 0 && half == 0) {
@@ -309,8 +331,9 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_prob_kernel(
 
   const float c2 = (w_scale ? *w_scale : 1.0f) * LOG2E;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
-  const int rows = (int)min((int64_t)G::BM, w.rows - m0) - wm - 4 * half;
+  const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
+  const int rows = (int)max((int64_t)0, min((int64_t)G::BM, w.rows - m0)) - wm - 4 * half;
+  const bool ragged = w.rows - m0 < G::BM;
   // token rows of BM 16-bit values and 16 bytes more, so that the rows that a
   // store touches start in different banks
   constexpr int PITCH = G::BM * 2 + 16;
@@ -321,24 +344,37 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_prob_kernel(
     const bool in = n < N;
     const int t = in ? targets[n] : T_NONE;
     const int64_t d = (int64_t)t - v0 - m0 - wm - 4 * half;
-    const int mine = t < 0 || d < 0 || d >= G::BM ? -1 : (int)d;
-    const float fn = in ? f[n] * pscale : 0.0f, l2 = in ? lse[n] * LOG2E : 0.0f;
-    const bool none = t == T_NONE;
+    const int mine = t < 0 || d < 0 || d >= G::WM ? -1 : (int)d;
+    // (an ignored row's x is zeros and its f 0: with any finite lse P is 0)
+    const float fn = in ? f[n] * pscale : 0.0f;
+    const float l2 = in && t != T_NONE ? lse[n] * LOG2E : 0.0f;
+    uint8_t* row = lds + col * PITCH + (wm + 4 * half) * 2;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float v[4];
+      for (int r = 0; r < 16; ++r)
+        acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c2, -l2));
+    if (__ballot(mine >= 0)) {  // (few tiles hold a target of their tokens)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int at_row = 32 * i + 8 * q + e;
-          const float p = __builtin_amdgcn_exp2f(acc[i][j][4 * q + e] * c2 - l2);
-          const float y = fn * (at_row == mine ? p - 1.0f : p);
-          v[e] = none || at_row >= rows ? 0.0f : y;
-        }
-        *reinterpret_cast<tg_u32x2*>(lds + col * PITCH + (wm + 4 * half + 32 * i + 8 * q) * 2) =
-            tg_u32x2{tg_pack2<CT>(v[0], v[1]), tg_pack2<CT>(v[2], v[3])};
-      }
+      for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * i + 8 * (r >> 2) + (r & 3) == mine) acc[i][j][r] -= 1.0f;
+    }
+    if (ragged) {
+#pragma unroll
+      for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * i + 8 * (r >> 2) + (r & 3) >= rows) acc[i][j][r] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<tg_u32x2*>(row + (32 * i + 8 * q) * 2) =
+            tg_u32x2{tg_pack2<CT>(acc[i][j][4 * q] * fn, acc[i][j][4 * q + 1] * fn),
+                     tg_pack2<CT>(acc[i][j][4 * q + 2] * fn, acc[i][j][4 * q + 3] * fn)};
   }
   __syncthreads();
   constexpr int CPR = G::BM / 8;  // 16-byte chunks a token row
@@ -367,7 +403,7 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_dx_kernel(TokenOp p, TokenOp w
   G::run(acc, p, w, m0, n0, K, (int)(kblocks * split / splits),
          (int)(kblocks * (split + 1) / splits), lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
+  const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   // what lies past N or D is left out by the descriptor (offsets past it)
   const int rows = (int)min((int64_t)G::BM, N - m0);
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
@@ -445,7 +481,7 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_dw_kernel(TokenOp p, TokenOp x
   G::run(acc, p, x, m0, n0, N, 0, (int)kblocks, lds);
   const float a = scal[0] * inv_pscale;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int wm = (wave & 1) * G::WM, wn = (wave >> 1) * G::WN;
+  const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   constexpr int OB = OT == F32 ? 4 : 2;
   const int rows = (int)min((int64_t)G::BM, vc - m0);
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
@@ -484,10 +520,57 @@ struct LossPlan {
   size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, total;
 };
 
-// Tiles of 256 x 256 (one workgroup a CU, 25% less LDS traffic an operation than
-// 128 x 128) where they make at least half a workgroup a CU, else 128 x 128.
-bool large_tiles(int64_t M, int64_t N) {
-  return ((M + 255) / 256) * ((N + 255) / 256) >= device_cu_count() / 2;
+// Time (us, on 256 CUs) of an M x N product of K, on tiles of 256 x 256 or 128 x
+// 128.  A CU runs one workgroup of the first (8 waves) or two of the second at a
+// time; measured at K 1024 and 4096 (8192 x 8192 and 8192 x 4096 tiles of
+// logits): 1.67 us a block of 64 K and 4.8 a tile, 0.965 and 4.1 a pair of
+// tiles.  A tile that has its CU to itself takes 0.65 of the pair's time.
+double product_us(int64_t M, int64_t N, int64_t K, bool big) {
+  const int64_t e = big ? 256 : 128, cus = device_cu_count();
+  const int64_t tiles = ((M + e - 1) / e) * ((N + e - 1) / e);
+  const double blocks = (double)((K + 63) / 64);
+  if (big) return (double)((tiles + cus - 1) / cus) * (1.67 * blocks + 4.8);
+  const int64_t rest = tiles % (2 * cus);
+  const double pair = 0.965 * blocks + 4.1;
+  return (double)(tiles / (2 * cus)) * pair + (rest == 0 ? 0.0 : rest <= cus ? 0.65 * pair : pair);
+}
+bool large_tiles(int64_t M, int64_t N, int64_t K) {
+  return product_us(M, N, K, true) <= product_us(M, N, K, false);
+}
+double best_us(int64_t M, int64_t N, int64_t K) {
+  return std::min(product_us(M, N, K, true), product_us(M, N, K, false));
+}
+
+// The rows of a piece (a multiple of 256): at most 128 MiB of P (and of the
+// table's 16-bit copy), so that what one product writes the next ones find in
+// the 256 MB cache; among the sizes that divide the vocabulary into about that
+// many pieces, the one whose products take the least time by the model above.
+int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, bool backward) {
+  const int64_t vr = (V + 255) / 256 * 256;
+  int64_t most = vr;
+  if (backward) most = std::min(most, ((int64_t)1 << 26) / std::max<int64_t>(N, 1));
+  if (copy_w) most = std::min(most, ((int64_t)1 << 26) / dp);
+  most = std::max<int64_t>(most / 256 * 256, std::min<int64_t>(vr, 1024));
+  if (most >= vr) return vr;
+  auto cost = [&](int64_t rows) {
+    if (rows == 0) return 0.0;
+    double us = best_us(rows, N, D) + 5.0;
+    if (backward) us += best_us(N, D, rows) + best_us(rows, D, N) + 10.0;
+    return us;
+  };
+  int64_t best = most;
+  double least = 0.0;
+  const int64_t few = (vr + most - 1) / most;
+  for (int64_t k = few; k < few + 6; ++k) {
+    // k equal pieces, or whole ones of `most` first (k == few)
+    for (int whole = 0; whole < 2; ++whole) {
+      const int64_t rows = whole ? most : ((V + k - 1) / k + 255) / 256 * 256;
+      if (rows > most) continue;
+      const double us = (double)(V / rows) * cost(rows) + cost(V % rows);
+      if (least == 0.0 || us < least) least = us, best = rows;
+    }
+  }
+  return best;
 }
 
 LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bool backward) {
@@ -499,21 +582,20 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   // blocks of 64
   p.copy_x = backward || x_dtype != p.ct || D % 64 != 0;
   p.copy_w = w_dtype != p.ct || D % 64 != 0;
-  const int64_t vr = (V + 255) / 256 * 256;
-  p.piece = std::min<int64_t>(vr, 8192);
-  if (backward)
-    p.piece = std::min(p.piece, std::max<int64_t>(1024, ((int64_t)1 << 29) / std::max<int64_t>(
-                                                                    2 * N, 1) / 256 * 256));
-  p.big_l = large_tiles(p.piece, N);
-  p.big_x = large_tiles(N, D);
-  p.big_w = large_tiles(p.piece, D);
+  p.piece = loss_piece(N, D, p.dp, V, p.copy_w, backward);
+  p.big_l = large_tiles(p.piece, N, D);
+  p.big_w = large_tiles(p.piece, D, N);
   p.vtiles = (V + (p.big_l ? 255 : 127)) / (p.big_l ? 256 : 128);
-  const int64_t tx = p.big_x ? 256 : 128;
-  const int64_t tiles = ((N + tx - 1) / tx) * ((D + tx - 1) / tx);
-  p.splits = 1;
-  while (p.splits < 16 && tiles * p.splits * 2 <= device_cu_count() &&
-         p.piece / 64 / (p.splits * 2) >= 4)
-    p.splits *= 2;
+  // grad_x: K split where its tiles leave CUs idle, at least 4 blocks each
+  const int64_t kb = p.piece / 64;
+  double least = 0.0;
+  for (int splits = 1; splits <= 16 && (splits == 1 || kb / splits >= 4); splits *= 2)
+    for (int big = 0; big < 2; ++big) {
+      // (the splits' sums are written and added: 2 us and their bytes at 4 TB/s)
+      const double us = product_us(N * splits, D, p.piece / splits, big) +
+                        (splits - 1) * (2.0 + (double)N * (double)D * 8.0 / 4e6);
+      if (least == 0.0 || us < least) least = us, p.splits = splits, p.big_x = big;
+    }
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t b = at;
@@ -592,8 +674,8 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
                    v0, N, targets, stats, p.vtiles, tl, tm, tn);
       return NOVAQ_OK;
     };
-    rc = p.big_l ? stats_of(TokenGemm<CT, false, false, 128, 128>{})
-                 : stats_of(TokenGemm<CT, false, false, 64, 64>{});
+    rc = p.big_l ? stats_of(TokenGemm<CT, false, false, 128, 64, 4>{})
+                 : stats_of(TokenGemm<CT, false, false, 64, 64, 2>{});
     if (rc != NOVAQ_OK) return rc;
   }
   hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, st, stats,
@@ -644,8 +726,8 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
                    N, targets, f, lse, pscale, P, pp, tm, tn);
       return NOVAQ_OK;
     };
-    rc = p.big_l ? prob(TokenGemm<CT, false, false, 128, 128>{})
-                 : prob(TokenGemm<CT, false, false, 64, 64>{});
+    rc = p.big_l ? prob(TokenGemm<CT, false, false, 128, 64, 4>{})
+                 : prob(TokenGemm<CT, false, false, 64, 64, 2>{});
     if (rc != NOVAQ_OK) return rc;
     auto dx = [&](auto g) -> int {
       using G = decltype(g);
@@ -655,8 +737,8 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
       return NOVAQ_OK;
     };
     if (gx) {
-      rc = p.big_x ? dx(TokenGemm<CT, false, true, 128, 128>{})
-                   : dx(TokenGemm<CT, false, true, 64, 64>{});
+      rc = p.big_x ? dx(TokenGemm<CT, false, true, 128, 64, 4>{})
+                   : dx(TokenGemm<CT, false, true, 64, 64, 2>{});
       if (rc != NOVAQ_OK) return rc;
     }
     auto dw = [&](auto g, auto ot) -> int {
@@ -669,8 +751,8 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
       return NOVAQ_OK;
     };
     auto dw_to = [&](auto ot) -> int {
-      return p.big_w ? dw(TokenGemm<CT, true, true, 128, 128>{}, ot)
-                     : dw(TokenGemm<CT, true, true, 64, 64>{}, ot);
+      return p.big_w ? dw(TokenGemm<CT, true, true, 128, 64, 4>{}, ot)
+                     : dw(TokenGemm<CT, true, true, 64, 64, 2>{}, ot);
     };
     if (gw) {
       rc = gw_dtype == F32   ? dw_to(std::integral_constant<int, F32>{})
