@@ -6,7 +6,7 @@
 // Each operand lies either K-contiguous (element (r, k) at r * ld + k) or
 // K-strided (at k * ld + r), ld a multiple of 8 elements and 16-byte aligned.
 // Tiles go from memory straight into LDS (buffer_load ... lds, 16 bytes a
-// lane) through two stages of 64 K; a K-contiguous tile is read into
+// lane) through a ring of stages of 64 or 32 K; a K-contiguous tile is read into
 // MFMA fragments with 16-byte reads, a K-strided one with gfx950's transposing
 // read (ds_read_b64_tr_b16; its lane order is in TokenTile::read), so no operand
 // needs a transposed copy.  What lies past a matrix's last row reads as zeros
@@ -59,6 +59,18 @@ __device__ __forceinline__ uint32_t tg_pack2(float lo, float hi) {
   }
 }
 
+// 16 bytes a lane from a buffer (descriptor rs, byte offset voff) straight into
+// LDS at lds + 16 * lane, lds the same in all lanes.  In assembly because the
+// compiler otherwise waits for every copy in flight before each transposing LDS
+// read (grad_W's product of 4096 x 4096 x 16384: 546 us so, 447 with this).  A copy
+// has no output registers; what reads LDS waits for it by vmcnt and a barrier.
+__device__ __forceinline__ void tg_copy16(const tg_u32x4& rs, uint32_t voff, uint8_t* lds) {
+  const uint32_t at = (uint32_t)(uintptr_t)(tg_lds_void*)lds;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at),
+               "v"(voff), "s"(rs)
+               : "memory", "m0");
+}
+
 // One operand of a product: rows (M or N) of K elements.
 struct TokenOp {
   const uint16_t* p;
@@ -66,19 +78,20 @@ struct TokenOp {
   int64_t ld;    // elements between rows (K-contiguous) or between K (K-strided)
 };
 
-// The LDS tile of one operand: R rows (or columns) of 64 K, 128 R bytes.
+// The LDS tile of one operand: R rows (or columns) of KB K, 2 KB R bytes.
 //   K-contiguous: row r holds 8 chunks of 16 bytes, chunk c at slot
 //     c ^ ((r >> 1) & 7): the 16 rows that one 16-byte read touches at a time
 //     fall in distinct banks.
 //   K-strided: K row k holds R / 8 chunks, chunk c at slot c ^ (4 (k & 3)):
 //     the four K rows that a transposing read touches lie in distinct 64-byte
 //     bank ranges.
-template <bool KS, int R, int NTH>
+template <bool KS, int R, int KB, int NTH>
 struct TokenTile {
-  static constexpr int bytes = R * 128;
-  static constexpr int loads = R * 8 / NTH;  // 16-byte loads a lane a stage
-  static constexpr int cpr = KS ? R / 8 : 8;  // chunks a row
-  static_assert(R % 32 == 0 && (R * 8) % NTH == 0 && NTH % cpr == 0, "tile shape");
+  static constexpr int bytes = R * KB * 2;
+  static constexpr int loads = R * KB / 8 / NTH;  // 16-byte loads a lane a stage
+  static constexpr int cpr = KS ? R / 8 : 8;      // chunks a row
+  static_assert(R % 32 == 0 && (R * KB / 8) % NTH == 0 && NTH % cpr == 0, "tile shape");
+  static_assert(KS || KB == 64, "a K-contiguous row is copied in whole 128-byte lines");
 
   // byte offsets of this lane's loads from the tile's base in memory
   struct Src {
@@ -107,19 +120,18 @@ struct TokenTile {
     return s;
   }
 
-  // Copies stage kb (64 K) to lds (this wave's part of every load).
-  __device__ static __forceinline__ void load(const Src& s, const TokenOp& op, int kb,
+  // Copies stage kb (KB K) to lds (this wave's part of every load); with `none`
+  // zeros, without touching memory.
+  __device__ static __forceinline__ void load(const Src& s, const TokenOp& op, int kb, bool none,
                                               uint8_t* lds, int wave) {
-    const int64_t at = KS ? (int64_t)kb * 64 * op.ld * 2 : (int64_t)kb * 128;
+    const int64_t at = KS ? (int64_t)kb * KB * op.ld * 2 : (int64_t)kb * 128;
     int64_t left = s.left - at;
-    left = left < 0 ? 0 : left > 0x7FFFFFFF ? 0x7FFFFFFF : left;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(s.base) + at), (short)0, (int)left,
-        0x00020000);
+    left = none || left < 0 ? 0 : left > 0x7FFFFFFF ? 0x7FFFFFFF : left;
+    const uint64_t from = (uint64_t)(reinterpret_cast<const uint8_t*>(s.base) + at);
+    const tg_u32x4 rs = {(uint32_t)from, (uint32_t)(from >> 32), (uint32_t)left, 0x00020000u};
 #pragma unroll
     for (int i = 0; i < loads; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rs, (tg_lds_void*)(lds + (i * NTH + wave * 64) * 16), 16, s.voff[i], 0, 0, 0);
+      tg_copy16(rs, s.voff[i], lds + (i * NTH + wave * 64) * 16);
   }
 
   // Lane's byte offset of fragment (32 rows from w0 + 32 i, K 16 s .. + 15):
@@ -163,17 +175,21 @@ __device__ __forceinline__ void tg_mix() {
 // The product of one BM x BN tile by WGM x WGN waves of WM x WN: K blocks kb0
 // to kb1 of 64.  acc[i][j]: rows wm + 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4,
 // column wn + 32 j + lane % 32.  After it returns every wave is done with LDS.
-template <int CT, bool AKS, bool BKS, int WM_, int WN_, int WGN_>
+//
+// KB K a stage, NS stages in LDS: NS - 1 are in flight or in use ahead of the one
+// that is multiplied.
+template <int CT, bool AKS, bool BKS, int WM_, int WN_, int WGN_, int KB_ = 64, int NS_ = 2>
 struct TokenGemm {
+  static constexpr int KB = KB_, NS = NS_, STEPS = KB / 16;
   static constexpr int WM = WM_, WN = WN_, WGM = 2, WGN = WGN_;
   static constexpr int BM = WGM * WM, BN = WGN * WN, NTH = 64 * WGM * WGN;
   static constexpr int MT = WM / 32, NT = WN / 32;
-  using A = TokenTile<AKS, BM, NTH>;
-  using B = TokenTile<BKS, BN, NTH>;
+  using A = TokenTile<AKS, BM, KB, NTH>;
+  using B = TokenTile<BKS, BN, KB, NTH>;
   static constexpr int stage = A::bytes + B::bytes;
   // (the epilogue that stores P passes its tile through LDS, rows padded)
   static constexpr int out_bytes = BN * (BM * 2 + 16);
-  static constexpr int lds_bytes = 2 * stage > out_bytes ? 2 * stage : out_bytes;
+  static constexpr int lds_bytes = NS * stage > out_bytes ? NS * stage : out_bytes;
   static constexpr int R = MT * (AKS ? 2 : 1) + NT * (BKS ? 2 : 1);  // LDS reads a step
   typedef tg_f32x16 Acc[MT][NT];
 
@@ -199,8 +215,8 @@ struct TokenGemm {
 
     auto issue = [&](int kb, int slot) {
       uint8_t* at = lds + slot * stage;
-      A::load(sa, oa, kb, at, wave);
-      B::load(sb, ob, kb, at + A::bytes, wave);
+      A::load(sa, oa, kb, kb >= kb1, at, wave);
+      B::load(sb, ob, kb, kb >= kb1, at + A::bytes, wave);
     };
     auto read = [&](Frags& f, int slot, const int s) {
       const uint8_t* at = lds + slot * stage;
@@ -215,52 +231,40 @@ struct TokenGemm {
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = tg_mfma<CT>(f.a[i], f.b[j], acc[i][j]);
     };
-    // Stage kb in four steps of 16 K, each step's fragments read while the one
-    // before is multiplied.  Before the last step: every wave's reads of stage kb
-    // and its copies of stage kb + 1 are done (counters, then the barrier), so
-    // stage kb + 2 may overwrite kb's slot, and step 0 of kb + 1 be read.
-    const int nb = kb1 - kb0;
-    if (nb <= 0) return;
-    auto wait_all = [&]() {
+    // Stage kb in steps of 16 K, each step's fragments read while the one before is
+    // multiplied.  Before the last step: this wave's reads of stage kb and its
+    // copies of stage kb + 1 are done (counters), and after the barrier every
+    // wave's, so the copy of stage kb + NS may overwrite kb's slot, and step 0 of
+    // kb + 1 be read.  Copies are issued past the end too (of zeros), so that the
+    // counters are the same in every stage.
+    if (kb0 >= kb1) return;
+    constexpr int L = A::loads + B::loads;
+    Frags f[2];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) issue(kb0 + i, i);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * L) : "memory");
+    read(f[0], 0, 0);
+    int slot = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int next = slot + 1 == NS ? 0 : slot + 1;
+#pragma unroll
+      for (int s = 0; s + 1 < STEPS; ++s) {
+        read(f[(s + 1) & 1], slot, s + 1);
+        multiply(f[s & 1]);
+        tg_mix<R, MT * NT>();
+      }
       __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * L) : "memory");
       __builtin_amdgcn_sched_barrier(0);
-    };
-    Frags f0, f1;
-    issue(kb0, 0);
-    if (nb > 1) {
-      issue(kb0 + 1, 1);
-      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(A::loads + B::loads) : "memory");
-    } else {
-      wait_all();
+      issue(kb + NS, slot);
+      read(f[0], next, 0);
+      multiply(f[(STEPS - 1) & 1]);
+      tg_mix<R, MT * NT>();
+      slot = next;
     }
-    read(f0, 0, 0);
-    for (int i = 0; i + 1 < nb; ++i) {
-      const int slot = i & 1;
-      read(f1, slot, 1);
-      multiply(f0);
-      tg_mix<R, MT * NT>();
-      read(f0, slot, 2);
-      multiply(f1);
-      tg_mix<R, MT * NT>();
-      read(f1, slot, 3);
-      multiply(f0);
-      tg_mix<R, MT * NT>();
-      wait_all();
-      if (i + 2 < nb) issue(kb0 + i + 2, slot);
-      read(f0, slot ^ 1, 0);
-      multiply(f1);
-      tg_mix<R, MT * NT>();
-    }
-    const int slot = (nb - 1) & 1;
-    read(f1, slot, 1);
-    multiply(f0);
-    read(f0, slot, 2);
-    multiply(f1);
-    read(f1, slot, 3);
-    multiply(f0);
-    multiply(f1);
-    wait_all();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   }
 };
 
