@@ -63,12 +63,16 @@ __device__ __forceinline__ uint32_t tg_pack2(float lo, float hi) {
 // LDS at lds + 16 * lane, lds the same in all lanes.  In assembly because the
 // compiler otherwise waits for every copy in flight before each transposing LDS
 // read (grad_W's product of 4096 x 4096 x 16384: 546 us so, 447 with this).  A copy
-// has no output registers; what reads LDS waits for it by vmcnt and a barrier.
+// has no vector output; m0 (its LDS address) is put back; what reads LDS waits for it by vmcnt and a barrier.
 __device__ __forceinline__ void tg_copy16(const tg_u32x4& rs, uint32_t voff, uint8_t* lds) {
   const uint32_t at = (uint32_t)(uintptr_t)(tg_lds_void*)lds;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at),
-               "v"(voff), "s"(rs)
-               : "memory", "m0");
+  uint32_t kept;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+      "buffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+      : "=&s"(kept)
+      : "s"(at), "v"(voff), "s"(rs)
+      : "memory");
 }
 
 // One operand of a product: rows (M or N) of K elements.

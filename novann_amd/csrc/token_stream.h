@@ -1,0 +1,183 @@
+// The vocabulary loss's logits for few tokens (at most 128): the table's codes
+// are read once, as stored, and what bounds the kernel is that read.
+//
+// A workgroup takes 128 table rows (32 a wave) and all tokens.  Stages of 128
+// bytes a row go straight into LDS (whole lines, 16-byte chunks swizzled as in
+// TokenTile) beside the tokens' matching K in the order of the MFMA fragments,
+// which a small kernel has laid out before: 1 KB a fragment, one coalesced copy.
+// A 16-byte chunk of a row holds E codes (8, 16 or 32) and feeds E / 8 MFMAs of
+// 16 K: lane half h of chunk pair c takes chunk 2 c + h, and MFMA u its codes 8 u
+// .. + 7, so the K of fragment (c, u) are E (2 c + h) + 8 u .. + 7 in both
+// operands.  Codes become 16-bit values by the packed converts, exactly.
+#pragma once
+
+#include "token_gemm.h"
+#include "token_io.h"
+
+namespace novaq {
+namespace {
+
+typedef __bf16 ts_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 ts_f16x2 __attribute__((ext_vector_type(2)));
+
+// 8 codes -> the 4 words of an MFMA fragment.  E4M3 / E5M2: words c0, c1; E2M1:
+// c0; 16-bit: the chunk itself (never called).
+template <int CT, int WT>
+__device__ __forceinline__ tg_u32x4 ts_decode8(uint32_t c0, uint32_t c1) {
+  tg_u32x4 o;
+#define NOVAQ_CVT(CVT, W, SEL) __builtin_bit_cast(uint32_t, CVT(W, 1.0f, SEL))
+  if constexpr (WT == E2M1) {
+    if constexpr (CT == BF16) {
+      o[0] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4, c0, 0);
+      o[1] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4, c0, 1);
+      o[2] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4, c0, 2);
+      o[3] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4, c0, 3);
+    } else {
+      o[0] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4, c0, 0);
+      o[1] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4, c0, 1);
+      o[2] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4, c0, 2);
+      o[3] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4, c0, 3);
+    }
+  } else if constexpr (WT == E4M3) {
+    if constexpr (CT == BF16) {
+      o[0] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8, c0, false);
+      o[1] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8, c0, true);
+      o[2] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8, c1, false);
+      o[3] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8, c1, true);
+    } else {
+      o[0] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8, c0, false);
+      o[1] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8, c0, true);
+      o[2] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8, c1, false);
+      o[3] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8, c1, true);
+    }
+  } else {
+    if constexpr (CT == BF16) {
+      o[0] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_bf8, c0, false);
+      o[1] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_bf8, c0, true);
+      o[2] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_bf8, c1, false);
+      o[3] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_bf16_bf8, c1, true);
+    } else {
+      o[0] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_bf8, c0, false);
+      o[1] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_bf8, c0, true);
+      o[2] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_bf8, c1, false);
+      o[3] = NOVAQ_CVT(__builtin_amdgcn_cvt_scalef32_pk_f16_bf8, c1, true);
+    }
+  }
+#undef NOVAQ_CVT
+  return o;
+}
+
+template <int CT, int WT, int NT_>
+struct TokenStream {
+  static constexpr int NT = NT_;                    // tiles of 32 tokens
+  static constexpr int E = 128 / dtype_bits(WT);    // codes a chunk
+  static constexpr int U = E / 8;                   // MFMAs a chunk
+  static constexpr int KS = 8 * E;                  // K a stage (128 bytes a row)
+  static constexpr int ROWS = 128, NTH = 256;
+  static constexpr int w_bytes = ROWS * 128, x_bytes = 4 * U * NT * 1024;
+  static constexpr int stage = w_bytes + x_bytes;
+  // two workgroups a CU where three stages leave room for it
+  static constexpr int NS = 3 * stage <= 80 * 1024 ? 3 : 2;
+  static constexpr int lds_bytes = NS * stage;
+  static constexpr int WL = 4, XL = U * NT, L = WL + XL;  // copies a lane a stage
+  static constexpr int kstages(int64_t D) { return (int)((D + KS - 1) / KS); }
+
+  typedef tg_f32x16 Acc[NT];
+
+  // acc[j]: table rows 32 wave + 8 (r / 4) + 4 (lane / 32) + r % 4 of r0 .., token
+  // 32 j + lane % 32.  xf: the tokens' fragments, stage by stage.
+  __device__ static __forceinline__ void run(Acc& acc, const uint8_t* w, int64_t rows,
+                                             int64_t row_bytes, int64_t r0, const uint8_t* xf,
+                                             int stages, uint8_t* lds) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int chunk = (tid & 7) ^ ((tid >> 4) & 7);  // of row tid / 8 (+ 32 i)
+    const int64_t left = min((int64_t)ROWS, rows - r0) * row_bytes;
+    const uint64_t from = (uint64_t)(w + r0 * row_bytes);
+    const uint64_t xfrom = (uint64_t)xf;
+    const tg_u32x4 xr = {(uint32_t)xfrom, (uint32_t)(xfrom >> 32),
+                         (uint32_t)(stages * x_bytes), 0x00020000u};
+    const tg_u32x4 wr = {(uint32_t)from, (uint32_t)(from >> 32), (uint32_t)left, 0x00020000u};
+    const uint32_t rb = (uint32_t)row_bytes;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][r] = 0.0f;
+
+    // chunks past a row's end and stages past the last one are zeros
+    auto issue = [&](int s, int slot) {
+      uint8_t* at = lds + slot * stage + wave * 1024;
+      const uint32_t c = (uint32_t)(s * 128 + chunk * 16);
+      const uint32_t base = c < rb && s < stages ? (uint32_t)(tid >> 3) * rb + c : 0x80000000u;
+#pragma unroll
+      for (int i = 0; i < WL; ++i) tg_copy16(wr, base + i * 32 * rb, at + i * 4096);
+      const uint32_t xb = s < stages ? (uint32_t)(s * x_bytes + tid * 16) : 0x80000000u;
+#pragma unroll
+      for (int i = 0; i < XL; ++i) tg_copy16(xr, xb + i * 4096, at + w_bytes + i * 4096);
+    };
+    const int r = lane & 31, h = lane >> 5;
+    const int wrow = (wave * 32 + r) * 128;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) issue(i, i);
+    int slot = 0;
+    for (int s = 0; s < stages; ++s) {
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * L) : "memory");
+      const uint8_t* at = lds + slot * stage;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const tg_u32x4 code = *reinterpret_cast<const tg_u32x4*>(
+            at + wrow + (((2 * c + h) ^ ((r >> 1) & 7)) << 4));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          tg_u32x4 a;
+          if constexpr (U == 1) a = code;
+          else if constexpr (U == 2) a = ts_decode8<CT, WT>(code[2 * u], code[2 * u + 1]);
+          else a = ts_decode8<CT, WT>(code[u], 0u);
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            acc[j] = tg_mfma<CT>(a,
+                                 *reinterpret_cast<const tg_u32x4*>(
+                                     at + w_bytes + ((c * U + u) * NT + j) * 1024 + lane * 16),
+                                 acc[j]);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      issue(s + NS, slot);
+      slot = slot + 1 == NS ? 0 : slot + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+};
+
+// The tokens' fragments: 16 bytes a thread, fragment ((stage 4 + c) U + u) NT + j
+// of 64 lanes; x (N x D) as ST, zeros past N and D.
+template <int CT, int ST>
+__global__ __launch_bounds__(256) void loss_fragments_kernel(const uint8_t* __restrict__ x,
+                                                             int64_t N, int64_t D, int E, int nt,
+                                                             int64_t total,
+                                                             uint16_t* __restrict__ out) {
+  const int U = E / 8;
+  const int64_t rb = row_bytes(ST, D);
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
+       q += (int64_t)gridDim.x * 256) {
+    const int lane = (int)(q & 63);
+    const int64_t fr = q >> 6;
+    const int j = (int)(fr % nt);
+    const int64_t step = fr / nt;
+    const int u = (int)(step % U);
+    const int64_t pair = step / U;  // of chunks
+    const int64_t n = j * 32 + (lane & 31), k = E * (2 * pair + (lane >> 5)) + 8 * u;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (n < N && k < D) {
+      if (D % 8 == 0) load8<ST, true>(x + n * rb, k, D, v);
+      else load8<ST, false>(x + n * rb, k, D, v);
+    }
+    tg_u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<tg_u32x4*>(out + q * 8) = o;
+  }
+}
+
+}  // namespace
+}  // namespace novaq

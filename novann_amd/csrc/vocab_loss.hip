@@ -37,6 +37,7 @@
 #include "novaq_internal.h"
 #include "token_gemm.h"
 #include "token_io.h"
+#include "token_stream.h"
 
 namespace novaq {
 namespace {
@@ -173,6 +174,73 @@ __device__ __forceinline__ void tile_of(int t, int tm, int tn, int& m, int& n) {
   n = rem / gm;
 }
 
+// log2(e) times the scale; 0 (all logits 0) becomes the smallest normal number,
+// which leaves them 0 and a product with an infinity infinite.
+__device__ __forceinline__ float logit_factor(const float* w_scale) {
+  const float c2 = (w_scale ? *w_scale : 1.0f) * LOG2E;
+  return c2 == 0.0f ? 0x1p-126f : c2;
+}
+
+// (maximum, sum of 2^(l2 - maximum)) of two disjoint sets of one token's logits.
+__device__ __forceinline__ float2 join_stats(const float2& a, const float2& b) {
+  const float m = fmaxf(a.x, b.x), z = m == -INFINITY ? 0.0f : m;
+  return float2{m, a.y * __builtin_amdgcn_exp2f(a.x - z) + b.y * __builtin_amdgcn_exp2f(b.x - z)};
+}
+
+// The statistics of one token's products in a wave's MT row tiles, both lane
+// halves.  at(i, r): the lane's product of row 32 i + 8 (r / 4) + r % 4 (from its
+// own first row); those from `rows` on do not exist.  mine: the row of the token's
+// target, or -1; its logit goes to *tlogit.
+template <int MT, class F>
+__device__ __forceinline__ float2 column_stats(F&& at, bool ragged, int rows, int mine, float c2,
+                                               float* tlogit) {
+  if (__ballot(mine >= 0)) {  // (few tiles hold a target of their tokens)
+    float l = 0.0f;
+    bool here = false;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool hit = 32 * i + 8 * (r >> 2) + (r & 3) == mine;
+        l = hit ? at(i, r) : l;
+        here |= hit;
+      }
+    if (here) *tlogit = l * c2;
+  }
+  if (ragged) {  // below every logit, in either sign of the scale
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (32 * i + 8 * (r >> 2) + (r & 3) >= rows) at(i, r) = c2 < 0.0f ? INFINITY : -INFINITY;
+  }
+  float top = at(0, 0);
+  if (c2 < 0.0f) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fminf(top, at(i, r));
+  } else {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, at(i, r));
+  }
+  const float m = top * c2, z = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(at(i, r), c2, -z));
+  return join_stats(float2{m, s}, float2{__shfl_xor(m, 32), __shfl_xor(s, 32)});
+}
+
+// The row of token n's target among the `many` rows from r0 on, or -1.
+__device__ __forceinline__ int target_row(int t, int64_t r0, int many) {
+  const int64_t d = (int64_t)t - r0;
+  return t < 0 || d < 0 || d >= many ? -1 : (int)d;
+}
+
 // The forward's tile: BM vocabulary rows (from v0 + m0) x BN tokens.  A lane
 // holds one token's logits of a column, so a row's maximum and sum stay in
 // registers but for one exchange between the lane halves and one between the
@@ -189,7 +257,7 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_stats_kernel(
   typename G::Acc acc;
   G::run(acc, w, x, m0, n0, dp, 0, (int)(dp / 64), lds);
 
-  const float c2 = (w_scale ? *w_scale : 1.0f) * LOG2E;
+  const float c2 = logit_factor(w_scale);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   const int rows = (int)min((int64_t)G::BM, w.rows - m0) - wm - 4 * half;  // of this lane
@@ -200,52 +268,9 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_stats_kernel(
   for (int j = 0; j < G::NT; ++j) {
     const int64_t n = n0 + wn + 32 * j + (lane & 31);
     const int t = n < N ? targets[n] : T_NONE;
-    const int64_t d = (int64_t)t - v0 - m0 - wm - 4 * half;
-    const int mine = t < 0 || d < 0 || d >= G::WM ? -1 : (int)d;
-    if (__ballot(mine >= 0)) {  // (few tiles hold a target of their tokens)
-      float l = 0.0f;
-      bool here = false;
-#pragma unroll
-      for (int i = 0; i < G::MT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool hit = 32 * i + 8 * (r >> 2) + (r & 3) == mine;
-          l = hit ? acc[i][j][r] : l;
-          here |= hit;
-        }
-      if (here) tlogit[n] = l * c2;
-    }
-    // rows past the vocabulary: below every logit (acc's sign makes it so in
-    // either sign of the scale)
-    if (ragged) {
-#pragma unroll
-      for (int i = 0; i < G::MT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * i + 8 * (r >> 2) + (r & 3) >= rows) acc[i][j][r] = c2 < 0.0f ? INFINITY : -INFINITY;
-    }
-    float top = acc[0][j][0];
-    if (c2 < 0.0f) {
-#pragma unroll
-      for (int i = 0; i < G::MT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fminf(top, acc[i][j][r]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < G::MT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
-    }
-    const float m = top * c2, z = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < G::MT; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c2, -z));
-    const float om = __shfl_xor(m, 32), os = __shfl_xor(s, 32), t2 = fmaxf(m, om);
-    const float tz = t2 == -INFINITY ? 0.0f : t2;
-    s = s * __builtin_amdgcn_exp2f(m - tz) + os * __builtin_amdgcn_exp2f(om - tz);
-    st[j] = float2{t2, s};
+    st[j] = column_stats<G::MT>([&](int i, int r) -> float& { return ((float*)&acc[i][j])[r]; },
+                                ragged, rows, target_row(t, v0 + m0 + wm + 4 * half, G::WM), c2,
+                                tlogit + n);
     if ((wave & 1) && half == 0) part[wn + 32 * j + (lane & 31)] = st[j];
     __builtin_amdgcn_sched_barrier(0);  // (a column's values at a time in registers)
   }
@@ -254,12 +279,43 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_stats_kernel(
 #pragma unroll
     for (int j = 0; j < G::NT; ++j) {
       const int64_t n = n0 + wn + 32 * j + (lane & 31);
-      const float2 o = part[wn + 32 * j + (lane & 31)];
-      const float m = fmaxf(st[j].x, o.x), z = m == -INFINITY ? 0.0f : m;
-      const float s = st[j].y * __builtin_amdgcn_exp2f(st[j].x - z) +
-                      o.y * __builtin_amdgcn_exp2f(o.x - z);
-      if (n < N) stats[n * vtiles + (v0 + m0) / G::BM] = float2{m, s};
+      const float2 o = join_stats(st[j], part[wn + 32 * j + (lane & 31)]);
+      if (n < N) stats[n * vtiles + (v0 + m0) / G::BM] = o;
     }
+  }
+}
+
+// The same for at most 128 tokens, the table read as stored: 128 rows a
+// workgroup.
+template <int CT, int WT, class S>
+__global__ __launch_bounds__(S::NTH, 1) void loss_stream_kernel(
+    const uint8_t* __restrict__ w, int64_t V, int64_t rb, const uint8_t* __restrict__ xf,
+    int stages, const float* __restrict__ w_scale, int64_t N, const int* __restrict__ targets,
+    float2* __restrict__ stats, int64_t vtiles, float* __restrict__ tlogit) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int64_t r0 = (int64_t)blockIdx.x * S::ROWS;
+  typename S::Acc acc;
+  S::run(acc, w, V, rb, r0, xf, stages, lds);
+
+  const float c2 = logit_factor(w_scale);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int rows = (int)min((int64_t)S::ROWS, V - r0) - 32 * wave - 4 * half;
+  const bool ragged = V - r0 < S::ROWS;
+  float2* part = reinterpret_cast<float2*>(lds);  // [waves][tokens]
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) {
+    const int64_t n = 32 * j + (lane & 31);
+    const int t = n < N ? targets[n] : T_NONE;
+    const float2 st = column_stats<1>([&](int, int r) -> float& { return ((float*)&acc[j])[r]; },
+                                      ragged, rows,
+                                      target_row(t, r0 + 32 * wave + 4 * half, 32), c2, tlogit + n);
+    if (half == 0) part[wave * 32 * S::NT + 32 * j + (lane & 31)] = st;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < 32 * S::NT && (int64_t)threadIdx.x < N) {
+    float2 o = part[threadIdx.x];
+    for (int v = 1; v < S::NTH / 64; ++v) o = join_stats(o, part[v * 32 * S::NT + threadIdx.x]);
+    stats[(int64_t)threadIdx.x * vtiles + blockIdx.x] = o;
   }
 }
 
@@ -273,22 +329,13 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* __restrict
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= N) return;
-  float m = -INFINITY, s = 0.0f;
-  for (int64_t i = lane; i < vtiles; i += 64) {
-    const float2 o = stats[n * vtiles + i];
-    const float t = fmaxf(m, o.x), z = t == -INFINITY ? 0.0f : t;
-    s = s * __builtin_amdgcn_exp2f(m - z) + o.y * __builtin_amdgcn_exp2f(o.x - z);
-    m = t;
-  }
+  float2 a = {-INFINITY, 0.0f};
+#pragma unroll 4
+  for (int64_t i = lane; i < vtiles; i += 64) a = join_stats(a, stats[n * vtiles + i]);
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float om = __shfl_xor(m, d), os = __shfl_xor(s, d);
-    const float t = fmaxf(m, om), z = t == -INFINITY ? 0.0f : t;
-    s = s * __builtin_amdgcn_exp2f(m - z) + os * __builtin_amdgcn_exp2f(om - z);
-    m = t;
-  }
+  for (int d = 32; d; d >>= 1) a = join_stats(a, float2{__shfl_xor(a.x, d), __shfl_xor(a.y, d)});
   if (lane == 0) {
-    const float l2 = m + log2f(s);
+    const float l2 = a.x + log2f(a.y);
     const int t = targets[n];
     lse[n] = l2 * LN2;
     // (the difference in base 2: the factor's rounding falls on the loss alone)
@@ -331,7 +378,7 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_prob_kernel(
   typename G::Acc acc;
   G::run(acc, w, x, m0, n0, dp, 0, (int)(dp / 64), lds);
 
-  const float c2 = (w_scale ? *w_scale : 1.0f) * LOG2E;
+  const float c2 = logit_factor(w_scale);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   const int rows = (int)max((int64_t)0, min((int64_t)G::BM, w.rows - m0)) - wm - 4 * half;
@@ -345,8 +392,7 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_prob_kernel(
     const int64_t n = n0 + col;
     const bool in = n < N;
     const int t = in ? targets[n] : T_NONE;
-    const int64_t d = (int64_t)t - v0 - m0 - wm - 4 * half;
-    const int mine = t < 0 || d < 0 || d >= G::WM ? -1 : (int)d;
+    const int mine = target_row(t, v0 + m0 + wm + 4 * half, G::WM);
     // (an ignored row's x is zeros and its f 0: with any finite lse P is 0)
     const float fn = in ? f[n] * pscale : 0.0f;
     const float l2 = in && t != T_NONE ? lse[n] * LOG2E : 0.0f;
@@ -520,6 +566,8 @@ struct LossPlan {
   int64_t vtiles;    // tiles of the vocabulary
   bool big_l, big_x, big_w;  // 256 x 256 tiles for the logits, grad_x, grad_W
   int splits;        // of grad_x's K
+  bool stream;       // forward: the table read as stored, for few tokens
+  int64_t frag_bytes;
   size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, total;
 };
 
@@ -576,6 +624,8 @@ int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, boo
   return best;
 }
 
+int stream_tiles(int64_t N) { return N <= 32 ? 1 : N <= 64 ? 2 : 4; }
+
 LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bool backward) {
   LossPlan p{};
   p.ct = x_dtype == F16 ? F16 : BF16;
@@ -588,6 +638,15 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   p.copy_w = w_dtype != p.ct || D % 64 != 0;
   p.piece = loss_piece(N, D, p.dp, V, p.copy_w, backward);
   p.big_l = large_tiles(p.piece, N, D);
+  // up to 128 rows of x, codes whose rows are whole 16-byte chunks, in a type that
+  // the kernel decodes (16-bit ones as they are)
+  p.stream = !backward && N <= 128 && row_bytes(w_dtype, D) % 16 == 0 &&
+             (is_quant(w_dtype) || w_dtype == p.ct);
+  if (p.stream) {
+    const int E = 128 / dtype_bits(w_dtype), nt = stream_tiles(N);
+    p.frag_bytes = ((D + 8 * E - 1) / (8 * E)) * 4 * (E / 8) * nt * 1024;
+    p.big_l = p.copy_x = p.copy_w = false;
+  }
   p.big_w = large_tiles(p.piece, D, N);
   p.vtiles = (V + (p.big_l ? 255 : 127)) / (p.big_l ? 256 : 128);
   // grad_x: K split where its tiles leave CUs idle, at least 4 blocks each
@@ -608,7 +667,7 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   };
   p.targets = take((size_t)N * 4);
   p.scal = take(16);
-  p.xc = take(p.copy_x ? (size_t)N * p.pitch * 2 : 0);
+  p.xc = take(p.stream ? (size_t)p.frag_bytes : p.copy_x ? (size_t)N * p.pitch * 2 : 0);
   p.wc = take(p.copy_w ? (size_t)p.piece * p.pitch * 2 : 0);
   if (backward) {
     p.f = take((size_t)N * 4);
@@ -640,6 +699,43 @@ int raise_lds(const void* kern, DeviceFlags& raised) {
   } while (0)
 
 template <int CT>
+int stream(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
+           int w_dtype, const float* w_scale, int64_t V, const int* targets, float2* stats,
+           float* tl, uint16_t* frags, hipStream_t st) {
+  const uint8_t* xb = static_cast<const uint8_t*>(x);
+  const int64_t total = p.frag_bytes / 16;
+  const int E = 128 / dtype_bits(w_dtype), nt = stream_tiles(N);
+  const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, 4096));
+  if (x_dtype == F32)
+    hipLaunchKernelGGL((loss_fragments_kernel<CT, F32>), grid, dim3(256), 0, st, xb, N, D, E, nt,
+                       total, frags);
+  else  // (f16 and bf16 x are in the products' type)
+    hipLaunchKernelGGL((loss_fragments_kernel<CT, CT>), grid, dim3(256), 0, st, xb, N, D, E, nt,
+                       total, frags);
+  int rc = check_launch();
+  if (rc != NOVAQ_OK) return rc;
+  auto go = [&](auto wt, auto tiles) -> int {
+    constexpr int WT = decltype(wt)::value;
+    using S = TokenStream<CT, WT, decltype(tiles)::value>;
+    NOVAQ_LAUNCH((loss_stream_kernel<CT, WT, S>), p.vtiles, S, st, static_cast<const uint8_t*>(w),
+                 V, row_bytes(w_dtype, D), reinterpret_cast<const uint8_t*>(frags),
+                 S::kstages(D), w_scale, N, targets, stats, p.vtiles, tl);
+    return NOVAQ_OK;
+  };
+  auto to = [&](auto wt) -> int {
+    return nt == 1   ? go(wt, std::integral_constant<int, 1>{})
+           : nt == 2 ? go(wt, std::integral_constant<int, 2>{})
+                     : go(wt, std::integral_constant<int, 4>{});
+  };
+  switch (w_dtype) {
+    case E4M3: return to(std::integral_constant<int, E4M3>{});
+    case E5M2: return to(std::integral_constant<int, E5M2>{});
+    case E2M1: return to(std::integral_constant<int, E2M1>{});
+    default: return to(std::integral_constant<int, CT>{});
+  }
+}
+
+template <int CT>
 int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
             int w_dtype, const float* w_scale, int64_t V, const void* ids, int bits,
             int64_t ignore, int reduction, float* loss, float* lse, uint8_t* ws, hipStream_t st) {
@@ -652,6 +748,11 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
                      (const float*)nullptr, 0, 0, targets, (float*)nullptr, scal);
   int rc = check_launch();
   if (rc != NOVAQ_OK) return rc;
+  if (p.stream) {
+    uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.xc);
+    rc = stream<CT>(p, x, x_dtype, N, D, w, w_dtype, w_scale, V, targets, stats, tl, d, st);
+    if (rc != NOVAQ_OK) return rc;
+  }
   const uint16_t* xc = reinterpret_cast<const uint16_t*>(x);
   if (p.copy_x) {
     uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.xc);
@@ -660,7 +761,7 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
     xc = d;
   }
   const TokenOp ox{xc, N, p.copy_x ? p.pitch : D};
-  for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+  for (int64_t v0 = 0; v0 < V && !p.stream; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, V - v0);
     const uint16_t* wc = reinterpret_cast<const uint16_t*>(w) + v0 * D;
     if (p.copy_w) {
