@@ -6,10 +6,16 @@
 // Two passes over memory: the first leaves one fp64 sum of squares a workgroup
 // (products and sums in fp64, so neither the largest fp32 gradient nor the
 // smallest one leaves the range), the second adds these in a fixed order in
-// every workgroup (from L2) and scales.  The tensors' addresses and lengths
-// travel in the kernels' arguments, 96 tensors a launch: nothing is copied to
-// the device and nothing about a tensor outlives the call.  Workgroups walk
-// runs of 4096 elements of one launch's tensors.
+// every workgroup (from L2) and scales.  Both are bound by memory.  The tensors'
+// addresses and lengths travel in the kernels' arguments, or, past 120 of them,
+// through the workspace, which small kernels fill from theirs: nothing is copied
+// from host memory and nothing about a tensor outlives the call.
+//
+// All tensors are cut into runs (of 2048 to 16384 elements: at most 8 for each of
+// 2048 workgroups where there are enough elements), which the workgroups take in
+// turn, each looked up by bisection in the tensors' first runs.  A lane loads 4
+// vectors of 8 elements before it uses the first.  The second pass walks the runs
+// backwards: what the first read last is still in the 256 MB cache.
 //
 // NaN or infinite gradients give a NaN or infinite norm: the factor is then
 // NaN or 0, as the formula says (min keeps a NaN).
@@ -24,27 +30,36 @@
 namespace novaq {
 namespace {
 
-constexpr int F64 = NOVAQ_F64;     // (only here: float64 gradients)
-constexpr int TENSORS = 96;        // a launch: 3 KB of kernel arguments
-constexpr int RUN = 4096;          // elements of one workgroup's step
-constexpr int SLOTS = 2048;        // workgroups (and fp64 sums) over all launches
+constexpr int F64 = NOVAQ_F64;  // (only here: float64 gradients)
+constexpr int ROWS = 120;       // tensors in a kernel's arguments (3840 bytes)
+constexpr int BLOCKS = 2048;    // workgroups of a pass: eight a CU
+constexpr int STEP = 2048;      // elements of one vector of every lane
 
-struct NormList {
-  const void* g[TENSORS];
-  void* out[TENSORS];
-  int64_t n[TENSORS];
-  uint32_t first[TENSORS];  // its first run among the launch's
-  uint8_t gt[TENSORS], ot[TENSORS];
-  int count;
-  uint32_t runs;
+struct NormRow {
+  const void* g;
+  void* out;
+  int64_t n;
+  uint32_t first;  // its first run
+  uint8_t gt, ot;
+};
+static_assert(sizeof(NormRow) == 32, "120 rows fit a kernel's arguments");
+
+struct NormRows {
+  NormRow row[ROWS];
 };
 
-// The tensor that holds run r of the list.
-__device__ __forceinline__ int tensor_of(const NormList& l, uint32_t r) {
-  int lo = 0, hi = l.count - 1;
+__global__ __launch_bounds__(128) void norm_rows_kernel(const NormRows l, int count,
+                                                        NormRow* __restrict__ table) {
+  if ((int)threadIdx.x < count) table[threadIdx.x] = l.row[threadIdx.x];
+}
+
+// The tensor that holds run r.
+template <class T>
+__device__ __forceinline__ int tensor_of(const T& rows, int count, uint32_t r) {
+  int lo = 0, hi = count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (l.first[mid] <= r) lo = mid;
+    if (rows[mid].first <= r) lo = mid;
     else hi = mid - 1;
   }
   return lo;
@@ -55,172 +70,207 @@ __device__ __forceinline__ double block_sum(double s, double* part) {
   for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  s = part[0];
-  for (int w = 1; w < (int)blockDim.x / 64; ++w) s += part[w];
+  s = part[0] + part[1] + part[2] + part[3];
   __syncthreads();
   return s;
 }
 
-// f(i, v, m): m (1 or V) values from element i on, over the run at e0.
-template <int GT, class F>
-__device__ __forceinline__ void each_of_run(const void* p, int64_t n, int64_t e0, F&& f) {
-  const int64_t e1 = min(n, e0 + RUN);
+// f8(i, v): 8 values from element i on; f1(i, v): one; over elements e0 .. e1 - 1
+// (e0 a multiple of 2048).
+template <int GT, class F8, class F1>
+__device__ __forceinline__ void each_of_run(const void* p, int64_t e0, int64_t e1, F8&& f8,
+                                            F1&& f1) {
   const uint8_t* b = static_cast<const uint8_t*>(p);
-  if constexpr (GT == F64) {
-    for (int64_t i = e0 + threadIdx.x; i < e1; i += blockDim.x) {
-      const double v[1] = {reinterpret_cast<const double*>(b)[i]};
-      f(i, v, 1);
+  int64_t i = e0;
+  if constexpr (GT != F64) {
+    if ((reinterpret_cast<uintptr_t>(b) & 15) == 0) {
+      for (; i + 4 * STEP <= e1; i += 4 * STEP) {
+        float v[4][8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) load8<GT, true>(b, i + k * STEP + threadIdx.x * 8, e1, v[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f8(i + k * STEP + threadIdx.x * 8, v[k]);
+      }
+      const int64_t whole = i + (e1 - i) / 8 * 8;
+      for (int64_t k = i + threadIdx.x * 8; k < whole; k += STEP) {
+        float v[8];
+        load8<GT, true>(b, k, e1, v);
+        f8(k, v);
+      }
+      i = whole;
     }
-  } else {
-    const bool vec = (reinterpret_cast<uintptr_t>(b) & 15) == 0;
-    const int64_t whole = vec ? e0 + (e1 - e0) / 8 * 8 : e0;
-#pragma unroll 2
-    for (int64_t i = e0 + threadIdx.x * 8; i < whole; i += blockDim.x * 8) {
-      float v[8];
-      load8<GT, true>(b, i, n, v);
-      f(i, v, 8);
-    }
-    for (int64_t i = whole + threadIdx.x; i < e1; i += blockDim.x) {
-      float v[1];
-      if constexpr (GT == F32) v[0] = reinterpret_cast<const float*>(b)[i];
-      else v[0] = u2f(decode<GT>(reinterpret_cast<const uint16_t*>(b)[i]));
-      f(i, v, 1);
-    }
+  }
+  for (int64_t k = i + threadIdx.x; k < e1; k += 256) {
+    if constexpr (GT == F64) f1(k, reinterpret_cast<const double*>(b)[k]);
+    else if constexpr (GT == F32) f1(k, reinterpret_cast<const float*>(b)[k]);
+    else f1(k, u2f(decode<GT>(reinterpret_cast<const uint16_t*>(b)[k])));
   }
 }
 
-__global__ __launch_bounds__(256) void norm_sum_kernel(const NormList l,
+template <class F8, class F1>
+__device__ __forceinline__ void each_of(int gt, const void* p, int64_t e0, int64_t e1, F8&& f8,
+                                        F1&& f1) {
+  switch (gt) {
+    case F32: each_of_run<F32>(p, e0, e1, f8, f1); break;
+    case F16: each_of_run<F16>(p, e0, e1, f8, f1); break;
+    case BF16: each_of_run<BF16>(p, e0, e1, f8, f1); break;
+    default: each_of_run<F64>(p, e0, e1, f8, f1); break;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ double sum_runs(const T& rows, int count, uint32_t runs, int run) {
+  double s = 0.0;
+  for (uint32_t r = blockIdx.x; r < runs; r += gridDim.x) {
+    const int t = tensor_of(rows, count, r);
+    const int64_t e0 = (int64_t)(r - rows[t].first) * run, e1 = min(rows[t].n, e0 + run);
+    each_of(
+        rows[t].gt, rows[t].g, e0, e1,
+        [&](int64_t, const float(&v)[8]) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) s = fma((double)v[k], (double)v[k], s);
+        },
+        [&](int64_t, auto v) { s = fma((double)v, (double)v, s); });
+  }
+  return s;
+}
+
+template <bool TABLE>
+__global__ __launch_bounds__(256) void norm_sum_kernel(const NormRows l,
+                                                       const NormRow* __restrict__ table,
+                                                       int count, uint32_t runs, int run,
                                                        double* __restrict__ slots) {
   __shared__ double part[4];
-  double s = 0.0;
-  auto add = [&](int64_t, const auto* v, int m) {
-    for (int i = 0; i < m; ++i) {
-      const double d = (double)v[i];
-      s = fma(d, d, s);
-    }
-  };
-  for (uint32_t r = blockIdx.x; r < l.runs; r += gridDim.x) {
-    const int t = tensor_of(l, r);
-    const int64_t e0 = (int64_t)(r - l.first[t]) * RUN;
-    switch (l.gt[t]) {
-      case F32: each_of_run<F32>(l.g[t], l.n[t], e0, add); break;
-      case F16: each_of_run<F16>(l.g[t], l.n[t], e0, add); break;
-      case BF16: each_of_run<BF16>(l.g[t], l.n[t], e0, add); break;
-      default: each_of_run<F64>(l.g[t], l.n[t], e0, add); break;
-    }
-  }
+  double s;
+  if constexpr (TABLE) s = sum_runs(table, count, runs, run);
+  else s = sum_runs(l.row, count, runs, run);
   s = block_sum(s, part);
   if (threadIdx.x == 0) slots[blockIdx.x] = s;
 }
 
-__device__ __forceinline__ void put(void* out, int ot, int64_t i, double v) {
+template <int OT>
+__device__ __forceinline__ void put(void* out, int64_t i, float v) {
+  if constexpr (OT == F32) reinterpret_cast<float*>(out)[i] = v;
+  else if constexpr (OT == F64) reinterpret_cast<double*>(out)[i] = (double)v;
+  else reinterpret_cast<uint16_t*>(out)[i] = (uint16_t)encode<OT>(f2u(v));
+}
+__device__ __forceinline__ void put(int ot, void* out, int64_t i, float v) {
   switch (ot) {
-    case F32: reinterpret_cast<float*>(out)[i] = (float)v; break;
-    case F16: reinterpret_cast<uint16_t*>(out)[i] = (uint16_t)encode<F16>(f2u((float)v)); break;
-    case BF16: reinterpret_cast<uint16_t*>(out)[i] = (uint16_t)encode<BF16>(f2u((float)v)); break;
-    default: reinterpret_cast<double*>(out)[i] = v; break;
+    case F32: put<F32>(out, i, v); break;
+    case F16: put<F16>(out, i, v); break;
+    case BF16: put<BF16>(out, i, v); break;
+    default: put<F64>(out, i, v); break;
   }
 }
 
-__global__ __launch_bounds__(256) void norm_scale_kernel(const NormList l,
+template <class T>
+__device__ __forceinline__ void scale_runs(const T& rows, int count, uint32_t runs, int run,
+                                           float coef) {
+  for (uint32_t b = blockIdx.x; b < runs; b += gridDim.x) {
+    const uint32_t r = runs - 1 - b;
+    const int t = tensor_of(rows, count, r);
+    void* out = rows[t].out;
+    if (!out) continue;
+    const int64_t e0 = (int64_t)(r - rows[t].first) * run, e1 = min(rows[t].n, e0 + run);
+    const int ot = rows[t].ot;
+    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    each_of(
+        rows[t].gt, rows[t].g, e0, e1,
+        [&](int64_t i, const float(&v)[8]) {
+          float y[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = v[k] * coef;
+          if (vec && ot == F32) store8<F32, true>(out, i, 8, y);
+          else if (vec && ot == F16) store8<F16, true>(out, i, 8, y);
+          else if (vec && ot == BF16) store8<BF16, true>(out, i, 8, y);
+          else
+            for (int k = 0; k < 8; ++k) put(ot, out, i + k, y[k]);
+        },
+        [&](int64_t i, auto v) {
+          if (sizeof(v) == 8 && ot == F64) reinterpret_cast<double*>(out)[i] = v * (double)coef;
+          else put(ot, out, i, (float)(v * (decltype(v))coef));
+        });
+  }
+}
+
+template <bool TABLE>
+__global__ __launch_bounds__(256) void norm_scale_kernel(const NormRows l,
+                                                         const NormRow* __restrict__ table,
+                                                         int count, uint32_t runs, int run,
                                                          const double* __restrict__ slots,
                                                          int nslots, float max_norm, float eps,
                                                          float* __restrict__ norm) {
   __shared__ double part[4];
   double s = 0.0;
   for (int i = threadIdx.x; i < nslots; i += 256) s += slots[i];
-  s = block_sum(s, part);
-  const float nv = (float)sqrt(s);
+  const float nv = (float)sqrt(block_sum(s, part));
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = nv;
   const float q = max_norm / (nv + eps), coef = q > 1.0f ? 1.0f : q;  // (NaN stays)
-  for (uint32_t r = blockIdx.x; r < l.runs; r += gridDim.x) {
-    const int t = tensor_of(l, r);
-    if (!l.out[t]) continue;
-    const int64_t e0 = (int64_t)(r - l.first[t]) * RUN;
-    void* out = l.out[t];
-    const int ot = l.ot[t];
-    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    auto scale = [&](int64_t i, const auto* v, int m) {
-      if (m == 8) {
-        float y[8];
-        for (int k = 0; k < 8; ++k) y[k] = (float)v[k] * coef;
-        if (vec && ot == F32) store8<F32, true>(out, i, 8, y);
-        else if (vec && ot == F16) store8<F16, true>(out, i, 8, y);
-        else if (vec && ot == BF16) store8<BF16, true>(out, i, 8, y);
-        else
-          for (int k = 0; k < 8; ++k) put(out, ot, i + k, (double)y[k]);
-      } else if constexpr (sizeof(v[0]) == 8) {
-        put(out, ot, i, v[0] * (double)coef);
-      } else {
-        put(out, ot, i, (double)(v[0] * coef));
-      }
-    };
-    switch (l.gt[t]) {
-      case F32: each_of_run<F32>(l.g[t], l.n[t], e0, scale); break;
-      case F16: each_of_run<F16>(l.g[t], l.n[t], e0, scale); break;
-      case BF16: each_of_run<BF16>(l.g[t], l.n[t], e0, scale); break;
-      default: each_of_run<F64>(l.g[t], l.n[t], e0, scale); break;
-    }
-  }
+  if constexpr (TABLE) scale_runs(table, count, runs, run, coef);
+  else scale_runs(l.row, count, runs, run, coef);
 }
 
 }  // namespace
 
 size_t clip_grad_norm_workspace(int64_t count) {
-  // one slot a workgroup; launches of at most SLOTS over all of them, at least
-  // one workgroup each
-  return (size_t)(SLOTS + (count + TENSORS - 1) / TENSORS) * 8;
+  return BLOCKS * sizeof(double) + (count > ROWS ? (size_t)count * sizeof(NormRow) : 0);
 }
 
 int clip_grad_norm_launch(const novaq_gradient* list, int64_t count, float max_norm, float eps,
                           float* norm, void* workspace, hipStream_t st) {
   double* slots = static_cast<double*>(workspace);
-  int64_t total = 0;
+  NormRow* table = reinterpret_cast<NormRow*>(slots + BLOCKS);
+  int64_t total = 0, kept = 0;
   bool outputs = false;
   for (int64_t i = 0; i < count; ++i) {
-    total += (list[i].n + RUN - 1) / RUN;
+    total += list[i].n;
+    kept += list[i].n > 0;
     outputs |= list[i].out != nullptr && list[i].n > 0;
   }
-  int used = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    int64_t at = 0;
-    bool first = true;
-    do {
-      NormList l;
-      l.count = 0;
-      int64_t runs = 0;
-      while (at < count && l.count < TENSORS) {
-        const novaq_gradient& g = list[at];
-        const int64_t r = (g.n + RUN - 1) / RUN;
-        if (runs + r > 0x7FFFFFFF && l.count) break;
-        ++at;
-        if (g.n == 0) continue;
-        l.g[l.count] = g.grad;
-        l.out[l.count] = g.out;
-        l.n[l.count] = g.n;
-        l.gt[l.count] = (uint8_t)g.grad_dtype;
-        l.ot[l.count] = (uint8_t)g.out_dtype;
-        l.first[l.count++] = (uint32_t)runs;
-        runs += r;
-      }
-      l.runs = (uint32_t)runs;
-      if (runs == 0 && !(pass == 1 && first)) continue;
-      if (pass == 0) {
-        const int blocks = (int)std::max<int64_t>(1, std::min(runs, runs * SLOTS / total));
-        hipLaunchKernelGGL(norm_sum_kernel, dim3(blocks), dim3(256), 0, st, l, slots + used);
-        used += blocks;
-      } else {
-        const int blocks = (int)std::max<int64_t>(1, outputs ? std::min<int64_t>(runs, SLOTS) : 1);
-        hipLaunchKernelGGL(norm_scale_kernel, dim3(blocks), dim3(256), 0, st, l, slots, used,
-                           max_norm, eps, norm);
-      }
-      first = false;
+  int64_t run = STEP;
+  while (run < 8 * STEP && total / run > BLOCKS) run *= 2;
+  int64_t runs = 0;
+  for (int64_t i = 0; i < count; ++i) runs += (list[i].n + run - 1) / run;
+  if (runs > 0x7FFFFFFF || kept > 0x7FFFFFFF) return NOVAQ_ENOTSUP;
+  const bool by_table = kept > ROWS;
+  NormRows l;
+  int64_t at = 0, first = 0, done = 0;
+  do {
+    int k = 0;
+    for (; at < count && k < ROWS; ++at) {
+      const novaq_gradient& g = list[at];
+      if (g.n == 0) continue;
+      l.row[k++] = NormRow{g.grad, g.out, g.n, (uint32_t)first, (uint8_t)g.grad_dtype,
+                           (uint8_t)g.out_dtype};
+      first += (g.n + run - 1) / run;
+    }
+    if (by_table && k > 0) {
+      hipLaunchKernelGGL(norm_rows_kernel, dim3(1), dim3(128), 0, st, l, k, table + done);
       const int rc = check_launch();
       if (rc != NOVAQ_OK) return rc;
-      if (pass == 1 && !outputs) return NOVAQ_OK;  // the norm is all that is asked for
-    } while (at < count);
+      done += k;
+    }
+  } while (at < count);
+  const int blocks = (int)std::min<int64_t>(runs, BLOCKS);
+  const int scalers = std::max(1, outputs ? blocks : 1);
+  if (blocks > 0) {
+    if (by_table)
+      hipLaunchKernelGGL(norm_sum_kernel<true>, dim3(blocks), dim3(256), 0, st, l, table,
+                         (int)kept, (uint32_t)runs, (int)run, slots);
+    else
+      hipLaunchKernelGGL(norm_sum_kernel<false>, dim3(blocks), dim3(256), 0, st, l, table,
+                         (int)kept, (uint32_t)runs, (int)run, slots);
+    const int rc = check_launch();
+    if (rc != NOVAQ_OK) return rc;
   }
-  return NOVAQ_OK;
+  const uint32_t scaled = outputs ? (uint32_t)runs : 0u;
+  if (by_table)
+    hipLaunchKernelGGL(norm_scale_kernel<true>, dim3(scalers), dim3(256), 0, st, l, table,
+                       (int)kept, scaled, (int)run, slots, blocks, max_norm, eps, norm);
+  else
+    hipLaunchKernelGGL(norm_scale_kernel<false>, dim3(scalers), dim3(256), 0, st, l, table,
+                       (int)kept, scaled, (int)run, slots, blocks, max_norm, eps, norm);
+  return check_launch();
 }
 
 }  // namespace novaq

@@ -149,43 +149,40 @@ _GRAD_TYPES = {torch.float32: DTYPES["f32"], torch.float16: DTYPES["f16"],
                torch.bfloat16: DTYPES["bf16"], torch.float64: _lib.F64}
 
 
-def _clip(grads, outs, max_norm: float, eps: float, dev) -> torch.Tensor:
-    """The C call: device gradients and, when clipped ones are asked for, where
-    they go (both contiguous)."""
-    types = _GRAD_TYPES
-    if outs is None:
-        rows = [(g.data_ptr(), 0, g.numel(), types[g.dtype]) for g in grads]
-    else:
-        rows = [(g.data_ptr(), o.data_ptr(), g.numel(), types[g.dtype] | types[o.dtype] << 32)
-                for g, o in zip(grads, outs)]
-    # the rows of novaq_gradient (address, address, count, the two types)
-    table = array("q", [v for row in rows for v in row])
+def _clip(rows, count: int, max_norm: float, eps: float, dev) -> torch.Tensor:
+    """The C call on the rows of novaq_gradient, flat (address, address, count,
+    the two types)."""
+    table = array("q", rows)
     lib = _lib.load()
-    nbytes = lib.novaq_clip_grad_norm_workspace(len(rows))
-    work = torch.empty(nbytes + 16, dtype=torch.uint8, device=dev)
+    nbytes = lib.novaq_clip_grad_norm_workspace(count)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    check(lib.novaq_clip_grad_norm(table.buffer_info()[0] if rows else None, len(rows), max_norm,
+    check(lib.novaq_clip_grad_norm(table.buffer_info()[0] if rows else None, count, max_norm,
                                    eps, norm.data_ptr(), work.data_ptr(), nbytes,
                                    torch._C._cuda_getCurrentRawStream(dev.index)),
           "clip_grad_norm")
     return norm
 
 
-def _check_device_grad(g, what: str) -> None:
-    if g.dtype not in _GRAD_TYPES:
+def _device_type(g, what: str) -> int:
+    """The type code of a device tensor that may be clipped."""
+    code = _GRAD_TYPES.get(g.dtype)
+    if code is None:
         raise TypeError(f"{what} must be fp32, f16, bf16 or float64, got {g.dtype}")
     if not g.is_cuda:
         raise ValueError(f"{what} must be CUDA (HIP) device tensors, got one on {g.device}")
+    return code
 
 
-def _gradients(items):
-    """[(holder or None, gradient)] of tensors, arrays or parameters with one."""
+def _gradients(items) -> list:
+    """The gradients among tensors, arrays and parameters (those with one)."""
     found = []
     for p in items:
-        if isinstance(p, (torch.Tensor, np.ndarray)):
-            found.append((None, p))
-        elif p.grad is not None:
-            found.append((p, p.grad))
+        if not isinstance(p, (torch.Tensor, np.ndarray)):
+            p = p.grad
+            if p is None:
+                continue
+        found.append(p)
     return found
 
 
@@ -194,7 +191,7 @@ def _upload(g) -> torch.Tensor:
         if g.dtype not in (np.float32, np.float64, np.float16):
             raise TypeError(f"gradients must be float arrays, got {g.dtype}")
         return torch.from_numpy(np.ascontiguousarray(g)).to(_device())
-    _check_device_grad(g, "gradients")
+    _device_type(g, "gradients")
     return g if g.is_contiguous() else g.contiguous()
 
 
@@ -202,9 +199,11 @@ def grad_norm(gradients: Iterable) -> torch.Tensor:
     """The 2-norm over all elements of all gradients (device tensors, numpy
     arrays, or parameters, whose ``grad`` counts), a 0-d fp32 device tensor.
     Squares are summed in fp64."""
-    dev_grads = [_upload(g) for _, g in _gradients(gradients)]
-    dev = dev_grads[0].device if dev_grads else _device()
-    return _clip(dev_grads, None, 0.0, 0.0, dev)
+    dev_grads = [_upload(g) for g in _gradients(gradients)]
+    rows = []
+    for g in dev_grads:
+        rows += (g.data_ptr(), 0, g.numel(), _GRAD_TYPES[g.dtype])
+    return _clip(rows, len(dev_grads), 0.0, 0.0, dev_grads[0].device if dev_grads else _device())
 
 
 def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
@@ -224,20 +223,29 @@ def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
     if not max_norm >= 0.0 or not eps >= 0.0:
         raise ValueError(f"max_norm and eps must not be negative, got {max_norm} and {eps}")
     found = _gradients(gradients)
-    dev_grads = [_upload(g) for _, g in found]
-    dev = dev_grads[0].device if dev_grads else _device()
+    rows = []
     if out is not None:
         outs = list(out)
-        if len(outs) != len(dev_grads):
-            raise ValueError(f"{len(outs)} outputs for {len(dev_grads)} gradients")
-        for g, o in zip(dev_grads, outs):
-            _check_device_grad(o, "out")
+        if len(outs) != len(found):
+            raise ValueError(f"{len(outs)} outputs for {len(found)} gradients")
+        kept = []
+        for g, o in zip(found, outs):
+            if type(g) is not torch.Tensor or not g.is_contiguous():
+                g = _upload(g)
+                kept.append(g)
+            types = _device_type(g, "gradients") | _device_type(o, "out") << 32
             if o.shape != g.shape or not o.is_contiguous():
                 raise ValueError(f"out must be contiguous with the gradient's shape "
                                  f"{tuple(g.shape)}, got {tuple(o.shape)}")
-        return _clip(dev_grads, outs, max_norm, eps, dev)
-    norm = _clip(dev_grads, dev_grads, max_norm, eps, dev)
-    for (_, g), d in zip(found, dev_grads):
+            rows += (g.data_ptr(), o.data_ptr(), g.numel(), types)
+        return _clip(rows, len(found), max_norm, eps, outs[0].device if outs else _device())
+    dev_grads = [_upload(g) for g in found]
+    for g in dev_grads:
+        at, code = g.data_ptr(), _GRAD_TYPES[g.dtype]
+        rows += (at, at, g.numel(), code | code << 32)
+    norm = _clip(rows, len(found), max_norm, eps,
+                 dev_grads[0].device if dev_grads else _device())
+    for g, d in zip(found, dev_grads):
         if isinstance(g, np.ndarray):
             g[...] = d.cpu().numpy()
         elif d is not g:
