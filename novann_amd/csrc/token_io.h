@@ -24,19 +24,32 @@ __host__ __device__ inline int64_t row_bytes(int dtype, int64_t D) {
   return (D * dtype_bits(dtype) + 7) / 8;
 }
 
+// A vector load or store, past the caches where what it touches is not used
+// again (NT; streams of hundreds of MB run half as fast again so).
+template <bool NT, class T>
+__device__ __forceinline__ T vload(const T* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool NT, class T>
+__device__ __forceinline__ void vstore(T* p, const T& v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+
 // Elements c .. c + 7 of a row of D as fp32 (zeros past D), c a multiple of
 // 8.  VEC: D % 8 == 0 and the row starts on a boundary of 8 elements, so the
 // run is one or two whole vector loads.
-template <int ST, bool VEC>
+template <int ST, bool VEC, bool NT = false>
 __device__ __forceinline__ void load8(const uint8_t* row, int64_t c, int64_t D, float (&v)[8]) {
   if constexpr (VEC) {
     if constexpr (ST == F32) {
       const ti_u32x4* p = reinterpret_cast<const ti_u32x4*>(row + c * 4);
-      const ti_u32x4 a = p[0], b = p[1];
+      const ti_u32x4 a = vload<NT>(p), b = vload<NT>(p + 1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = u2f(a[i]), v[4 + i] = u2f(b[i]);
     } else if constexpr (ST == F16 || ST == BF16) {
-      const ti_u32x4 a = *reinterpret_cast<const ti_u32x4*>(row + c * 2);
+      const ti_u32x4 a = vload<NT>(reinterpret_cast<const ti_u32x4*>(row + c * 2));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t w = a[i];
@@ -44,14 +57,14 @@ __device__ __forceinline__ void load8(const uint8_t* row, int64_t c, int64_t D, 
         v[2 * i + 1] = u2f(decode<ST>(w >> 16));
       }
     } else if constexpr (ST == E4M3 || ST == E5M2) {
-      const ti_u32x2 a = *reinterpret_cast<const ti_u32x2*>(row + c);
+      const ti_u32x2 a = vload<NT>(reinterpret_cast<const ti_u32x2*>(row + c));
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t w = a[i >> 2];
         v[i] = u2f(decode<ST>((w >> (8 * (i & 3))) & 0xFFu));
       }
     } else {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(row + c / 2);
+      const uint32_t w = vload<NT>(reinterpret_cast<const uint32_t*>(row + c / 2));
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = u2f(decode<E2M1>((w >> (4 * i)) & 0xFu));
     }
@@ -74,7 +87,7 @@ __device__ __forceinline__ void load8(const uint8_t* row, int64_t c, int64_t D, 
 
 // 8 fp32 values stored as OT (F32, F16, BF16) at element e of out; whole
 // vectors (VEC: e on a boundary of 8 and 16-byte aligned) or the first `left`.
-template <int OT, bool VEC>
+template <int OT, bool VEC, bool NT = false>
 __device__ __forceinline__ void store8(void* out, int64_t e, int64_t left, const float (&v)[8]) {
   if constexpr (OT == F32) {
     float* p = reinterpret_cast<float*>(out) + e;
@@ -82,8 +95,8 @@ __device__ __forceinline__ void store8(void* out, int64_t e, int64_t left, const
       ti_u32x4 a, b;
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = f2u(v[i]), b[i] = f2u(v[4 + i]);
-      reinterpret_cast<ti_u32x4*>(p)[0] = a;
-      reinterpret_cast<ti_u32x4*>(p)[1] = b;
+      vstore<NT>(reinterpret_cast<ti_u32x4*>(p), a);
+      vstore<NT>(reinterpret_cast<ti_u32x4*>(p) + 1, b);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -98,7 +111,7 @@ __device__ __forceinline__ void store8(void* out, int64_t e, int64_t left, const
         if constexpr (OT == BF16) a[i] = pack_bf16x2(f2u(v[2 * i]), f2u(v[2 * i + 1]));
         else a[i] = encode<F16>(f2u(v[2 * i])) | (encode<F16>(f2u(v[2 * i + 1])) << 16);
       }
-      *reinterpret_cast<ti_u32x4*>(p) = a;
+      vstore<NT>(reinterpret_cast<ti_u32x4*>(p), a);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)

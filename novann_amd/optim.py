@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 from array import array
+from operator import attrgetter
 from typing import Iterable, List, Optional
 
 import numpy as np
@@ -149,61 +150,82 @@ _GRAD_TYPES = {torch.float32: DTYPES["f32"], torch.float16: DTYPES["f16"],
                torch.bfloat16: DTYPES["bf16"], torch.float64: _lib.F64}
 
 
-def _clip(rows, count: int, max_norm: float, eps: float, dev) -> torch.Tensor:
-    """The C call on the rows of novaq_gradient, flat (address, address, count,
-    the two types)."""
-    table = array("q", rows)
+# (what follows handles hundreds of tensors a call: whole lists at a time, a
+# few tenths of a microsecond a tensor)
+_data_ptr, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
+_contiguous = torch.Tensor.is_contiguous
+_dtype, _is_cuda = attrgetter("dtype"), attrgetter("is_cuda")
+
+
+def _type_codes(tensors, what: str) -> list:
+    """The type codes of device tensors that may be clipped (else TypeError or
+    ValueError)."""
+    codes = list(map(_GRAD_TYPES.get, map(_dtype, tensors)))
+    if None in codes:
+        raise TypeError(f"{what} must be fp32, f16, bf16 or float64, got "
+                        f"{tensors[codes.index(None)].dtype}")
+    if not all(map(_is_cuda, tensors)):
+        raise ValueError(f"{what} must be CUDA (HIP) device tensors, got one on the host")
+    return codes
+
+
+def _clip(grads, outs, max_norm: float, eps: float) -> torch.Tensor:
+    """The C call on contiguous device tensors; outs: where the clipped ones go,
+    or None."""
+    n = len(grads)
+    dev = grads[0].device if n else _device()
+    # the rows of novaq_gradient: address, address, count, the two types
+    types = _type_codes(grads, "gradients")
+    counts = array("q", map(_numel, grads))
+    table = array("q", bytes(32 * n))
+    table[0::4] = array("q", map(_data_ptr, grads))
+    table[2::4] = counts
+    if outs is not None:
+        if outs is not grads and array("q", map(_numel, outs)) != counts:
+            raise ValueError("every out must have as many elements as its gradient")
+        to = types if outs is grads else _type_codes(outs, "out")
+        types = [a | b << 32 for a, b in zip(types, to)]
+        table[1::4] = array("q", map(_data_ptr, outs))
+    table[3::4] = array("q", types)
     lib = _lib.load()
-    nbytes = lib.novaq_clip_grad_norm_workspace(count)
+    nbytes = lib.novaq_clip_grad_norm_workspace(n)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    check(lib.novaq_clip_grad_norm(table.buffer_info()[0] if rows else None, count, max_norm,
-                                   eps, norm.data_ptr(), work.data_ptr(), nbytes,
+    check(lib.novaq_clip_grad_norm(table.buffer_info()[0] if n else None, n, max_norm, eps,
+                                   norm.data_ptr(), work.data_ptr(), nbytes,
                                    torch._C._cuda_getCurrentRawStream(dev.index)),
           "clip_grad_norm")
     return norm
 
 
-def _device_type(g, what: str) -> int:
-    """The type code of a device tensor that may be clipped."""
-    code = _GRAD_TYPES.get(g.dtype)
-    if code is None:
-        raise TypeError(f"{what} must be fp32, f16, bf16 or float64, got {g.dtype}")
-    if not g.is_cuda:
-        raise ValueError(f"{what} must be CUDA (HIP) device tensors, got one on {g.device}")
-    return code
-
-
 def _gradients(items) -> list:
     """The gradients among tensors, arrays and parameters (those with one)."""
-    found = []
-    for p in items:
-        if not isinstance(p, (torch.Tensor, np.ndarray)):
-            p = p.grad
-            if p is None:
-                continue
-        found.append(p)
-    return found
+    items = list(items)
+    if set(map(type, items)) == {torch.Tensor}:
+        return items
+    found = (p if isinstance(p, (torch.Tensor, np.ndarray)) else p.grad for p in items)
+    return [g for g in found if g is not None]
 
 
-def _upload(g) -> torch.Tensor:
-    if isinstance(g, np.ndarray):
-        if g.dtype not in (np.float32, np.float64, np.float16):
-            raise TypeError(f"gradients must be float arrays, got {g.dtype}")
-        return torch.from_numpy(np.ascontiguousarray(g)).to(_device())
-    _device_type(g, "gradients")
-    return g if g.is_contiguous() else g.contiguous()
+def _uploaded(grads) -> list:
+    """The gradients as contiguous tensors, arrays on the device."""
+    def upload(g):
+        if isinstance(g, np.ndarray):
+            if g.dtype not in (np.float32, np.float64, np.float16):
+                raise TypeError(f"gradients must be float arrays, got {g.dtype}")
+            return torch.from_numpy(np.ascontiguousarray(g)).to(_device())
+        return g.contiguous()
+
+    if set(map(type, grads)) == {torch.Tensor} and all(map(_contiguous, grads)):
+        return grads
+    return [upload(g) for g in grads]
 
 
 def grad_norm(gradients: Iterable) -> torch.Tensor:
     """The 2-norm over all elements of all gradients (device tensors, numpy
     arrays, or parameters, whose ``grad`` counts), a 0-d fp32 device tensor.
     Squares are summed in fp64."""
-    dev_grads = [_upload(g) for g in _gradients(gradients)]
-    rows = []
-    for g in dev_grads:
-        rows += (g.data_ptr(), 0, g.numel(), _GRAD_TYPES[g.dtype])
-    return _clip(rows, len(dev_grads), 0.0, 0.0, dev_grads[0].device if dev_grads else _device())
+    return _clip(_uploaded(_gradients(gradients)), None, 0.0, 0.0)
 
 
 def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
@@ -214,8 +236,8 @@ def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
 
     gradients: device tensors (fp32, f16, bf16, float64, mixed), numpy arrays, or
     parameters, whose ``grad`` is taken; those without one are passed over.  They
-    are clipped in place, or, with ``out`` (a device tensor of the same shape for
-    each, contiguous, of any of these types), written there: bf16 gradients to the
+    are clipped in place, or, with ``out`` (for each a contiguous device tensor of as
+    many elements, of any of these types), written there: bf16 gradients to the
     fp32 ones an optimizer steps with in the same pass.  A NaN norm makes every
     gradient NaN.  Stands for the clipping of the reference's SGD
     (novann/optim/sgd.py:37-82), before any optimizer's step."""
@@ -223,29 +245,16 @@ def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
     if not max_norm >= 0.0 or not eps >= 0.0:
         raise ValueError(f"max_norm and eps must not be negative, got {max_norm} and {eps}")
     found = _gradients(gradients)
-    rows = []
+    grads = _uploaded(found)
     if out is not None:
         outs = list(out)
-        if len(outs) != len(found):
-            raise ValueError(f"{len(outs)} outputs for {len(found)} gradients")
-        kept = []
-        for g, o in zip(found, outs):
-            if type(g) is not torch.Tensor or not g.is_contiguous():
-                g = _upload(g)
-                kept.append(g)
-            types = _device_type(g, "gradients") | _device_type(o, "out") << 32
-            if o.shape != g.shape or not o.is_contiguous():
-                raise ValueError(f"out must be contiguous with the gradient's shape "
-                                 f"{tuple(g.shape)}, got {tuple(o.shape)}")
-            rows += (g.data_ptr(), o.data_ptr(), g.numel(), types)
-        return _clip(rows, len(found), max_norm, eps, outs[0].device if outs else _device())
-    dev_grads = [_upload(g) for g in found]
-    for g in dev_grads:
-        at, code = g.data_ptr(), _GRAD_TYPES[g.dtype]
-        rows += (at, at, g.numel(), code | code << 32)
-    norm = _clip(rows, len(found), max_norm, eps,
-                 dev_grads[0].device if dev_grads else _device())
-    for g, d in zip(found, dev_grads):
+        if len(outs) != len(grads):
+            raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
+        if not all(map(_contiguous, outs)):
+            raise ValueError("every out must be contiguous")
+        return _clip(grads, outs, max_norm, eps)
+    norm = _clip(grads, grads, max_norm, eps)
+    for g, d in zip(found, grads):
         if isinstance(g, np.ndarray):
             g[...] = d.cpu().numpy()
         elif d is not g:
