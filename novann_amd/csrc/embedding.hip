@@ -24,47 +24,61 @@
 namespace novaq {
 namespace {
 
-// A row per token, 8 elements a thread; a token outside the table gives a row
-// of NaN.
+// A row per token, 8 elements a thread and four such units a thread, whose ids
+// and then codes are all loaded before the first store; a token outside the table
+// gives a row of NaN.
 template <int ST, int OT, bool VEC>
 __global__ __launch_bounds__(256) void embedding_kernel(const void* __restrict__ ids, int bits,
-                                                        int64_t N,
                                                         const uint8_t* __restrict__ table,
                                                         const float* __restrict__ scale,
                                                         int64_t V, int64_t D, float factor,
-                                                        void* __restrict__ out) {
-  const int64_t per = (D + 7) / 8, rb = row_bytes(ST, D);
+                                                        int64_t i0, uint32_t units, uint32_t per,
+                                                        FastDiv by_per, void* __restrict__ out) {
+  constexpr int A = 4;
+  const int64_t rb = row_bytes(ST, D);
   const float a = (scale ? *scale : 1.0f) * factor;
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < N * per;
-       q += (int64_t)gridDim.x * 256) {
-    const int64_t i = q / per, c = (q - i * per) * 8;
-    const int64_t t = token_at(ids, bits, i);
-    float v[8];
-    if (t >= 0 && t < V) {
-      load8<ST, VEC>(table + t * rb, c, D, v);
+  const uint32_t q0 = blockIdx.x * (256 * A) + threadIdx.x;
+  int64_t t[A], i[A], c[A];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= a;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = u2f(0x7FC00000u);
-    }
-    store8<OT, VEC>(out, i * D + c, D - c, v);
+  for (int k = 0; k < A; ++k) {
+    const uint32_t q = min(q0 + k * 256, units - 1), r = fdiv(q, by_per);
+    i[k] = i0 + r;
+    c[k] = (int64_t)(q - r * per) * 8;
+    t[k] = token_at(ids, bits, i[k]);
   }
+  float v[A][8];
+#pragma unroll
+  for (int k = 0; k < A; ++k) {
+    const bool in = t[k] >= 0 && t[k] < V;
+    load8<ST, VEC>(table + (in ? t[k] : 0) * rb, c[k], D, v[k]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[k][e] = in ? v[k][e] * a : u2f(0x7FC00000u);
+  }
+#pragma unroll
+  for (int k = 0; k < A; ++k)
+    if (q0 + k * 256 < units) store8<OT, VEC>(out, i[k] * D + c[k], D - c[k], v[k]);
 }
 
 template <int ST, int OT>
 int lookup(const void* ids, int bits, int64_t N, const void* table, const float* scale, int64_t V,
            int64_t D, float factor, void* out, hipStream_t st) {
-  const int64_t units = N * ((D + 7) / 8);
-  const dim3 grid((unsigned)std::min<int64_t>((units + 255) / 256, 1 << 20));
+  const int64_t per = (D + 7) / 8, most = (int64_t)1 << 30;  // units a launch
   const uint8_t* t = static_cast<const uint8_t*>(table);
-  if (D % 8 == 0)
-    hipLaunchKernelGGL((embedding_kernel<ST, OT, true>), grid, dim3(256), 0, st, ids, bits, N, t,
-                       scale, V, D, factor, out);
-  else
-    hipLaunchKernelGGL((embedding_kernel<ST, OT, false>), grid, dim3(256), 0, st, ids, bits, N, t,
-                       scale, V, D, factor, out);
-  return check_launch();
+  for (int64_t i0 = 0; i0 < N; i0 += most / per) {
+    const uint32_t units = (uint32_t)(std::min(N - i0, most / per) * per);
+    const dim3 grid((units + 1023) / 1024);
+    if (D % 8 == 0)
+      hipLaunchKernelGGL((embedding_kernel<ST, OT, true>), grid, dim3(256), 0, st, ids, bits, t,
+                         scale, V, D, factor, i0, units, (uint32_t)per, fast_div((uint32_t)per),
+                         out);
+    else
+      hipLaunchKernelGGL((embedding_kernel<ST, OT, false>), grid, dim3(256), 0, st, ids, bits, t,
+                         scale, V, D, factor, i0, units, (uint32_t)per, fast_div((uint32_t)per),
+                         out);
+    const int rc = check_launch();
+    if (rc != NOVAQ_OK) return rc;
+  }
+  return NOVAQ_OK;
 }
 
 template <int ST>
@@ -79,11 +93,34 @@ int lookup_to(int ot, const void* ids, int bits, int64_t N, const void* table, c
 }
 
 // --------------------------------------------------------------------------
-// the sort
+// the sort, and the zeros under it
 
 constexpr int DIGIT = 9, BINS = 1 << DIGIT;
+constexpr int BATCH = 1024;     // entries of a block's batch: 4 a lane
 constexpr int BLOCKS = 128;     // at most, of a pass
+constexpr int SMALL = 2048;     // entries that one workgroup sorts in LDS
 constexpr int CHUNK = 16;       // sorted entries a wave sums
+
+// The rows that get no gradient must be zero: the sort's launches, which use few
+// workgroups, carry the table's zeros in their other ones (32768 tokens, a table
+// of 205 MB: 31 us of sorting and 28 of writing one after the other).
+struct Zeros {
+  uint8_t* p;
+  int64_t from, to;  // bytes, multiples of 16 but for the table's end
+};
+
+__device__ __forceinline__ void write_zeros(const Zeros& z, int block, int blocks, int threads) {
+  ti_u32x4* p = reinterpret_cast<ti_u32x4*>(z.p + z.from);
+  const int64_t n16 = (z.to - z.from) / 16;
+  for (int64_t i = (int64_t)block * threads + threadIdx.x; i < n16; i += (int64_t)blocks * threads)
+    p[i] = ti_u32x4{0u, 0u, 0u, 0u};
+  if (block == 0 && (int64_t)threadIdx.x < (z.to - z.from) % 16)
+    z.p[z.from + n16 * 16 + threadIdx.x] = 0;
+}
+
+__global__ __launch_bounds__(256) void embedding_zero_kernel(Zeros z) {
+  write_zeros(z, blockIdx.x, gridDim.x, 256);
+}
 
 // The sort's key of position i: the token, or V where it is none of the
 // table's (those sort last and are left out).
@@ -92,18 +129,127 @@ __device__ __forceinline__ uint32_t token_key(const void* ids, int bits, int64_t
   return t >= 0 && t < V ? (uint32_t)t : (uint32_t)V;
 }
 
+// Exclusive prefix sums of 64 lanes' values.
+__device__ __forceinline__ uint32_t wave_before(uint32_t v, int lane, uint32_t& total) {
+  uint32_t s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(s, d);
+    if (lane >= d) s += o;
+  }
+  total = __shfl(s, 63);
+  return s - v;
+}
+
+// Where the wave's 64 entries of digit d go: cnt[d] holds the next place of each
+// digit; equal digits are ranked by ballots and the place moved on by the first of
+// them (after the reads of this step, before those of the next).
+__device__ __forceinline__ uint32_t place(uint32_t* cnt, uint32_t d, bool in, int lane) {
+  uint64_t same = __ballot(in);
+#pragma unroll
+  for (int bit = 0; bit < DIGIT; ++bit) {
+    const uint64_t m = __ballot((d >> bit) & 1);
+    same &= (d >> bit) & 1 ? m : ~m;
+  }
+  const uint32_t rank = __popcll(same & ((1ull << lane) - 1));
+  uint32_t at = 0;
+  if (in) at = cnt[d] + rank;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (in && rank == 0) cnt[d] += (uint32_t)__popcll(same);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return at;
+}
+
+// Up to SMALL entries sorted by one workgroup in LDS, all passes; the other
+// workgroups write zeros.
+__global__ __launch_bounds__(512) void sort_small_kernel(const void* __restrict__ ids, int bits,
+                                                         int64_t V, int N, int passes,
+                                                         uint32_t* __restrict__ keys_out,
+                                                         uint32_t* __restrict__ pos_out,
+                                                         Zeros z) {
+  if (blockIdx.x > 0) {
+    write_zeros(z, blockIdx.x - 1, gridDim.x - 1, 512);
+    return;
+  }
+  constexpr int W = 8, PER = SMALL / 512;  // waves; entries a lane
+  __shared__ uint32_t key[SMALL], pos[SMALL], cnt[W][BINS], sums[W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // wave w holds entries w 64 PER .. : step i's are 64 i + lane of them
+  uint32_t k[PER], p[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = wave * 64 * PER + i * 64 + lane;
+    k[i] = e < N ? token_key(ids, bits, e, V) : 0u;
+    p[i] = (uint32_t)e;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * DIGIT;
+    for (int w = 0; w < W; ++w) cnt[w][tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (wave * 64 * PER + i * 64 + lane < N) atomicAdd(&cnt[wave][(k[i] >> shift) & (BINS - 1)], 1u);
+    __syncthreads();
+    // digit tid: its entries in all waves, then the digits before it
+    uint32_t all = 0, of_wave;
+    for (int w = 0; w < W; ++w) all += cnt[w][tid];
+    uint32_t at = wave_before(all, lane, of_wave);
+    if (lane == 0) sums[wave] = of_wave;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) at += sums[w];
+    for (int w = 0; w < W; ++w) {
+      const uint32_t c = cnt[w][tid];
+      cnt[w][tid] = at;
+      at += c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool in = wave * 64 * PER + i * 64 + lane < N;
+      const uint32_t to = place(cnt[wave], (k[i] >> shift) & (BINS - 1), in, lane);
+      if (in) key[to] = k[i], pos[to] = p[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = wave * 64 * PER + i * 64 + lane;
+      if (e < N) k[i] = key[e], p[i] = pos[e];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = wave * 64 * PER + i * 64 + lane;
+    if (e < N) keys_out[e] = k[i], pos_out[e] = p[i];
+  }
+}
+
 // Digit counts of each block's `per` entries: hist[block][digit].
 __global__ __launch_bounds__(256) void sort_hist_kernel(const uint32_t* __restrict__ keys,
                                                         const void* __restrict__ ids, int bits,
-                                                        int64_t V, int N, int per, int shift,
-                                                        uint32_t* __restrict__ hist) {
+                                                        int64_t V, int N, int per, int nb,
+                                                        int shift, uint32_t* __restrict__ hist,
+                                                        Zeros z) {
+  if ((int)blockIdx.x >= nb) {
+    write_zeros(z, blockIdx.x - nb, gridDim.x - nb, 256);
+    return;
+  }
   __shared__ uint32_t cnt[BINS];
   for (int d = threadIdx.x; d < BINS; d += 256) cnt[d] = 0;
   __syncthreads();
   const int from = blockIdx.x * per, to = min(N, from + per);
-  for (int i = from + threadIdx.x; i < to; i += 256) {
-    const uint32_t k = ids ? token_key(ids, bits, i, V) : keys[i];
-    atomicAdd(&cnt[(k >> shift) & (BINS - 1)], 1u);
+  for (int i0 = from + threadIdx.x; i0 < to; i0 += BATCH) {
+    uint32_t k[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = min(i0 + 256 * x, to - 1);
+      k[x] = ids ? token_key(ids, bits, i, V) : keys[i];
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (i0 + 256 * x < to) atomicAdd(&cnt[(k[x] >> shift) & (BINS - 1)], 1u);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < BINS; d += 256) hist[blockIdx.x * BINS + d] = cnt[d];
@@ -111,80 +257,69 @@ __global__ __launch_bounds__(256) void sort_hist_kernel(const uint32_t* __restri
 
 // One stable pass: entry i of digit d goes behind all entries of smaller
 // digits, those of d in earlier blocks, and those of d before it in its block.
-// Each wave takes a contiguous quarter of the block, 64 entries a step; equal
-// digits within a step are ranked by ballots.
+// Each wave takes a contiguous quarter of the block, 64 entries a step.
 __global__ __launch_bounds__(256) void sort_scatter_kernel(
     const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
-    const void* __restrict__ ids, int bits, int64_t V, int N, int per, int shift,
+    const void* __restrict__ ids, int bits, int64_t V, int N, int per, int nb, int shift,
     const uint32_t* __restrict__ hist, uint32_t* __restrict__ keys_out,
-    uint32_t* __restrict__ pos_out) {
-  __shared__ uint32_t base[BINS], cnt[4][BINS], sums[256];
+    uint32_t* __restrict__ pos_out, Zeros z) {
+  if ((int)blockIdx.x >= nb) {
+    write_zeros(z, blockIdx.x - nb, gridDim.x - nb, 256);
+    return;
+  }
+  __shared__ uint32_t cnt[4][BINS], sums[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int nb = gridDim.x, b = blockIdx.x;
+  const int b = blockIdx.x;
+  const int quarter = per / 4, from = b * per + wave * quarter, to = min(N, from + quarter);
+  auto batch = [&](int i0, uint32_t(&k)[4], uint32_t(&p)[4]) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = min(i0 + 64 * x + lane, to - 1);
+      k[x] = ids ? token_key(ids, bits, i, V) : keys[i];
+      p[x] = ids ? (uint32_t)i : pos[i];
+    }
+  };
+  // the waves' own counts
+  for (int w = 0; w < 4; ++w) cnt[w][2 * tid] = 0, cnt[w][2 * tid + 1] = 0;
+  uint32_t k[4], p[4];
+  if (from < to) batch(from, k, p);
+  __syncthreads();
+  for (int i0 = from; i0 < to; i0 += 256) {
+    if (i0 > from) batch(i0, k, p);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (i0 + 64 * x + lane < to) atomicAdd(&cnt[wave][(k[x] >> shift) & (BINS - 1)], 1u);
+  }
   // digits 2 tid and 2 tid + 1: entries of earlier blocks, and of all
   uint32_t before[2] = {0, 0}, all[2] = {0, 0};
 #pragma unroll 8
   for (int i = 0; i < nb; ++i) {
     const uint2 h = reinterpret_cast<const uint2*>(hist + i * BINS)[tid];
     all[0] += h.x, all[1] += h.y;
-    if (i < b) before[0] += h.x, before[1] += h.y;
+    before[0] += i < b ? h.x : 0u, before[1] += i < b ? h.y : 0u;
   }
-  sums[tid] = all[0] + all[1];
-  for (int w = 0; w < 4; ++w) cnt[w][2 * tid] = 0, cnt[w][2 * tid + 1] = 0;
+  uint32_t of_wave;
+  uint32_t first = wave_before(all[0] + all[1], lane, of_wave);
+  if (lane == 0) sums[wave] = of_wave;
   __syncthreads();
-  for (int d = 1; d < 256; d <<= 1) {
-    const uint32_t o = tid >= d ? sums[tid - d] : 0;
-    __syncthreads();
-    sums[tid] += o;
-    __syncthreads();
-  }
-  const uint32_t first = sums[tid] - all[0] - all[1];
-  base[2 * tid] = first + before[0];
-  base[2 * tid + 1] = first + all[0] + before[1];
-  // the waves' own counts
-  const int quarter = per / 4, from = b * per + wave * quarter,
-            to = min(N, from + quarter);
-  for (int i = from + lane; i < to; i += 64) {
-    const uint32_t k = ids ? token_key(ids, bits, i, V) : keys[i];
-    atomicAdd(&cnt[wave][(k >> shift) & (BINS - 1)], 1u);
-  }
-  __syncthreads();
-  for (int d = tid; d < BINS; d += 256) {
-    uint32_t at = base[d];
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t c = cnt[w][d];
-      cnt[w][d] = at;
-      at += c;
-    }
-  }
-  __syncthreads();
-  for (int i0 = from; i0 < to; i0 += 64) {
-    const int i = i0 + lane;
-    const bool in = i < to;
-    uint32_t k = 0, p = 0;
-    if (in) {
-      k = ids ? token_key(ids, bits, i, V) : keys[i];
-      p = ids ? (uint32_t)i : pos[i];
-    }
-    const uint32_t d = (k >> shift) & (BINS - 1);
-    uint64_t same = __ballot(in);
+  for (int w = 0; w < wave; ++w) first += sums[w];
+  uint32_t at[2] = {first + before[0], first + all[0] + before[1]};
 #pragma unroll
-    for (int bit = 0; bit < DIGIT; ++bit) {
-      const uint64_t m = __ballot((d >> bit) & 1);
-      same &= (d >> bit) & 1 ? m : ~m;
+  for (int w = 0; w < 4; ++w)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint32_t c = cnt[w][2 * tid + x];
+      cnt[w][2 * tid + x] = at[x];
+      at[x] += c;
     }
-    const uint32_t rank = __popcll(same & ((1ull << lane) - 1));
-    uint32_t at = 0;
-    if (in) at = cnt[wave][d] + rank;
-    // (the reads above come before the first lane's write, the next step's after)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (in && rank == 0) cnt[wave][d] += (uint32_t)__popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (in) {
-      keys_out[at] = k;
-      pos_out[at] = p;
+  __syncthreads();
+  for (int i0 = from; i0 < to; i0 += 256) {
+    if (quarter > 256) batch(i0, k, p);  // (a single batch is still in registers)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const bool in = i0 + 64 * x + lane < to;
+      const uint32_t o = place(cnt[wave], (k[x] >> shift) & (BINS - 1), in, lane);
+      if (in) keys_out[o] = k[x], pos_out[o] = p[x];
     }
   }
 }
@@ -193,17 +328,17 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(
 // the sums
 
 // VEC elements from p as fp32 (VEC 8: 16-byte loads; 4: one load).
-template <int GT, int VEC>
+template <int GT, int VEC, bool NT = false>
 __device__ __forceinline__ void loadv(const uint8_t* p, float (&v)[VEC]) {
   if constexpr (VEC == 8) {
-    load8<GT, true>(p, 0, 8, v);
+    load8<GT, true, NT>(p, 0, 8, v);
   } else if constexpr (VEC == 4) {
     if constexpr (GT == F32) {
-      const ti_u32x4 a = *reinterpret_cast<const ti_u32x4*>(p);
+      const ti_u32x4 a = vload<NT>(reinterpret_cast<const ti_u32x4*>(p));
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = u2f(a[i]);
     } else {
-      const ti_u32x2 a = *reinterpret_cast<const ti_u32x2*>(p);
+      const ti_u32x2 a = vload<NT>(reinterpret_cast<const ti_u32x2*>(p));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint32_t w = a[i];
@@ -267,7 +402,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(
   for (int i = 0; i < CHUNK; ++i) {
     const int e = e0 + min(i, n - 1);
     k[i] = keys[e];
-    loadv<GT, VEC>(grad + ((int64_t)pos[e] * D + c) * GB, v[i]);
+    loadv<GT, VEC, true>(grad + ((int64_t)pos[e] * D + c) * GB, v[i]);
   }
   const bool from_before = chunk > 0 && keys[e0 - 1] == k[0];
   const bool goes_on = e0 + n < N && keys[e0 + n] == k[n - 1];
@@ -347,13 +482,6 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(
   put_row<OT, VEC>(out + ((int64_t)k * D + c) * OB, sum, factor, accumulate);
 }
 
-__global__ __launch_bounds__(256) void embedding_zero_kernel(ti_u32x4* __restrict__ p, int64_t n16,
-                                                             uint16_t* __restrict__ rest, int nr) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256)
-    p[i] = ti_u32x4{0u, 0u, 0u, 0u};
-  if (blockIdx.x == 0 && (int)threadIdx.x < nr) rest[threadIdx.x] = 0;
-}
-
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct EmbedPlan {
@@ -367,8 +495,8 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D) {
   int bits = 1;
   while (bits < 33 && ((int64_t)1 << bits) <= V) ++bits;  // keys 0 .. V
   p.passes = (bits + DIGIT - 1) / DIGIT;
-  // 2048 entries a block, more when that makes over 128 blocks; 256 divide it
-  p.per = (int)std::max<int64_t>(2048, ((N + BLOCKS - 1) / BLOCKS + 255) / 256 * 256);
+  // whole batches a block, at most 128 blocks
+  p.per = (int)(((N + BLOCKS - 1) / BLOCKS + BATCH - 1) / BATCH * BATCH);
   p.blocks = (int)((N + p.per - 1) / p.per);
   p.chunks = (N + CHUNK - 1) / CHUNK;
   size_t at = 0;
@@ -437,32 +565,55 @@ int embedding_backward_launch(const void* grad, int g_dtype, const void* ids, in
                               int64_t V, int64_t D, float factor, int accumulate, void* out,
                               int o_dtype, void* workspace, hipStream_t st) {
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (!accumulate) {
-    const int64_t bytes = V * D * (o_dtype == F32 ? 4 : 2), n16 = bytes / 16;
-    const unsigned blocks = (unsigned)std::min<int64_t>(std::max<int64_t>((n16 + 255) / 256, 1), 8192);
-    hipLaunchKernelGGL(embedding_zero_kernel, dim3(blocks), dim3(256), 0, st,
-                       static_cast<ti_u32x4*>(out), n16,
-                       reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(out) + n16 * 16),
-                       (int)(bytes % 16 / 2));
-    const int rc = check_launch();
-    if (rc != NOVAQ_OK) return rc;
+  const int64_t bytes = accumulate ? 0 : V * D * (o_dtype == F32 ? 4 : 2);
+  uint8_t* table = static_cast<uint8_t*>(out);
+  // workgroups of `threads` that write n bytes of zeros: 16 vectors a lane, 4096 waves
+  auto zero_blocks = [](int64_t n, int threads) {
+    return (unsigned)std::min<int64_t>((n + threads * 256 - 1) / (threads * 256),
+                                       262144 / threads);
+  };
+  if (N == 0) {
+    if (bytes == 0) return NOVAQ_OK;
+    hipLaunchKernelGGL(embedding_zero_kernel, dim3(zero_blocks(bytes, 256)), dim3(256), 0, st,
+                       Zeros{table, 0, bytes});
+    return check_launch();
   }
-  if (N == 0) return NOVAQ_OK;
   const EmbedPlan p = embed_plan(N, V, D);
   uint32_t* hist = reinterpret_cast<uint32_t*>(ws + p.hist);
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws + p.keys[0]),
                        reinterpret_cast<uint32_t*>(ws + p.keys[1])};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + p.pos[0]),
                       reinterpret_cast<uint32_t*>(ws + p.pos[1])};
-  for (int i = 0; i < p.passes; ++i) {
+  if (N <= SMALL) {
+    hipLaunchKernelGGL(sort_small_kernel, dim3(1 + zero_blocks(bytes, 512)), dim3(512), 0, st, ids,
+                       bits, V, (int)N, p.passes, keys[p.passes & 1], pos[p.passes & 1],
+                       Zeros{table, 0, bytes});
+    const int rc = check_launch();
+    if (rc != NOVAQ_OK) return rc;
+  }
+  // the zeros' share of a launch: one part beside the counts, three beside the
+  // scatter, which takes about three times as long
+  int64_t zero_at = 0;
+  int parts = 0;
+  auto share = [&](int more) {
+    parts += more;
+    const int64_t from = zero_at;
+    zero_at = parts == 4 * p.passes ? bytes : bytes / (4 * p.passes) * parts / 16 * 16;
+    return Zeros{table, from, zero_at};
+  };
+  for (int i = 0; i < p.passes && N > SMALL; ++i) {
     const void* raw = i == 0 ? ids : nullptr;
     const int in = i & 1, to = in ^ 1;
-    hipLaunchKernelGGL(sort_hist_kernel, dim3(p.blocks), dim3(256), 0, st, keys[in], raw, bits, V,
-                       (int)N, p.per, i * DIGIT, hist);
+    Zeros z = share(1);
+    hipLaunchKernelGGL(sort_hist_kernel, dim3(p.blocks + zero_blocks(z.to - z.from, 256)),
+                       dim3(256), 0, st, keys[in], raw, bits, V, (int)N, p.per, p.blocks,
+                       i * DIGIT, hist, z);
     int rc = check_launch();
     if (rc != NOVAQ_OK) return rc;
-    hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.blocks), dim3(256), 0, st, keys[in], pos[in],
-                       raw, bits, V, (int)N, p.per, i * DIGIT, hist, keys[to], pos[to]);
+    z = share(3);
+    hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.blocks + zero_blocks(z.to - z.from, 256)),
+                       dim3(256), 0, st, keys[in], pos[in], raw, bits, V, (int)N, p.per, p.blocks,
+                       i * DIGIT, hist, keys[to], pos[to], z);
     rc = check_launch();
     if (rc != NOVAQ_OK) return rc;
   }
