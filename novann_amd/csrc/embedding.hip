@@ -464,11 +464,17 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(
   for (int x = 0; x < VEC; ++x) sum[x] = 0.0f;
   if (c < D) {
     if (wave == 0) loadv<F32, VEC>((const uint8_t*)(tail + (int64_t)chunk * D + c), sum);
-    for (int h = chunk + 1 + wave; h < end; h += 8) {
-      float v[VEC];
-      loadv<F32, VEC>((const uint8_t*)(head + (int64_t)h * D + c), v);
+    for (int h = chunk + 1 + wave; h < end; h += 32) {
+      float v[4][VEC];  // (all four loaded before the first is added)
 #pragma unroll
-      for (int x = 0; x < VEC; ++x) sum[x] += v[x];
+      for (int y = 0; y < 4; ++y)
+        loadv<F32, VEC>((const uint8_t*)(head + (int64_t)min(h + 8 * y, end - 1) * D + c), v[y]);
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (h + 8 * y < end) {
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) sum[x] += v[y][x];
+        }
     }
   }
 #pragma unroll

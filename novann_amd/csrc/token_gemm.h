@@ -64,15 +64,22 @@ __device__ __forceinline__ uint32_t tg_pack2(float lo, float hi) {
 // compiler otherwise waits for every copy in flight before each transposing LDS
 // read (grad_W's product of 4096 x 4096 x 16384: 546 us so, 447 with this).  A copy
 // has no vector output; m0 (its LDS address) is put back; what reads LDS waits for it by vmcnt and a barrier.
+// NT: past the caches, for what is read once.
+template <bool NT = false>
 __device__ __forceinline__ void tg_copy16(const tg_u32x4& rs, uint32_t voff, uint8_t* lds) {
   const uint32_t at = (uint32_t)(uintptr_t)(tg_lds_void*)lds;
   uint32_t kept;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
-      "buffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-      : "=&s"(kept)
-      : "s"(at), "v"(voff), "s"(rs)
-      : "memory");
+#define NOVAQ_COPY16(MORE)                                    \
+  asm volatile(                                               \
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"   \
+      "buffer_load_dwordx4 %2, %3, 0 offen" MORE              \
+      " lds\n\ts_mov_b32 m0, %0"                              \
+      : "=&s"(kept)                                           \
+      : "s"(at), "v"(voff), "s"(rs)                           \
+      : "memory")
+  if constexpr (NT) NOVAQ_COPY16(" nt");
+  else NOVAQ_COPY16("");
+#undef NOVAQ_COPY16
 }
 
 // One operand of a product: rows (M or N) of K elements.

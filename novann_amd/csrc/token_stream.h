@@ -4,7 +4,7 @@
 // A workgroup takes 128 table rows (32 a wave) and all tokens.  Stages of 128
 // bytes a row go straight into LDS (whole lines, 16-byte chunks swizzled as in
 // TokenTile) beside the tokens' matching K in the order of the MFMA fragments,
-// which a small kernel has laid out before: 1 KB a fragment, one coalesced copy.
+// which the call's first kernel lays out: 1 KB a fragment, one coalesced copy.
 // A 16-byte chunk of a row holds E codes (8, 16 or 32) and feeds E / 8 MFMAs of
 // 16 K: lane half h of chunk pair c takes chunk 2 c + h, and MFMA u its codes 8 u
 // .. + 7, so the K of fragment (c, u) are E (2 c + h) + 8 u .. + 7 in both
@@ -110,7 +110,7 @@ struct TokenStream {
       const uint32_t c = (uint32_t)(s * 128 + chunk * 16);
       const uint32_t base = c < rb && s < stages ? (uint32_t)(tid >> 3) * rb + c : 0x80000000u;
 #pragma unroll
-      for (int i = 0; i < WL; ++i) tg_copy16(wr, base + i * 32 * rb, at + i * 4096);
+      for (int i = 0; i < WL; ++i) tg_copy16<true>(wr, base + i * 32 * rb, at + i * 4096);
       const uint32_t xb = s < stages ? (uint32_t)(s * x_bytes + tid * 16) : 0x80000000u;
 #pragma unroll
       for (int i = 0; i < XL; ++i) tg_copy16(xr, xb + i * 4096, at + w_bytes + i * 4096);
@@ -148,36 +148,6 @@ struct TokenStream {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
 };
-
-// The tokens' fragments: 16 bytes a thread, fragment ((stage 4 + c) U + u) NT + j
-// of 64 lanes; x (N x D) as ST, zeros past N and D.
-template <int CT, int ST>
-__global__ __launch_bounds__(256) void loss_fragments_kernel(const uint8_t* __restrict__ x,
-                                                             int64_t N, int64_t D, int E, int nt,
-                                                             int64_t total,
-                                                             uint16_t* __restrict__ out) {
-  const int U = E / 8;
-  const int64_t rb = row_bytes(ST, D);
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
-       q += (int64_t)gridDim.x * 256) {
-    const int lane = (int)(q & 63);
-    const int64_t fr = q >> 6;
-    const int j = (int)(fr % nt);
-    const int64_t step = fr / nt;
-    const int u = (int)(step % U);
-    const int64_t pair = step / U;  // of chunks
-    const int64_t n = j * 32 + (lane & 31), k = E * (2 * pair + (lane >> 5)) + 8 * u;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (n < N && k < D) {
-      if (D % 8 == 0) load8<ST, true>(x + n * rb, k, D, v);
-      else load8<ST, false>(x + n * rb, k, D, v);
-    }
-    tg_u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<tg_u32x4*>(out + q * 8) = o;
-  }
-}
 
 }  // namespace
 }  // namespace novaq

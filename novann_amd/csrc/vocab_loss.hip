@@ -53,113 +53,207 @@ constexpr int64_t row_pitch(int64_t width) { return width + 128; }
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// dst (rows x dp, 16 bits, dp % 64 == 0) = src (rows x D, ST) as CT, zeros past
-// D; rows whose target is T_NONE become zeros (targets may be null).
-template <int ST, int CT, bool VEC>
-__global__ __launch_bounds__(256) void loss_copy_kernel(const uint8_t* __restrict__ src,
-                                                        int64_t rows, int64_t D, int64_t dp,
-                                                        int64_t pitch,
-                                                        const int* __restrict__ targets,
-                                                        uint16_t* __restrict__ dst) {
-  const int64_t per = dp / 8, total = rows * per, rb = row_bytes(ST, D);
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
-       q += (int64_t)gridDim.x * 256) {
-    const int64_t row = q / per, c = (q - row * per) * 8;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (c < D && !(targets && targets[row] == T_NONE))
-      load8<ST, VEC>(src + row * rb, c, D, v);
-    ti_u32x4 o;
+// A 16-bit copy: dst (rows x dp, pitch elements apart, dp % 64 == 0) = src (rows x
+// D, stored as st) in the products' type, zeros past D and in the rows whose id is
+// `ignore` (ids may be null).
+struct CopyJob {
+  const uint8_t* src;
+  uint16_t* dst;
+  int64_t rows, D, dp, pitch;
+  int st;
+  const void* ids;
+  int bits;
+  int64_t ignore;
+  FastDiv by_per;  // of dp / 8
+};
+
+template <int CT, int ST, bool VEC>
+__device__ __forceinline__ void copy_rows(const CopyJob& j, int64_t first, int64_t step) {
+  constexpr int A = 4;  // units of 8 elements loaded before the first is stored
+  const uint32_t per = (uint32_t)(j.dp / 8);
+  const int64_t total = j.rows * per, rb = row_bytes(ST, j.D);
+  for (int64_t q0 = first; q0 < total; q0 += A * step) {
+    float v[A][8];
+    uint16_t* to[A];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<ti_u32x4*>(dst + row * pitch + c) = o;
+    for (int x = 0; x < A; ++x) {
+      const int64_t q = min(q0 + x * step, total - 1);
+      const int64_t row = total < ((int64_t)1 << 31) ? (int64_t)fdiv((uint32_t)q, j.by_per)
+                                                     : q / per;
+      const int64_t c = (q - row * per) * 8;
+      to[x] = j.dst + row * j.pitch + c;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[x][i] = 0.0f;
+      if (c < j.D && !(j.ids && token_at(j.ids, j.bits, row) == j.ignore))
+        load8<ST, VEC, true>(j.src + row * rb, c, j.D, v[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < A; ++x) {
+      if (q0 + x * step >= total) break;
+      ti_u32x4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[x][2 * i], v[x][2 * i + 1]);
+      *reinterpret_cast<ti_u32x4*>(to[x]) = o;
+    }
   }
 }
 
 template <int CT>
-int copy_launch(const void* src, int st, int64_t rows, int64_t D, int64_t dp, int64_t pitch,
-                const int* targets, uint16_t* dst, hipStream_t stream) {
-  if (rows == 0) return NOVAQ_OK;
-  const int64_t units = rows * (dp / 8);
-  const dim3 grid((unsigned)std::min<int64_t>((units + 255) / 256, 16384));
-  const uint8_t* s = static_cast<const uint8_t*>(src);
-#define NOVAQ_COPY(ST)                                                                        \
-  case ST:                                                                                    \
-    if (D % 8 == 0)                                                                           \
-      hipLaunchKernelGGL((loss_copy_kernel<ST, CT, true>), grid, dim3(256), 0, stream, s,     \
-                         rows, D, dp, pitch, targets, dst);                                        \
-    else                                                                                      \
-      hipLaunchKernelGGL((loss_copy_kernel<ST, CT, false>), grid, dim3(256), 0, stream, s,    \
-                         rows, D, dp, pitch, targets, dst);                                        \
+__device__ __forceinline__ void copy_job(const CopyJob& j, int64_t first, int64_t step) {
+  const bool vec = j.D % 8 == 0;
+  switch (j.st) {
+#define NOVAQ_COPY(ST)                                     \
+  case ST:                                                 \
+    if (vec) copy_rows<CT, ST, true>(j, first, step);      \
+    else copy_rows<CT, ST, false>(j, first, step);         \
     break;
-  switch (st) {
     NOVAQ_COPY(F32)
     NOVAQ_COPY(F16)
     NOVAQ_COPY(BF16)
     NOVAQ_COPY(E4M3)
     NOVAQ_COPY(E5M2)
     NOVAQ_COPY(E2M1)
-    default: return NOVAQ_EDTYPE;
-  }
 #undef NOVAQ_COPY
-  return check_launch();
+  }
 }
 
-// Per-row state, by one workgroup: targets as int32 (T_NONE, T_BAD), the row
-// factors f (NaN for T_BAD, so its gradients show) and scal[0] = g, scal[1] =
-// the number of rows with a loss.  grad: one value, or one a row
-// (per_row), or null (1).
-__global__ __launch_bounds__(1024) void loss_rows_kernel(const void* __restrict__ ids, int bits,
-                                                         int64_t ignore, int64_t N, int64_t V,
-                                                         const float* __restrict__ grad,
-                                                         int per_row, int mean,
-                                                         int* __restrict__ targets,
-                                                         float* __restrict__ f,
-                                                         float* __restrict__ scal) {
-  __shared__ int cnt[16];
-  __shared__ float top[16];
+// The tokens' fragments of the kernel for few rows (token_stream.h): 16 bytes a
+// thread, fragment ((stage 4 + c) U + u) nt + j of 64 lanes; x (N x D) as st,
+// zeros past N and D.
+struct FragmentJob {
+  const uint8_t* x;
+  uint16_t* dst;
+  int64_t N, D, total;
+  int st, E, nt;
+};
+
+template <int CT, int ST, bool VEC>
+__device__ __forceinline__ void fragments(const FragmentJob& f, int64_t first, int64_t step) {
+  const int U = f.E / 8;
+  const int64_t rb = row_bytes(ST, f.D);
+  for (int64_t q = first; q < f.total; q += step) {
+    const int lane = (int)(q & 63);
+    const int64_t fr = q >> 6;
+    const int j = (int)(fr % f.nt);
+    const int64_t at = fr / f.nt, pair = at / U;  // of chunks
+    const int u = (int)(at % U);
+    const int64_t n = j * 32 + (lane & 31), k = f.E * (2 * pair + (lane >> 5)) + 8 * u;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (n < f.N && k < f.D) load8<ST, VEC>(f.x + n * rb, k, f.D, v);
+    ti_u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<ti_u32x4*>(f.dst + q * 8) = o;
+  }
+}
+
+// Per-row state: targets as int32 (T_NONE, T_BAD), the row factors f (NaN for
+// T_BAD, so its gradients show; may be null), scal[0] = g, scal[1] = the number
+// of rows with a loss.
+// grad: one value, or one a row (per_row), or null (1).
+struct RowsJob {
+  const void* ids;
+  int bits;
+  int64_t ignore, N, V;
+  const float* grad;
+  int per_row, mean;
+  int* targets;
+  float* f;
+  float* scal;
+};
+
+__device__ __forceinline__ float nan_max(float a, float b) {
+  return a != a || b != b ? u2f(0x7FC00000u) : fmaxf(a, b);
+}
+
+__device__ __forceinline__ void rows_job(const RowsJob& r, int* cnt, float* top) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int c = 0;
   float m = 0.0f;
-  bool nan = false;
-  for (int64_t n = tid; n < N; n += 1024) {
-    const int64_t t = token_at(ids, bits, n);
-    const int k = t == ignore ? T_NONE : t < 0 || t >= V ? T_BAD : (int)t;
-    targets[n] = k;
-    c += k != T_NONE;
-    if (per_row && k != T_NONE) {
-      const float a = fabsf(grad[n]);
-      nan |= a != a;
-      m = fmaxf(m, a);
+  for (int64_t n0 = tid; n0 < r.N; n0 += 2048) {
+    int64_t t[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) t[x] = token_at(r.ids, r.bits, min(n0 + 256 * x, r.N - 1));
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int64_t n = n0 + 256 * x;
+      if (n >= r.N) continue;
+      const int k = t[x] == r.ignore ? T_NONE : t[x] < 0 || t[x] >= r.V ? T_BAD : (int)t[x];
+      r.targets[n] = k;
+      c += k != T_NONE;
+      if (r.per_row && k != T_NONE) m = nan_max(m, fabsf(r.grad[n]));
+      if (r.f && !r.per_row) r.f[n] = k == T_NONE ? 0.0f : k == T_BAD ? u2f(0x7FC00000u) : 1.0f;
     }
   }
-  if (nan) m = u2f(0x7FC00000u);
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     c += __shfl_xor(c, d);
-    const float o = __shfl_xor(m, d);
-    m = m != m || o != o ? u2f(0x7FC00000u) : fmaxf(m, o);
+    m = nan_max(m, __shfl_xor(m, d));
   }
   if (lane == 0) cnt[wave] = c, top[wave] = m;
   __syncthreads();
   c = 0, m = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    c += cnt[w];
-    m = m != m || top[w] != top[w] ? u2f(0x7FC00000u) : fmaxf(m, top[w]);
+  for (int w = 0; w < 4; ++w) c += cnt[w], m = nan_max(m, top[w]);
+  if (tid == 0) {
+    float g = r.per_row ? m : r.grad ? *r.grad : 1.0f;
+    if (r.mean) g = c > 0 ? g / (float)c : 0.0f;
+    r.scal[0] = g;
+    r.scal[1] = (float)c;
   }
-  if (tid == 0 && scal) {
-    float g = per_row ? m : grad ? *grad : 1.0f;
-    if (mean) g = c > 0 ? g / (float)c : 0.0f;
-    scal[0] = g;
-    scal[1] = (float)c;
-  }
-  if (f)
-    for (int64_t n = tid; n < N; n += 1024) {
-      const int k = targets[n];
-      float v = k == T_NONE ? 0.0f : 1.0f;
-      if (per_row && k != T_NONE) v = m > 0.0f ? grad[n] / m : m;  // (all zero: 0; NaN: NaN)
-      f[n] = k == T_BAD ? u2f(0x7FC00000u) : v;
+  if (r.f && r.per_row)
+    for (int64_t n = tid; n < r.N; n += 256) {
+      const int k = r.targets[n];
+      // (all zero: 0; NaN: NaN)
+      r.f[n] = k == T_NONE ? 0.0f : k == T_BAD ? u2f(0x7FC00000u) : m > 0.0f ? r.grad[n] / m : m;
     }
+}
+
+// What a call needs before its products, in one launch: workgroup 0 the rows, the
+// next ones x's copy (or fragments), the rest the table's first piece; and for the
+// later pieces their copies alone (rows.N, x.rows and frag.total 0).
+template <int CT>
+__global__ __launch_bounds__(256) void loss_prep_kernel(RowsJob rows, CopyJob x, FragmentJob frag,
+                                                         CopyJob w, int xblocks) {
+  __shared__ int cnt[4];
+  __shared__ float top[4];
+  int b = blockIdx.x;
+  if (rows.N > 0) {
+    if (b == 0) {
+      rows_job(rows, cnt, top);
+      return;
+    }
+    --b;
+  }
+  if (b < xblocks) {
+    const int64_t first = (int64_t)b * 256 + threadIdx.x, step = (int64_t)xblocks * 256;
+    if (x.rows > 0) copy_job<CT>(x, first, step);
+    else if (frag.st == F32) {
+      if (frag.D % 8 == 0) fragments<CT, F32, true>(frag, first, step);
+      else fragments<CT, F32, false>(frag, first, step);
+    } else {  // (f16 and bf16 x are in the products' type)
+      if (frag.D % 8 == 0) fragments<CT, CT, true>(frag, first, step);
+      else fragments<CT, CT, false>(frag, first, step);
+    }
+    return;
+  }
+  b -= xblocks;
+  const int wblocks = gridDim.x - xblocks - (rows.N > 0);
+  copy_job<CT>(w, (int64_t)b * 256 + threadIdx.x, (int64_t)wblocks * 256);
+}
+
+template <int CT>
+int prep_launch(const RowsJob& rows, CopyJob x, const FragmentJob& frag, CopyJob w,
+                hipStream_t stream) {
+  auto blocks = [](int64_t units) { return (int)std::min<int64_t>((units + 1023) / 1024, 16384); };
+  if (x.rows > 0) x.by_per = fast_div((uint32_t)(x.dp / 8));
+  if (w.rows > 0) w.by_per = fast_div((uint32_t)(w.dp / 8));
+  const int xb = blocks(x.rows > 0 ? x.rows * (x.dp / 8) : frag.total);
+  const int wb = blocks(w.rows * (w.dp / 8));
+  const int all = (rows.N > 0) + xb + wb;
+  if (all == 0) return NOVAQ_OK;
+  hipLaunchKernelGGL(loss_prep_kernel<CT>, dim3(all), dim3(256), 0, stream, rows, x, frag, w, xb);
+  return check_launch();
 }
 
 // 8 workgroups in a row go to the 8 XCDs: those of one XCD take a compact
@@ -319,37 +413,12 @@ __global__ __launch_bounds__(S::NTH, 1) void loss_stream_kernel(
   }
 }
 
-// One wave a row joins the tiles' (maximum, sum) pairs: lse and the loss.
-__global__ __launch_bounds__(256) void loss_join_kernel(const float2* __restrict__ stats,
-                                                        int64_t vtiles, int64_t N,
-                                                        const int* __restrict__ targets,
-                                                        const float* __restrict__ tlogit,
-                                                        float* __restrict__ lse,
-                                                        float* __restrict__ loss) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= N) return;
-  float2 a = {-INFINITY, 0.0f};
-#pragma unroll 4
-  for (int64_t i = lane; i < vtiles; i += 64) a = join_stats(a, stats[n * vtiles + i]);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) a = join_stats(a, float2{__shfl_xor(a.x, d), __shfl_xor(a.y, d)});
-  if (lane == 0) {
-    const float l2 = a.x + log2f(a.y);
-    const int t = targets[n];
-    lse[n] = l2 * LN2;
-    // (the difference in base 2: the factor's rounding falls on the loss alone)
-    loss[n] = t == T_NONE ? 0.0f : t == T_BAD ? u2f(0x7FC00000u) : (l2 - tlogit[n]) * LN2;
-  }
-}
-
-// The rows' losses summed in fp64 in a fixed order, over the count for mean
-// (0 where no row has a loss).
-__global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict__ each, int64_t N,
-                                                        int mean, const float* __restrict__ scal,
-                                                        float* __restrict__ out) {
-  __shared__ double part[16];
+// The rows' losses summed in fp64 in a fixed order by 16 waves, over the count for
+// mean (0 where no row has a loss).
+__device__ __forceinline__ void sum_losses(const float* each, int64_t N, int mean,
+                                           const float* scal, float* out, double* part) {
   double s = 0.0;
+#pragma unroll 4
   for (int64_t n = threadIdx.x; n < N; n += 1024) s += (double)each[n];
 #pragma unroll
   for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
@@ -361,6 +430,43 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict_
     if (mean) s = scal[1] > 0.0f ? s / (double)scal[1] : 0.0;
     *out = (float)s;
   }
+}
+
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict__ each, int64_t N,
+                                                        int mean, const float* __restrict__ scal,
+                                                        float* __restrict__ out) {
+  __shared__ double part[16];
+  sum_losses(each, N, mean, scal, out, part);
+}
+
+// One wave a row joins the tiles' (maximum, sum) pairs: lse and the loss.  A
+// single workgroup (grid 1) takes all rows and sums their losses into `out`.
+__global__ __launch_bounds__(1024) void loss_join_kernel(const float2* __restrict__ stats,
+                                                         int64_t vtiles, int64_t N,
+                                                         const int* __restrict__ targets,
+                                                         const float* __restrict__ tlogit,
+                                                         float* __restrict__ lse, float* loss,
+                                                         int mean, const float* __restrict__ scal,
+                                                         float* __restrict__ out) {
+  __shared__ double part[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int64_t n = (int64_t)blockIdx.x * 16 + wave; n < N; n += (int64_t)gridDim.x * 16) {
+    float2 a = {-INFINITY, 0.0f};
+#pragma unroll 4
+    for (int64_t i = lane; i < vtiles; i += 64) a = join_stats(a, stats[n * vtiles + i]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) a = join_stats(a, float2{__shfl_xor(a.x, d), __shfl_xor(a.y, d)});
+    if (lane == 0) {
+      const float l2 = a.x + log2f(a.y);
+      const int t = targets[n];
+      lse[n] = l2 * LN2;
+      // (the difference in base 2: the factor's rounding falls on the loss alone)
+      loss[n] = t == T_NONE ? 0.0f : t == T_BAD ? u2f(0x7FC00000u) : (l2 - tlogit[n]) * LN2;
+    }
+  }
+  if (gridDim.x > 1 || !out) return;
+  __syncthreads();
+  sum_losses(loss, N, mean, scal, out, part);
 }
 
 // The backward's P of one piece: the forward's tile, then f (2^(l2 - lse2) -
@@ -434,22 +540,34 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_prob_kernel(
   }
 }
 
-// grad_x's share of one piece: P (N x K) times the piece's rows (K x D), K
+// The gradients' products of one piece.
+struct GradsJob {
+  TokenOp p, pt;        // P: N rows of K; and as K-strided rows of the vocabulary
+  TokenOp w, x;         // the piece and x, both K-strided
+  int64_t N, D, vc;     // vc: the piece's rows
+  int vblocks, nblocks; // K blocks of the two products
+  int splits, first;    // of grad_x's K; the first piece stores, the others add
+  float* sums;          // grad_x's fp32 sums, split by split, pitch dp
+  int64_t dp;
+  const float* scal;
+  float inv_pscale;
+  uint8_t* gw;
+  int xtm, xtn, wtm, wtn;  // tiles; wtm 0: no grad_W
+};
+
+// grad_x's share of one piece: P (N x vc) times the piece's rows (vc x D), K
 // blocks of this split, added to (or, first, stored in) the split's fp32 sums.
 template <int CT, class G>
-__global__ __launch_bounds__(G::NTH, 1) void loss_dx_kernel(TokenOp p, TokenOp w, int64_t K,
-                                                            int64_t kblocks, int splits,
-                                                            float* __restrict__ sums, int64_t N,
-                                                            int64_t dp, int64_t D, int first,
-                                                            int tm, int tn) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+__device__ __forceinline__ void dx_tile(const GradsJob& g, int b, uint8_t* lds) {
   int mi, ni;
-  const int split = blockIdx.x / (tm * tn);
-  tile_of(blockIdx.x % (tm * tn), tm, tn, mi, ni);
-  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN;
+  const int split = b / (g.xtm * g.xtn);
+  tile_of(b % (g.xtm * g.xtn), g.xtm, g.xtn, mi, ni);
+  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN, N = g.N, D = g.D, dp = g.dp;
+  float* sums = g.sums;
+  const int first = g.first;
   typename G::Acc acc;
-  G::run(acc, p, w, m0, n0, K, (int)(kblocks * split / splits),
-         (int)(kblocks * (split + 1) / splits), lds);
+  G::run(acc, g.p, g.w, m0, n0, g.vc, (int)((int64_t)g.vblocks * split / g.splits),
+         (int)((int64_t)g.vblocks * (split + 1) / g.splits), lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   // what lies past N or D is left out by the descriptor (offsets past it)
@@ -480,54 +598,16 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_dx_kernel(TokenOp p, TokenOp w
   }
 }
 
-// grad_x = the splits' sums, in order, times g s / pscale, as OT.
-template <int OT>
-__global__ __launch_bounds__(256) void loss_dx_store_kernel(const float* __restrict__ sums,
-                                                            int splits, int64_t N, int64_t dp,
-                                                            int64_t D,
-                                                            const float* __restrict__ scal,
-                                                            const float* __restrict__ w_scale,
-                                                            float inv_pscale,
-                                                            const int* __restrict__ targets,
-                                                            void* __restrict__ out) {
-  const float a = scal[0] * (w_scale ? *w_scale : 1.0f) * inv_pscale;
-  const int64_t per = dp / 8, total = N * per;
-  const bool vec = D % 8 == 0;
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
-       q += (int64_t)gridDim.x * 256) {
-    const int64_t n = q / per, c = (q - n * per) * 8;
-    if (c >= D) continue;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int s = 0; s < splits; ++s) {
-      const float4* p = reinterpret_cast<const float4*>(sums + ((int64_t)s * N + n) * dp + c);
-      const float4 lo = p[0], hi = p[1];
-      v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-      v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
-    }
-    const bool none = targets[n] == T_NONE;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = none ? 0.0f : v[i] * a;
-    if (vec) store8<OT, true>(out, n * D + c, 8, v);
-    else store8<OT, false>(out, n * D + c, D - c, v);
-  }
-}
-
 // grad_W's rows of one piece: P^T (vc x N) times x (N x D), times g / pscale.
 template <int CT, int OT, class G>
-__global__ __launch_bounds__(G::NTH, 1) void loss_dw_kernel(TokenOp p, TokenOp x, int64_t N,
-                                                            int64_t kblocks, int64_t vc,
-                                                            int64_t D,
-                                                            const float* __restrict__ scal,
-                                                            float inv_pscale,
-                                                            uint8_t* __restrict__ out, int tm,
-                                                            int tn) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+__device__ __forceinline__ void dw_tile(const GradsJob& g, int b, uint8_t* lds) {
   int mi, ni;
-  tile_of(blockIdx.x, tm, tn, mi, ni);
-  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN;
+  tile_of(b, g.wtm, g.wtn, mi, ni);
+  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN, D = g.D, vc = g.vc;
   typename G::Acc acc;
-  G::run(acc, p, x, m0, n0, N, 0, (int)kblocks, lds);
-  const float a = scal[0] * inv_pscale;
+  G::run(acc, g.pt, g.x, m0, n0, g.N, 0, g.nblocks, lds);
+  const float a = g.scal[0] * g.inv_pscale;
+  uint8_t* out = g.gw;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   constexpr int OB = OT == F32 ? 4 : 2;
@@ -554,6 +634,62 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_dw_kernel(TokenOp p, TokenOp x
   }
 }
 
+// Both gradients' tiles in one launch, grad_x's first: each product alone leaves
+// CUs idle in its last round (8192 x 1024 x 8192: 128 tiles of 256 x 256 each).
+template <int CT, int OT, class GX, class GW>
+__global__ __launch_bounds__(GX::NTH, 1) void loss_grads_kernel(GradsJob g) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int nx = g.xtm * g.xtn * g.splits;
+  if ((int)blockIdx.x < nx) dx_tile<CT, GX>(g, blockIdx.x, lds);
+  else dw_tile<CT, OT, GW>(g, blockIdx.x - nx, lds);
+}
+
+// grad_x = the splits' sums, in order, times g s / pscale, as OT: four columns a
+// thread.
+template <int OT>
+__global__ __launch_bounds__(256) void loss_dx_store_kernel(const float* __restrict__ sums,
+                                                            int splits, int64_t N, int64_t dp,
+                                                            int64_t D,
+                                                            const float* __restrict__ scal,
+                                                            const float* __restrict__ w_scale,
+                                                            float inv_pscale,
+                                                            const int* __restrict__ targets,
+                                                            void* __restrict__ out) {
+  const float a = scal[0] * (w_scale ? *w_scale : 1.0f) * inv_pscale;
+  const int64_t per = dp / 4, total = N * per;
+  const bool vec = D % 4 == 0;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
+       q += (int64_t)gridDim.x * 256) {
+    const int64_t n = q / per, c = (q - n * per) * 4;
+    if (c >= D) continue;
+    float v[4] = {0, 0, 0, 0};
+    const float* p = sums + n * dp + c;
+#pragma unroll 16
+    for (int s = 0; s < splits; ++s) {
+      const float4 o = *reinterpret_cast<const float4*>(p + (int64_t)s * N * dp);
+      v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
+    }
+    const bool none = targets[n] == T_NONE;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = none ? 0.0f : v[i] * a;
+    const int64_t e = n * D + c;
+    if constexpr (OT == F32) {
+      float* o = reinterpret_cast<float*>(out) + e;
+      if (vec) *reinterpret_cast<float4*>(o) = float4{v[0], v[1], v[2], v[3]};
+      else
+        for (int i = 0; i < 4; ++i)
+          if (c + i < D) o[i] = v[i];
+    } else {
+      uint16_t* o = reinterpret_cast<uint16_t*>(out) + e;
+      const tg_u32x2 w = {tg_pack2<OT>(v[0], v[1]), tg_pack2<OT>(v[2], v[3])};
+      if (vec) *reinterpret_cast<tg_u32x2*>(o) = w;
+      else
+        for (int i = 0; i < 4; ++i)
+          if (c + i < D) o[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
 // --------------------------------------------------------------------------
 // the plan of a call: what its shapes and types make of the workspace
 
@@ -564,7 +700,7 @@ struct LossPlan {
   bool copy_x, copy_w;
   int64_t piece;     // vocabulary rows a piece (a multiple of 256)
   int64_t vtiles;    // tiles of the vocabulary
-  bool big_l, big_x, big_w;  // 256 x 256 tiles for the logits, grad_x, grad_W
+  bool big_l, big_g;  // 256 x 256 tiles for the logits, the gradients
   int splits;        // of grad_x's K
   bool stream;       // forward: the table read as stored, for few tokens
   int64_t frag_bytes;
@@ -592,6 +728,44 @@ double best_us(int64_t M, int64_t N, int64_t K) {
   return std::min(product_us(M, N, K, true), product_us(M, N, K, false));
 }
 
+// Both gradients' products in one launch: grad_x's tiles (K split) fill the
+// workgroups' slots in rounds, grad_W's go where one is free first.
+struct GradsPlan {
+  double us;
+  bool big;
+  int splits;
+};
+GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece) {
+  const int64_t cus = device_cu_count();
+  GradsPlan best{0.0, false, 1};
+  const int64_t kx = (piece + 63) / 64, kw = (N + 63) / 64;
+  for (int big = 0; big < 2; ++big) {
+    const int64_t e = big ? 256 : 128, slots = big ? cus : 2 * cus, cols = (D + e - 1) / e;
+    const double block = big ? 1.67 : 0.965, tile = big ? 4.8 : 4.1;
+    const int64_t nw = ((piece + e - 1) / e) * cols;
+    for (int splits = 1; splits <= 64 && (splits == 1 || kx / splits >= 4); splits *= 2) {
+      const int64_t nx = ((N + e - 1) / e) * cols * splits;
+      const double tx = block * (double)((kx + splits - 1) / splits) + tile;
+      const double tw = block * (double)kw + tile;
+      // two groups of slots: those with one tile of grad_x more than the others
+      int64_t count[2] = {nx % slots, slots - nx % slots}, left = nw;
+      double at[2] = {(double)(nx / slots + 1) * tx, (double)(nx / slots) * tx};
+      double end = count[0] ? at[0] : at[1];
+      while (left > 0) {
+        const int g = count[0] == 0 || at[1] <= at[0] ? 1 : 0;
+        at[g] += tw;
+        end = std::max(end, at[g]);
+        left -= count[g];
+      }
+      if (!big && nx + nw <= cus) end *= 0.65;
+      // (the splits' sums: written and read once, 16 at a time)
+      const double us = end + (double)splits * ((double)N * (double)D * 8.0 / 4e6 + 0.1);
+      if (best.us == 0.0 || us < best.us) best = GradsPlan{us, big != 0, splits};
+    }
+  }
+  return best;
+}
+
 // The rows of a piece (a multiple of 256): at most 128 MiB of P (and of the
 // table's 16-bit copy), so that what one product writes the next ones find in
 // the 256 MB cache; among the sizes that divide the vocabulary into about that
@@ -606,7 +780,7 @@ int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, boo
   auto cost = [&](int64_t rows) {
     if (rows == 0) return 0.0;
     double us = best_us(rows, N, D) + 5.0;
-    if (backward) us += best_us(N, D, rows) + best_us(rows, D, N) + 10.0;
+    if (backward) us += grads_plan(N, D, rows).us + 5.0;
     return us;
   };
   int64_t best = most;
@@ -647,18 +821,12 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
     p.frag_bytes = ((D + 8 * E - 1) / (8 * E)) * 4 * (E / 8) * nt * 1024;
     p.big_l = p.copy_x = p.copy_w = false;
   }
-  p.big_w = large_tiles(p.piece, D, N);
   p.vtiles = (V + (p.big_l ? 255 : 127)) / (p.big_l ? 256 : 128);
-  // grad_x: K split where its tiles leave CUs idle, at least 4 blocks each
-  const int64_t kb = p.piece / 64;
-  double least = 0.0;
-  for (int splits = 1; splits <= 16 && (splits == 1 || kb / splits >= 4); splits *= 2)
-    for (int big = 0; big < 2; ++big) {
-      // (the splits' sums are written and added: 2 us and their bytes at 4 TB/s)
-      const double us = product_us(N * splits, D, p.piece / splits, big) +
-                        (splits - 1) * (2.0 + (double)N * (double)D * 8.0 / 4e6);
-      if (least == 0.0 || us < least) least = us, p.splits = splits, p.big_x = big;
-    }
+  if (backward) {
+    const GradsPlan g = grads_plan(N, D, p.piece);
+    p.big_g = g.big;
+    p.splits = g.splits;
+  }
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t b = at;
@@ -699,21 +867,10 @@ int raise_lds(const void* kern, DeviceFlags& raised) {
   } while (0)
 
 template <int CT>
-int stream(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
-           int w_dtype, const float* w_scale, int64_t V, const int* targets, float2* stats,
-           float* tl, uint16_t* frags, hipStream_t st) {
-  const uint8_t* xb = static_cast<const uint8_t*>(x);
-  const int64_t total = p.frag_bytes / 16;
-  const int E = 128 / dtype_bits(w_dtype), nt = stream_tiles(N);
-  const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, 4096));
-  if (x_dtype == F32)
-    hipLaunchKernelGGL((loss_fragments_kernel<CT, F32>), grid, dim3(256), 0, st, xb, N, D, E, nt,
-                       total, frags);
-  else  // (f16 and bf16 x are in the products' type)
-    hipLaunchKernelGGL((loss_fragments_kernel<CT, CT>), grid, dim3(256), 0, st, xb, N, D, E, nt,
-                       total, frags);
-  int rc = check_launch();
-  if (rc != NOVAQ_OK) return rc;
+int stream(const LossPlan& p, int64_t N, int64_t D, const void* w, int w_dtype,
+           const float* w_scale, int64_t V, const int* targets, float2* stats, float* tl,
+           const uint16_t* frags, hipStream_t st) {
+  const int nt = stream_tiles(N);
   auto go = [&](auto wt, auto tiles) -> int {
     constexpr int WT = decltype(wt)::value;
     using S = TokenStream<CT, WT, decltype(tiles)::value>;
@@ -744,34 +901,33 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
   float2* stats = reinterpret_cast<float2*>(ws + p.stats);
   float* tl = reinterpret_cast<float*>(ws + p.tlogit);
   float* each = reduction == NOVAQ_REDUCE_NONE ? loss : reinterpret_cast<float*>(ws + p.each);
-  hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, st, ids, bits, ignore, N, V,
-                     (const float*)nullptr, 0, 0, targets, (float*)nullptr, scal);
-  int rc = check_launch();
-  if (rc != NOVAQ_OK) return rc;
+  uint16_t* xw = reinterpret_cast<uint16_t*>(ws + p.xc);
+  uint16_t* ww = reinterpret_cast<uint16_t*>(ws + p.wc);
+  RowsJob rows{ids, bits, ignore, N, V, nullptr, 0, 0, targets, nullptr, scal};
+  CopyJob cx{};
+  FragmentJob fx{};
+  if (p.stream)
+    fx = FragmentJob{static_cast<const uint8_t*>(x), xw, N, D, p.frag_bytes / 16, x_dtype,
+                     128 / dtype_bits(w_dtype), stream_tiles(N)};
+  else if (p.copy_x)
+    cx = CopyJob{static_cast<const uint8_t*>(x), xw, N, D, p.dp, p.pitch, x_dtype, nullptr, 0, 0, {}};
+  int rc = NOVAQ_OK;
   if (p.stream) {
-    uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.xc);
-    rc = stream<CT>(p, x, x_dtype, N, D, w, w_dtype, w_scale, V, targets, stats, tl, d, st);
+    rc = prep_launch<CT>(rows, cx, fx, CopyJob{}, st);
+    if (rc == NOVAQ_OK) rc = stream<CT>(p, N, D, w, w_dtype, w_scale, V, targets, stats, tl, xw, st);
     if (rc != NOVAQ_OK) return rc;
   }
-  const uint16_t* xc = reinterpret_cast<const uint16_t*>(x);
-  if (p.copy_x) {
-    uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.xc);
-    rc = copy_launch<CT>(x, x_dtype, N, D, p.dp, p.pitch, nullptr, d, st);
-    if (rc != NOVAQ_OK) return rc;
-    xc = d;
-  }
-  const TokenOp ox{xc, N, p.copy_x ? p.pitch : D};
+  const TokenOp ox{p.copy_x ? xw : static_cast<const uint16_t*>(x), N, p.copy_x ? p.pitch : D};
   for (int64_t v0 = 0; v0 < V && !p.stream; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, V - v0);
-    const uint16_t* wc = reinterpret_cast<const uint16_t*>(w) + v0 * D;
-    if (p.copy_w) {
-      uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.wc);
-      rc = copy_launch<CT>(static_cast<const uint8_t*>(w) + v0 * row_bytes(w_dtype, D), w_dtype,
-                           vc, D, p.dp, p.pitch, nullptr, d, st);
-      if (rc != NOVAQ_OK) return rc;
-      wc = d;
-    }
-    const TokenOp ow{wc, vc, p.copy_w ? p.pitch : D};
+    const uint8_t* from = static_cast<const uint8_t*>(w) + v0 * row_bytes(w_dtype, D);
+    CopyJob cw{};
+    if (p.copy_w) cw = CopyJob{from, ww, vc, D, p.dp, p.pitch, w_dtype, nullptr, 0, 0, {}};
+    rc = prep_launch<CT>(rows, cx, fx, cw, st);
+    if (rc != NOVAQ_OK) return rc;
+    rows.N = cx.rows = 0;  // (done with the first piece)
+    const TokenOp ow{p.copy_w ? ww : reinterpret_cast<const uint16_t*>(from), vc,
+                     p.copy_w ? p.pitch : D};
     auto stats_of = [&](auto g) -> int {
       using G = decltype(g);
       const int tm = (int)((vc + G::BM - 1) / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
@@ -783,12 +939,16 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
                  : stats_of(TokenGemm<CT, false, false, 64, 64, 2>{});
     if (rc != NOVAQ_OK) return rc;
   }
-  hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, st, stats,
-                     p.vtiles, N, targets, tl, lse, each);
+  // (one workgroup, that sums the losses too, for up to 16 rows)
+  const bool alone = N <= 16;
+  float* out = reduction == NOVAQ_REDUCE_NONE ? nullptr : loss;
+  hipLaunchKernelGGL(loss_join_kernel, dim3(alone ? 1u : (unsigned)((N + 15) / 16)), dim3(1024), 0,
+                     st, stats, p.vtiles, N, targets, tl, lse, each,
+                     reduction == NOVAQ_REDUCE_MEAN, scal, out);
   rc = check_launch();
-  if (rc != NOVAQ_OK || reduction == NOVAQ_REDUCE_NONE) return rc;
+  if (rc != NOVAQ_OK || alone || !out) return rc;
   hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, each, N,
-                     reduction == NOVAQ_REDUCE_MEAN, scal, loss);
+                     reduction == NOVAQ_REDUCE_MEAN, scal, out);
   return check_launch();
 }
 
@@ -802,28 +962,25 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
   float* f = reinterpret_cast<float*>(ws + p.f);
   uint16_t* P = reinterpret_cast<uint16_t*>(ws + p.P);
   float* sums = reinterpret_cast<float*>(ws + p.sums);
-  uint16_t* xc = reinterpret_cast<uint16_t*>(ws + p.xc);
+  uint16_t* xw = reinterpret_cast<uint16_t*>(ws + p.xc);
+  uint16_t* ww = reinterpret_cast<uint16_t*>(ws + p.wc);
   const float pscale = CT == F16 ? 0x1p14f : 1.0f, inv = 1.0f / pscale;
-  hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, st, ids, bits, ignore, N, V, grad,
-                     reduction == NOVAQ_REDUCE_NONE && grad ? 1 : 0,
-                     reduction == NOVAQ_REDUCE_MEAN, targets, f, scal);
-  int rc = check_launch();
-  if (rc != NOVAQ_OK) return rc;
-  rc = copy_launch<CT>(x, x_dtype, N, D, p.dp, p.pitch, targets, xc, st);
-  if (rc != NOVAQ_OK) return rc;
-  const TokenOp ox{xc, N, p.copy_x ? p.pitch : D};
+  RowsJob rows{ids, bits, ignore, N, V, grad, reduction == NOVAQ_REDUCE_NONE && grad ? 1 : 0,
+               reduction == NOVAQ_REDUCE_MEAN, targets, f, scal};
+  CopyJob cx{static_cast<const uint8_t*>(x), xw, N, D, p.dp, p.pitch, x_dtype, ids, bits, ignore, {}};
+  int rc = NOVAQ_OK;
+  const TokenOp ox{xw, N, p.pitch};
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, V - v0), vp = (vc + 255) / 256 * 256;
-    const uint16_t* wc = reinterpret_cast<const uint16_t*>(w) + v0 * D;
-    if (p.copy_w) {
-      uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.wc);
-      rc = copy_launch<CT>(static_cast<const uint8_t*>(w) + v0 * row_bytes(w_dtype, D), w_dtype,
-                           vc, D, p.dp, p.pitch, nullptr, d, st);
-      if (rc != NOVAQ_OK) return rc;
-      wc = d;
-    }
+    const uint8_t* from = static_cast<const uint8_t*>(w) + v0 * row_bytes(w_dtype, D);
+    CopyJob cw{};
+    if (p.copy_w) cw = CopyJob{from, ww, vc, D, p.dp, p.pitch, w_dtype, nullptr, 0, 0, {}};
+    rc = prep_launch<CT>(rows, cx, FragmentJob{}, cw, st);
+    if (rc != NOVAQ_OK) return rc;
+    rows.N = cx.rows = 0;  // (done with the first piece)
     const int64_t pp = row_pitch(vp);
-    const TokenOp ow{wc, vc, p.copy_w ? p.pitch : D}, op{P, N, pp}, opt{P, vp, pp};
+    const TokenOp ow{p.copy_w ? ww : reinterpret_cast<const uint16_t*>(from), vc,
+                     p.copy_w ? p.pitch : D};
     auto prob = [&](auto g) -> int {
       using G = decltype(g);
       const int tm = (int)(vp / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
@@ -834,40 +991,40 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
     rc = p.big_l ? prob(TokenGemm<CT, false, false, 128, 64, 4>{})
                  : prob(TokenGemm<CT, false, false, 64, 64, 2>{});
     if (rc != NOVAQ_OK) return rc;
-    auto dx = [&](auto g) -> int {
-      using G = decltype(g);
-      const int tm = (int)((N + G::BM - 1) / G::BM), tn = (int)((D + G::BN - 1) / G::BN);
-      NOVAQ_LAUNCH((loss_dx_kernel<CT, G>), (int64_t)tm * tn * p.splits, G, st, op, ow, vc,
-                   vp / 64, p.splits, sums, N, p.dp, D, v0 == 0 ? 1 : 0, tm, tn);
-      return NOVAQ_OK;
-    };
-    if (gx) {
-      rc = p.big_x ? dx(TokenGemm<CT, false, true, 128, 64, 4>{})
-                   : dx(TokenGemm<CT, false, true, 64, 64, 2>{});
-      if (rc != NOVAQ_OK) return rc;
-    }
-    auto dw = [&](auto g, auto ot) -> int {
-      using G = decltype(g);
+    auto grads = [&](auto ot, auto gx_, auto gw_) -> int {
+      using GX = decltype(gx_);
+      using GW = decltype(gw_);
       constexpr int OT = decltype(ot)::value;
-      const int tm = (int)((vc + G::BM - 1) / G::BM), tn = (int)((D + G::BN - 1) / G::BN);
-      uint8_t* out = static_cast<uint8_t*>(gw) + v0 * D * (OT == F32 ? 4 : 2);
-      NOVAQ_LAUNCH((loss_dw_kernel<CT, OT, G>), (int64_t)tm * tn, G, st, opt, ox, N,
-                   (N + G::KB - 1) / G::KB, vc, D, scal, inv, out, tm, tn);
+      GradsJob j{TokenOp{P, N, pp}, TokenOp{P, vp, pp}, ow, ox, N, D, vc, (int)(vp / 64),
+                 (int)((N + 63) / 64), p.splits, v0 == 0 ? 1 : 0, sums, p.dp, scal, inv,
+                 static_cast<uint8_t*>(gw) + v0 * D * (OT == F32 ? 4 : 2), 0, 0, 0, 0};
+      if (gx) {
+        j.xtm = (int)((N + GX::BM - 1) / GX::BM);
+        j.xtn = (int)((D + GX::BN - 1) / GX::BN);
+      } else {
+        j.xtm = j.xtn = 0;
+      }
+      if (gw) {
+        j.wtm = (int)((vc + GW::BM - 1) / GW::BM);
+        j.wtn = (int)((D + GW::BN - 1) / GW::BN);
+      }
+      const int64_t tiles = (int64_t)j.xtm * j.xtn * j.splits + (int64_t)j.wtm * j.wtn;
+      NOVAQ_LAUNCH((loss_grads_kernel<CT, OT, GX, GW>), tiles, GX, st, j);
       return NOVAQ_OK;
     };
-    auto dw_to = [&](auto ot) -> int {
-      return p.big_w ? dw(TokenGemm<CT, true, true, 128, 64, 4>{}, ot)
-                     : dw(TokenGemm<CT, true, true, 64, 64, 2>{}, ot);
+    auto grads_to = [&](auto ot) -> int {
+      return p.big_g ? grads(ot, TokenGemm<CT, false, true, 128, 64, 4>{},
+                             TokenGemm<CT, true, true, 128, 64, 4>{})
+                     : grads(ot, TokenGemm<CT, false, true, 64, 64, 2>{},
+                             TokenGemm<CT, true, true, 64, 64, 2>{});
     };
-    if (gw) {
-      rc = gw_dtype == F32   ? dw_to(std::integral_constant<int, F32>{})
-           : gw_dtype == F16 ? dw_to(std::integral_constant<int, F16>{})
-                             : dw_to(std::integral_constant<int, BF16>{});
-      if (rc != NOVAQ_OK) return rc;
-    }
+    rc = gw_dtype == F32   ? grads_to(std::integral_constant<int, F32>{})
+         : gw_dtype == F16 ? grads_to(std::integral_constant<int, F16>{})
+                           : grads_to(std::integral_constant<int, BF16>{});
+    if (rc != NOVAQ_OK) return rc;
   }
   if (gx) {
-    const dim3 grid((unsigned)std::min<int64_t>((N * (p.dp / 8) + 255) / 256, 4096));
+    const dim3 grid((unsigned)std::min<int64_t>((N * (p.dp / 4) + 255) / 256, 8192));
     switch (x_dtype) {
       case F32:
         hipLaunchKernelGGL(loss_dx_store_kernel<F32>, grid, dim3(256), 0, st, sums, p.splits, N,
