@@ -1,7 +1,7 @@
 // The vocabulary loss's logits for few tokens (at most 128): the table's codes
 // are read once, as stored, and what bounds the kernel is that read.
 //
-// A workgroup takes 128 table rows (32 a wave) and all tokens.  Stages of 128
+// A workgroup takes 128 or 256 table rows (32 a wave) and all tokens.  Stages of 128
 // bytes a row go straight into LDS (whole lines, 16-byte chunks swizzled as in
 // TokenTile) beside the tokens' matching K in the order of the MFMA fragments,
 // which the call's first kernel lays out: 1 KB a fragment, one coalesced copy.
@@ -67,19 +67,29 @@ __device__ __forceinline__ tg_u32x4 ts_decode8(uint32_t c0, uint32_t c1) {
   return o;
 }
 
+// Table rows a workgroup, 32 a wave (E codes a chunk, nt tiles of tokens): 128, so
+// that two workgroups share a CU and one computes while the other waits (one row
+// of 4096 x 131072 E4M3: 94 us, with 256 rows 121), but 256 where the tokens'
+// fragments are larger than 128 rows' codes and more rows must share them (37
+// rows of 1024 x 50000 E2M1: 13.6 us, with 128 19.6), while two stages fit.
+constexpr int stream_rows(int E, int nt) { return E * nt > 32 && E * nt < 128 ? 256 : 128; }
+
 template <int CT, int WT, int NT_>
 struct TokenStream {
   static constexpr int NT = NT_;                    // tiles of 32 tokens
   static constexpr int E = 128 / dtype_bits(WT);    // codes a chunk
   static constexpr int U = E / 8;                   // MFMAs a chunk
   static constexpr int KS = 8 * E;                  // K a stage (128 bytes a row)
-  static constexpr int ROWS = 128, NTH = 256;
+  static constexpr int ROWS = stream_rows(E, NT), NTH = 2 * ROWS;
   static constexpr int w_bytes = ROWS * 128, x_bytes = 4 * U * NT * 1024;
-  static constexpr int stage = w_bytes + x_bytes;
-  // two workgroups a CU where three stages leave room for it
-  static constexpr int NS = 3 * stage <= 80 * 1024 ? 3 : 2;
+  static constexpr int PASS = NTH * 16;  // bytes that one copy of every lane covers
+  static constexpr int WL = w_bytes / PASS, XL = (x_bytes + PASS - 1) / PASS, L = WL + XL;
+  static constexpr int stage = w_bytes + XL * PASS;
+  // as many stages as leave room for two workgroups a CU, or for one
+  static constexpr int ROOM = (2 * stage <= 80 * 1024 ? 80 : 160) * 1024;
+  static constexpr int NS = 3 * stage <= ROOM ? 3 : 2;
   static constexpr int lds_bytes = NS * stage;
-  static constexpr int WL = 4, XL = U * NT, L = WL + XL;  // copies a lane a stage
+  static_assert(lds_bytes <= 160 * 1024, "LDS");
   static constexpr int kstages(int64_t D) { return (int)((D + KS - 1) / KS); }
 
   typedef tg_f32x16 Acc[NT];
@@ -91,8 +101,8 @@ struct TokenStream {
                                              int stages, uint8_t* lds) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int chunk = (tid & 7) ^ ((tid >> 4) & 7);  // of row tid / 8 (+ 32 i)
-    const int64_t left = min((int64_t)ROWS, rows - r0) * row_bytes;
+    const int chunk = (tid & 7) ^ ((tid >> 4) & 7);  // of row tid / 8 (+ NTH / 8 i)
+    const int64_t left = min((int64_t)ROWS, rows - r0) * row_bytes;  // (below 2^30)
     const uint64_t from = (uint64_t)(w + r0 * row_bytes);
     const uint64_t xfrom = (uint64_t)xf;
     const tg_u32x4 xr = {(uint32_t)xfrom, (uint32_t)(xfrom >> 32),
@@ -110,10 +120,14 @@ struct TokenStream {
       const uint32_t c = (uint32_t)(s * 128 + chunk * 16);
       const uint32_t base = c < rb && s < stages ? (uint32_t)(tid >> 3) * rb + c : 0x80000000u;
 #pragma unroll
-      for (int i = 0; i < WL; ++i) tg_copy16<true>(wr, base + i * 32 * rb, at + i * 4096);
-      const uint32_t xb = s < stages ? (uint32_t)(s * x_bytes + tid * 16) : 0x80000000u;
+      for (int i = 0; i < WL; ++i)
+        tg_copy16<true>(wr, base + i * (NTH / 8) * rb, at + i * PASS);
 #pragma unroll
-      for (int i = 0; i < XL; ++i) tg_copy16(xr, xb + i * 4096, at + w_bytes + i * 4096);
+      for (int i = 0; i < XL; ++i) {
+        const bool in = s < stages && (x_bytes % PASS == 0 || tid * 16 + i * PASS < x_bytes);
+        tg_copy16(xr, in ? (uint32_t)(s * x_bytes + tid * 16 + i * PASS) : 0x80000000u,
+                  at + w_bytes + i * PASS);
+      }
     };
     const int r = lane & 31, h = lane >> 5;
     const int wrow = (wave * 32 + r) * 128;

@@ -379,8 +379,7 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_stats_kernel(
   }
 }
 
-// The same for at most 128 tokens, the table read as stored: 128 rows a
-// workgroup.
+// The same for at most 128 tokens, the table read as stored.
 template <int CT, int WT, class S>
 __global__ __launch_bounds__(S::NTH, 1) void loss_stream_kernel(
     const uint8_t* __restrict__ w, int64_t V, int64_t rb, const uint8_t* __restrict__ xf,
@@ -812,6 +811,7 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   p.copy_w = w_dtype != p.ct || D % 64 != 0;
   p.piece = loss_piece(N, D, p.dp, V, p.copy_w, backward);
   p.big_l = large_tiles(p.piece, N, D);
+  p.vtiles = (V + (p.big_l ? 255 : 127)) / (p.big_l ? 256 : 128);
   // up to 128 rows of x, codes whose rows are whole 16-byte chunks, in a type that
   // the kernel decodes (16-bit ones as they are)
   p.stream = !backward && N <= 128 && row_bytes(w_dtype, D) % 16 == 0 &&
@@ -820,8 +820,8 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
     const int E = 128 / dtype_bits(w_dtype), nt = stream_tiles(N);
     p.frag_bytes = ((D + 8 * E - 1) / (8 * E)) * 4 * (E / 8) * nt * 1024;
     p.big_l = p.copy_x = p.copy_w = false;
+    p.vtiles = (V + stream_rows(E, nt) - 1) / stream_rows(E, nt);
   }
-  p.vtiles = (V + (p.big_l ? 255 : 127)) / (p.big_l ? 256 : 128);
   if (backward) {
     const GradsPlan g = grads_plan(N, D, p.piece);
     p.big_g = g.big;
