@@ -643,9 +643,10 @@ __global__ __launch_bounds__(GX::NTH, 1) void loss_grads_kernel(GradsJob g) {
   else dw_tile<CT, OT, GW>(g, blockIdx.x - nx, lds);
 }
 
-// grad_x = the splits' sums, in order, times g s / pscale, as OT: four columns a
-// thread.
-template <int OT>
+// grad_x = the splits' sums times g s / pscale, as OT: four columns a thread, or,
+// with SHARE, four threads (one in each wave) that take every fourth split each and
+// add up in their order.
+template <int OT, bool SHARE>
 __global__ __launch_bounds__(256) void loss_dx_store_kernel(const float* __restrict__ sums,
                                                             int splits, int64_t N, int64_t dp,
                                                             int64_t D,
@@ -654,20 +655,33 @@ __global__ __launch_bounds__(256) void loss_dx_store_kernel(const float* __restr
                                                             float inv_pscale,
                                                             const int* __restrict__ targets,
                                                             void* __restrict__ out) {
+  __shared__ float4 part[SHARE ? 3 * 64 : 1];
   const float a = scal[0] * (w_scale ? *w_scale : 1.0f) * inv_pscale;
   const int64_t per = dp / 4, total = N * per;
+  constexpr int STEP = SHARE ? 4 : 1, UNITS = 256 / STEP;
+  const int from = SHARE ? threadIdx.x >> 6 : 0, unit = SHARE ? threadIdx.x & 63 : threadIdx.x;
   const bool vec = D % 4 == 0;
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
-       q += (int64_t)gridDim.x * 256) {
+  for (int64_t q0 = (int64_t)blockIdx.x * UNITS; q0 < total; q0 += (int64_t)gridDim.x * UNITS) {
+    const int64_t q = min(q0 + unit, total - 1);
     const int64_t n = q / per, c = (q - n * per) * 4;
-    if (c >= D) continue;
     float v[4] = {0, 0, 0, 0};
     const float* p = sums + n * dp + c;
-#pragma unroll 16
-    for (int s = 0; s < splits; ++s) {
+#pragma unroll 8
+    for (int s = from; s < splits; s += STEP) {
       const float4 o = *reinterpret_cast<const float4*>(p + (int64_t)s * N * dp);
       v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
     }
+    if constexpr (SHARE) {
+      if (from > 0) part[(from - 1) * 64 + unit] = float4{v[0], v[1], v[2], v[3]};
+      __syncthreads();
+      if (from == 0)
+        for (int w = 0; w < 3; ++w) {
+          const float4 o = part[w * 64 + unit];
+          v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
+        }
+      __syncthreads();
+    }
+    if (from > 0 || q0 + unit >= total || c >= D) continue;
     const bool none = targets[n] == T_NONE;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = none ? 0.0f : v[i] * a;
@@ -757,7 +771,7 @@ GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece) {
         left -= count[g];
       }
       if (!big && nx + nw <= cus) end *= 0.65;
-      // (the splits' sums: written and read once, 16 at a time)
+      // (the splits' sums: written and read once, a few at a time)
       const double us = end + (double)splits * ((double)N * (double)D * 8.0 / 4e6 + 0.1);
       if (best.us == 0.0 || us < best.us) best = GradsPlan{us, big != 0, splits};
     }
@@ -1024,20 +1038,20 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
     if (rc != NOVAQ_OK) return rc;
   }
   if (gx) {
-    const dim3 grid((unsigned)std::min<int64_t>((N * (p.dp / 4) + 255) / 256, 8192));
-    switch (x_dtype) {
-      case F32:
-        hipLaunchKernelGGL(loss_dx_store_kernel<F32>, grid, dim3(256), 0, st, sums, p.splits, N,
-                           p.dp, D, scal, w_scale, inv, targets, gx);
-        break;
-      case F16:
-        hipLaunchKernelGGL(loss_dx_store_kernel<F16>, grid, dim3(256), 0, st, sums, p.splits, N,
-                           p.dp, D, scal, w_scale, inv, targets, gx);
-        break;
-      default:
-        hipLaunchKernelGGL(loss_dx_store_kernel<BF16>, grid, dim3(256), 0, st, sums, p.splits, N,
-                           p.dp, D, scal, w_scale, inv, targets, gx);
-    }
+    auto store = [&](auto ot, auto share) {
+      constexpr bool SHARE = decltype(share)::value;
+      const int64_t units = SHARE ? 64 : 256;
+      const dim3 grid((unsigned)std::min<int64_t>((N * (p.dp / 4) + units - 1) / units, 8192));
+      hipLaunchKernelGGL((loss_dx_store_kernel<decltype(ot)::value, SHARE>), grid, dim3(256), 0, st,
+                         sums, p.splits, N, p.dp, D, scal, w_scale, inv, targets, gx);
+    };
+    auto to = [&](auto ot) {
+      if (p.splits >= 8) store(ot, std::true_type{});
+      else store(ot, std::false_type{});
+    };
+    if (x_dtype == F32) to(std::integral_constant<int, F32>{});
+    else if (x_dtype == F16) to(std::integral_constant<int, F16>{});
+    else to(std::integral_constant<int, BF16>{});
     rc = check_launch();
   }
   return rc;
