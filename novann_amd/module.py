@@ -15,7 +15,8 @@ forward and backward; both call the GPU operators in ``functional``.
 ``BatchNorm2d`` / ``BatchNorm1d`` hold the reference's parameters and running
 statistics (batchnorm2d.py:33-55, batchnorm1d.py:33-55) and ``ReLU`` stands
 for novann's ReLU layer; on this path they run fused into the product before
-them (``fuse``), in eval mode.
+them (``fuse``), in eval mode.  ``Embedding`` and ``LinearCrossEntropy`` are the
+two ends of a token model, in the same manner.
 """
 from __future__ import annotations
 
@@ -251,6 +252,111 @@ class Linear(Layer):
     def __repr__(self) -> str:
         return (f"Linear(in_features={self.in_features}, out_features={self.out_features}, "
                 f"bias={self.use_bias})")
+
+
+def _token_table(layer, rows: int, cols: int, name: str):
+    """A (rows, cols) weight drawn as Linear draws its own, stored in the layer's
+    weight_dtype (with the fp32 master) when it has one."""
+    init = layer.init_fn or DEFAULT_NORMAL_INIT_MAP["default"]
+    w = Parameters(np.asarray(init((rows, cols)), dtype=np.float32))
+    if layer.weight_dtype is not None:
+        w = QuantizedParameters.from_float(w, layer.weight_dtype, keep_master=True)
+    w.name = name
+    return w
+
+
+class Embedding(Layer):
+    """Rows of a (num_tokens, width) table by token, times ``factor``.
+
+    The table is drawn and stored as Linear's weight (``init``,
+    ``weight_dtype``); forward returns tokens.shape + (width,) in ``out_dtype``.
+    ``backward`` sets weight.grad, or adds to it where the table is another
+    layer's weight as well (``tied``) and that one's gradient is already there.
+    No counterpart in the reference, which has no token layers."""
+
+    def __init__(self, num_tokens: int, width: int, init=None,
+                 weight_dtype: Optional[str] = None, factor: float = 1.0,
+                 out_dtype: str = "f32", tied: bool = False) -> None:
+        super().__init__()
+        self.num_tokens, self.width = num_tokens, width
+        self.init_fn, self.weight_dtype = init, weight_dtype
+        self.factor, self.out_dtype, self.tied = factor, out_dtype, tied
+        self._cache_tokens = None
+        self.weight = _token_table(self, num_tokens, width, "embedding weight")
+
+    def forward(self, tokens):
+        from . import functional as F
+        self._cache_tokens = tokens
+        return F.embedding(tokens, self.weight, factor=self.factor, out_dtype=self.out_dtype)
+
+    def backward(self, grad):
+        """Sets (tied: adds to) weight.grad; tokens have no gradient."""
+        from . import functional as F
+        there = self.weight.grad if self.tied else None
+        add = isinstance(there, torch.Tensor)
+        g = F.embedding_backward(_as_f32(grad), self._cache_tokens, self.weight,
+                                 factor=self.factor, out=there if add else None, accumulate=add)
+        self.weight.grad = g
+
+    def parameters(self):
+        return [self.weight]
+
+    def __repr__(self) -> str:
+        return f"Embedding(num_tokens={self.num_tokens}, width={self.width})"
+
+
+class LinearCrossEntropy(Layer):
+    """The output layer of a token model and its loss in one: a bias-free linear
+    layer onto num_tokens classes and the softmax cross entropy of its logits,
+    which are never stored (functional.linear_cross_entropy).
+
+    ``weight``: another layer's (num_tokens, in_features) weight to share (an
+    Embedding's), else one is drawn and stored as Linear's.  Called with the
+    hidden states (N, in_features) and the targets (N,); ``backward`` takes the
+    loss's own gradient (default 1), sets weight.grad and returns the hidden
+    states' gradient.  Stands for Linear with CrossEntropyLoss
+    (novann/losses/loss_functions.py:8-167)."""
+
+    def __init__(self, in_features: int, num_tokens: int, init=None,
+                 weight_dtype: Optional[str] = None, weight=None, ignore_index: int = -100,
+                 reduction: str = "mean") -> None:
+        super().__init__()
+        self.in_features, self.num_tokens = in_features, num_tokens
+        self.init_fn, self.weight_dtype = init, weight_dtype
+        self.ignore_index, self.reduction = ignore_index, reduction
+        self._cache = None
+        if weight is not None and tuple(weight.shape) != (num_tokens, in_features):
+            raise ValueError(f"weight {tuple(weight.shape)} is not {(num_tokens, in_features)}")
+        self.shared = weight is not None
+        self.weight = weight if self.shared else _token_table(self, num_tokens, in_features,
+                                                              "output weight")
+
+    def __call__(self, x, targets):
+        return self.forward(x, targets)
+
+    def forward(self, x, targets):
+        from . import functional as F
+        x = _as_f32(x)
+        loss, lse = F.linear_cross_entropy(x, self.weight, targets,
+                                           ignore_index=self.ignore_index,
+                                           reduction=self.reduction, extras=True)
+        self._cache = (x, targets, lse)
+        return loss
+
+    def backward(self, grad=None):
+        from . import functional as F
+        x, targets, lse = self._cache
+        gx, self.weight.grad = F.linear_cross_entropy_backward(
+            x, self.weight, targets, lse, grad=grad, ignore_index=self.ignore_index,
+            reduction=self.reduction)
+        return gx
+
+    def parameters(self):
+        return [] if self.shared else [self.weight]
+
+    def __repr__(self) -> str:
+        return (f"LinearCrossEntropy(in_features={self.in_features}, "
+                f"num_tokens={self.num_tokens})")
 
 
 class Conv2d(Layer):
