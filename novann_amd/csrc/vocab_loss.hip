@@ -748,7 +748,7 @@ struct GradsPlan {
   bool big;
   int splits;
 };
-GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece) {
+GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece, int most = 64) {
   const int64_t cus = device_cu_count();
   GradsPlan best{0.0, false, 1};
   const int64_t kx = (piece + 63) / 64, kw = (N + 63) / 64;
@@ -756,7 +756,7 @@ GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece) {
     const int64_t e = big ? 256 : 128, slots = big ? cus : 2 * cus, cols = (D + e - 1) / e;
     const double block = big ? 1.67 : 0.965, tile = big ? 4.8 : 4.1;
     const int64_t nw = ((piece + e - 1) / e) * cols;
-    for (int splits = 1; splits <= 64 && (splits == 1 || kx / splits >= 4); splits *= 2) {
+    for (int splits = 1; splits <= most && (splits == 1 || kx / splits >= 4); splits *= 2) {
       const int64_t nx = ((N + e - 1) / e) * cols * splits;
       const double tx = block * (double)((kx + splits - 1) / splits) + tile;
       const double tw = block * (double)kw + tile;
@@ -995,6 +995,12 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
     const int64_t pp = row_pitch(vp);
     const TokenOp ow{p.copy_w ? ww : reinterpret_cast<const uint16_t*>(from), vc,
                      p.copy_w ? p.pitch : D};
+    // a last, smaller piece may do better on other tiles (the first has set all the
+    // splits' sums)
+    const bool rest = v0 > 0 && vc < p.piece;
+    const bool big_l = rest ? large_tiles(vc, N, D) : p.big_l;
+    const GradsPlan gp = rest ? grads_plan(N, D, vc, p.splits)
+                              : GradsPlan{0.0, p.big_g, p.splits};
     auto prob = [&](auto g) -> int {
       using G = decltype(g);
       const int tm = (int)(vp / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
@@ -1002,7 +1008,7 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
                    N, targets, f, lse, pscale, P, pp, tm, tn);
       return NOVAQ_OK;
     };
-    rc = p.big_l ? prob(TokenGemm<CT, false, false, 128, 64, 4>{})
+    rc = big_l ? prob(TokenGemm<CT, false, false, 128, 64, 4>{})
                  : prob(TokenGemm<CT, false, false, 64, 64, 2>{});
     if (rc != NOVAQ_OK) return rc;
     auto grads = [&](auto ot, auto gx_, auto gw_) -> int {
@@ -1010,7 +1016,7 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
       using GW = decltype(gw_);
       constexpr int OT = decltype(ot)::value;
       GradsJob j{TokenOp{P, N, pp}, TokenOp{P, vp, pp}, ow, ox, N, D, vc, (int)(vp / 64),
-                 (int)((N + 63) / 64), p.splits, v0 == 0 ? 1 : 0, sums, p.dp, scal, inv,
+                 (int)((N + 63) / 64), gp.splits, v0 == 0 ? 1 : 0, sums, p.dp, scal, inv,
                  static_cast<uint8_t*>(gw) + v0 * D * (OT == F32 ? 4 : 2), 0, 0, 0, 0};
       if (gx) {
         j.xtm = (int)((N + GX::BM - 1) / GX::BM);
@@ -1027,7 +1033,7 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
       return NOVAQ_OK;
     };
     auto grads_to = [&](auto ot) -> int {
-      return p.big_g ? grads(ot, TokenGemm<CT, false, true, 128, 64, 4>{},
+      return gp.big ? grads(ot, TokenGemm<CT, false, true, 128, 64, 4>{},
                              TokenGemm<CT, true, true, 128, 64, 4>{})
                      : grads(ot, TokenGemm<CT, false, true, 64, 64, 2>{},
                              TokenGemm<CT, true, true, 64, 64, 2>{});
