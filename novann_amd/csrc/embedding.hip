@@ -7,8 +7,8 @@
 // The lookup moves one row a token and is bound by memory; 8 elements a lane.
 //
 // The gradient sorts the tokens (stable, radix digits of 9 bits), so that a
-// row's positions lie together in rising order, and sums runs of 16 sorted
-// entries a wave.  A token with many positions spans several of these chunks:
+// row's positions lie together in rising order, and sums chunks of 16 (few tokens:
+// 4) sorted entries a wave.  A token with many positions spans several of these chunks:
 // each then leaves its part in the workspace and a last kernel adds a run's
 // parts in order.  No atomics touch floating-point values: the sums' order
 // depends on the tokens alone, and the result is the same bit for bit in every
@@ -17,6 +17,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "novaq_internal.h"
 #include "token_io.h"
@@ -98,8 +99,9 @@ int lookup_to(int ot, const void* ids, int bits, int64_t N, const void* table, c
 constexpr int DIGIT = 9, BINS = 1 << DIGIT;
 constexpr int BATCH = 1024;     // entries of a block's batch: 4 a lane
 constexpr int BLOCKS = 128;     // at most, of a pass
-constexpr int SMALL = 2048;     // entries that one workgroup sorts in LDS
-constexpr int CHUNK = 16;       // sorted entries a wave sums
+// Entries that one workgroup sorts in LDS (4096: 15 us against 21 for the four
+// launches of the passes over blocks; 8192: 24 against 21).
+constexpr int SMALL = 4096;
 
 // The rows that get no gradient must be zero: the sort's launches, which use few
 // workgroups, carry the table's zeros in their other ones (32768 tokens, a table
@@ -162,68 +164,82 @@ __device__ __forceinline__ uint32_t place(uint32_t* cnt, uint32_t d, bool in, in
   return at;
 }
 
-// Up to SMALL entries sorted by one workgroup in LDS, all passes; the other
+// Up to 1024 PER entries sorted by one workgroup in LDS, all passes; the other
 // workgroups write zeros.
-__global__ __launch_bounds__(512) void sort_small_kernel(const void* __restrict__ ids, int bits,
-                                                         int64_t V, int N, int passes,
-                                                         uint32_t* __restrict__ keys_out,
-                                                         uint32_t* __restrict__ pos_out,
-                                                         Zeros z) {
+template <int PER>
+struct SmallSort {
+  static constexpr int W = 16, N = 1024 * PER;
+  static constexpr size_t lds = (size_t)(2 * N + W * BINS + W) * 4;
+};
+
+template <int PER>
+__global__ __launch_bounds__(1024) void sort_small_kernel(const void* __restrict__ ids, int bits,
+                                                          int64_t V, int N, int passes,
+                                                          uint32_t* __restrict__ keys_out,
+                                                          uint32_t* __restrict__ pos_out,
+                                                          Zeros z) {
   if (blockIdx.x > 0) {
-    write_zeros(z, blockIdx.x - 1, gridDim.x - 1, 512);
+    write_zeros(z, blockIdx.x - 1, gridDim.x - 1, 1024);
     return;
   }
-  constexpr int W = 8, PER = SMALL / 512;  // waves; entries a lane
-  __shared__ uint32_t key[SMALL], pos[SMALL], cnt[W][BINS], sums[W];
+  constexpr int W = SmallSort<PER>::W;
+  extern __shared__ uint32_t small_lds[];
+  uint32_t* key = small_lds;
+  uint32_t* pos = key + SmallSort<PER>::N;
+  uint32_t(*cnt)[BINS] = reinterpret_cast<uint32_t(*)[BINS]>(pos + SmallSort<PER>::N);
+  uint32_t* sums = &cnt[W][0];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // wave w holds entries w 64 PER .. : step i's are 64 i + lane of them
+  const int e0 = wave * 64 * PER + lane;
   uint32_t k[PER], p[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = wave * 64 * PER + i * 64 + lane;
+    const int e = e0 + i * 64;
     k[i] = e < N ? token_key(ids, bits, e, V) : 0u;
     p[i] = (uint32_t)e;
   }
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * DIGIT;
-    for (int w = 0; w < W; ++w) cnt[w][tid] = 0;
+    for (int i = tid; i < W * BINS; i += 1024) cnt[0][i] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (wave * 64 * PER + i * 64 + lane < N) atomicAdd(&cnt[wave][(k[i] >> shift) & (BINS - 1)], 1u);
+      if (e0 + i * 64 < N) atomicAdd(&cnt[wave][(k[i] >> shift) & (BINS - 1)], 1u);
     __syncthreads();
-    // digit tid: its entries in all waves, then the digits before it
-    uint32_t all = 0, of_wave;
-    for (int w = 0; w < W; ++w) all += cnt[w][tid];
-    uint32_t at = wave_before(all, lane, of_wave);
-    if (lane == 0) sums[wave] = of_wave;
+    // digit tid (of the first 8 waves): its entries in all waves, then the digits
+    // before it
+    uint32_t all = 0, of_wave, at = 0;
+    if (tid < BINS) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) all += cnt[w][tid];
+      at = wave_before(all, lane, of_wave);
+      if (lane == 0) sums[wave] = of_wave;
+    }
     __syncthreads();
-    for (int w = 0; w < wave; ++w) at += sums[w];
-    for (int w = 0; w < W; ++w) {
-      const uint32_t c = cnt[w][tid];
-      cnt[w][tid] = at;
-      at += c;
+    if (tid < BINS) {
+      for (int w = 0; w < wave; ++w) at += sums[w];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const uint32_t c = cnt[w][tid];
+        cnt[w][tid] = at;
+        at += c;
+      }
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const bool in = wave * 64 * PER + i * 64 + lane < N;
+      const bool in = e0 + i * 64 < N;
       const uint32_t to = place(cnt[wave], (k[i] >> shift) & (BINS - 1), in, lane);
       if (in) key[to] = k[i], pos[to] = p[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = wave * 64 * PER + i * 64 + lane;
-      if (e < N) k[i] = key[e], p[i] = pos[e];
-    }
-    __syncthreads();
+    for (int i = 0; i < PER; ++i)
+      if (e0 + i * 64 < N) k[i] = key[e0 + i * 64], p[i] = pos[e0 + i * 64];
   }
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = wave * 64 * PER + i * 64 + lane;
-    if (e < N) keys_out[e] = k[i], pos_out[e] = p[i];
-  }
+  for (int i = 0; i < PER; ++i)
+    if (e0 + i * 64 < N) keys_out[e0 + i * 64] = k[i], pos_out[e0 + i * 64] = p[i];
 }
 
 // Digit counts of each block's `per` entries: hist[block][digit].
@@ -384,7 +400,7 @@ __device__ __forceinline__ void put_row(uint8_t* out, const float (&sum)[VEC], f
 // before the first sum; a run that ends inside the chunk is stored, one that
 // began in an earlier chunk leaves its sum at head[chunk], one that goes on
 // past the chunk at tail[chunk].
-template <int GT, int OT, int VEC>
+template <int GT, int OT, int VEC, int CHUNK>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(
     const uint8_t* __restrict__ grad, const uint32_t* __restrict__ keys,
     const uint32_t* __restrict__ pos, int N, int64_t V, int64_t D, float factor, int accumulate,
@@ -438,7 +454,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(
 // sums are added in the waves' order.
 template <int OT, int VEC>
 __global__ __launch_bounds__(512) void embedding_join_kernel(
-    const uint32_t* __restrict__ keys, int N, int64_t V, int64_t D, float factor, int accumulate,
+    const uint32_t* __restrict__ keys, int N, int CHUNK, int64_t V, int64_t D, float factor, int accumulate,
     const float* __restrict__ head, const float* __restrict__ tail, uint8_t* __restrict__ out) {
   constexpr int OB = OT == F32 ? 4 : 2;
   __shared__ float part[8][64 * VEC];
@@ -491,7 +507,7 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct EmbedPlan {
-  int passes, per, blocks;
+  int passes, per, blocks, chunk;
   int64_t chunks;
   size_t hist, keys[2], pos[2], head, tail, total;
 };
@@ -504,7 +520,8 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D) {
   // whole batches a block, at most 128 blocks
   p.per = (int)(((N + BLOCKS - 1) / BLOCKS + BATCH - 1) / BATCH * BATCH);
   p.blocks = (int)((N + p.per - 1) / p.per);
-  p.chunks = (N + CHUNK - 1) / CHUNK;
+  p.chunk = N <= SMALL ? 4 : 16;
+  p.chunks = (N + p.chunk - 1) / p.chunk;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t b = at;
@@ -526,13 +543,17 @@ int sums(const EmbedPlan& p, const uint8_t* grad, const uint32_t* keys, const ui
   float* head = reinterpret_cast<float*>(ws + p.head);
   float* tail = reinterpret_cast<float*>(ws + p.tail);
   const unsigned cols = (unsigned)((D + 64 * VEC - 1) / (64 * VEC));
-  hipLaunchKernelGGL((embedding_sum_kernel<GT, OT, VEC>),
-                     dim3((unsigned)((p.chunks + 3) / 4), cols), dim3(256), 0, st, grad, keys, pos,
-                     (int)N, V, D, factor, accumulate, head, tail, out);
+  const dim3 grid((unsigned)((p.chunks + 3) / 4), cols);
+  if (p.chunk == 4)
+    hipLaunchKernelGGL((embedding_sum_kernel<GT, OT, VEC, 4>), grid, dim3(256), 0, st, grad, keys,
+                       pos, (int)N, V, D, factor, accumulate, head, tail, out);
+  else
+    hipLaunchKernelGGL((embedding_sum_kernel<GT, OT, VEC, 16>), grid, dim3(256), 0, st, grad, keys,
+                       pos, (int)N, V, D, factor, accumulate, head, tail, out);
   int rc = check_launch();
   if (rc != NOVAQ_OK || p.chunks < 2) return rc;
   hipLaunchKernelGGL((embedding_join_kernel<OT, VEC>), dim3((unsigned)p.chunks, cols), dim3(512),
-                     0, st, keys, (int)N, V, D, factor, accumulate, head, tail, out);
+                     0, st, keys, (int)N, p.chunk, V, D, factor, accumulate, head, tail, out);
   return check_launch();
 }
 
@@ -591,10 +612,20 @@ int embedding_backward_launch(const void* grad, int g_dtype, const void* ids, in
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + p.pos[0]),
                       reinterpret_cast<uint32_t*>(ws + p.pos[1])};
   if (N <= SMALL) {
-    hipLaunchKernelGGL(sort_small_kernel, dim3(1 + zero_blocks(bytes, 512)), dim3(512), 0, st, ids,
-                       bits, V, (int)N, p.passes, keys[p.passes & 1], pos[p.passes & 1],
-                       Zeros{table, 0, bytes});
-    const int rc = check_launch();
+    auto small = [&](auto per) -> int {
+      constexpr int PER = decltype(per)::value;
+      static DeviceFlags raised;
+      const int rc = allow_lds(raised, reinterpret_cast<const void*>(&sort_small_kernel<PER>),
+                               SmallSort<PER>::lds, SmallSort<PER>::lds);
+      if (rc != NOVAQ_OK) return rc;
+      hipLaunchKernelGGL(sort_small_kernel<PER>, dim3(1 + zero_blocks(bytes, 1024)), dim3(1024),
+                         SmallSort<PER>::lds, st, ids, bits, V, (int)N, p.passes,
+                         keys[p.passes & 1], pos[p.passes & 1], Zeros{table, 0, bytes});
+      return check_launch();
+    };
+    const int rc = N <= 1024   ? small(std::integral_constant<int, 1>{})
+                   : N <= 2048 ? small(std::integral_constant<int, 2>{})
+                               : small(std::integral_constant<int, 4>{});
     if (rc != NOVAQ_OK) return rc;
   }
   // the zeros' share of a launch: one part beside the counts, three beside the
