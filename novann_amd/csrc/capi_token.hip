@@ -39,7 +39,8 @@ int check_loss(const void* x, int x_dtype, int64_t N, int64_t D, const void* w, 
   int rc = check_table(w_dtype, w_scale, V, D);
   if (rc != NOVAQ_OK) return rc;
   if (N < 0 || reduction < NOVAQ_REDUCE_NONE || reduction > NOVAQ_REDUCE_SUM) return NOVAQ_EINVAL;
-  if (N >= INT - 1024) return NOVAQ_ENOTSUP;
+  // (tiles of 128 x 128 are counted in 31 bits)
+  if (N >= INT - 1024 || ((N + 127) / 128) * ((V + 127) / 128) > INT) return NOVAQ_ENOTSUP;
   rc = check_ids(targets, bits);
   if (rc != NOVAQ_OK) return rc;
   if (!w || (N > 0 && (!x || !targets))) return NOVAQ_EINVAL;

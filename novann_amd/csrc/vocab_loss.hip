@@ -786,7 +786,8 @@ GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece, int most = 64) {
 int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, bool backward) {
   const int64_t vr = (V + 255) / 256 * 256;
   int64_t most = vr;
-  if (backward) most = std::min(most, ((int64_t)1 << 26) / std::max<int64_t>(N, 1));
+  // (256 rows of P within 31 bits of bytes, whatever N)
+  if (backward) most = std::min(most, ((int64_t)1 << 26) / std::max<int64_t>(N, 32));
   if (copy_w) most = std::min(most, ((int64_t)1 << 26) / dp);
   most = std::max<int64_t>(most / 256 * 256, std::min<int64_t>(vr, 1024));
   if (most >= vr) return vr;

@@ -592,6 +592,8 @@ def _ids_arg(ids, limit: Optional[int], what: str, ignore: Optional[int] = None)
     host are checked against 0 .. limit - 1 (ValueError); what a kernel does
     with an id on the device that lies outside is said by each operator."""
     if isinstance(ids, torch.Tensor):
+        if ids.is_cuda and ids.dtype is torch.int64 and ids.is_contiguous():
+            return ids, 64
         if not ids.is_cuda:
             ids = ids.detach().numpy()
     elif not isinstance(ids, np.ndarray):
@@ -615,28 +617,46 @@ def _ids_arg(ids, limit: Optional[int], what: str, ignore: Optional[int] = None)
     raise TypeError(f"{what} must be integers, got {ids.dtype}")
 
 
+def _table_shape(weight):
+    if isinstance(weight, tuple):
+        shape = weight
+    elif isinstance(weight, QuantizedParameters):
+        shape = weight.shape
+    else:
+        shape = tuple((weight.data if isinstance(weight, Parameters) else weight).shape)
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"weight must be a (rows, columns) table, got shape {tuple(shape)}")
+    return shape
+
+
 def _table_arg(weight, dev: torch.device):
     """(codes, dtype code, scale or None, (V, D)) of a 2-D table: quantized
     codes, or fp32 / bf16 / f16 data as stored (other types become fp32)."""
+    shape = _table_shape(weight)
     if isinstance(weight, QuantizedParameters):
-        w, dt, scale = _weight_args(weight, dev)
-        shape = weight.shape
-    else:
-        data = weight.data if isinstance(weight, Parameters) else weight
-        if isinstance(data, torch.Tensor) and data.is_cuda and data.dtype in _TOKEN_FLOATS:
-            w, dt, scale = _aligned(data.contiguous()), DTYPES[_TOKEN_FLOATS[data.dtype]], None
-        else:
-            w, dt, scale = _to_device_f32(data, "weight")[0], DTYPES["f32"], None
-        shape = tuple(w.shape)
-    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
-        raise ValueError(f"weight must be a (rows, columns) table, got shape {tuple(shape)}")
-    return w, dt, scale, shape
+        # (_weight_args, at less cost where everything is in place: its checks
+        # take longer than a kernel that looks up one row)
+        codes, scale, at = weight.codes, weight.scale, dev.index
+        row = (shape[1] + 1) // 2 if weight.dtype == "e2m1" else shape[1]
+        if codes.get_device() == at and scale.get_device() == at and codes.is_contiguous() \
+                and codes.element_size() == 1 and codes.numel() >= shape[0] * row \
+                and codes.data_ptr() % 16 == 0:
+            return codes, DTYPES[weight.dtype], scale, shape
+        return (*_weight_args(weight, dev), shape)
+    data = weight.data if isinstance(weight, Parameters) else weight
+    if isinstance(data, torch.Tensor) and data.is_cuda and data.dtype in _TOKEN_FLOATS:
+        return _aligned(data.contiguous()), DTYPES[_TOKEN_FLOATS[data.dtype]], None, shape
+    return _to_device_f32(data, "weight")[0], DTYPES["f32"], None, shape
 
 
 def _float_arg(a, what: str):
     """(contiguous fp32 / bf16 / f16 device tensor, dtype code, was numpy)."""
-    if isinstance(a, torch.Tensor) and a.is_cuda and a.dtype in _TOKEN_FLOATS:
-        return _aligned(a.contiguous()), DTYPES[_TOKEN_FLOATS[a.dtype]], False
+    if isinstance(a, torch.Tensor) and a.is_cuda:
+        name = _TOKEN_FLOATS.get(a.dtype)
+        if name is not None:
+            if not a.is_contiguous() or a.data_ptr() % 16:
+                a = _aligned(a.contiguous())
+            return a, DTYPES[name], False
     t, was_numpy = _to_device_f32(a, what)
     return t, DTYPES["f32"], was_numpy
 
@@ -688,14 +708,7 @@ def embedding_backward(grad, tokens, weight, *, factor: float = 1.0, out=None,
     that is the output layer's too.  Sums are fp32 in an order that depends on the
     tokens alone: equal calls give equal bits.  Tokens outside the table add
     nothing.  weight: as in ``embedding``, or its (V, D) shape."""
-    if isinstance(weight, tuple):
-        shape = weight
-    else:
-        shape = weight.shape if isinstance(weight, QuantizedParameters) else tuple(
-            (weight.data if isinstance(weight, Parameters) else weight).shape)
-    if len(shape) != 2:
-        raise ValueError(f"weight must be a (rows, columns) table, got shape {tuple(shape)}")
-    V, D = shape
+    V, D = _table_shape(weight)
     g, gdt, was_numpy = _float_arg(grad, "grad")
     ids, bits = _ids_arg(tokens, V, "tokens")
     if tuple(g.shape) != (*ids.shape, D):

@@ -74,7 +74,7 @@ class QuantizedParameters:
                  amax: Optional[torch.Tensor] = None, name: Optional[str] = None,
                  master: Optional[torch.Tensor] = None):
         self.codes = codes
-        self.shape = tuple(int(d) for d in shape)
+        self.shape = tuple(map(int, shape))
         self.dtype = dtype
         self.scale = scale
         self.amax = amax

@@ -199,12 +199,21 @@ def _clip(grads, outs, max_norm: float, eps: float) -> torch.Tensor:
 
 
 def _gradients(items) -> list:
-    """The gradients among tensors, arrays and parameters (those with one)."""
+    """The gradients among tensors, arrays and parameters (those with one; a
+    parameter that is named twice, as a shared weight may be, counts once)."""
     items = list(items)
     if set(map(type, items)) == {torch.Tensor}:
         return items
-    found = (p if isinstance(p, (torch.Tensor, np.ndarray)) else p.grad for p in items)
-    return [g for g in found if g is not None]
+    found, seen = [], set()
+    for p in items:
+        if not isinstance(p, (torch.Tensor, np.ndarray)):
+            if id(p) in seen:
+                continue
+            seen.add(id(p))
+            p = p.grad
+        if p is not None:
+            found.append(p)
+    return found
 
 
 def _uploaded(grads) -> list:

@@ -132,3 +132,11 @@ def test_stream_and_graph():
         again = [torch.empty_like(o) for o in outs]
         assert torch.equal(norm, optim.clip_grad_norm(grads, 1.0, out=again))
         assert all(torch.equal(a, b) for a, b in zip(outs, again))
+
+
+def test_a_shared_parameter_counts_once():
+    p = Parameters(np.zeros((2, 3), np.float32))
+    p.grad = np.full((2, 3), 2.0, np.float32)
+    assert abs(float(optim.grad_norm([p, p])) - np.sqrt(24)) <= 2.0 ** -23 * np.sqrt(24)
+    optim.clip_grad_norm([p, p], np.sqrt(24) / 2, eps=0.0)
+    assert np.allclose(p.grad, 1.0, rtol=6 * 2.0 ** -24, atol=0)

@@ -255,3 +255,22 @@ def test_views_streams_and_graph():
         want, lse = F.linear_cross_entropy(fixed, w, at, extras=True)
         gx, gw = F.linear_cross_entropy_backward(fixed, w, at, lse)
         assert torch.equal(got, want) and torch.equal(gx, gx2) and torch.equal(gw, gw2)
+
+
+def test_more_classes_than_one_piece_of_few_rows():
+    """A vocabulary of millions: P's row pitch, the pieces and the tiles' counts
+    stay within their types."""
+    N, D, V = 2, 8, 3_000_001
+    rng = np.random.default_rng(11)
+    w = floats(rng, (V, D), "bf16", 0.5)
+    x = floats(rng, (N, D), "bf16")
+    t = np.array([V - 1, 17])
+    ids = torch.from_numpy(t).cuda()
+    each, lse = F.linear_cross_entropy(x, w, ids, reduction="none", extras=True)
+    x64, w64 = host(x), host(w)
+    want, want_lse, _ = cross_entropy(x64, w64, t)
+    e = logit_error(x64, w64, want_lse)
+    assert np.abs(host(each) - want).max() <= 2 * e and np.abs(host(lse) - want_lse).max() <= e
+    gx, gw = F.linear_cross_entropy_backward(x, w, ids, lse, reduction="sum",
+                                             weight_grad_dtype="f32")
+    check_grads(x, w, w64, t, np.ones(N), gx, gw, "bf16")
