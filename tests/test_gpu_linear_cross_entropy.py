@@ -274,3 +274,38 @@ def test_more_classes_than_one_piece_of_few_rows():
     gx, gw = F.linear_cross_entropy_backward(x, w, ids, lse, reduction="sum",
                                              weight_grad_dtype="f32")
     check_grads(x, w, w64, t, np.ones(N), gx, gw, "bf16")
+
+
+@pytest.mark.parametrize("N,D,V,wdtype,xdtype", [(5000, 700, 33000, "e4m3", "bf16"),
+                                                 (2048, 512, 20011, "e2m1", "f16"),
+                                                 (4096, 256, 40000, "bf16", "bf16")])
+def test_large_products(N, D, V, wdtype, xdtype):
+    """256 x 256 tiles, several pieces with a smaller last one, split sums: the
+    bounds of this file with the formulas in float64 on the device."""
+    x, w, w64, t = inputs(N, D, V, wdtype, xdtype, seed=5)
+    ids = torch.from_numpy(t).cuda()
+    loss, lse = F.linear_cross_entropy(x, w, ids, extras=True)
+    gx, gw = F.linear_cross_entropy_backward(x, w, ids, lse)
+    kept = ids != -100
+    n = int(kept.sum())
+    X, W = x.double() * kept.unsqueeze(1), torch.from_numpy(w64).cuda()
+    l = X @ W.t().contiguous()
+    want_lse = torch.logsumexp(l, 1)
+    e = float(np.sqrt(D) * 2.0 ** -23 * (X.abs() @ W.abs().t().contiguous()).max()
+              + 2.0 ** -20 * (1 + want_lse.abs().max()))
+    assert (lse.double() - want_lse).abs()[kept].max() <= e
+    at = torch.where(kept, ids, 0).unsqueeze(1)
+    each = torch.where(kept, want_lse - l.gather(1, at).squeeze(1), 0.0)
+    assert abs(float(loss) - float(each.sum()) / n) <= 2 * e
+    P = (l - want_lse.unsqueeze(1)).exp_()
+    del l
+    P.scatter_add_(1, at, torch.full_like(at, -1, dtype=torch.float64))
+    P *= kept.unsqueeze(1) / n
+    rel = HALF_ULP[xdtype] * 1.01 + 2 * e
+    floor = 2.0 ** -39 / n if xdtype == "f16" else 0.0
+    for got, want, size, few in ((gx, P @ W, P.abs() @ W.abs(), W.abs().sum(0)),
+                                 (gw, P.t().contiguous() @ X, P.abs().t().contiguous() @ X.abs(),
+                                  X.abs().sum(0))):
+        bound = rel * size + HALF_ULP[xdtype] * 1.01 * want.abs() + HALF_MIN[xdtype] + floor * few
+        bad = (got.double() - want).abs() > bound
+        assert not bad.any(), (int(bad.sum()), bad.nonzero()[:3])
