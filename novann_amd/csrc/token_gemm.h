@@ -27,6 +27,7 @@ namespace novaq {
 namespace {
 
 typedef float tg_f32x16 __attribute__((ext_vector_type(16)));
+typedef float tg_f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t tg_u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t tg_u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 tg_bf16x8 __attribute__((ext_vector_type(8)));
@@ -35,7 +36,8 @@ typedef __bf16 tg_bf16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) tg_bf16x4 tg_lds_bf16x4;
 typedef __attribute__((address_space(3))) void tg_lds_void;
 
-// One 32 x 32 x 16 MFMA on fragments held as raw words (CT: BF16 or F16).
+// MFMAs on fragments held as raw words (CT: BF16 or F16): 32 x 32 x 16, and 16 x
+// 16 x 32, which moves half as many accumulators an operation.
 template <int CT>
 __device__ __forceinline__ tg_f32x16 tg_mfma(const tg_u32x4& a, const tg_u32x4& b,
                                              const tg_f32x16& c) {
@@ -44,6 +46,16 @@ __device__ __forceinline__ tg_f32x16 tg_mfma(const tg_u32x4& a, const tg_u32x4& 
                                                    __builtin_bit_cast(tg_bf16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(tg_f16x8, a),
+                                                  __builtin_bit_cast(tg_f16x8, b), c, 0, 0, 0);
+}
+template <int CT>
+__device__ __forceinline__ tg_f32x4 tg_mfma(const tg_u32x4& a, const tg_u32x4& b,
+                                            const tg_f32x4& c) {
+  if constexpr (CT == BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(tg_bf16x8, a),
+                                                   __builtin_bit_cast(tg_bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(tg_f16x8, a),
                                                   __builtin_bit_cast(tg_f16x8, b), c, 0, 0, 0);
 }
 
@@ -93,9 +105,9 @@ struct TokenOp {
 //   K-contiguous: row r holds 8 chunks of 16 bytes, chunk c at slot
 //     c ^ ((r >> 1) & 7): the 16 rows that one 16-byte read touches at a time
 //     fall in distinct banks.
-//   K-strided: K row k holds R / 8 chunks, chunk c at slot c ^ (4 (k & 3)):
-//     the four K rows that a transposing read touches lie in distinct 64-byte
-//     bank ranges.
+//   K-strided: K row k holds R / 8 chunks, chunk c at slot c ^ (4 (k & 3)) ^
+//     (2 (k / 8 & 1)): the K rows k .. k + 3 and k + 8 .. k + 11 that half a
+//     wave's transposing read touches lie in distinct 32-byte bank ranges.
 template <bool KS, int R, int KB, int NTH>
 struct TokenTile {
   static constexpr int bytes = R * KB * 2;
@@ -125,7 +137,7 @@ struct TokenTile {
 #pragma unroll
     for (int i = 0; i < loads; ++i) {
       const int r = row0 + i * step;
-      const int c = (tid % cpr) ^ (KS ? 4 * (r & 3) : ((r >> 1) & 7));
+      const int c = (tid % cpr) ^ (KS ? 4 * (r & 3) ^ 2 * ((r >> 3) & 1) : ((r >> 1) & 7));
       s.voff[i] = (uint32_t)r * (uint32_t)(op.ld * 2) + c * 16;
     }
     return s;
@@ -145,18 +157,18 @@ struct TokenTile {
       tg_copy16(rs, s.voff[i], lds + (i * NTH + wave * 64) * 16);
   }
 
-  // Lane's byte offset of fragment (32 rows from w0 + 32 i, K 16 s .. + 15):
-  //   K-contiguous: lane l reads row l % 32, K 8 (l / 32) .. + 7.
+  // Fragment of 16 rows (from w0 + 16 i) and 32 K (from 32 s): lane l holds row l %
+  // 16, K 8 (l / 16) .. + 7.
   //   K-strided: in each group of 16 lanes lane p names 8 bytes (K row p / 4,
   //     columns 4 (p % 4) .. + 3 of a 4 x 16 block) and receives column p of
   //     the block; the second read is 4 K rows further.
   __device__ static __forceinline__ tg_u32x4 read(const uint8_t* lds, int w0, int i, int s,
                                                   int lane) {
+    const int q = lane >> 4;
     if constexpr (KS) {
-      const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
-      const int byte = ((w0 + i * 32) * 2 ^ ((k & 3) * 64)) +
-                       (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
-      const uint8_t* p = lds + (16 * s + k) * (R * 2) + byte;
+      const int k = 8 * q + ((lane & 15) >> 2);
+      const int byte = ((w0 + i * 16) * 2 ^ ((k & 3) * 64) ^ ((q & 1) * 32)) + (lane & 3) * 8;
+      const uint8_t* p = lds + (32 * s + k) * (R * 2) + byte;
       const tg_u32x2 lo = __builtin_bit_cast(
           tg_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((tg_lds_bf16x4*)p));
       const tg_u32x2 hi = __builtin_bit_cast(
@@ -164,9 +176,9 @@ struct TokenTile {
           __builtin_amdgcn_ds_read_tr16_b64_v4bf16((tg_lds_bf16x4*)(p + 4 * (R * 2))));
       return tg_u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
-      const int r = lane & 31, h = lane >> 5;
-      return *reinterpret_cast<const tg_u32x4*>(lds + (w0 + i * 32 + r) * 128 +
-                                                (((2 * s + h) ^ ((r >> 1) & 7)) << 4));
+      const int r = lane & 15;
+      return *reinterpret_cast<const tg_u32x4*>(lds + (w0 + i * 16 + r) * 128 +
+                                                (((4 * s + q) ^ ((r >> 1) & 7)) << 4));
     }
   }
 };
@@ -184,17 +196,17 @@ __device__ __forceinline__ void tg_mix() {
 }
 
 // The product of one BM x BN tile by WGM x WGN waves of WM x WN: K blocks kb0
-// to kb1 of 64.  acc[i][j]: rows wm + 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4,
-// column wn + 32 j + lane % 32.  After it returns every wave is done with LDS.
+// to kb1 of 64.  acc[i][j]: rows wm + 16 i + 4 (lane / 16) + r, column wn + 16 j +
+// lane % 16.  After it returns every wave is done with LDS.
 //
 // KB K a stage, NS stages in LDS: NS - 1 are in flight or in use ahead of the one
 // that is multiplied.
 template <int CT, bool AKS, bool BKS, int WM_, int WN_, int WGN_, int KB_ = 64, int NS_ = 2>
 struct TokenGemm {
-  static constexpr int KB = KB_, NS = NS_, STEPS = KB / 16;
+  static constexpr int KB = KB_, NS = NS_, STEPS = KB / 32;
   static constexpr int WM = WM_, WN = WN_, WGM = 2, WGN = WGN_;
   static constexpr int BM = WGM * WM, BN = WGN * WN, NTH = 64 * WGM * WGN;
-  static constexpr int MT = WM / 32, NT = WN / 32;
+  static constexpr int MT = WM / 16, NT = WN / 16;
   using A = TokenTile<AKS, BM, KB, NTH>;
   using B = TokenTile<BKS, BN, KB, NTH>;
   static constexpr int stage = A::bytes + B::bytes;
@@ -202,7 +214,7 @@ struct TokenGemm {
   static constexpr int out_bytes = BN * (BM * 2 + 16);
   static constexpr int lds_bytes = NS * stage > out_bytes ? NS * stage : out_bytes;
   static constexpr int R = MT * (AKS ? 2 : 1) + NT * (BKS ? 2 : 1);  // LDS reads a step
-  typedef tg_f32x16 Acc[MT][NT];
+  typedef tg_f32x4 Acc[MT][NT];
 
   struct Frags {
     tg_u32x4 a[MT];
@@ -222,7 +234,7 @@ struct TokenGemm {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = 0.0f;
 
     auto issue = [&](int kb, int slot) {
       uint8_t* at = lds + slot * stage;
@@ -242,7 +254,7 @@ struct TokenGemm {
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = tg_mfma<CT>(f.a[i], f.b[j], acc[i][j]);
     };
-    // Stage kb in steps of 16 K, each step's fragments read while the one before is
+    // Stage kb in steps of 32 K, each step's fragments read while the one before is
     // multiplied.  Before the last step: this wave's reads of stage kb and its
     // copies of stage kb + 1 are done (counters), and after the barrier every
     // wave's, so the copy of stage kb + NS may overwrite kb's slot, and step 0 of

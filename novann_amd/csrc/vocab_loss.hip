@@ -281,21 +281,21 @@ __device__ __forceinline__ float2 join_stats(const float2& a, const float2& b) {
   return float2{m, a.y * __builtin_amdgcn_exp2f(a.x - z) + b.y * __builtin_amdgcn_exp2f(b.x - z)};
 }
 
-// The statistics of one token's products in a wave's MT row tiles, both lane
-// halves.  at(i, r): the lane's product of row 32 i + 8 (r / 4) + r % 4 (from its
-// own first row); those from `rows` on do not exist.  mine: the row of the token's
-// target, or -1; its logit goes to *tlogit.
-template <int MT, class F>
-__device__ __forceinline__ float2 column_stats(F&& at, bool ragged, int rows, int mine, float c2,
-                                               float* tlogit) {
+// The statistics of the I x R products of one token that a lane holds.  at(i, r)
+// is the product of row row(i, r) (from the lane's own first row); those from
+// `rows` on do not exist.  mine: the row of the token's target, or -1; its logit
+// goes to *tlogit.
+template <int I, int R, class F, class G>
+__device__ __forceinline__ float2 column_stats(F&& at, G&& row, bool ragged, int rows, int mine,
+                                               float c2, float* tlogit) {
   if (__ballot(mine >= 0)) {  // (few tiles hold a target of their tokens)
     float l = 0.0f;
     bool here = false;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const bool hit = 32 * i + 8 * (r >> 2) + (r & 3) == mine;
+      for (int r = 0; r < R; ++r) {
+        const bool hit = row(i, r) == mine;
         l = hit ? at(i, r) : l;
         here |= hit;
       }
@@ -303,30 +303,35 @@ __device__ __forceinline__ float2 column_stats(F&& at, bool ragged, int rows, in
   }
   if (ragged) {  // below every logit, in either sign of the scale
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (32 * i + 8 * (r >> 2) + (r & 3) >= rows) at(i, r) = c2 < 0.0f ? INFINITY : -INFINITY;
+      for (int r = 0; r < R; ++r)
+        if (row(i, r) >= rows) at(i, r) = c2 < 0.0f ? INFINITY : -INFINITY;
   }
   float top = at(0, 0);
   if (c2 < 0.0f) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fminf(top, at(i, r));
+      for (int r = 0; r < R; ++r) top = fminf(top, at(i, r));
   } else {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, at(i, r));
+      for (int r = 0; r < R; ++r) top = fmaxf(top, at(i, r));
   }
   const float m = top * c2, z = m == -INFINITY ? 0.0f : m;
   float s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < I; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(at(i, r), c2, -z));
-  return join_stats(float2{m, s}, float2{__shfl_xor(m, 32), __shfl_xor(s, 32)});
+    for (int r = 0; r < R; ++r) s += __builtin_amdgcn_exp2f(fmaf(at(i, r), c2, -z));
+  return float2{m, s};
+}
+
+// The same of the lanes `d` apart, joined.
+__device__ __forceinline__ float2 across(const float2& a, int d) {
+  return join_stats(a, float2{__shfl_xor(a.x, d), __shfl_xor(a.y, d)});
 }
 
 // The row of token n's target among the `many` rows from r0 on, or -1.
@@ -337,8 +342,8 @@ __device__ __forceinline__ int target_row(int t, int64_t r0, int many) {
 
 // The forward's tile: BM vocabulary rows (from v0 + m0) x BN tokens.  A lane
 // holds one token's logits of a column, so a row's maximum and sum stay in
-// registers but for one exchange between the lane halves and one between the
-// two waves that share the tokens.
+// registers but for the exchange between the four lanes and the two waves that
+// share the tokens.
 template <int CT, class G>
 __global__ __launch_bounds__(G::NTH, 1) void loss_stats_kernel(
     TokenOp w, TokenOp x, int64_t dp, const float* __restrict__ w_scale, int64_t v0, int64_t N,
@@ -352,28 +357,29 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_stats_kernel(
   G::run(acc, w, x, m0, n0, dp, 0, (int)(dp / 64), lds);
 
   const float c2 = logit_factor(w_scale);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, c = lane & 15;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
-  const int rows = (int)min((int64_t)G::BM, w.rows - m0) - wm - 4 * half;  // of this lane
+  const int rows = (int)min((int64_t)G::BM, w.rows - m0) - wm - 4 * q;  // of this lane
   const bool ragged = w.rows - m0 < G::BM;
   float2* part = reinterpret_cast<float2*>(lds);  // [BN]
   float2 st[G::NT];
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
-    const int64_t n = n0 + wn + 32 * j + (lane & 31);
+    const int64_t n = n0 + wn + 16 * j + c;
     const int t = n < N ? targets[n] : T_NONE;
-    st[j] = column_stats<G::MT>([&](int i, int r) -> float& { return ((float*)&acc[i][j])[r]; },
-                                ragged, rows, target_row(t, v0 + m0 + wm + 4 * half, G::WM), c2,
-                                tlogit + n);
-    if ((wave & 1) && half == 0) part[wn + 32 * j + (lane & 31)] = st[j];
+    st[j] = column_stats<G::MT, 4>([&](int i, int r) -> float& { return ((float*)&acc[i][j])[r]; },
+                                   [](int i, int r) { return 16 * i + r; }, ragged, rows,
+                                   target_row(t, v0 + m0 + wm + 4 * q, G::WM), c2, tlogit + n);
+    st[j] = across(across(st[j], 16), 32);
+    if ((wave & 1) && q == 0) part[wn + 16 * j + c] = st[j];
     __builtin_amdgcn_sched_barrier(0);  // (a column's values at a time in registers)
   }
   __syncthreads();
-  if ((wave & 1) == 0 && half == 0) {
+  if ((wave & 1) == 0 && q == 0) {
 #pragma unroll
     for (int j = 0; j < G::NT; ++j) {
-      const int64_t n = n0 + wn + 32 * j + (lane & 31);
-      const float2 o = join_stats(st[j], part[wn + 32 * j + (lane & 31)]);
+      const int64_t n = n0 + wn + 16 * j + c;
+      const float2 o = join_stats(st[j], part[wn + 16 * j + c]);
       if (n < N) stats[n * vtiles + (v0 + m0) / G::BM] = o;
     }
   }
@@ -399,9 +405,11 @@ __global__ __launch_bounds__(S::NTH, 1) void loss_stream_kernel(
   for (int j = 0; j < S::NT; ++j) {
     const int64_t n = 32 * j + (lane & 31);
     const int t = n < N ? targets[n] : T_NONE;
-    const float2 st = column_stats<1>([&](int, int r) -> float& { return ((float*)&acc[j])[r]; },
-                                      ragged, rows,
-                                      target_row(t, r0 + 32 * wave + 4 * half, 32), c2, tlogit + n);
+    const float2 st = across(
+        column_stats<1, 16>([&](int, int r) -> float& { return ((float*)&acc[j])[r]; },
+                            [](int, int r) { return 8 * (r >> 2) + (r & 3); }, ragged, rows,
+                            target_row(t, r0 + 32 * wave + 4 * half, 32), c2, tlogit + n),
+        32);
     if (half == 0) part[wave * 32 * S::NT + 32 * j + (lane & 31)] = st;
   }
   __syncthreads();
@@ -484,50 +492,48 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_prob_kernel(
   G::run(acc, w, x, m0, n0, dp, 0, (int)(dp / 64), lds);
 
   const float c2 = logit_factor(w_scale);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
-  const int rows = (int)max((int64_t)0, min((int64_t)G::BM, w.rows - m0)) - wm - 4 * half;
+  const int rows = (int)max((int64_t)0, min((int64_t)G::BM, w.rows - m0)) - wm - 4 * q;
   const bool ragged = w.rows - m0 < G::BM;
   // token rows of BM 16-bit values and 16 bytes more, so that the rows that a
   // store touches start in different banks
   constexpr int PITCH = G::BM * 2 + 16;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
-    const int col = wn + 32 * j + (lane & 31);
+    const int col = wn + 16 * j + (lane & 15);
     const int64_t n = n0 + col;
     const bool in = n < N;
     const int t = in ? targets[n] : T_NONE;
-    const int mine = target_row(t, v0 + m0 + wm + 4 * half, G::WM);
+    const int mine = target_row(t, v0 + m0 + wm + 4 * q, G::WM);
     // (an ignored row's x is zeros and its f 0: with any finite lse P is 0)
     const float fn = in ? f[n] * pscale : 0.0f;
     const float l2 = in && t != T_NONE ? lse[n] * LOG2E : 0.0f;
-    uint8_t* row = lds + col * PITCH + (wm + 4 * half) * 2;
+    uint8_t* row = lds + col * PITCH + (wm + 4 * q) * 2;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
+      for (int r = 0; r < 4; ++r)
         acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c2, -l2));
     if (__ballot(mine >= 0)) {  // (few tiles hold a target of their tokens)
 #pragma unroll
       for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * i + 8 * (r >> 2) + (r & 3) == mine) acc[i][j][r] -= 1.0f;
+        for (int r = 0; r < 4; ++r)
+          if (16 * i + r == mine) acc[i][j][r] -= 1.0f;
     }
     if (ragged) {
 #pragma unroll
       for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * i + 8 * (r >> 2) + (r & 3) >= rows) acc[i][j][r] = 0.0f;
+        for (int r = 0; r < 4; ++r)
+          if (16 * i + r >= rows) acc[i][j][r] = 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < G::MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<tg_u32x2*>(row + (32 * i + 8 * q) * 2) =
-            tg_u32x2{tg_pack2<CT>(acc[i][j][4 * q] * fn, acc[i][j][4 * q + 1] * fn),
-                     tg_pack2<CT>(acc[i][j][4 * q + 2] * fn, acc[i][j][4 * q + 3] * fn)};
+      *reinterpret_cast<tg_u32x2*>(row + 32 * i) =
+          tg_u32x2{tg_pack2<CT>(acc[i][j][0] * fn, acc[i][j][1] * fn),
+                   tg_pack2<CT>(acc[i][j][2] * fn, acc[i][j][3] * fn)};
   }
   __syncthreads();
   constexpr int CPR = G::BM / 8;  // 16-byte chunks a token row
@@ -567,7 +573,7 @@ __device__ __forceinline__ void dx_tile(const GradsJob& g, int b, uint8_t* lds) 
   typename G::Acc acc;
   G::run(acc, g.p, g.w, m0, n0, g.vc, (int)((int64_t)g.vblocks * split / g.splits),
          (int)((int64_t)g.vblocks * (split + 1) / g.splits), lds);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   // what lies past N or D is left out by the descriptor (offsets past it)
   const int rows = (int)min((int64_t)G::BM, N - m0);
@@ -576,23 +582,23 @@ __device__ __forceinline__ void dx_tile(const GradsJob& g, int b, uint8_t* lds) 
   const uint32_t pitch = (uint32_t)dp * 4;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
-    const int64_t d = n0 + wn + 32 * j + (lane & 31);
-    const uint32_t at = d < D ? (uint32_t)(wm + 4 * half) * pitch + (uint32_t)d * 4 : 0x80000000u;
+    const int64_t d = n0 + wn + 16 * j + (lane & 15);
+    const uint32_t at = d < D ? (uint32_t)(wm + 4 * q) * pitch + (uint32_t)d * 4 : 0x80000000u;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
-      float old[16];
+      float old[4];
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
+      for (int r = 0; r < 4; ++r)
         old[r] = first ? 0.0f
                        : u2f(__builtin_amdgcn_raw_buffer_load_b32(
-                             rs, at + (32 * i + 8 * (r >> 2) + (r & 3)) * pitch, 0, 0));
+                             rs, at + (16 * i + r) * pitch, 0, 0));
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
+      for (int r = 0; r < 4; ++r)
         __builtin_amdgcn_raw_buffer_store_b32(f2u(old[r] + acc[i][j][r]), rs,
-                                              at + (32 * i + 8 * (r >> 2) + (r & 3)) * pitch, 0,
+                                              at + (16 * i + r) * pitch, 0,
                                               0);
       // (16 loads in flight at a time: all of a tile's would not fit the registers)
-      __builtin_amdgcn_sched_barrier(0);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -607,7 +613,7 @@ __device__ __forceinline__ void dw_tile(const GradsJob& g, int b, uint8_t* lds) 
   G::run(acc, g.pt, g.x, m0, n0, g.N, 0, g.nblocks, lds);
   const float a = g.scal[0] * g.inv_pscale;
   uint8_t* out = g.gw;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
   constexpr int OB = OT == F32 ? 4 : 2;
   const int rows = (int)min((int64_t)G::BM, vc - m0);
@@ -616,19 +622,19 @@ __device__ __forceinline__ void dw_tile(const GradsJob& g, int b, uint8_t* lds) 
   const uint32_t pitch = (uint32_t)D * OB;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
-    const int64_t d = n0 + wn + 32 * j + (lane & 31);
-    const uint32_t at = d < D ? (uint32_t)(wm + 4 * half) * pitch + (uint32_t)d * OB : 0x80000000u;
+    const int64_t d = n0 + wn + 16 * j + (lane & 15);
+    const uint32_t at = d < D ? (uint32_t)(wm + 4 * q) * pitch + (uint32_t)d * OB : 0x80000000u;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const uint32_t o = at + (32 * i + 8 * (r >> 2) + (r & 3)) * pitch;
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t o = at + (16 * i + r) * pitch;
         const float y = acc[i][j][r] * a;
         if constexpr (OT == F32) __builtin_amdgcn_raw_buffer_store_b32(f2u(y), rs, o, 0, 0);
         else
           __builtin_amdgcn_raw_buffer_store_b16((uint16_t)tg_pack2<OT>(y, 0.0f), rs, o, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
