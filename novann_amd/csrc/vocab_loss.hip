@@ -726,19 +726,27 @@ struct LossPlan {
   size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, total;
 };
 
-// Time (us, on 256 CUs) of an M x N product of K, on tiles of 256 x 256 or 128 x
-// 128.  A CU runs one workgroup of the first (8 waves) or two of the second at a
-// time; measured at K 1024 and 4096 (8192 x 8192 and 8192 x 4096 tiles of
-// logits): 1.67 us a block of 64 K and 4.8 a tile, 0.965 and 4.1 a pair of
-// tiles.  A tile that has its CU to itself takes 0.65 of the pair's time.
+// Time (us) of a round of tiles of 256 x 256 (a CU runs one workgroup of 8 waves) or
+// of 128 x 128 (two of 4 waves) with K in blocks of 64.  Measured: the logits of 8192
+// x 8192 at K 512 and 1024 take 85 and 131 us in 4 rounds of the first, 119 and 174
+// in 8 of the second; those of 4096 x 16384 at K 4096 437 and 578, the gradients
+// from them (512 blocks in 5 rounds, 1024 in 10) 916 and 1110.  A small tile that
+// has its CU to itself takes 0.85 of the pair's time (2048 x 2048 and 2048 x 4096
+// logits at K 1024: 20.6 and 24.3 us).
+double round_us(bool big, double blocks, bool strided = false) {
+  return big ? (strided ? 1.72 : 1.6) * blocks + 7.0 : 1.03 * blocks + 5.5;
+}
+constexpr double LONE = 0.85;
+
+// Time of an M x N product of K.
 double product_us(int64_t M, int64_t N, int64_t K, bool big) {
   const int64_t e = big ? 256 : 128, cus = device_cu_count();
   const int64_t tiles = ((M + e - 1) / e) * ((N + e - 1) / e);
   const double blocks = (double)((K + 63) / 64);
-  if (big) return (double)((tiles + cus - 1) / cus) * (1.67 * blocks + 4.8);
+  const double round = round_us(big, blocks);
+  if (big) return (double)((tiles + cus - 1) / cus) * round;
   const int64_t rest = tiles % (2 * cus);
-  const double pair = 0.965 * blocks + 4.1;
-  return (double)(tiles / (2 * cus)) * pair + (rest == 0 ? 0.0 : rest <= cus ? 0.65 * pair : pair);
+  return (double)(tiles / (2 * cus)) * round + (rest == 0 ? 0.0 : rest <= cus ? LONE * round : round);
 }
 bool large_tiles(int64_t M, int64_t N, int64_t K) {
   return product_us(M, N, K, true) <= product_us(M, N, K, false);
@@ -760,12 +768,11 @@ GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece, int most = 64) {
   const int64_t kx = (piece + 63) / 64, kw = (N + 63) / 64;
   for (int big = 0; big < 2; ++big) {
     const int64_t e = big ? 256 : 128, slots = big ? cus : 2 * cus, cols = (D + e - 1) / e;
-    const double block = big ? 1.67 : 0.965, tile = big ? 4.8 : 4.1;
     const int64_t nw = ((piece + e - 1) / e) * cols;
     for (int splits = 1; splits <= most && (splits == 1 || kx / splits >= 4); splits *= 2) {
       const int64_t nx = ((N + e - 1) / e) * cols * splits;
-      const double tx = block * (double)((kx + splits - 1) / splits) + tile;
-      const double tw = block * (double)kw + tile;
+      const double tx = round_us(big != 0, (double)((kx + splits - 1) / splits), true);
+      const double tw = round_us(big != 0, (double)kw, true);
       // two groups of slots: those with one tile of grad_x more than the others
       int64_t count[2] = {nx % slots, slots - nx % slots}, left = nw;
       double at[2] = {(double)(nx / slots + 1) * tx, (double)(nx / slots) * tx};
@@ -776,7 +783,7 @@ GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece, int most = 64) {
         end = std::max(end, at[g]);
         left -= count[g];
       }
-      if (!big && nx + nw <= cus) end *= 0.65;
+      if (!big && nx + nw <= cus) end *= LONE;
       // (the splits' sums: written and read once, a few at a time)
       const double us = end + (double)splits * ((double)N * (double)D * 8.0 / 4e6 + 0.1);
       if (best.us == 0.0 || us < best.us) best = GradsPlan{us, big != 0, splits};
