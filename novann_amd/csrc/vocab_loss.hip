@@ -73,7 +73,10 @@ __device__ __forceinline__ void copy_rows(const CopyJob& j, int64_t first, int64
   const uint32_t per = (uint32_t)(j.dp / 8);
   const int64_t total = j.rows * per, rb = row_bytes(ST, j.D);
   for (int64_t q0 = first; q0 < total; q0 += A * step) {
+    // codes stay codes until they are stored: two a convert
+    constexpr bool codes = VEC && (ST == E4M3 || ST == E5M2 || ST == E2M1);
     float v[A][8];
+    ti_u32x2 code[A];
     uint16_t* to[A];
 #pragma unroll
     for (int x = 0; x < A; ++x) {
@@ -82,17 +85,30 @@ __device__ __forceinline__ void copy_rows(const CopyJob& j, int64_t first, int64
                                                      : q / per;
       const int64_t c = (q - row * per) * 8;
       to[x] = j.dst + row * j.pitch + c;
+      const bool here = c < j.D && !(j.ids && token_at(j.ids, j.bits, row) == j.ignore);
+      if constexpr (codes) {
+        code[x] = ti_u32x2{0, 0};
+        const uint8_t* p = j.src + row * rb + (ST == E2M1 ? c / 2 : c);
+        if (here) {
+          if constexpr (ST == E2M1) code[x][0] = vload<true>(reinterpret_cast<const uint32_t*>(p));
+          else code[x] = vload<true>(reinterpret_cast<const ti_u32x2*>(p));
+        }
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[x][i] = 0.0f;
-      if (c < j.D && !(j.ids && token_at(j.ids, j.bits, row) == j.ignore))
-        load8<ST, VEC, true>(j.src + row * rb, c, j.D, v[x]);
+        for (int i = 0; i < 8; ++i) v[x][i] = 0.0f;
+        if (here) load8<ST, VEC, true>(j.src + row * rb, c, j.D, v[x]);
+      }
     }
 #pragma unroll
     for (int x = 0; x < A; ++x) {
       if (q0 + x * step >= total) break;
       ti_u32x4 o;
+      if constexpr (codes) {
+        o = ts_decode8<CT, ST>(code[x][0], code[x][1]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[x][2 * i], v[x][2 * i + 1]);
+        for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[x][2 * i], v[x][2 * i + 1]);
+      }
       *reinterpret_cast<ti_u32x4*>(to[x]) = o;
     }
   }
