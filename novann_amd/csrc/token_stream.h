@@ -95,10 +95,13 @@ struct TokenStream {
   typedef tg_f32x16 Acc[NT];
 
   // acc[j]: table rows 32 wave + 8 (r / 4) + 4 (lane / 32) + r % 4 of r0 .., token
-  // 32 j + lane % 32.  xf: the tokens' fragments, stage by stage.
+  // 32 j + lane % 32.  xf: the tokens' fragments, stage by stage.  Stages are taken
+  // from `first` on, around the end: workgroups at the same columns of rows a power
+  // of two apart would all read the same few memory channels (one row of 4096 x
+  // 131072 E4M3: 94 us all from 0, 78 with every workgroup of an XCD elsewhere).
   __device__ static __forceinline__ void run(Acc& acc, const uint8_t* w, int64_t rows,
                                              int64_t row_bytes, int64_t r0, const uint8_t* xf,
-                                             int stages, uint8_t* lds) {
+                                             int stages, int first, uint8_t* lds) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int chunk = (tid & 7) ^ ((tid >> 4) & 7);  // of row tid / 8 (+ NTH / 8 i)
@@ -115,16 +118,17 @@ struct TokenStream {
       for (int r = 0; r < 16; ++r) acc[j][r] = 0.0f;
 
     // chunks past a row's end and stages past the last one are zeros
-    auto issue = [&](int s, int slot) {
+    auto issue = [&](int i0, int slot) {
       uint8_t* at = lds + slot * stage + wave * 1024;
+      const int s = i0 + first - (i0 + first >= stages ? stages : 0);
       const uint32_t c = (uint32_t)(s * 128 + chunk * 16);
-      const uint32_t base = c < rb && s < stages ? (uint32_t)(tid >> 3) * rb + c : 0x80000000u;
+      const uint32_t base = c < rb && i0 < stages ? (uint32_t)(tid >> 3) * rb + c : 0x80000000u;
 #pragma unroll
       for (int i = 0; i < WL; ++i)
         tg_copy16<true>(wr, base + i * (NTH / 8) * rb, at + i * PASS);
 #pragma unroll
       for (int i = 0; i < XL; ++i) {
-        const bool in = s < stages && (x_bytes % PASS == 0 || tid * 16 + i * PASS < x_bytes);
+        const bool in = i0 < stages && (x_bytes % PASS == 0 || tid * 16 + i * PASS < x_bytes);
         tg_copy16(xr, in ? (uint32_t)(s * x_bytes + tid * 16 + i * PASS) : 0x80000000u,
                   at + w_bytes + i * PASS);
       }

@@ -409,7 +409,8 @@ __global__ __launch_bounds__(S::NTH, 1) void loss_stream_kernel(
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int64_t r0 = (int64_t)blockIdx.x * S::ROWS;
   typename S::Acc acc;
-  S::run(acc, w, V, rb, r0, xf, stages, lds);
+  // (8 workgroups in a row are on 8 XCDs)
+  S::run(acc, w, V, rb, r0, xf, stages, (int)((blockIdx.x >> 3) % (unsigned)stages), lds);
 
   const float c2 = logit_factor(w_scale);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
