@@ -105,17 +105,28 @@ constexpr int SMALL = 4096;
 
 // The rows that get no gradient must be zero: the sort's launches, which use few
 // workgroups, carry the table's zeros in their other ones (32768 tokens, a table
-// of 205 MB: 31 us of sorting and 28 of writing one after the other).
+// of 205 MB: 31 us of sorting and 28 of writing one after the other, 46 together).
 struct Zeros {
   uint8_t* p;
   int64_t from, to;  // bytes, multiples of 16 but for the table's end
+  bool past;         // past the caches
 };
 
+// A table of more than half the 256 MB cache is written past it: what else the
+// cache holds is read next (lookup and gradient of 32768 tokens, 205 MB: 104 us
+// through it, 100 past it; of 1000 tokens, 94 MB: 26.3 and 29.3).
+constexpr int64_t PAST = (int64_t)128 << 20;
+
+template <bool NT>
+__device__ __forceinline__ void write_vectors(ti_u32x4* p, int64_t n, int64_t first, int64_t step) {
+  for (int64_t i = first; i < n; i += step) vstore<NT>(p + i, ti_u32x4{0u, 0u, 0u, 0u});
+}
 __device__ __forceinline__ void write_zeros(const Zeros& z, int block, int blocks, int threads) {
   ti_u32x4* p = reinterpret_cast<ti_u32x4*>(z.p + z.from);
-  const int64_t n16 = (z.to - z.from) / 16;
-  for (int64_t i = (int64_t)block * threads + threadIdx.x; i < n16; i += (int64_t)blocks * threads)
-    p[i] = ti_u32x4{0u, 0u, 0u, 0u};
+  const int64_t n16 = (z.to - z.from) / 16, step = (int64_t)blocks * threads;
+  const int64_t first = (int64_t)block * threads + threadIdx.x;
+  if (z.past) write_vectors<true>(p, n16, first, step);
+  else write_vectors<false>(p, n16, first, step);
   if (block == 0 && (int64_t)threadIdx.x < (z.to - z.from) % 16)
     z.p[z.from + n16 * 16 + threadIdx.x] = 0;
 }
@@ -602,7 +613,7 @@ int embedding_backward_launch(const void* grad, int g_dtype, const void* ids, in
   if (N == 0) {
     if (bytes == 0) return NOVAQ_OK;
     hipLaunchKernelGGL(embedding_zero_kernel, dim3(zero_blocks(bytes, 256)), dim3(256), 0, st,
-                       Zeros{table, 0, bytes});
+                       Zeros{table, 0, bytes, bytes > PAST});
     return check_launch();
   }
   const EmbedPlan p = embed_plan(N, V, D);
@@ -620,7 +631,7 @@ int embedding_backward_launch(const void* grad, int g_dtype, const void* ids, in
       if (rc != NOVAQ_OK) return rc;
       hipLaunchKernelGGL(sort_small_kernel<PER>, dim3(1 + zero_blocks(bytes, 1024)), dim3(1024),
                          SmallSort<PER>::lds, st, ids, bits, V, (int)N, p.passes,
-                         keys[p.passes & 1], pos[p.passes & 1], Zeros{table, 0, bytes});
+                         keys[p.passes & 1], pos[p.passes & 1], Zeros{table, 0, bytes, bytes > PAST});
       return check_launch();
     };
     const int rc = N <= 1024   ? small(std::integral_constant<int, 1>{})
@@ -636,7 +647,7 @@ int embedding_backward_launch(const void* grad, int g_dtype, const void* ids, in
     parts += more;
     const int64_t from = zero_at;
     zero_at = parts == 4 * p.passes ? bytes : bytes / (4 * p.passes) * parts / 16 * 16;
-    return Zeros{table, from, zero_at};
+    return Zeros{table, from, zero_at, bytes > PAST};
   };
   for (int i = 0; i < p.passes && N > SMALL; ++i) {
     const void* raw = i == 0 ? ids : nullptr;

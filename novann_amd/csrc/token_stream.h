@@ -67,11 +67,12 @@ __device__ __forceinline__ tg_u32x4 ts_decode8(uint32_t c0, uint32_t c1) {
   return o;
 }
 
-// Table rows a workgroup, 32 a wave (E codes a chunk, nt tiles of tokens): 128, so
-// that two workgroups share a CU and one computes while the other waits (one row
-// of 4096 x 131072 E4M3: 94 us, with 256 rows 121), but 256 where the tokens'
-// fragments are larger than 128 rows' codes and more rows must share them (37
-// rows of 1024 x 50000 E2M1: 13.6 us, with 128 19.6), while two stages fit.
+// Table rows a workgroup, 32 a wave (E codes a chunk, nt tiles of tokens): 128, which
+// spreads a small table over more CUs (64 rows of 512 x 10000 E4M3, with gradients:
+// 51.8 us, with 256 rows 53.8; of a large table the two are equal), but 256 where
+// the tokens' fragments are larger than 128 rows' codes and more rows must share
+// them (37 rows of 1024 x 50000 E2M1: 20.1 us a call, with 128 27.5), while two
+// stages fit.
 constexpr int stream_rows(int E, int nt) { return E * nt > 32 && E * nt < 128 ? 256 : 128; }
 
 template <int CT, int WT, int NT_>
