@@ -6,13 +6,15 @@
 //
 // The lookup moves one row a token and is bound by memory; 8 elements a lane.
 //
-// The gradient sorts the tokens (stable, radix digits of 9 bits), so that a
-// row's positions lie together in rising order, and sums chunks of 16 (few tokens:
-// 4) sorted entries a wave.  A token with many positions spans several of these chunks:
-// each then leaves its part in the workspace and a last kernel adds a run's
-// parts in order.  No atomics touch floating-point values: the sums' order
-// depends on the tokens alone, and the result is the same bit for bit in every
-// call.  Sums are fp32; the factor is applied once to the whole sum.
+// The gradient of few tokens is one launch in which each token's first position
+// looks for the others (embedding_few_kernel).  For more it sorts the tokens
+// (stable, radix digits of 9 bits), so that a row's positions lie together in
+// rising order, and sums chunks of 16 (up to 4096 tokens: 4) sorted entries a
+// wave.  A token with many positions spans several of these chunks: each then
+// leaves its part in the workspace and a last kernel adds a run's parts in order.
+// No atomics touch floating-point values: the sums' order depends on the tokens
+// alone, and the result is the same bit for bit in every call.  Sums are fp32; the
+// factor is applied once to the whole sum.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -515,9 +517,131 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(
   put_row<OT, VEC>(out + ((int64_t)k * D + c) * OB, sum, factor, accumulate);
 }
 
+// --------------------------------------------------------------------------
+// few tokens, without a sort
+
+// At most so many tokens, and workgroups for them (each reads all tokens), and a
+// table that the caches hold.  The gradient on this path and by the sort: 64 tokens
+// of 512, a table of 10000 rows: 5.6 us and 10.8; 512 of 64, 1000 rows: 4.2 and
+// 11.8; 512 of 784, 30001 rows: 16.7 and 18.9, all of them one token 30.5 and 22.4
+// (its rows then go through one CU).  1000 of 784 would be 21.3 and 20.5, 64 of 4096
+// in a table of 2.1 GB 423 and 395.
+constexpr int FEW = 512, FEW_WORK = 1024;
+static_assert(FEW == 512, "a token a thread");
+constexpr int FEW_ROWS = 1024;  // of the table, at most, of a workgroup that writes zeros
+
+// One launch.  The workgroups x < N take position x and 64 VEC columns each: all tokens are compared with the position's own, and where it is the
+// token's first its positions' rows are summed, every eighth by a wave and the
+// waves' sums in order.  The others take rows of the table: they mark those of
+// the tokens and write zeros to the rest.
+template <int GT, int OT, int VEC>
+__global__ __launch_bounds__(512) void embedding_few_kernel(
+    const uint8_t* __restrict__ grad, const void* __restrict__ ids, int bits, int N, int64_t V,
+    int64_t D, float factor, int accumulate, int rows, FastDiv by_per,
+    uint8_t* __restrict__ out) {
+  constexpr int GB = GT == F32 ? 4 : 2, OB = OT == F32 ? 4 : 2;
+  __shared__ union {
+    struct {
+      float part[8][64 * VEC];
+      uint64_t mask[8];
+      uint16_t list[FEW];
+    };
+    uint32_t marked[FEW_ROWS / 32];
+  } sh;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t t = tid < N ? token_at(ids, bits, tid) : -1;
+  if ((int)blockIdx.x >= N) {
+    const int64_t r0 = ((int64_t)(blockIdx.x - N) * gridDim.y + blockIdx.y) * rows;
+    if (r0 >= V) return;
+    const int n = (int)min((int64_t)rows, V - r0);
+    for (int i = tid; i < FEW_ROWS / 32; i += 512) sh.marked[i] = 0;
+    __syncthreads();
+    if (t >= r0 && t < r0 + n) atomicOr(&sh.marked[(t - r0) >> 5], 1u << ((t - r0) & 31));
+    __syncthreads();
+    // words of 16 bytes, or what 4 elements or 1 are
+    using W = std::conditional_t<
+        VEC == 8 || (VEC == 4 && OB == 4), ti_u32x4,
+        std::conditional_t<VEC == 4, ti_u32x2, std::conditional_t<OB == 4, uint32_t, uint16_t>>>;
+    const uint32_t per = (uint32_t)(D * OB / (int)sizeof(W)), all = per * (uint32_t)n;
+    W* p = reinterpret_cast<W*>(out + r0 * D * OB);
+    const W zero = {};
+    for (uint32_t i0 = tid; i0 < all; i0 += 4 * 512) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t i = i0 + 512 * x, r = fdiv(min(i, all - 1), by_per);
+        if (i < all && !(sh.marked[r >> 5] >> (r & 31) & 1)) p[i] = zero;
+      }
+    }
+    return;
+  }
+  const int at = (int)blockIdx.x;
+  const int64_t mine = token_at(ids, bits, at);
+  if (mine < 0 || mine >= V) return;
+  const uint64_t here = __ballot(t == mine);
+  if (lane == 0) sh.mask[wave] = here;
+  __syncthreads();
+  // the positions in rising order
+  int count = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const uint64_t m = sh.mask[w];
+    // (one before `at`: that one's workgroup sums the row)
+    if (w < at / 64 ? m != 0 : w == at / 64 && (m & ((1ull << (at & 63)) - 1)) != 0) return;
+    if (w < wave) before += __popcll(m);
+    count += __popcll(m);
+  }
+  if (t == mine) sh.list[before + __popcll(here & ((1ull << lane) - 1))] = (uint16_t)tid;
+  __syncthreads();
+  const int64_t c = (int64_t)blockIdx.y * 64 * VEC + lane * VEC;
+  float sum[VEC];
+#pragma unroll
+  for (int x = 0; x < VEC; ++x) sum[x] = 0.0f;
+  if (c < D)
+    for (int e = wave; e < count; e += 64) {
+      float v[8][VEC];  // (all eight loaded before the first is added)
+#pragma unroll
+      for (int y = 0; y < 8; ++y)
+        loadv<GT, VEC, true>(grad + ((int64_t)sh.list[min(e + 8 * y, count - 1)] * D + c) * GB,
+                             v[y]);
+#pragma unroll
+      for (int y = 0; y < 8; ++y)
+        if (e + 8 * y < count) {
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) sum[x] += v[y][x];
+        }
+    }
+  if (count > 1) {
+#pragma unroll
+    for (int x = 0; x < VEC; ++x) sh.part[wave][lane * VEC + x] = sum[x];
+    __syncthreads();
+    if (wave == 0)
+      for (int w = 1; w < min(8, count); ++w)
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) sum[x] += sh.part[w][lane * VEC + x];
+  }
+  if (wave == 0 && c < D)
+    put_row<OT, VEC>(out + (mine * D + c) * OB, sum, factor, accumulate);
+}
+
+template <int GT, int OT, int VEC>
+int few_launch(const uint8_t* grad, const void* ids, int bits, int64_t N, int64_t V, int64_t D,
+               float factor, int accumulate, uint8_t* out, hipStream_t st) {
+  constexpr int OB = OT == F32 ? 4 : 2;
+  constexpr int word = VEC == 8 ? 16 : VEC * OB;
+  const int cols = (int)((D + 64 * VEC - 1) / (64 * VEC));
+  const int rows = (int)std::min<int64_t>((V + 1023) / 1024, FEW_ROWS);
+  const int64_t zeros = accumulate ? 0 : ((V + rows - 1) / rows + cols - 1) / cols;
+  hipLaunchKernelGGL((embedding_few_kernel<GT, OT, VEC>), dim3((unsigned)(N + zeros), cols),
+                     dim3(512), 0, st, grad, ids, bits, (int)N, V, D, factor, accumulate, rows,
+                     fast_div((uint32_t)(D * OB / word)), out);
+  return check_launch();
+}
+
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct EmbedPlan {
+  bool few;
   int passes, per, blocks, chunk;
   int64_t chunks;
   size_t hist, keys[2], pos[2], head, tail, total;
@@ -525,6 +649,8 @@ struct EmbedPlan {
 
 EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D) {
   EmbedPlan p{};
+  const int64_t width = D % 8 == 0 ? 512 : D % 4 == 0 ? 256 : 64;  // columns a workgroup
+  p.few = N <= FEW && N * ((D + width - 1) / width) <= FEW_WORK && V * D <= PAST / 4;
   int bits = 1;
   while (bits < 33 && ((int64_t)1 << bits) <= V) ++bits;  // keys 0 .. V
   p.passes = (bits + DIGIT - 1) / DIGIT;
@@ -569,11 +695,17 @@ int sums(const EmbedPlan& p, const uint8_t* grad, const uint32_t* keys, const ui
 }
 
 template <int GT, int OT>
-int sums_by_width(const EmbedPlan& p, const void* grad, const uint32_t* keys, const uint32_t* pos,
+int sums_by_width(const EmbedPlan& p, const void* grad, const void* ids, int bits,
+                  const uint32_t* keys, const uint32_t* pos,
                   int64_t N, int64_t V, int64_t D, float factor, int accumulate, uint8_t* ws,
                   void* out, hipStream_t st) {
   const uint8_t* g = static_cast<const uint8_t*>(grad);
   uint8_t* o = static_cast<uint8_t*>(out);
+  if (p.few) {
+    if (D % 8 == 0) return few_launch<GT, OT, 8>(g, ids, bits, N, V, D, factor, accumulate, o, st);
+    if (D % 4 == 0) return few_launch<GT, OT, 4>(g, ids, bits, N, V, D, factor, accumulate, o, st);
+    return few_launch<GT, OT, 1>(g, ids, bits, N, V, D, factor, accumulate, o, st);
+  }
   if (D % 8 == 0) return sums<GT, OT, 8>(p, g, keys, pos, N, V, D, factor, accumulate, ws, o, st);
   if (D % 4 == 0) return sums<GT, OT, 4>(p, g, keys, pos, N, V, D, factor, accumulate, ws, o, st);
   return sums<GT, OT, 1>(p, g, keys, pos, N, V, D, factor, accumulate, ws, o, st);
@@ -622,7 +754,7 @@ int embedding_backward_launch(const void* grad, int g_dtype, const void* ids, in
                        reinterpret_cast<uint32_t*>(ws + p.keys[1])};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + p.pos[0]),
                       reinterpret_cast<uint32_t*>(ws + p.pos[1])};
-  if (N <= SMALL) {
+  if (!p.few && N <= SMALL) {
     auto small = [&](auto per) -> int {
       constexpr int PER = decltype(per)::value;
       static DeviceFlags raised;
@@ -668,7 +800,7 @@ int embedding_backward_launch(const void* grad, int g_dtype, const void* ids, in
   const uint32_t* k = keys[p.passes & 1];
   const uint32_t* q = pos[p.passes & 1];
 #define NOVAQ_SUMS(G, O) \
-  return sums_by_width<G, O>(p, grad, k, q, N, V, D, factor, accumulate, ws, out, st)
+  return sums_by_width<G, O>(p, grad, ids, bits, k, q, N, V, D, factor, accumulate, ws, out, st)
 #define NOVAQ_SUMS_TO(G)                  \
   if (o_dtype == F32) NOVAQ_SUMS(G, F32); \
   if (o_dtype == F16) NOVAQ_SUMS(G, F16); \

@@ -101,6 +101,22 @@ def test_gradient_orders(kind, n):
     check_gradient(t, g, got, V, 1.0)
 
 
+@pytest.mark.parametrize("n,V,D", [(512, 300, 72), (513, 300, 72), (512, 90, 1032), (300, 700, 130),
+                                   (400, 700, 130), (1000, 64, 16), (3000, 5000, 40),
+                                   (16, 70000, 512), (600, 70000, 512)])
+def test_gradient_of_few_tokens_and_large_tables(n, V, D):
+    rng = np.random.default_rng(n + D)
+    g = floats(rng, (n, D), "bf16")
+    for t in (np.full(n, V - 1), rng.integers(-1, V + 1, n), rng.integers(0, 3, n) * (V // 3),
+              np.arange(n)[::-1] % V):
+        out = torch.full((V, D), float("nan"), device="cuda")
+        F.embedding_backward(g, torch.from_numpy(t.copy()).cuda(), (V, D), out=out)
+        check_gradient(t, g, out, V, 1.0)
+        twice = F.embedding_backward(g, torch.from_numpy(t.copy()).cuda(), (V, D), out=out.clone(),
+                                     accumulate=True)
+        assert torch.equal(twice, out + out)
+
+
 def test_gradient_is_the_difference_of_the_lookup():
     rng = np.random.default_rng(3)
     V, D, n = 40, 12, 100
