@@ -573,6 +573,8 @@ struct GradsJob {
   const float* scal;
   float inv_pscale;
   uint8_t* gw;
+  float* wsums;            // where grad_W's K is split: fp32 sums as above, of the piece
+  int wsplits;
   int xtm, xtn, wtm, wtn;  // tiles; wtm 0: no grad_W
 };
 
@@ -619,23 +621,42 @@ __device__ __forceinline__ void dx_tile(const GradsJob& g, int b, uint8_t* lds) 
   }
 }
 
-// grad_W's rows of one piece: P^T (vc x N) times x (N x D), times g / pscale.
+// A product rounded to fp32 before it is converted: the compiler makes one mixed
+// instruction of a multiply and a conversion to f16, and a gradient in f16 would
+// then differ from the fp32 one's rounding at ties.
+__device__ __forceinline__ float rounded(float y) {
+  asm("" : "+v"(y));
+  return y;
+}
+
+// grad_W's rows of one piece: P^T (vc x N) times x (N x D), times g / pscale, as
+// OT; or (OT SUMS), where its K is split, this split's fp32 sums.
+constexpr int SUMS = -1;
 template <int CT, int OT, class G>
 __device__ __forceinline__ void dw_tile(const GradsJob& g, int b, uint8_t* lds) {
-  int mi, ni;
+  int mi, ni, split = 0;
+  if constexpr (OT == SUMS) split = b / (g.wtm * g.wtn), b %= g.wtm * g.wtn;
   tile_of(b, g.wtm, g.wtn, mi, ni);
   const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN, D = g.D, vc = g.vc;
+  int k0 = 0, k1 = g.nblocks;
+  if constexpr (OT == SUMS) {
+    k0 = (int)((int64_t)g.nblocks * split / g.wsplits);
+    k1 = (int)((int64_t)g.nblocks * (split + 1) / g.wsplits);
+  }
   typename G::Acc acc;
-  G::run(acc, g.pt, g.x, m0, n0, g.N, 0, g.nblocks, lds);
-  const float a = g.scal[0] * g.inv_pscale;
+  G::run(acc, g.pt, g.x, m0, n0, g.N, k0, k1, lds);
+  const float a = OT == SUMS ? 1.0f : g.scal[0] * g.inv_pscale;
   uint8_t* out = g.gw;
+  int64_t ld = D;
+  if constexpr (OT == SUMS) out = (uint8_t*)(g.wsums + split * vc * g.dp), ld = g.dp;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
   const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
-  constexpr int OB = OT == F32 ? 4 : 2;
+  constexpr bool F = OT == F32 || OT == SUMS;
+  constexpr int OB = F ? 4 : 2;
   const int rows = (int)min((int64_t)G::BM, vc - m0);
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-      out + m0 * D * OB, (short)0, rows * (int)D * OB, 0x00020000);
-  const uint32_t pitch = (uint32_t)D * OB;
+      out + m0 * ld * OB, (short)0, rows * (int)ld * OB, 0x00020000);
+  const uint32_t pitch = (uint32_t)ld * OB;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
     const int64_t d = n0 + wn + 16 * j + (lane & 15);
@@ -645,8 +666,8 @@ __device__ __forceinline__ void dw_tile(const GradsJob& g, int b, uint8_t* lds) 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const uint32_t o = at + (16 * i + r) * pitch;
-        const float y = acc[i][j][r] * a;
-        if constexpr (OT == F32) __builtin_amdgcn_raw_buffer_store_b32(f2u(y), rs, o, 0, 0);
+        const float y = OT == F16 ? rounded(acc[i][j][r] * a) : acc[i][j][r] * a;
+        if constexpr (F) __builtin_amdgcn_raw_buffer_store_b32(f2u(y), rs, o, 0, 0);
         else
           __builtin_amdgcn_raw_buffer_store_b16((uint16_t)tg_pack2<OT>(y, 0.0f), rs, o, 0, 0);
       }
@@ -665,11 +686,11 @@ __global__ __launch_bounds__(GX::NTH, 1) void loss_grads_kernel(GradsJob g) {
   else dw_tile<CT, OT, GW>(g, blockIdx.x - nx, lds);
 }
 
-// grad_x = the splits' sums times g s / pscale, as OT: four columns a thread, or,
-// with SHARE, four threads (one in each wave) that take every fourth split each and
+// A gradient = its splits' sums times g s / pscale, as OT (rows of ignored targets 0;
+// grad_W has neither s nor targets): four columns a thread, or, with SHARE, four threads (one in each wave) that take every fourth split each and
 // add up in their order.
 template <int OT, bool SHARE>
-__global__ __launch_bounds__(256) void loss_dx_store_kernel(const float* __restrict__ sums,
+__global__ __launch_bounds__(256) void loss_sums_store_kernel(const float* __restrict__ sums,
                                                             int splits, int64_t N, int64_t dp,
                                                             int64_t D,
                                                             const float* __restrict__ scal,
@@ -704,9 +725,9 @@ __global__ __launch_bounds__(256) void loss_dx_store_kernel(const float* __restr
       __syncthreads();
     }
     if (from > 0 || q0 + unit >= total || c >= D) continue;
-    const bool none = targets[n] == T_NONE;
+    const bool none = targets && targets[n] == T_NONE;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = none ? 0.0f : v[i] * a;
+    for (int i = 0; i < 4; ++i) v[i] = none ? 0.0f : rounded(v[i] * a);
     const int64_t e = n * D + c;
     if constexpr (OT == F32) {
       float* o = reinterpret_cast<float*>(out) + e;
@@ -736,10 +757,10 @@ struct LossPlan {
   int64_t piece;     // vocabulary rows a piece (a multiple of 256)
   int64_t vtiles;    // tiles of the vocabulary
   bool big_l, big_g;  // 256 x 256 tiles for the logits, the gradients
-  int splits;        // of grad_x's K
+  int splits, wsplits;  // of grad_x's K, of grad_W's
   bool stream;       // forward: the table read as stored, for few tokens
   int64_t frag_bytes;
-  size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, total;
+  size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, wsums, total;
 };
 
 // Time (us) of a round of tiles of 256 x 256 (a CU runs one workgroup of 8 waves) or
@@ -776,34 +797,41 @@ double best_us(int64_t M, int64_t N, int64_t K) {
 struct GradsPlan {
   double us;
   bool big;
-  int splits;
+  int splits, wsplits;
 };
 GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece, int most = 64) {
   const int64_t cus = device_cu_count();
-  GradsPlan best{0.0, false, 1};
+  GradsPlan best{0.0, false, 1, 1};
   const int64_t kx = (piece + 63) / 64, kw = (N + 63) / 64;
   for (int big = 0; big < 2; ++big) {
     const int64_t e = big ? 256 : 128, slots = big ? cus : 2 * cus, cols = (D + e - 1) / e;
     const int64_t nw = ((piece + e - 1) / e) * cols;
-    for (int splits = 1; splits <= most && (splits == 1 || kx / splits >= 4); splits *= 2) {
-      const int64_t nx = ((N + e - 1) / e) * cols * splits;
-      const double tx = round_us(big != 0, (double)((kx + splits - 1) / splits), true);
-      const double tw = round_us(big != 0, (double)kw, true);
-      // two groups of slots: those with one tile of grad_x more than the others
-      int64_t count[2] = {nx % slots, slots - nx % slots}, left = nw;
-      double at[2] = {(double)(nx / slots + 1) * tx, (double)(nx / slots) * tx};
-      double end = count[0] ? at[0] : at[1];
-      while (left > 0) {
-        const int g = count[0] == 0 || at[1] <= at[0] ? 1 : 0;
-        at[g] += tw;
-        end = std::max(end, at[g]);
-        left -= count[g];
+    // (grad_W's K, the tokens, is split where its tiles leave slots empty; each split's
+    // sums cost a store, and a launch joins them.  The backward of 32768 x 512 x 256
+    // classes: 120 us, unsplit 451; of 8192 x 1024 x 848, such as the last piece of
+    // 50000 classes is: 103 and 159)
+    for (int wsplits = 1; wsplits == 1 || (nw * wsplits <= 2 * slots && kw / wsplits >= 4);
+         wsplits *= 2)
+      for (int splits = 1; splits <= most && (splits == 1 || kx / splits >= 4); splits *= 2) {
+        const int64_t nx = ((N + e - 1) / e) * cols * splits;
+        const double tx = round_us(big != 0, (double)((kx + splits - 1) / splits), true);
+        const double tw = round_us(big != 0, (double)((kw + wsplits - 1) / wsplits), true);
+        // two groups of slots: those with one tile of grad_x more than the others
+        int64_t count[2] = {nx % slots, slots - nx % slots}, left = nw * wsplits;
+        double at[2] = {(double)(nx / slots + 1) * tx, (double)(nx / slots) * tx};
+        double end = count[0] ? at[0] : at[1];
+        while (left > 0) {
+          const int g = count[0] == 0 || at[1] <= at[0] ? 1 : 0;
+          at[g] += tw;
+          end = std::max(end, at[g]);
+          left -= count[g];
+        }
+        if (!big && nx + nw * wsplits <= cus) end *= LONE;
+        // (the splits' sums: written and read once, a few at a time)
+        double us = end + (double)splits * ((double)N * (double)D * 8.0 / 4e6 + 0.1);
+        if (wsplits > 1) us += (double)wsplits * ((double)piece * (double)D * 8.0 / 4e6 + 0.1) + 5.0;
+        if (best.us == 0.0 || us < best.us) best = GradsPlan{us, big != 0, splits, wsplits};
       }
-      if (!big && nx + nw <= cus) end *= LONE;
-      // (the splits' sums: written and read once, a few at a time)
-      const double us = end + (double)splits * ((double)N * (double)D * 8.0 / 4e6 + 0.1);
-      if (best.us == 0.0 || us < best.us) best = GradsPlan{us, big != 0, splits};
-    }
   }
   return best;
 }
@@ -870,6 +898,7 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
     const GradsPlan g = grads_plan(N, D, p.piece);
     p.big_g = g.big;
     p.splits = g.splits;
+    p.wsplits = g.wsplits;
   }
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -885,6 +914,12 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
     p.f = take((size_t)N * 4);
     p.P = take((size_t)N * row_pitch(p.piece) * 2);
     p.sums = take((size_t)p.splits * N * p.dp * 4);
+    auto parts = [&](int splits, int64_t rows) {
+      return splits > 1 ? (size_t)splits * rows * p.dp * 4 : 0;
+    };
+    const int64_t rest = V % p.piece;
+    const size_t last = V > p.piece && rest ? parts(grads_plan(N, D, rest, p.splits).wsplits, rest) : 0;
+    p.wsums = take(std::max(parts(p.wsplits, std::min(p.piece, V)), last));
   } else {
     p.stats = take((size_t)N * p.vtiles * 8);
     p.tlogit = take((size_t)N * 4);
@@ -997,6 +1032,22 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
   return check_launch();
 }
 
+template <int OT>
+int store_sums(const float* sums, int splits, int64_t rows, int64_t dp, int64_t D,
+               const float* scal, const float* w_scale, float inv, const int* targets, void* out,
+               hipStream_t st) {
+  auto go = [&](auto share) {
+    constexpr bool SHARE = decltype(share)::value;
+    const int64_t units = SHARE ? 64 : 256;
+    const dim3 grid((unsigned)std::min<int64_t>((rows * (dp / 4) + units - 1) / units, 8192));
+    hipLaunchKernelGGL((loss_sums_store_kernel<OT, SHARE>), grid, dim3(256), 0, st, sums, splits,
+                       rows, dp, D, scal, w_scale, inv, targets, out);
+  };
+  if (splits >= 8) go(std::true_type{});
+  else go(std::false_type{});
+  return check_launch();
+}
+
 template <int CT>
 int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
              int w_dtype, const float* w_scale, int64_t V, const void* ids, int bits,
@@ -1031,7 +1082,7 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
     const bool rest = v0 > 0 && vc < p.piece;
     const bool big_l = rest ? large_tiles(vc, N, D) : p.big_l;
     const GradsPlan gp = rest ? grads_plan(N, D, vc, p.splits)
-                              : GradsPlan{0.0, p.big_g, p.splits};
+                              : GradsPlan{0.0, p.big_g, p.splits, p.wsplits};
     auto prob = [&](auto g) -> int {
       using G = decltype(g);
       const int tm = (int)(vp / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
@@ -1048,7 +1099,8 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
       constexpr int OT = decltype(ot)::value;
       GradsJob j{TokenOp{P, N, pp}, TokenOp{P, vp, pp}, ow, ox, N, D, vc, (int)(vp / 64),
                  (int)((N + 63) / 64), gp.splits, v0 == 0 ? 1 : 0, sums, p.dp, scal, inv,
-                 static_cast<uint8_t*>(gw) + v0 * D * (OT == F32 ? 4 : 2), 0, 0, 0, 0};
+                 static_cast<uint8_t*>(gw) + v0 * D * (OT == F32 ? 4 : 2),
+                 reinterpret_cast<float*>(ws + p.wsums), gp.wsplits, 0, 0, 0, 0};
       if (gx) {
         j.xtm = (int)((N + GX::BM - 1) / GX::BM);
         j.xtn = (int)((D + GX::BN - 1) / GX::BN);
@@ -1059,9 +1111,13 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
         j.wtm = (int)((vc + GW::BM - 1) / GW::BM);
         j.wtn = (int)((D + GW::BN - 1) / GW::BN);
       }
-      const int64_t tiles = (int64_t)j.xtm * j.xtn * j.splits + (int64_t)j.wtm * j.wtn;
-      NOVAQ_LAUNCH((loss_grads_kernel<CT, OT, GX, GW>), tiles, GX, st, j);
-      return NOVAQ_OK;
+      const int64_t tiles = (int64_t)j.xtm * j.xtn * j.splits + (int64_t)j.wtm * j.wtn * j.wsplits;
+      if (!gw || gp.wsplits == 1) {
+        NOVAQ_LAUNCH((loss_grads_kernel<CT, OT, GX, GW>), tiles, GX, st, j);
+        return NOVAQ_OK;
+      }
+      NOVAQ_LAUNCH((loss_grads_kernel<CT, SUMS, GX, GW>), tiles, GX, st, j);
+      return store_sums<OT>(j.wsums, gp.wsplits, vc, p.dp, D, scal, nullptr, inv, nullptr, j.gw, st);
     };
     auto grads_to = [&](auto ot) -> int {
       return gp.big ? grads(ot, TokenGemm<CT, false, true, 128, 64, 4>{},
@@ -1074,24 +1130,14 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
                            : grads_to(std::integral_constant<int, BF16>{});
     if (rc != NOVAQ_OK) return rc;
   }
-  if (gx) {
-    auto store = [&](auto ot, auto share) {
-      constexpr bool SHARE = decltype(share)::value;
-      const int64_t units = SHARE ? 64 : 256;
-      const dim3 grid((unsigned)std::min<int64_t>((N * (p.dp / 4) + units - 1) / units, 8192));
-      hipLaunchKernelGGL((loss_dx_store_kernel<decltype(ot)::value, SHARE>), grid, dim3(256), 0, st,
-                         sums, p.splits, N, p.dp, D, scal, w_scale, inv, targets, gx);
-    };
-    auto to = [&](auto ot) {
-      if (p.splits >= 8) store(ot, std::true_type{});
-      else store(ot, std::false_type{});
-    };
-    if (x_dtype == F32) to(std::integral_constant<int, F32>{});
-    else if (x_dtype == F16) to(std::integral_constant<int, F16>{});
-    else to(std::integral_constant<int, BF16>{});
-    rc = check_launch();
-  }
-  return rc;
+  if (!gx) return rc;
+  auto store = [&](auto ot) {
+    return store_sums<decltype(ot)::value>(sums, p.splits, N, p.dp, D, scal, w_scale, inv, targets,
+                                           gx, st);
+  };
+  return x_dtype == F32   ? store(std::integral_constant<int, F32>{})
+         : x_dtype == F16 ? store(std::integral_constant<int, F16>{})
+                          : store(std::integral_constant<int, BF16>{});
 }
 
 #undef NOVAQ_LAUNCH

@@ -309,3 +309,18 @@ def test_large_products(N, D, V, wdtype, xdtype):
         bound = rel * size + HALF_ULP[xdtype] * 1.01 * want.abs() + HALF_MIN[xdtype] + floor * few
         bad = (got.double() - want).abs() > bound
         assert not bad.any(), (int(bad.sum()), bad.nonzero()[:3])
+
+
+@pytest.mark.parametrize("N,D,V,wdtype,xdtype", [(8192, 96, 300, "bf16", "bf16"),
+                                                 (20000, 200, 70, "e5m2", "f16"),
+                                                 (4100, 1030, 900, "e4m3", "bf16")])
+def test_many_tokens_of_few_classes(N, D, V, wdtype, xdtype):
+    """grad_W's products are split over the tokens; its types are roundings of one sum."""
+    test_large_products(N, D, V, wdtype, xdtype)
+    x, w, _, t = inputs(N, D, V, wdtype, xdtype, seed=6)
+    ids = torch.from_numpy(t).cuda()
+    _, lse = F.linear_cross_entropy(x, w, ids, extras=True)
+    full = F.linear_cross_entropy_backward(x, w, ids, lse, weight_grad_dtype="f32")[1]
+    for name in ("bf16", "f16"):
+        got = F.linear_cross_entropy_backward(x, w, ids, lse, weight_grad_dtype=name)[1]
+        assert torch.equal(got, full.to(got.dtype))
