@@ -5,7 +5,9 @@ per-tensor amax scaling, and the Linear / Conv2d forward products on
 quantized weights, all as HIP kernels for gfx950 in ``libnovaq.so`` behind
 the C ABI of ``include/novaq.h``.  This package is the host side: it mirrors
 NovaNN's ``functional.linear`` / ``functional.conv2d`` and its ``Linear`` /
-``Conv2d`` layers.
+``Conv2d`` layers.  For token models it adds ``functional.embedding``,
+``functional.linear_cross_entropy`` (with their backward functions and layers)
+and ``optim.clip_grad_norm``.
 """
 from . import _lib
 from ._lib import LIB_PATH, load

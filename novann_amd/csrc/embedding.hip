@@ -29,7 +29,8 @@ namespace {
 
 // A row per token, 8 elements a thread and four such units a thread, whose ids
 // and then codes are all loaded before the first store; a token outside the table
-// gives a row of NaN.
+// gives a row of NaN.  32768 tokens of 1024 E4M3 to bf16: 17 us, 67 MB written and
+// 19 read at 5.0 TB/s.
 template <int ST, int OT, bool VEC>
 __global__ __launch_bounds__(256) void embedding_kernel(const void* __restrict__ ids, int bits,
                                                         const uint8_t* __restrict__ table,
@@ -107,7 +108,7 @@ constexpr int SMALL = 4096;
 
 // The rows that get no gradient must be zero: the sort's launches, which use few
 // workgroups, carry the table's zeros in their other ones (32768 tokens, a table
-// of 205 MB: 31 us of sorting and 28 of writing one after the other, 46 together).
+// of 205 MB: 31 us of sorting and 28 of writing one after the other, 44 together).
 struct Zeros {
   uint8_t* p;
   int64_t from, to;  // bytes, multiples of 16 but for the table's end
@@ -467,8 +468,9 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(
 // sums are added in the waves' order.
 template <int OT, int VEC>
 __global__ __launch_bounds__(512) void embedding_join_kernel(
-    const uint32_t* __restrict__ keys, int N, int CHUNK, int64_t V, int64_t D, float factor, int accumulate,
-    const float* __restrict__ head, const float* __restrict__ tail, uint8_t* __restrict__ out) {
+    const uint32_t* __restrict__ keys, int N, int CHUNK, int64_t V, int64_t D, float factor,
+    int accumulate, const float* __restrict__ head, const float* __restrict__ tail,
+    uint8_t* __restrict__ out) {
   constexpr int OB = OT == F32 ? 4 : 2;
   __shared__ float part[8][64 * VEC];
   const int chunk = blockIdx.x, lane = threadIdx.x & 63;
@@ -530,10 +532,11 @@ constexpr int FEW = 512, FEW_WORK = 1024;
 static_assert(FEW == 512, "a token a thread");
 constexpr int FEW_ROWS = 1024;  // of the table, at most, of a workgroup that writes zeros
 
-// One launch.  The workgroups x < N take position x and 64 VEC columns each: all tokens are compared with the position's own, and where it is the
-// token's first its positions' rows are summed, every eighth by a wave and the
-// waves' sums in order.  The others take rows of the table: they mark those of
-// the tokens and write zeros to the rest.
+// One launch.  The workgroups x < N take position x and 64 VEC columns each: all
+// tokens are compared with the position's own, and where it is the token's first
+// its positions' rows are summed, every eighth by a wave and the waves' sums in
+// order.  The others take rows of the table: they mark those of the tokens and
+// write zeros to the rest.
 template <int GT, int OT, int VEC>
 __global__ __launch_bounds__(512) void embedding_few_kernel(
     const uint8_t* __restrict__ grad, const void* __restrict__ ids, int bits, int N, int64_t V,
