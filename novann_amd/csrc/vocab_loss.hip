@@ -18,7 +18,8 @@
 // backward computes a piece's logits again, stores P of that piece in 16 bits
 // and multiplies it with the piece (grad_x, summed over the pieces in fp32)
 // and with x (grad_W's rows of the piece): 8 N V D operations for both, 6 of
-// them needed by any method.
+// them needed by any method.  Where the logits are so few that their tiles leave
+// CUs idle, the products' K is split and the fp32 parts stored (loss_logits_kernel).
 //
 // Types: the products run in 16 bits, f16 where x is f16 and bf16 otherwise;
 // FP8 and FP4 codes are exact in both, fp32 x or W and 16-bit W of the other
@@ -564,6 +565,110 @@ __global__ __launch_bounds__(G::NTH, 1) void loss_prob_kernel(
   }
 }
 
+// --------------------------------------------------------------------------
+// few tiles of logits: their K split over the CUs
+
+// This split's fp32 products of one tile, at sums[split][n][v] (pitch vp).
+template <int CT, class G>
+__global__ __launch_bounds__(G::NTH, 1) void loss_logits_kernel(TokenOp w, TokenOp x, int64_t dp,
+                                                                int64_t N, int splits,
+                                                                float* __restrict__ sums,
+                                                                int64_t vp, int tm, int tn) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int mi, ni;
+  const int split = blockIdx.x / (tm * tn), blocks = (int)(dp / 64);
+  tile_of(blockIdx.x % (tm * tn), tm, tn, mi, ni);
+  const int64_t m0 = (int64_t)mi * G::BM, n0 = (int64_t)ni * G::BN;
+  typename G::Acc acc;
+  G::run(acc, w, x, m0, n0, dp, blocks * split / splits, blocks * (split + 1) / splits, lds);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
+  const int wm = (wave % G::WGM) * G::WM, wn = (wave / G::WGM) * G::WN;
+#pragma unroll
+  for (int j = 0; j < G::NT; ++j) {
+    const int64_t n = n0 + wn + 16 * j + (lane & 15);
+    float* p = sums + ((int64_t)split * N + n) * vp + m0 + wm + 4 * q;
+    if (n < N) {
+#pragma unroll
+      for (int i = 0; i < G::MT; ++i) *reinterpret_cast<tg_f32x4*>(p + 16 * i) = acc[i][j];
+    }
+  }
+}
+
+// Four products of token n from v on, their splits added in order.
+__device__ __forceinline__ tg_f32x4 split_sum(const float* sums, int splits, int64_t N, int64_t vp,
+                                              int64_t n, int64_t v) {
+  tg_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) {
+    const tg_f32x4 o = *reinterpret_cast<const tg_f32x4*>(sums + ((int64_t)k * N + n) * vp + v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] += o[i];
+  }
+  return s;
+}
+
+// A token's lse and loss from its split logits, one workgroup.
+__global__ __launch_bounds__(256) void loss_rows_kernel(const float* __restrict__ sums, int splits,
+                                                        int64_t N, int64_t V, int64_t vp,
+                                                        const float* __restrict__ w_scale,
+                                                        const int* __restrict__ targets,
+                                                        float* __restrict__ lse, float* loss) {
+  __shared__ float2 part[4];
+  __shared__ float tlogit;
+  const int64_t n = blockIdx.x;
+  const int t = targets[n];
+  const float c2 = logit_factor(w_scale);
+  float2 a = {-INFINITY, 0.0f};
+  for (int64_t v = threadIdx.x * 4; v < V; v += 1024) {
+    const tg_f32x4 s = split_sum(sums, splits, N, vp, n, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (v + i >= V) continue;
+      a = join_stats(a, float2{s[i] * c2, 1.0f});
+      if (v + i == t) tlogit = s[i] * c2;
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) a = across(a, d);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
+  __syncthreads();
+  if (threadIdx.x > 0) return;
+  for (int w = 1; w < 4; ++w) a = join_stats(a, part[w]);
+  const float l2 = a.x + log2f(a.y);
+  lse[n] = l2 * LN2;
+  loss[n] = t == T_NONE ? 0.0f : t == T_BAD ? u2f(0x7FC00000u) : (l2 - tlogit) * LN2;
+}
+
+// The backward's P (as in loss_prob_kernel) from the split logits: 8 classes a
+// thread, a token a grid row.
+template <int CT>
+__global__ __launch_bounds__(256) void loss_prob_rows_kernel(
+    const float* __restrict__ sums, int splits, int64_t N, int64_t V, int64_t vp,
+    const float* __restrict__ w_scale, const int* __restrict__ targets,
+    const float* __restrict__ f, const float* __restrict__ lse, float pscale,
+    uint16_t* __restrict__ P, int64_t pitch) {
+  const int64_t n = blockIdx.y, v = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (v >= vp) return;
+  const int t = targets[n];
+  const float c2 = logit_factor(w_scale), fn = f[n] * pscale;
+  const float l2 = t != T_NONE ? lse[n] * LOG2E : 0.0f;
+  tg_u32x4 o = {0, 0, 0, 0};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (v + 4 * h >= V) break;
+    tg_f32x4 s = split_sum(sums, splits, N, vp, n, v + 4 * h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = v + 4 * h + i;
+      const float e = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -l2)) - (at == t ? 1.0f : 0.0f);
+      s[i] = at < V ? e * fn : 0.0f;
+    }
+    o[2 * h] = tg_pack2<CT>(s[0], s[1]);
+    o[2 * h + 1] = tg_pack2<CT>(s[2], s[3]);
+  }
+  *reinterpret_cast<tg_u32x4*>(P + n * pitch + v) = o;
+}
+
 // The gradients' products of one piece.
 struct GradsJob {
   TokenOp p, pt;        // P: N rows of K; and as K-strided rows of the vocabulary
@@ -764,9 +869,10 @@ struct LossPlan {
   int64_t vtiles;    // tiles of the vocabulary
   bool big_l, big_g;  // 256 x 256 tiles for the logits, the gradients
   int splits, wsplits;  // of grad_x's K, of grad_W's
+  int lsplits;       // of the logits' K (1: their tiles are not stored)
   bool stream;       // forward: the table read as stored, for few tokens
   int64_t frag_bytes;
-  size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, wsums, total;
+  size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, wsums, lsums, total;
 };
 
 // Time (us) of a round of tiles of 256 x 256 (a CU runs one workgroup of 8 waves) or
@@ -876,6 +982,24 @@ int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, boo
   return best;
 }
 
+// The splits of the logits' K where their tiles leave CUs idle, by the same model:
+// each split's sums cost a store and a load, and a launch joins them (backward of
+// 103 x 2560 x 1280 classes: 57 us, split 38; of 1 x 4096 x 1280: 67 and 33; forward
+// of 300 x 4096 x 2000: 54 and 29).
+int logit_splits(int64_t N, int64_t V, int64_t D, double* us) {
+  const int64_t cus = device_cu_count(), blocks = (D + 63) / 64;
+  const int64_t tiles = ((V + 127) / 128) * ((N + 127) / 128);
+  *us = best_us(V, N, D);
+  int best = 1;
+  for (int s = 2; s <= 64 && blocks / s >= 2 && tiles * s <= 2 * cus; s *= 2) {
+    const double round = round_us(false, (double)((blocks + s - 1) / s));
+    const double t = (tiles * s <= cus ? LONE * round : round) + 5.0 +
+                     s * ((double)N * (double)V * 8.0 / 4e6 + 0.3);
+    if (t < *us) *us = t, best = s;
+  }
+  return best;
+}
+
 int stream_tiles(int64_t N) { return N <= 32 ? 1 : N <= 64 ? 2 : 4; }
 
 LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bool backward) {
@@ -891,10 +1015,24 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   p.piece = loss_piece(N, D, p.dp, V, p.copy_w, backward);
   p.big_l = large_tiles(p.piece, N, D);
   p.vtiles = (V + (p.big_l ? 255 : 127)) / (p.big_l ? 256 : 128);
+  double logits_us = 0.0;
+  p.lsplits = p.piece >= V ? logit_splits(N, V, D, &logits_us) : 1;
   // up to 128 rows of x, codes whose rows are whole 16-byte chunks, in a type that
   // the kernel decodes (16-bit ones as they are)
   p.stream = !backward && N <= 128 && row_bytes(w_dtype, D) % 16 == 0 &&
              (is_quant(w_dtype) || w_dtype == p.ct);
+  if (p.stream) {
+    const int E = 128 / dtype_bits(w_dtype), nt = stream_tiles(N);
+    // a small table's few workgroups take their stages one after another, each the
+    // longer the more fragments it copies: 0.54 us for one tile of tokens with E4M3
+    // codes, 1.6 for four, 2.9 with E2M1 ones (the split logits trade the join for a
+    // copy of the table: 2 us less than the model's; 103 tokens of 2560, 1280 classes
+    // E4M3: 44 us so, 21 split; 1 token: 18.9 so)
+    const int64_t stages = (D + 8 * E - 1) / (8 * E);
+    if (p.lsplits > 1 && (double)stages * (0.2 + 0.17 * (E / 8) * nt) > logits_us - 2.0)
+      p.stream = false;
+    else p.lsplits = 1;
+  }
   if (p.stream) {
     const int E = 128 / dtype_bits(w_dtype), nt = stream_tiles(N);
     p.frag_bytes = ((D + 8 * E - 1) / (8 * E)) * 4 * (E / 8) * nt * 1024;
@@ -915,6 +1053,7 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   };
   p.targets = take((size_t)N * 4);
   p.scal = take(16);
+  p.lsums = take(p.lsplits > 1 ? (size_t)p.lsplits * N * ((V + 255) / 256 * 256) * 4 : 0);
   p.xc = take(p.stream ? (size_t)p.frag_bytes : p.copy_x ? (size_t)N * p.pitch * 2 : 0);
   p.wc = take(p.copy_w ? (size_t)p.piece * p.pitch * 2 : 0);
   if (backward) {
@@ -980,6 +1119,17 @@ int stream(const LossPlan& p, int64_t N, int64_t D, const void* w, int w_dtype,
 }
 
 template <int CT>
+int logits(const LossPlan& p, const TokenOp& ow, const TokenOp& ox, int64_t N, uint8_t* ws,
+           hipStream_t st) {
+  using G = TokenGemm<CT, false, false, 64, 64, 2>;
+  const int tm = (int)((ow.rows + G::BM - 1) / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
+  NOVAQ_LAUNCH((loss_logits_kernel<CT, G>), (int64_t)tm * tn * p.lsplits, G, st, ow, ox, p.dp, N,
+               p.lsplits, reinterpret_cast<float*>(ws + p.lsums), (ow.rows + 255) / 256 * 256, tm,
+               tn);
+  return NOVAQ_OK;
+}
+
+template <int CT>
 int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D, const void* w,
             int w_dtype, const float* w_scale, int64_t V, const void* ids, int bits,
             int64_t ignore, int reduction, float* loss, float* lse, uint8_t* ws, hipStream_t st) {
@@ -1015,6 +1165,16 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
     rows.N = cx.rows = 0;  // (done with the first piece)
     const TokenOp ow{p.copy_w ? ww : reinterpret_cast<const uint16_t*>(from), vc,
                      p.copy_w ? p.pitch : D};
+    if (p.lsplits > 1) {
+      rc = logits<CT>(p, ow, ox, N, ws, st);
+      if (rc != NOVAQ_OK) return rc;
+      hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)N), dim3(256), 0, st,
+                         reinterpret_cast<const float*>(ws + p.lsums), p.lsplits, N, V,
+                         (V + 255) / 256 * 256, w_scale, targets, lse, each);
+      rc = check_launch();
+      if (rc != NOVAQ_OK) return rc;
+      break;
+    }
     auto stats_of = [&](auto g) -> int {
       using G = decltype(g);
       const int tm = (int)((vc + G::BM - 1) / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
@@ -1026,14 +1186,17 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
                  : stats_of(TokenGemm<CT, false, false, 64, 64, 2>{});
     if (rc != NOVAQ_OK) return rc;
   }
-  // (one workgroup, that sums the losses too, for up to 16 rows; for the 37 of 1024 x
-  // 50000 23.5 us a call, with a launch for the sum 20.0)
-  const bool alone = N <= 16;
   float* out = reduction == NOVAQ_REDUCE_NONE ? nullptr : loss;
-  hipLaunchKernelGGL(loss_join_kernel, dim3(alone ? 1u : (unsigned)((N + 15) / 16)), dim3(1024), 0,
-                     st, stats, p.vtiles, N, targets, tl, lse, each,
-                     reduction == NOVAQ_REDUCE_MEAN, scal, out);
-  rc = check_launch();
+  bool alone = false;
+  if (p.lsplits == 1) {
+    // (one workgroup, that sums the losses too, for up to 16 rows; for the 37 of 1024 x
+    // 50000 23.5 us a call, with a launch for the sum 20.0)
+    alone = N <= 16;
+    hipLaunchKernelGGL(loss_join_kernel, dim3(alone ? 1u : (unsigned)((N + 15) / 16)), dim3(1024), 0,
+                       st, stats, p.vtiles, N, targets, tl, lse, each,
+                       reduction == NOVAQ_REDUCE_MEAN, scal, out);
+    rc = check_launch();
+  }
   if (rc != NOVAQ_OK || alone || !out) return rc;
   hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, each, N,
                      reduction == NOVAQ_REDUCE_MEAN, scal, out);
@@ -1098,8 +1261,17 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
                    N, targets, f, lse, pscale, P, pp, tm, tn);
       return NOVAQ_OK;
     };
-    rc = big_l ? prob(TokenGemm<CT, false, false, 128, 64, 4>{})
+    if (p.lsplits > 1) {
+      rc = logits<CT>(p, ow, ox, N, ws, st);
+      if (rc != NOVAQ_OK) return rc;
+      hipLaunchKernelGGL(loss_prob_rows_kernel<CT>, dim3((unsigned)((vp + 2047) / 2048), (unsigned)N),
+                         dim3(256), 0, st, reinterpret_cast<const float*>(ws + p.lsums), p.lsplits,
+                         N, V, vp, w_scale, targets, f, lse, pscale, P, pp);
+      rc = check_launch();
+    } else {
+      rc = big_l ? prob(TokenGemm<CT, false, false, 128, 64, 4>{})
                  : prob(TokenGemm<CT, false, false, 64, 64, 2>{});
+    }
     if (rc != NOVAQ_OK) return rc;
     auto grads = [&](auto ot, auto gx_, auto gw_) -> int {
       using GX = decltype(gx_);

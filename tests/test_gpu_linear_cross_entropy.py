@@ -324,3 +324,42 @@ def test_many_tokens_of_few_classes(N, D, V, wdtype, xdtype):
     for name in ("bf16", "f16"):
         got = F.linear_cross_entropy_backward(x, w, ids, lse, weight_grad_dtype=name)[1]
         assert torch.equal(got, full.to(got.dtype))
+
+
+@pytest.mark.parametrize("N,D,V,wdtype,xdtype", [(1, 4096, 1280, "e4m3", "bf16"),
+                                                 (103, 2560, 1001, "e2m1", "f16"),
+                                                 (300, 4090, 258, "bf16", "bf16"),
+                                                 (130, 1100, 7, "bf16", "f16")])
+def test_wide_rows_of_few_classes(N, D, V, wdtype, xdtype):
+    """The logits' products are split over the width."""
+    test_loss(N, D, V, wdtype, xdtype)
+    test_gradients(N, D, V, wdtype, xdtype)
+
+
+def test_wide_rows_show_bad_targets_and_ignore_others():
+    N, D, V = 40, 2048, 600
+    x, w, _, t = inputs(N, D, V, "e4m3", "bf16", seed=9)
+    t[0], t[1] = V, -100
+    ids = torch.from_numpy(t).cuda()
+    each, lse = F.linear_cross_entropy(x, w, ids, reduction="none", extras=True)
+    assert torch.isnan(each[0]) and each[1] == 0 and torch.isfinite(each[1:]).all()
+    gx, gw = F.linear_cross_entropy_backward(x, w, ids, lse, reduction="none",
+                                             grad=torch.ones(N, device="cuda"))
+    assert torch.isnan(gx[0]).all() and (gx[1] == 0).all() and torch.isfinite(gx[1:].float()).all()
+    assert torch.isnan(gw).all()
+
+
+@pytest.mark.parametrize("N,D", [(17, 2048), (5, 40)])
+def test_one_class(N, D):
+    """The softmax is 1 and its gradients 0: what is left of 1 - 1 is the rounding of
+    the logit and of lse, twice logit_error of the softmax, times f and the operand."""
+    x, w, w64, t = inputs(N, D, 1, "e5m2", "bf16")
+    test_loss(N, D, 1, "e5m2", "bf16")
+    ids = torch.from_numpy(t).cuda()
+    _, lse = F.linear_cross_entropy(x, w, ids, extras=True)
+    gx, gw = F.linear_cross_entropy_backward(x, w, ids, lse)
+    x64 = np.where((t != -100)[:, None], host(x), 0.0)
+    e = 2 * logit_error(x64, w64, cross_entropy(x64, w64, t)[1]) / max(1, (t != -100).sum())
+    assert (np.abs(host(gx)) <= 1.01 * e * np.abs(w64)).all()
+    assert (np.abs(host(gw)) <= 1.01 * e * np.abs(x64).sum(0)).all()
+    assert (host(gx)[t == -100] == 0).all()
