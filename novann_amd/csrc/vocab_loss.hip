@@ -639,11 +639,11 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const float* __restrict_
   loss[n] = t == T_NONE ? 0.0f : t == T_BAD ? u2f(0x7FC00000u) : (l2 - tlogit) * LN2;
 }
 
-// The backward's P (as in loss_prob_kernel) from the split logits: 8 classes a
-// thread, a token a grid row.
+// The backward's P (as in loss_prob_kernel) of a piece from its split logits: 8
+// classes a thread, a token a grid row.
 template <int CT>
 __global__ __launch_bounds__(256) void loss_prob_rows_kernel(
-    const float* __restrict__ sums, int splits, int64_t N, int64_t V, int64_t vp,
+    const float* __restrict__ sums, int splits, int64_t N, int64_t vc, int64_t vp, int64_t v0,
     const float* __restrict__ w_scale, const int* __restrict__ targets,
     const float* __restrict__ f, const float* __restrict__ lse, float pscale,
     uint16_t* __restrict__ P, int64_t pitch) {
@@ -655,13 +655,13 @@ __global__ __launch_bounds__(256) void loss_prob_rows_kernel(
   tg_u32x4 o = {0, 0, 0, 0};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    if (v + 4 * h >= V) break;
+    if (v + 4 * h >= vc) break;
     tg_f32x4 s = split_sum(sums, splits, N, vp, n, v + 4 * h);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t at = v + 4 * h + i;
-      const float e = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -l2)) - (at == t ? 1.0f : 0.0f);
-      s[i] = at < V ? e * fn : 0.0f;
+      const float e = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -l2)) - (v0 + at == t ? 1.0f : 0.0f);
+      s[i] = at < vc ? e * fn : 0.0f;
     }
     o[2 * h] = tg_pack2<CT>(s[0], s[1]);
     o[2 * h + 1] = tg_pack2<CT>(s[2], s[3]);
@@ -949,39 +949,6 @@ GradsPlan grads_plan(int64_t N, int64_t D, int64_t piece, int most = 64) {
   return best;
 }
 
-// The rows of a piece (a multiple of 256): at most 128 MiB of P (and of the
-// table's 16-bit copy), so that what one product writes the next ones find in
-// the 256 MB cache; among the sizes that divide the vocabulary into about that
-// many pieces, the one whose products take the least time by the model above.
-int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, bool backward) {
-  const int64_t vr = (V + 255) / 256 * 256;
-  int64_t most = vr;
-  // (256 rows of P within 31 bits of bytes, whatever N)
-  if (backward) most = std::min(most, ((int64_t)1 << 26) / std::max<int64_t>(N, 32));
-  if (copy_w) most = std::min(most, ((int64_t)1 << 26) / dp);
-  most = std::max<int64_t>(most / 256 * 256, std::min<int64_t>(vr, 1024));
-  if (most >= vr) return vr;
-  auto cost = [&](int64_t rows) {
-    if (rows == 0) return 0.0;
-    double us = best_us(rows, N, D) + 5.0;
-    if (backward) us += grads_plan(N, D, rows).us + 5.0;
-    return us;
-  };
-  int64_t best = most;
-  double least = 0.0;
-  const int64_t few = (vr + most - 1) / most;
-  for (int64_t k = few; k < few + 6; ++k) {
-    // k equal pieces, or whole ones of `most` first (k == few)
-    for (int whole = 0; whole < 2; ++whole) {
-      const int64_t rows = whole ? most : ((V + k - 1) / k + 255) / 256 * 256;
-      if (rows > most) continue;
-      const double us = (double)(V / rows) * cost(rows) + cost(V % rows);
-      if (least == 0.0 || us < least) least = us, best = rows;
-    }
-  }
-  return best;
-}
-
 // The splits of the logits' K where their tiles leave CUs idle, by the same model:
 // each split's sums cost a store and a load, and a launch joins them (backward of
 // 103 x 2560 x 1280 classes: 57 us, split 38; of 1 x 4096 x 1280: 67 and 33; forward
@@ -996,6 +963,40 @@ int logit_splits(int64_t N, int64_t V, int64_t D, double* us) {
     const double t = (tiles * s <= cus ? LONE * round : round) + 5.0 +
                      s * ((double)N * (double)V * 8.0 / 4e6 + 0.3);
     if (t < *us) *us = t, best = s;
+  }
+  return best;
+}
+
+// The rows of a piece (a multiple of 256): at most 128 MiB of P (and of the
+// table's 16-bit copy), so that what one product writes the next ones find in
+// the 256 MB cache; among the sizes that divide the vocabulary into about that
+// many pieces, the one whose products take the least time by the model above.
+int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, bool backward) {
+  const int64_t vr = (V + 255) / 256 * 256;
+  int64_t most = vr;
+  // (256 rows of P within 31 bits of bytes, whatever N)
+  if (backward) most = std::min(most, ((int64_t)1 << 26) / std::max<int64_t>(N, 32));
+  if (copy_w) most = std::min(most, ((int64_t)1 << 26) / dp);
+  most = std::max<int64_t>(most / 256 * 256, std::min<int64_t>(vr, 1024));
+  if (most >= vr) return vr;
+  auto cost = [&](int64_t rows) {
+    if (rows == 0) return 0.0;
+    double us = best_us(rows, N, D);
+    if (!backward) return us + 5.0;
+    logit_splits(N, rows, D, &us);
+    return us + grads_plan(N, D, rows).us + 10.0;
+  };
+  int64_t best = most;
+  double least = 0.0;
+  const int64_t few = (vr + most - 1) / most;
+  for (int64_t k = few; k < few + 6; ++k) {
+    // k equal pieces, or whole ones of `most` first (k == few)
+    for (int whole = 0; whole < 2; ++whole) {
+      const int64_t rows = whole ? most : ((V + k - 1) / k + 255) / 256 * 256;
+      if (rows > most) continue;
+      const double us = (double)(V / rows) * cost(rows) + cost(V % rows);
+      if (least == 0.0 || us < least) least = us, best = rows;
+    }
   }
   return best;
 }
@@ -1016,7 +1017,9 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   p.big_l = large_tiles(p.piece, N, D);
   p.vtiles = (V + (p.big_l ? 255 : 127)) / (p.big_l ? 256 : 128);
   double logits_us = 0.0;
-  p.lsplits = p.piece >= V ? logit_splits(N, V, D, &logits_us) : 1;
+  // (the forward's rows are joined from one piece)
+  p.lsplits = 1;
+  if (backward || p.piece >= V) p.lsplits = logit_splits(N, std::min(p.piece, V), D, &logits_us);
   // up to 128 rows of x, codes whose rows are whole 16-byte chunks, in a type that
   // the kernel decodes (16-bit ones as they are)
   p.stream = !backward && N <= 128 && row_bytes(w_dtype, D) % 16 == 0 &&
@@ -1053,9 +1056,15 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   };
   p.targets = take((size_t)N * 4);
   p.scal = take(16);
-  p.lsums = take(p.lsplits > 1 ? (size_t)p.lsplits * N * ((V + 255) / 256 * 256) * 4 : 0);
   p.xc = take(p.stream ? (size_t)p.frag_bytes : p.copy_x ? (size_t)N * p.pitch * 2 : 0);
   p.wc = take(p.copy_w ? (size_t)p.piece * p.pitch * 2 : 0);
+  auto logit_parts = [&](int splits, int64_t rows) {
+    return splits > 1 ? (size_t)splits * N * ((rows + 255) / 256 * 256) * 4 : 0;
+  };
+  size_t lparts = logit_parts(p.lsplits, std::min(p.piece, V));
+  if (backward && V > p.piece && V % p.piece)
+    lparts = std::max(lparts, logit_parts(logit_splits(N, V % p.piece, D, &logits_us), V % p.piece));
+  p.lsums = take(lparts);
   if (backward) {
     p.f = take((size_t)N * 4);
     p.P = take((size_t)N * row_pitch(p.piece) * 2);
@@ -1119,12 +1128,12 @@ int stream(const LossPlan& p, int64_t N, int64_t D, const void* w, int w_dtype,
 }
 
 template <int CT>
-int logits(const LossPlan& p, const TokenOp& ow, const TokenOp& ox, int64_t N, uint8_t* ws,
-           hipStream_t st) {
+int logits(const LossPlan& p, int splits, const TokenOp& ow, const TokenOp& ox, int64_t N,
+           uint8_t* ws, hipStream_t st) {
   using G = TokenGemm<CT, false, false, 64, 64, 2>;
   const int tm = (int)((ow.rows + G::BM - 1) / G::BM), tn = (int)((N + G::BN - 1) / G::BN);
-  NOVAQ_LAUNCH((loss_logits_kernel<CT, G>), (int64_t)tm * tn * p.lsplits, G, st, ow, ox, p.dp, N,
-               p.lsplits, reinterpret_cast<float*>(ws + p.lsums), (ow.rows + 255) / 256 * 256, tm,
+  NOVAQ_LAUNCH((loss_logits_kernel<CT, G>), (int64_t)tm * tn * splits, G, st, ow, ox, p.dp, N,
+               splits, reinterpret_cast<float*>(ws + p.lsums), (ow.rows + 255) / 256 * 256, tm,
                tn);
   return NOVAQ_OK;
 }
@@ -1166,7 +1175,7 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
     const TokenOp ow{p.copy_w ? ww : reinterpret_cast<const uint16_t*>(from), vc,
                      p.copy_w ? p.pitch : D};
     if (p.lsplits > 1) {
-      rc = logits<CT>(p, ow, ox, N, ws, st);
+      rc = logits<CT>(p, p.lsplits, ow, ox, N, ws, st);
       if (rc != NOVAQ_OK) return rc;
       hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)N), dim3(256), 0, st,
                          reinterpret_cast<const float*>(ws + p.lsums), p.lsplits, N, V,
@@ -1261,12 +1270,14 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
                    N, targets, f, lse, pscale, P, pp, tm, tn);
       return NOVAQ_OK;
     };
-    if (p.lsplits > 1) {
-      rc = logits<CT>(p, ow, ox, N, ws, st);
+    double us;
+    const int lsplits = rest ? logit_splits(N, vc, D, &us) : p.lsplits;
+    if (lsplits > 1) {
+      rc = logits<CT>(p, lsplits, ow, ox, N, ws, st);
       if (rc != NOVAQ_OK) return rc;
       hipLaunchKernelGGL(loss_prob_rows_kernel<CT>, dim3((unsigned)((vp + 2047) / 2048), (unsigned)N),
-                         dim3(256), 0, st, reinterpret_cast<const float*>(ws + p.lsums), p.lsplits,
-                         N, V, vp, w_scale, targets, f, lse, pscale, P, pp);
+                         dim3(256), 0, st, reinterpret_cast<const float*>(ws + p.lsums), lsplits, N,
+                         vc, vp, v0, w_scale, targets, f, lse, pscale, P, pp);
       rc = check_launch();
     } else {
       rc = big_l ? prob(TokenGemm<CT, false, false, 128, 64, 4>{})

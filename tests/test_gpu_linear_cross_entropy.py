@@ -363,3 +363,8 @@ def test_one_class(N, D):
     assert (np.abs(host(gx)) <= 1.01 * e * np.abs(w64)).all()
     assert (np.abs(host(gw)) <= 1.01 * e * np.abs(x64).sum(0)).all()
     assert (host(gx)[t == -100] == 0).all()
+
+
+def test_few_rows_of_several_pieces():
+    """Each piece's logits are split over the width, the last, smaller one further."""
+    test_large_products(90, 4096, 18000, "e4m3", "bf16")
