@@ -292,10 +292,17 @@ class Embedding(Layer):
     def backward(self, grad):
         """Sets (tied: adds to) weight.grad; tokens have no gradient."""
         from . import functional as F
+        grad = _as_f32(grad)
         there = self.weight.grad if self.tied else None
-        add = isinstance(there, torch.Tensor)
-        g = F.embedding_backward(_as_f32(grad), self._cache_tokens, self.weight,
-                                 factor=self.factor, out=there if add else None, accumulate=add)
+        out = there
+        if there is not None and not (isinstance(there, torch.Tensor) and there.is_cuda):
+            # (an array, as the output layer leaves it for arrays: its sum with this
+            # one is made on the device)
+            out = torch.tensor(np.asarray(there, dtype=np.float32), device=F._device())
+        g = F.embedding_backward(grad, self._cache_tokens, self.weight, factor=self.factor,
+                                 out=out, accumulate=out is not None)
+        if out is not there and isinstance(grad, np.ndarray):
+            g = g.cpu().numpy()
         self.weight.grad = g
 
     def parameters(self):
