@@ -488,8 +488,9 @@ int novaq_linear_cross_entropy_backward(const void *x, int x_dtype, int64_t N, i
                                         void *stream);
 
 /* One gradient of novaq_clip_grad_norm: n elements at grad, and where the
- * clipped ones go: out (grad itself to clip in place, NULL for none).  Types:
- * F32, F16, BF16 or NOVAQ_F64, element-aligned. */
+ * clipped ones go: out (grad itself to clip in place, in a type of the same size;
+ * NULL for none).  Types: F32, F16, BF16 or NOVAQ_F64, element-aligned.  Bytes of
+ * an out may be no other row's out or (where that row has one) grad: NOVAQ_EINVAL. */
 typedef struct novaq_gradient {
   const void *grad;
   void *out;

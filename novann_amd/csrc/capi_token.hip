@@ -3,6 +3,10 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <memory>
+#include <new>
+
 #include "novaq_convert.h"
 #include "novaq_internal.h"
 #include "token_io.h"
@@ -45,6 +49,43 @@ int check_loss(const void* x, int x_dtype, int64_t N, int64_t D, const void* w, 
   if (rc != NOVAQ_OK) return rc;
   if (!w || (N > 0 && (!x || !targets))) return NOVAQ_EINVAL;
   if (!aligned(x, 16) || !aligned(w, 16)) return NOVAQ_EALIGN;
+  return NOVAQ_OK;
+}
+
+unsigned float_size(int dt) { return dt == NOVAQ_F64 ? 8u : dt == F32 ? 4u : 2u; }
+
+// NOVAQ_EINVAL where a clipped gradient's bytes are another one's as well, or are
+// read as another gradient (or as its own, but not in place) while they are written:
+// workgroups would race on them.
+int check_outputs(const novaq_gradient* list, int64_t count) {
+  struct Span {
+    uintptr_t from, to;
+    bool written;
+  };
+  Span few[256];  // (of up to 128 gradients: no allocation)
+  std::unique_ptr<Span[]> many;
+  Span* span = few;
+  if (count > 128) {
+    many.reset(count < INT ? new (std::nothrow) Span[2 * count] : nullptr);
+    span = many.get();
+    if (!span) return NOVAQ_ESCRATCH;
+  }
+  int64_t spans = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const novaq_gradient& g = list[i];
+    if (g.n == 0 || !g.out) continue;
+    const unsigned gb = float_size(g.grad_dtype), ob = float_size(g.out_dtype);
+    const uintptr_t in = reinterpret_cast<uintptr_t>(g.grad), out = reinterpret_cast<uintptr_t>(g.out);
+    span[spans++] = Span{out, out + (uintptr_t)g.n * ob, true};
+    if (in != out || gb != ob) span[spans++] = Span{in, in + (uintptr_t)g.n * gb, false};
+  }
+  std::sort(span, span + spans, [](const Span& a, const Span& b) { return a.from < b.from; });
+  uintptr_t any = 0, written = 0;  // where the spans so far, and the written ones, end
+  for (int64_t i = 0; i < spans; ++i) {
+    if (span[i].from < (span[i].written ? any : written)) return NOVAQ_EINVAL;
+    any = std::max(any, span[i].to);
+    if (span[i].written) written = std::max(written, span[i].to);
+  }
   return NOVAQ_OK;
 }
 
@@ -168,13 +209,15 @@ int novaq_clip_grad_norm(const novaq_gradient* list, int64_t count, float max_no
     const bool has_out = g.out != nullptr;
     if (!(plain_float(g.grad_dtype) || g.grad_dtype == NOVAQ_F64)) return NOVAQ_EDTYPE;
     if (has_out && !(plain_float(g.out_dtype) || g.out_dtype == NOVAQ_F64)) return NOVAQ_EDTYPE;
-    if (g.n < 0 || (g.n > 0 && !g.grad)) return NOVAQ_EINVAL;
-    auto size = [](int dt) { return dt == NOVAQ_F64 ? 8u : dt == F32 ? 4u : 2u; };
-    if (!aligned(g.grad, size(g.grad_dtype)) || (has_out && !aligned(g.out, size(g.out_dtype))))
+    if (g.n < 0 || g.n > INT64_MAX / 16 || (g.n > 0 && !g.grad)) return NOVAQ_EINVAL;
+    if (!aligned(g.grad, float_size(g.grad_dtype)) ||
+        (has_out && !aligned(g.out, float_size(g.out_dtype))))
       return NOVAQ_EALIGN;
   }
   if (!aligned(workspace, 16) || !aligned(norm, 4)) return NOVAQ_EALIGN;
   if (workspace_bytes < clip_grad_norm_workspace(count)) return NOVAQ_EINVAL;
+  const int rc = check_outputs(list, count);
+  if (rc != NOVAQ_OK) return rc;
   return clip_grad_norm_launch(list, count, max_norm, eps, norm, workspace,
                                static_cast<hipStream_t>(stream));
 }
