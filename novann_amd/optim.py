@@ -16,6 +16,7 @@ array steps in float32 (the reference's float32 parameters).
 from __future__ import annotations
 
 import ctypes
+import math
 from array import array
 from operator import attrgetter
 from typing import Iterable, List, Optional
@@ -198,22 +199,39 @@ def _clip(grads, outs, max_norm: float, eps: float) -> torch.Tensor:
     return norm
 
 
+def _elements(g):
+    """The memory that a gradient's elements lie in: address, type and layout."""
+    if isinstance(g, np.ndarray):
+        whole, at = g.flags.c_contiguous, g.__array_interface__["data"][0]
+        return at, g.dtype, g.size if whole else (g.shape, g.strides)
+    return g.data_ptr(), g.dtype, g.numel() if g.is_contiguous() else (g.shape, g.stride())
+
+
+def _distinct(grads) -> list:
+    """The gradients, one whose elements an earlier one names left out: it would
+    count twice, and be scaled twice in place."""
+    if set(map(type, grads)) == {torch.Tensor} and \
+            len(set(map(_data_ptr, grads))) == len(grads):
+        return grads
+    kept, seen = [], set()
+    for g in grads:
+        if isinstance(g, (torch.Tensor, np.ndarray)) and math.prod(g.shape) > 0:
+            at = _elements(g)
+            if at in seen:
+                continue
+            seen.add(at)
+        kept.append(g)
+    return kept
+
+
 def _gradients(items) -> list:
-    """The gradients among tensors, arrays and parameters (those with one; a
-    parameter that is named twice, as a shared weight may be, counts once)."""
+    """The gradients among tensors, arrays and parameters (those with one; one that
+    is named twice, as a shared weight's may be, counts once)."""
     items = list(items)
     if set(map(type, items)) == {torch.Tensor}:
-        return items
-    found, seen = [], set()
-    for p in items:
-        if not isinstance(p, (torch.Tensor, np.ndarray)):
-            if id(p) in seen:
-                continue
-            seen.add(id(p))
-            p = p.grad
-        if p is not None:
-            found.append(p)
-    return found
+        return _distinct(items)
+    found = [p if isinstance(p, (torch.Tensor, np.ndarray)) else p.grad for p in items]
+    return _distinct([g for g in found if g is not None])
 
 
 def _uploaded(grads) -> list:
@@ -233,7 +251,7 @@ def _uploaded(grads) -> list:
 def grad_norm(gradients: Iterable) -> torch.Tensor:
     """The 2-norm over all elements of all gradients (device tensors, numpy
     arrays, or parameters, whose ``grad`` counts), a 0-d fp32 device tensor.
-    Squares are summed in fp64."""
+    Squares are summed in fp64; one gradient named twice counts once."""
     return _clip(_uploaded(_gradients(gradients)), None, 0.0, 0.0)
 
 
@@ -244,10 +262,12 @@ def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
     for the device unless a gradient is a numpy array).
 
     gradients: device tensors (fp32, f16, bf16, float64, mixed), numpy arrays, or
-    parameters, whose ``grad`` is taken; those without one are passed over.  They
-    are clipped in place, or, with ``out`` (for each a contiguous device tensor of as
+    parameters, whose ``grad`` is taken; those without one are passed over, and one
+    named twice (a shared weight's) counts and is scaled once.  They are clipped in
+    place, or, with ``out`` (for each that counts a contiguous device tensor of as
     many elements, of any of these types), written there: bf16 gradients to the
-    fp32 ones an optimizer steps with in the same pass.  A NaN norm makes every
+    fp32 ones an optimizer steps with in the same pass.  Contiguous ones that share
+    memory otherwise, and outs that do, are a ValueError.  A NaN norm makes every
     gradient NaN.  Stands for the clipping of the reference's SGD
     (novann/optim/sgd.py:37-82), before any optimizer's step."""
     max_norm, eps = float(max_norm), float(eps)

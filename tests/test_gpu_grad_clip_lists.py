@@ -1,10 +1,30 @@
 """Lists of gradients that overlap, or name one more than once."""
+import numpy as np
 import pytest
 import torch
 
 from novann_amd import optim
 
 pytestmark = pytest.mark.gpu
+
+
+def test_one_gradient_named_twice_counts_once():
+    g = torch.full((3000,), 2.0, device="cuda")
+    h = torch.full((16,), 1.0, device="cuda")
+    a = np.full(9, 2.0, np.float32)
+    n = np.sqrt(4 * 3000 + 16 + 4 * 9)
+    lists = [g, h, g, a, g.view(30, 100), a, g[:0], h[:0], a.reshape(3, 3)]
+    assert abs(float(optim.grad_norm(lists)) - n) <= 2.0 ** -23 * n
+    norm = optim.clip_grad_norm(lists, n / 2, eps=0.0)
+    assert abs(float(norm) - n) <= 2.0 ** -23 * n
+    assert ((g - 1.0).abs() <= 6 * 2.0 ** -24).all() and ((h - 0.5).abs() <= 6 * 2.0 ** -24).all()
+    assert (np.abs(a - 1.0) <= 6 * 2.0 ** -24).all()
+    # with outputs, as for a parameter that is named twice: one for each that counts
+    outs = [torch.empty(3000, device="cuda"), torch.empty(16, device="cuda")]
+    optim.clip_grad_norm([g, g, h], 1e9, out=outs)
+    assert torch.equal(outs[0], g) and torch.equal(outs[1], h)
+    with pytest.raises(ValueError):
+        optim.clip_grad_norm([g, g], 1.0, out=outs)
 
 
 def test_overlapping_gradients_are_refused():
