@@ -225,12 +225,14 @@ def _distinct(grads) -> list:
 
 
 def _gradients(items) -> list:
-    """The gradients among tensors, arrays and parameters (those with one; one that
-    is named twice, as a shared weight's may be, counts once)."""
+    """The gradients among tensors, arrays and parameters, torch's own among them
+    (those with one; one that is named twice, as a shared weight's may be, counts
+    once)."""
     items = list(items)
     if set(map(type, items)) == {torch.Tensor}:
         return _distinct(items)
-    found = [p if isinstance(p, (torch.Tensor, np.ndarray)) else p.grad for p in items]
+    found = [p if isinstance(p, (torch.Tensor, np.ndarray))
+             and not isinstance(p, torch.nn.Parameter) else p.grad for p in items]
     return _distinct([g for g in found if g is not None])
 
 
@@ -262,7 +264,7 @@ def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
     for the device unless a gradient is a numpy array).
 
     gradients: device tensors (fp32, f16, bf16, float64, mixed), numpy arrays, or
-    parameters, whose ``grad`` is taken; those without one are passed over, and one
+    parameters (torch.nn's too), whose ``grad`` is taken; those without one are passed over, and one
     named twice (a shared weight's) counts and is scaled once.  They are clipped in
     place, or, with ``out`` (for each that counts a contiguous device tensor of as
     many elements, of any of these types), written there: bf16 gradients to the

@@ -35,3 +35,13 @@ def test_other_views_are_other_gradients():
     empty = [m[:0], m[:0], torch.empty(0), torch.empty(0)]
     assert same(optim._gradients(empty), empty)
     assert optim._gradients([]) == []
+
+
+def test_torch_parameters_stand_for_their_gradients():
+    a, b, c = (torch.nn.Parameter(torch.ones(3)) for _ in range(3))
+    a.grad = torch.full((3,), 2.0)
+    c.grad = a.grad
+    h = torch.ones(5)
+    assert same(optim._gradients([a, b, c]), [a.grad])
+    assert same(optim._gradients([h, a]), [h, a.grad])
+    assert optim._gradients([b]) == []

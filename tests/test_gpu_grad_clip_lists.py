@@ -1,4 +1,4 @@
-"""Lists of gradients that overlap, or name one more than once."""
+"""Lists of gradients that overlap or name one more than once, and torch's parameters."""
 import numpy as np
 import pytest
 import torch
@@ -45,3 +45,15 @@ def test_overlapping_gradients_are_refused():
     norm = optim.clip_grad_norm([m[:, :4], m[:, 4:]], 4.0, eps=0.0)
     assert abs(float(norm) - 8) <= 2.0 ** -20 and ((m - 0.5).abs() <= 6 * 2.0 ** -24).all()
     assert ((buf - 0.5).abs() <= 6 * 2.0 ** -24).all()
+
+
+def test_torch_parameters_are_clipped_by_their_gradients():
+    a = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    b = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    c = torch.nn.Parameter(torch.ones(3, device="cuda"))
+    a.grad, b.grad = torch.full((5,), 2.0, device="cuda"), torch.full((4,), 2.0, device="cuda")
+    assert abs(float(optim.grad_norm([a, b, c])) - 6.0) <= 2.0 ** -23 * 6
+    optim.clip_grad_norm([a, b, c], 3.0, eps=0.0)
+    assert all((p == 1).all() for p in (a, b, c)) and c.grad is None
+    for p in (a, b):
+        assert ((p.grad - 1.0).abs() <= 6 * 2.0 ** -24).all()
