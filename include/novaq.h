@@ -477,8 +477,9 @@ int novaq_linear_cross_entropy(const void *x, int x_dtype, int64_t N, int64_t D,
  * softmax is computed again from lse, a piece of the vocabulary at a time, and
  * rounded to the products' 16-bit type before its two products (fp32 sums);
  * each output is rounded once.  Rows that are ignored get a zero gradient and
- * add nothing, whatever x holds there; a target outside the vocabulary makes
- * its gradients NaN. */
+ * add nothing, whatever x (and, with a gradient for each row, that) holds there; a
+ * target outside the vocabulary makes its gradients NaN.  A row's own gradient, were
+ * it infinite or NaN, shows in that row of grad_input alone, and in grad_weight. */
 int novaq_linear_cross_entropy_backward(const void *x, int x_dtype, int64_t N, int64_t D,
                                         const void *w_q, int w_dtype, const float *w_scale,
                                         int64_t V, const void *targets, int target_bits,

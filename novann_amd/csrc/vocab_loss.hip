@@ -9,8 +9,11 @@
 //   grad_x   = g s P dec(W),  grad_W = g P^T x
 //
 // f[n] is 0 for ignored rows and else 1 (reduction mean: g = upstream / count,
-// sum: g = upstream) or, with a gradient for each row, that gradient over the
-// largest of them in magnitude (which is g).
+// sum: g = upstream).  With a gradient for each row (u[n]; row_factors) P takes its
+// digits and at most 12 of its binary places, grad_x's rows the power of two that
+// is left when they are stored, and grad_W's product a copy of x with the rest of
+// it: rows of very different gradients, infinite ones and NaN among them, leave
+// one another's grad_x alone.
 //
 // The vocabulary is walked in pieces.  The forward multiplies a piece's rows
 // with x and reduces each tile of logits to one (maximum, sum of 2^(l2 -
@@ -26,7 +29,8 @@
 // type are rounded to nearest even.  P is rounded to the same type before its
 // products (half an ulp of 2^-8 or 2^-11: the size of the gradients' own
 // rounding where they are stored in 16 bits); in f16 it carries a factor of
-// 2^14, which keeps probabilities down to 2^-28 in its normal range.  Logits,
+// 2^14, which keeps probabilities down to 2^-28 in its normal range (2^-16 in a row
+// whose own gradient is 2^-23 of the largest or less).  Logits,
 // maxima, sums, lse and all accumulation are fp32; the loss over the rows is
 // summed in fp64.
 #include <hip/hip_runtime.h>
@@ -165,7 +169,7 @@ __device__ __forceinline__ void fragments(const FragmentJob& f, int64_t first, i
 // Per-row state: targets as int32 (T_NONE, T_BAD), the row factors f (NaN for
 // T_BAD, so its gradients show; may be null), scal[0] = g, scal[1] = the number
 // of rows with a loss.
-// grad: one value, or one a row (per_row), or null (1).
+// grad: one value, or one a row (per_row; then fx and fw too), or null (1).
 struct RowsJob {
   const void* ids;
   int bits;
@@ -175,10 +179,34 @@ struct RowsJob {
   int* targets;
   float* f;
   float* scal;
+  float *fx, *fw;  // what grad_x's rows are scaled by, and x's for grad_W
 };
 
-__device__ __forceinline__ float nan_max(float a, float b) {
-  return a != a || b != b ? u2f(0x7FC00000u) : fmaxf(a, b);
+// The exponent e of a finite a > 0: 2^e <= a < 2^(e + 1).
+__device__ __forceinline__ int exponent(float a) {
+  const int e = (int)(f2u(a) >> 23);
+  return e > 0 ? e - 127 : 31 - __clz(f2u(a)) - 149;
+}
+
+// The gradient u of one row as f fx = u and f fw 2^top = u, 2^top being the power of
+// two in the largest finite one.  With d the places that u lies below that: f is u's
+// digits (1 <= |f| < 2) moved down by half of d, but 12 places at most, fw = 2^-(the
+// other places), both exact.  So P in f16 (a factor of 2^14 above one) holds
+// probabilities down to 2^-16 in its normal range however small a row's gradient is,
+// and x fw loses bits only where it falls under 2^-14.  An infinite or NaN u is kept
+// out of P, which both products read.
+__device__ __forceinline__ void row_factors(float u, int top, float& f, float& fx, float& fw) {
+  const float a = fabsf(u);
+  if (!(a < INFINITY)) {
+    f = 1.0f, fx = fw = u;
+  } else if (a == 0.0f) {
+    f = 0.0f, fx = fw = 1.0f;
+  } else {
+    const int e = exponent(a), d = top - e, down = min(d - d / 2, 12);
+    f = ldexpf(u, -e - down);
+    fx = ldexpf(1.0f, e + down);
+    fw = ldexpf(1.0f, down - d);
+  }
 }
 
 __device__ __forceinline__ void rows_job(const RowsJob& r, int* cnt, float* top) {
@@ -196,22 +224,23 @@ __device__ __forceinline__ void rows_job(const RowsJob& r, int* cnt, float* top)
       const int k = t[x] == r.ignore ? T_NONE : t[x] < 0 || t[x] >= r.V ? T_BAD : (int)t[x];
       r.targets[n] = k;
       c += k != T_NONE;
-      if (r.per_row && k != T_NONE) m = nan_max(m, fabsf(r.grad[n]));
+      if (r.per_row && k != T_NONE && fabsf(r.grad[n]) < INFINITY) m = fmaxf(m, fabsf(r.grad[n]));
       if (r.f && !r.per_row) r.f[n] = k == T_NONE ? 0.0f : k == T_BAD ? u2f(0x7FC00000u) : 1.0f;
     }
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     c += __shfl_xor(c, d);
-    m = nan_max(m, __shfl_xor(m, d));
+    m = fmaxf(m, __shfl_xor(m, d));
   }
   if (lane == 0) cnt[wave] = c, top[wave] = m;
   __syncthreads();
   c = 0, m = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) c += cnt[w], m = nan_max(m, top[w]);
+  for (int w = 0; w < 4; ++w) c += cnt[w], m = fmaxf(m, top[w]);
+  const int e = m > 0.0f ? exponent(m) : 0;
   if (tid == 0) {
-    float g = r.per_row ? m : r.grad ? *r.grad : 1.0f;
+    float g = r.per_row ? ldexpf(1.0f, e) : r.grad ? *r.grad : 1.0f;
     if (r.mean) g = c > 0 ? g / (float)c : 0.0f;
     r.scal[0] = g;
     r.scal[1] = (float)c;
@@ -219,8 +248,9 @@ __device__ __forceinline__ void rows_job(const RowsJob& r, int* cnt, float* top)
   if (r.f && r.per_row)
     for (int64_t n = tid; n < r.N; n += 256) {
       const int k = r.targets[n];
-      // (all zero: 0; NaN: NaN)
-      r.f[n] = k == T_NONE ? 0.0f : k == T_BAD ? u2f(0x7FC00000u) : m > 0.0f ? r.grad[n] / m : m;
+      float f = k == T_NONE ? 0.0f : u2f(0x7FC00000u), fx = 1.0f, fw = 1.0f;
+      if (k >= 0) row_factors(r.grad[n], e, f, fx, fw);
+      r.f[n] = f, r.fx[n] = fx, r.fw[n] = fw;
     }
 }
 
@@ -270,6 +300,28 @@ int prep_launch(const RowsJob& rows, CopyJob x, const FragmentJob& frag, CopyJob
   if (all == 0) return NOVAQ_OK;
   hipLaunchKernelGGL(loss_prep_kernel<CT>, dim3(all), dim3(256), 0, stream, rows, x, frag, w, xb);
   return check_launch();
+}
+
+// x's rows times fw, for grad_W's product where each row has a gradient of its own:
+// N x dp 16-bit values (pitch elements apart), 8 a thread.
+template <int CT>
+__global__ __launch_bounds__(256) void loss_scaled_x_kernel(const uint16_t* __restrict__ x,
+                                                            const float* __restrict__ fw, int64_t N,
+                                                            int64_t dp, int64_t pitch,
+                                                            uint16_t* __restrict__ out) {
+  const int64_t per = dp / 8, total = N * per;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
+    const int64_t n = q / per, at = n * pitch + (q - n * per) * 8;
+    const float a = fw[n];
+    float v[8];
+    load8<CT, true>(reinterpret_cast<const uint8_t*>(x), at, 0, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= a;
+    tg_u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = tg_pack2<CT>(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<tg_u32x4*>(out + at) = o;
+  }
 }
 
 // 8 workgroups in a row go to the 8 XCDs: those of one XCD take a compact
@@ -797,8 +849,8 @@ __global__ __launch_bounds__(GX::NTH, 1) void loss_grads_kernel(GradsJob g) {
 }
 
 // A gradient = its splits' sums times g s / pscale, as OT (rows of ignored targets
-// 0; grad_W has neither s nor targets): four columns a thread, or, with SHARE, four
-// threads (one in each wave) that take every fourth split each and add up in their
+// 0; with fx that of each row in g's place; grad_W has neither s nor targets): four
+// columns a thread, or, with SHARE, four threads (one in each wave) that take every fourth split each and add up in their
 // order.
 template <int OT, bool SHARE>
 __global__ __launch_bounds__(256) void loss_sums_store_kernel(const float* __restrict__ sums,
@@ -808,9 +860,10 @@ __global__ __launch_bounds__(256) void loss_sums_store_kernel(const float* __res
                                                             const float* __restrict__ w_scale,
                                                             float inv_pscale,
                                                             const int* __restrict__ targets,
+                                                            const float* __restrict__ fx,
                                                             void* __restrict__ out) {
   __shared__ float4 part[SHARE ? 3 * 64 : 1];
-  const float a = scal[0] * (w_scale ? *w_scale : 1.0f) * inv_pscale;
+  const float s = w_scale ? *w_scale : 1.0f, all = scal[0] * s * inv_pscale;
   const int64_t per = dp / 4, total = N * per;
   constexpr int STEP = SHARE ? 4 : 1, UNITS = 256 / STEP;
   const int from = SHARE ? threadIdx.x >> 6 : 0, unit = SHARE ? threadIdx.x & 63 : threadIdx.x;
@@ -837,6 +890,7 @@ __global__ __launch_bounds__(256) void loss_sums_store_kernel(const float* __res
     }
     if (from > 0 || q0 + unit >= total || c >= D) continue;
     const bool none = targets && targets[n] == T_NONE;
+    const float a = fx ? fx[n] * s * inv_pscale : all;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = none ? 0.0f : rounded(v[i] * a);
     const int64_t e = n * D + c;
@@ -872,7 +926,7 @@ struct LossPlan {
   int lsplits;       // of the logits' K (1: their tiles are not stored)
   bool stream;       // forward: the table read as stored, for few tokens
   int64_t frag_bytes;
-  size_t xc, wc, stats, tlogit, targets, each, scal, f, P, sums, wsums, lsums, total;
+  size_t xc, wc, stats, tlogit, targets, each, scal, f, fx, fw, xs, P, sums, wsums, lsums, total;
 };
 
 // Time (us) of a round of tiles of 256 x 256 (a CU runs one workgroup of 8 waves) or
@@ -1067,6 +1121,9 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
   p.lsums = take(lparts);
   if (backward) {
     p.f = take((size_t)N * 4);
+    p.fx = take((size_t)N * 4);  // (these three where each row has a gradient of its own)
+    p.fw = take((size_t)N * 4);
+    p.xs = take((size_t)N * p.pitch * 2);
     p.P = take((size_t)N * row_pitch(p.piece) * 2);
     p.sums = take((size_t)p.splits * N * p.dp * 4);
     auto parts = [&](int splits, int64_t rows) {
@@ -1149,7 +1206,7 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
   float* each = reduction == NOVAQ_REDUCE_NONE ? loss : reinterpret_cast<float*>(ws + p.each);
   uint16_t* xw = reinterpret_cast<uint16_t*>(ws + p.xc);
   uint16_t* ww = reinterpret_cast<uint16_t*>(ws + p.wc);
-  RowsJob rows{ids, bits, ignore, N, V, nullptr, 0, 0, targets, nullptr, scal};
+  RowsJob rows{ids, bits, ignore, N, V, nullptr, 0, 0, targets, nullptr, scal, nullptr, nullptr};
   CopyJob cx{};
   FragmentJob fx{};
   if (p.stream)
@@ -1214,14 +1271,14 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
 
 template <int OT>
 int store_sums(const float* sums, int splits, int64_t rows, int64_t dp, int64_t D,
-               const float* scal, const float* w_scale, float inv, const int* targets, void* out,
-               hipStream_t st) {
+               const float* scal, const float* w_scale, float inv, const int* targets,
+               const float* fx, void* out, hipStream_t st) {
   auto go = [&](auto share) {
     constexpr bool SHARE = decltype(share)::value;
     const int64_t units = SHARE ? 64 : 256;
     const dim3 grid((unsigned)std::min<int64_t>((rows * (dp / 4) + units - 1) / units, 8192));
     hipLaunchKernelGGL((loss_sums_store_kernel<OT, SHARE>), grid, dim3(256), 0, st, sums, splits,
-                       rows, dp, D, scal, w_scale, inv, targets, out);
+                       rows, dp, D, scal, w_scale, inv, targets, fx, out);
   };
   if (splits >= 8) go(std::true_type{});
   else go(std::false_type{});
@@ -1241,11 +1298,15 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
   uint16_t* xw = reinterpret_cast<uint16_t*>(ws + p.xc);
   uint16_t* ww = reinterpret_cast<uint16_t*>(ws + p.wc);
   const float pscale = CT == F16 ? 0x1p14f : 1.0f, inv = 1.0f / pscale;
-  RowsJob rows{ids, bits, ignore, N, V, grad, reduction == NOVAQ_REDUCE_NONE && grad ? 1 : 0,
-               reduction == NOVAQ_REDUCE_MEAN, targets, f, scal};
+  const bool per_row = reduction == NOVAQ_REDUCE_NONE && grad;
+  float* fx = reinterpret_cast<float*>(ws + p.fx);
+  float* fw = reinterpret_cast<float*>(ws + p.fw);
+  uint16_t* xs = reinterpret_cast<uint16_t*>(ws + p.xs);
+  RowsJob rows{ids, bits, ignore, N, V, grad, per_row ? 1 : 0, reduction == NOVAQ_REDUCE_MEAN,
+               targets, f, scal, fx, fw};
   CopyJob cx{static_cast<const uint8_t*>(x), xw, N, D, p.dp, p.pitch, x_dtype, ids, bits, ignore, {}};
   int rc = NOVAQ_OK;
-  const TokenOp ox{xw, N, p.pitch};
+  const TokenOp ox{xw, N, p.pitch}, oxs{per_row && gw ? xs : xw, N, p.pitch};
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, V - v0), vp = (vc + 255) / 256 * 256;
     const uint8_t* from = static_cast<const uint8_t*>(w) + v0 * row_bytes(w_dtype, D);
@@ -1254,6 +1315,13 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
     rc = prep_launch<CT>(rows, cx, FragmentJob{}, cw, st);
     if (rc != NOVAQ_OK) return rc;
     rows.N = cx.rows = 0;  // (done with the first piece)
+    if (per_row && gw && v0 == 0) {
+      const dim3 grid((unsigned)std::min<int64_t>((N * (p.dp / 8) + 255) / 256, 8192));
+      hipLaunchKernelGGL(loss_scaled_x_kernel<CT>, grid, dim3(256), 0, st, xw, fw, N, p.dp, p.pitch,
+                         xs);
+      rc = check_launch();
+      if (rc != NOVAQ_OK) return rc;
+    }
     const int64_t pp = row_pitch(vp);
     const TokenOp ow{p.copy_w ? ww : reinterpret_cast<const uint16_t*>(from), vc,
                      p.copy_w ? p.pitch : D};
@@ -1288,7 +1356,7 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
       using GX = decltype(gx_);
       using GW = decltype(gw_);
       constexpr int OT = decltype(ot)::value;
-      GradsJob j{TokenOp{P, N, pp}, TokenOp{P, vp, pp}, ow, ox, N, D, vc, (int)(vp / 64),
+      GradsJob j{TokenOp{P, N, pp}, TokenOp{P, vp, pp}, ow, oxs, N, D, vc, (int)(vp / 64),
                  (int)((N + 63) / 64), gp.splits, v0 == 0 ? 1 : 0, sums, p.dp, scal, inv,
                  static_cast<uint8_t*>(gw) + v0 * D * (OT == F32 ? 4 : 2),
                  reinterpret_cast<float*>(ws + p.wsums), gp.wsplits, 0, 0, 0, 0};
@@ -1308,7 +1376,8 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
         return NOVAQ_OK;
       }
       NOVAQ_LAUNCH((loss_grads_kernel<CT, SUMS, GX, GW>), tiles, GX, st, j);
-      return store_sums<OT>(j.wsums, gp.wsplits, vc, p.dp, D, scal, nullptr, inv, nullptr, j.gw, st);
+      return store_sums<OT>(j.wsums, gp.wsplits, vc, p.dp, D, scal, nullptr, inv, nullptr, nullptr, j.gw,
+                            st);
     };
     auto grads_to = [&](auto ot) -> int {
       return gp.big ? grads(ot, TokenGemm<CT, false, true, 128, 64, 4>{},
@@ -1324,7 +1393,7 @@ int backward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D
   if (!gx) return rc;
   auto store = [&](auto ot) {
     return store_sums<decltype(ot)::value>(sums, p.splits, N, p.dp, D, scal, w_scale, inv, targets,
-                                           gx, st);
+                                           per_row ? fx : nullptr, gx, st);
   };
   return x_dtype == F32   ? store(std::integral_constant<int, F32>{})
          : x_dtype == F16 ? store(std::integral_constant<int, F16>{})
