@@ -504,13 +504,14 @@ typedef struct novaq_gradient {
 size_t novaq_clip_grad_norm_workspace(int64_t count);
 
 /* *norm = sqrt(sum of g^2 over all elements of all gradients), summed in fp64,
- * and out = g * min(1, max_norm / (norm + eps)) (one fp32 multiply, fp64 for
- * F64 gradients, rounded to out's type) for each gradient that has an out.  The list is host memory, read
- * before the call returns.  A NaN norm makes every output NaN; an infinite one
+ * and out = g * min(1, max_norm / (norm + eps)) for each gradient that has an out:
+ * the factor in fp64, rounded to fp32 for one fp32 multiply where the gradient is
+ * not F64, the product rounded to out's type.  *norm is rounded to fp32 (infinite
+ * past its range).  The list is host memory, read before the call returns.  A NaN norm makes every output NaN; an infinite one
  * makes finite gradients 0.
  * Stands for the clipping inside SGD.step (novann/optim/sgd.py:37-82), for any
  * optimizer. */
-int novaq_clip_grad_norm(const novaq_gradient *list, int64_t count, float max_norm, float eps,
+int novaq_clip_grad_norm(const novaq_gradient *list, int64_t count, double max_norm, double eps,
                          float *norm, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus

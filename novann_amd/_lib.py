@@ -102,7 +102,7 @@ SIGNATURES = {
                                                    _vp, _i32, _i64, _i32, _f32p, _f32p, _vp, _vp,
                                                    _i32, _vp, ctypes.c_size_t, _vp]),
     "novaq_clip_grad_norm_workspace": (ctypes.c_size_t, [_i64]),
-    "novaq_clip_grad_norm": (_i32, [_vp, _i64, ctypes.c_float, ctypes.c_float, _f32p, _vp,
+    "novaq_clip_grad_norm": (_i32, [_vp, _i64, ctypes.c_double, ctypes.c_double, _f32p, _vp,
                                     ctypes.c_size_t, _vp]),
 }
 

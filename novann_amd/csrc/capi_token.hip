@@ -200,10 +200,10 @@ size_t novaq_clip_grad_norm_workspace(int64_t count) {
   return clip_grad_norm_workspace(count < 0 ? 0 : count);
 }
 
-int novaq_clip_grad_norm(const novaq_gradient* list, int64_t count, float max_norm, float eps,
+int novaq_clip_grad_norm(const novaq_gradient* list, int64_t count, double max_norm, double eps,
                          float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   if (count < 0 || (count > 0 && !list) || !norm || !workspace) return NOVAQ_EINVAL;
-  if (!(max_norm >= 0.0f) || !(eps >= 0.0f)) return NOVAQ_EINVAL;
+  if (!(max_norm >= 0.0) || !(eps >= 0.0)) return NOVAQ_EINVAL;
   for (int64_t i = 0; i < count; ++i) {
     const novaq_gradient& g = list[i];
     const bool has_out = g.out != nullptr;

@@ -20,6 +20,9 @@
 // two 16-byte stores of fp32: 573 us for the second pass, 390 = 5.4 TB/s with 4).
 // Neither fewer registers nor fp32 products change the times.
 //
+// The factor is worked out in fp64 too, and float64 gradients are multiplied by it as
+// it is; the others by its fp32 rounding (a norm past fp32's range still scales them).
+//
 // NaN or infinite gradients give a NaN or infinite norm: the factor is then
 // NaN or 0, as the formula says (min keeps a NaN).
 #include <hip/hip_runtime.h>
@@ -192,8 +195,9 @@ __device__ __forceinline__ void put(void* out, int64_t i, float v) {
 }
 template <int GT, int OT>
 __device__ __forceinline__ void scale_run(const void* g, void* out, int64_t e0, int64_t e1,
-                                          float coef) {
+                                          double coef64) {
   constexpr int W = GT == F32 || OT == F32 ? 4 : 8;
+  const float coef = (float)coef64;
   each_of_run<GT, W, true>(
       g, e0, e1, OT != F64 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
       [&](int64_t i, const float(&v)[W]) {
@@ -205,14 +209,15 @@ __device__ __forceinline__ void scale_run(const void* g, void* out, int64_t e0, 
         }
       },
       [&](int64_t i, auto v) {
-        if constexpr (GT == F64 && OT == F64) reinterpret_cast<double*>(out)[i] = v * (double)coef;
-        else put<OT>(out, i, (float)(v * (decltype(v))coef));
+        if constexpr (GT == F64 && OT == F64) reinterpret_cast<double*>(out)[i] = v * coef64;
+        else if constexpr (GT == F64) put<OT>(out, i, (float)(v * coef64));
+        else put<OT>(out, i, v * coef);
       });
 }
 
 template <int GT>
 __device__ __forceinline__ void scale_run(int ot, const void* g, void* out, int64_t e0, int64_t e1,
-                                          float coef) {
+                                          double coef) {
   switch (ot) {
     case F32: scale_run<GT, F32>(g, out, e0, e1, coef); break;
     case F16: scale_run<GT, F16>(g, out, e0, e1, coef); break;
@@ -223,7 +228,7 @@ __device__ __forceinline__ void scale_run(int ot, const void* g, void* out, int6
 
 template <class T>
 __device__ __forceinline__ void scale_runs(const T& rows, int count, uint32_t runs, int run,
-                                           float coef) {
+                                           double coef) {
   for (uint32_t r = blockIdx.x; r < runs; r += gridDim.x) {
     const int t = tensor_of(rows, count, r);
     void* out = rows[t].out;
@@ -243,14 +248,14 @@ __global__ __launch_bounds__(256) void norm_scale_kernel(const NormRows l,
                                                          const NormRow* __restrict__ table,
                                                          int count, uint32_t runs, int run,
                                                          const double* __restrict__ slots,
-                                                         int nslots, float max_norm, float eps,
+                                                         int nslots, double max_norm, double eps,
                                                          float* __restrict__ norm) {
   __shared__ double part[4];
   double s = 0.0;
   for (int i = threadIdx.x; i < nslots; i += 256) s += slots[i];
-  const float nv = (float)sqrt(block_sum(s, part));
-  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = nv;
-  const float q = max_norm / (nv + eps), coef = q > 1.0f ? 1.0f : q;  // (NaN stays)
+  const double nv = sqrt(block_sum(s, part));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nv;
+  const double q = max_norm / (nv + eps), coef = q > 1.0 ? 1.0 : q;  // (NaN stays)
   if constexpr (TABLE) scale_runs(table, count, runs, run, coef);
   else scale_runs(l.row, count, runs, run, coef);
 }
@@ -261,7 +266,7 @@ size_t clip_grad_norm_workspace(int64_t count) {
   return BLOCKS * sizeof(double) + (count > ROWS ? (size_t)count * sizeof(NormRow) : 0);
 }
 
-int clip_grad_norm_launch(const novaq_gradient* list, int64_t count, float max_norm, float eps,
+int clip_grad_norm_launch(const novaq_gradient* list, int64_t count, double max_norm, double eps,
                           float* norm, void* workspace, hipStream_t st) {
   double* slots = static_cast<double*>(workspace);
   NormRow* table = reinterpret_cast<NormRow*>(slots + BLOCKS);

@@ -231,7 +231,7 @@ int vocab_loss_backward_launch(const void* x, int x_dtype, int64_t N, int64_t D,
                                const float* lse, void* gx, void* gw, int gw_dtype, void* ws,
                                hipStream_t stream);
 size_t clip_grad_norm_workspace(int64_t count);
-int clip_grad_norm_launch(const novaq_gradient* list, int64_t count, float max_norm, float eps,
+int clip_grad_norm_launch(const novaq_gradient* list, int64_t count, double max_norm, double eps,
                           float* norm, void* workspace, hipStream_t stream);
 
 }  // namespace novaq
