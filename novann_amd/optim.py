@@ -161,10 +161,14 @@ _dtype, _is_cuda = attrgetter("dtype"), attrgetter("is_cuda")
 def _type_codes(tensors, what: str) -> list:
     """The type codes of device tensors that may be clipped (else TypeError or
     ValueError)."""
-    codes = list(map(_GRAD_TYPES.get, map(_dtype, tensors)))
+    types = list(map(_dtype, tensors))
+    if types and types.count(types[0]) == len(types):  # (the ordinary list)
+        codes = [_GRAD_TYPES.get(types[0])] * len(types)
+    else:
+        codes = list(map(_GRAD_TYPES.get, types))
     if None in codes:
         raise TypeError(f"{what} must be fp32, f16, bf16 or float64, got "
-                        f"{tensors[codes.index(None)].dtype}")
+                        f"{types[codes.index(None)]}")
     if not all(map(_is_cuda, tensors)):
         raise ValueError(f"{what} must be CUDA (HIP) device tensors, got one on the host")
     return codes
@@ -175,18 +179,19 @@ def _clip(grads, outs, max_norm: float, eps: float) -> torch.Tensor:
     or None."""
     n = len(grads)
     dev = grads[0].device if n else _device()
-    # the rows of novaq_gradient: address, address, count, the two types
+    # the rows of novaq_gradient: address, address, count, the two types (an array
+    # is made of a list in less time than of an iterator)
     types = _type_codes(grads, "gradients")
-    counts = array("q", map(_numel, grads))
+    counts = list(map(_numel, grads))
     table = array("q", bytes(32 * n))
-    table[0::4] = array("q", map(_data_ptr, grads))
-    table[2::4] = counts
+    table[0::4] = at = array("q", list(map(_data_ptr, grads)))
+    table[2::4] = array("q", counts)
     if outs is not None:
-        if outs is not grads and array("q", map(_numel, outs)) != counts:
+        if outs is not grads and list(map(_numel, outs)) != counts:
             raise ValueError("every out must have as many elements as its gradient")
         to = types if outs is grads else _type_codes(outs, "out")
         types = [a | b << 32 for a, b in zip(types, to)]
-        table[1::4] = array("q", map(_data_ptr, outs))
+        table[1::4] = at if outs is grads else array("q", list(map(_data_ptr, outs)))
     table[3::4] = array("q", types)
     lib = _lib.load()
     nbytes = lib.novaq_clip_grad_norm_workspace(n)
