@@ -320,8 +320,9 @@ class LinearCrossEntropy(Layer):
     ``weight``: another layer's (num_tokens, in_features) weight to share (an
     Embedding's), else one is drawn and stored as Linear's.  Called with the
     hidden states (N, in_features) and the targets (N,); ``backward`` takes the
-    loss's own gradient (default 1), sets weight.grad and returns the hidden
-    states' gradient.  Stands for Linear with CrossEntropyLoss
+    loss's own gradient (default 1), sets weight.grad (fp32, as a lookup in the same
+    table may add to it and an optimizer steps with it) and returns the hidden states'
+    gradient in their type.  Stands for Linear with CrossEntropyLoss
     (novann/losses/loss_functions.py:8-167)."""
 
     def __init__(self, in_features: int, num_tokens: int, init=None,
@@ -355,7 +356,7 @@ class LinearCrossEntropy(Layer):
         x, targets, lse = self._cache
         gx, self.weight.grad = F.linear_cross_entropy_backward(
             x, self.weight, targets, lse, grad=grad, ignore_index=self.ignore_index,
-            reduction=self.reduction)
+            reduction=self.reduction, weight_grad_dtype="f32")
         return gx
 
     def parameters(self):

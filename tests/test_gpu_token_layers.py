@@ -78,3 +78,37 @@ def test_tied_gradient_after_zeros():
         assert isinstance(embed.weight.grad, torch.Tensor)
         # fp32 sums of at most N terms
         assert (np.abs(host(embed.weight.grad) - want) <= N * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("tie", [True, False])
+@pytest.mark.parametrize("xdtype", [torch.bfloat16, torch.float16])
+def test_tables_gradient_is_fp32_for_16_bit_hidden_states(xdtype, tie):
+    """Each class's gradient is far below the smallest f16 number; a token that comes
+    4000 times would stop growing in 16 bits."""
+    np.random.seed(3)
+    classes, width, n = 64, 16, 8000
+    embed = Embedding(classes, width, init=lambda s: np.random.standard_normal(s) / 8, tied=tie)
+    head = LinearCrossEntropy(width, classes, weight=embed.weight) if tie else \
+        LinearCrossEntropy(width, classes, init=lambda s: np.random.standard_normal(s) / 8)
+    x = torch.full((n, width), 2.0 ** -8, device="cuda", dtype=xdtype)
+    target = torch.from_numpy(np.arange(n) % 2).cuda()
+    head(x, target)
+    gx = head.backward(2.0 ** -10)
+    assert gx.dtype == xdtype
+    g = head.weight.grad
+    assert g.dtype == torch.float32
+    w = head.weight.data.astype(np.float32)
+    w = bf16(w) if xdtype == torch.bfloat16 else host(torch.from_numpy(w).to(torch.float16))
+    P, _, want = cross_entropy_grads(host(x), w, target.cpu().numpy(), np.full(n, 2.0 ** -10 / n))
+    u = 2.0 ** -8 if xdtype == torch.bfloat16 else 2.0 ** -11
+    # (P rounded to 16 bits: at most u of its size, and fp32 sums)
+    bound = 1.05 * u * (np.abs(P).T @ np.abs(host(x)))
+    assert np.abs(want).min() > 0 and np.abs(want[2:]).max() < 2.0 ** -20
+    assert (np.abs(host(g) - want) <= bound).all()
+    if tie:
+        t = torch.full((n,), 7, device="cuda")
+        embed(t)
+        embed.backward(torch.full((n, width), 2.0 ** -9, device="cuda", dtype=xdtype))
+        assert embed.weight.grad is g
+        want[7] += n * 2.0 ** -9
+        assert (np.abs(host(g) - want) <= bound + 2.0 ** -20 * np.abs(want)).all()
