@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import numbers
 from dataclasses import dataclass
 from typing import Any, Optional, Tuple, Union
 
@@ -790,8 +791,10 @@ def linear_cross_entropy_backward(input, weight, targets, lse, *, grad=None,
     it): (grad_input (N, D) in input's type, grad_weight (V, D) in
     ``weight_grad_dtype``, input's type by default).
 
-    grad: the loss's own gradient, a number or fp32 tensor (one value, or (N,)
-    with reduction 'none'; default 1).  grad_weight is the gradient of the
+    grad: the loss's own gradient, a number (Python's or numpy's; with reduction
+    'none' every row's) or an fp32 tensor or array (one value, or (N,) with 'none');
+    default 1.  Gradients of single rows, whatever their sizes, leave the other rows'
+    grad_input alone.  grad_weight is the gradient of the
     dequantized table.  The softmax is rounded to the products' 16-bit type
     before it is multiplied, sums are fp32.  Ignored rows get and give no
     gradient, whatever they hold.  ndarrays in -> ndarrays out (fp32, f16)."""
@@ -805,7 +808,8 @@ def linear_cross_entropy_backward(input, weight, targets, lse, *, grad=None,
         raise ValueError(f"lse {tuple(l.shape)} does not match {N} rows")
     g = None
     if grad is not None:
-        if isinstance(grad, (int, float)):
+        # (a loss of arrays is a numpy number)
+        if isinstance(grad, numbers.Real) or isinstance(grad, np.ndarray) and grad.ndim == 0:
             g = torch.full((N,) if reduction == "none" else (1,), float(grad), device=x.device)
         else:
             g, _ = _to_device_f32(grad, "grad")

@@ -113,3 +113,21 @@ def test_gradients_of_the_whole_range():
     assert (np.abs(gx - want_x) <= bx).all() and (np.abs(gw - want_w) <= bw).all()
     x, w, t, gx, gw = run(N, D, V, "e4m3", "bf16", np.zeros(N, np.float32))
     assert not gx.any() and not gw.any()
+
+
+@pytest.mark.parametrize("grad", [np.float32(0.25), np.float64(0.25), 0.25, np.array(0.25),
+                                  np.array([0.25], np.float32)])
+def test_numbers_as_upstream_gradients(grad):
+    """The loss of arrays is an np.float32; so may its gradient be."""
+    rng = np.random.default_rng(5)
+    x, w = rng.standard_normal((6, 16)).astype(np.float32), rng.standard_normal((9, 16))
+    w, t = Parameters(w.astype(np.float32)), rng.integers(0, 9, 6)
+    _, lse = F.linear_cross_entropy(x, w, t, extras=True)
+    gx, gw = F.linear_cross_entropy_backward(x, w, t, lse, grad=grad)
+    full_x, full_w = F.linear_cross_entropy_backward(x, w, t, lse)
+    # (a quarter is exact in every step)
+    assert np.array_equal(gx, 0.25 * full_x) and np.array_equal(gw, 0.25 * full_w)
+    if np.ndim(grad) == 0:
+        rows = F.linear_cross_entropy_backward(x, w, t, lse, grad=grad, reduction="none")[0]
+        want = F.linear_cross_entropy_backward(x, w, t, lse, reduction="sum")[0]
+        assert np.array_equal(rows, 0.25 * want)
