@@ -460,7 +460,8 @@ size_t novaq_linear_cross_entropy_backward_workspace(int64_t N, int64_t D, int64
  * of target_bits (32 or 64) bits, element-aligned.  The products run in f16
  * where x is F16, else in bf16, on operands rounded to that type (FP8 / FP4
  * codes are exact in both), with fp32 sums, maxima and exponentials.  A target
- * outside 0 .. V - 1 that is not ignore_index gives a NaN loss.  loss: N values
+ * outside 0 .. V - 1 that is not ignore_index gives a NaN loss.  N up to 2^27, V
+ * up to 2^31 - 256, N D and min(V, 2^21) D below 2^37 (NOVAQ_ENOTSUP).  loss: N values
  * (NOVAQ_REDUCE_NONE) or one; lse: N values, for the backward.
  * No reference counterpart as one call: it stands for F.linear followed by
  * CrossEntropyLoss (novann/losses/loss_functions.py:8-167), on logits instead

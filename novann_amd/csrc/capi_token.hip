@@ -37,14 +37,26 @@ int check_ids(const void* ids, int bits) {
   return NOVAQ_OK;
 }
 
+// The vocabulary loss's sizes: a launch's threads stay below 2^32.  N (whose pieces of
+// the vocabulary have 1024 rows at least) by the logits' tiles, V by the kernel that
+// reads it as stored, 256 rows a workgroup; N and a piece of V (2^21 rows at most) with
+// D by the gradients' tiles.
+int check_loss_sizes(int64_t N, int64_t V, int64_t D) {
+  auto tiles = [](int64_t a) { return (a + 127) / 128; };
+  if (N > ((int64_t)1 << 27) || V > INT - 255) return NOVAQ_ENOTSUP;
+  const int64_t piece = std::min<int64_t>(V, 1 << 21);
+  if (std::max(tiles(N), tiles(piece)) * tiles(D) >= (1 << 23)) return NOVAQ_ENOTSUP;
+  return NOVAQ_OK;
+}
+
 int check_loss(const void* x, int x_dtype, int64_t N, int64_t D, const void* w, int w_dtype,
                const float* w_scale, int64_t V, const void* targets, int bits, int reduction) {
   if (!plain_float(x_dtype)) return NOVAQ_EDTYPE;
   int rc = check_table(w_dtype, w_scale, V, D);
   if (rc != NOVAQ_OK) return rc;
   if (N < 0 || reduction < NOVAQ_REDUCE_NONE || reduction > NOVAQ_REDUCE_SUM) return NOVAQ_EINVAL;
-  // (tiles of 128 x 128 are counted in 31 bits)
-  if (N >= INT - 1024 || ((N + 127) / 128) * ((V + 127) / 128) > INT) return NOVAQ_ENOTSUP;
+  rc = check_loss_sizes(N, V, D);
+  if (rc != NOVAQ_OK) return rc;
   rc = check_ids(targets, bits);
   if (rc != NOVAQ_OK) return rc;
   if (!w || (N > 0 && (!x || !targets))) return NOVAQ_EINVAL;
@@ -136,16 +148,16 @@ int novaq_embedding_backward(const void* grad, int grad_dtype, const void* ids, 
 
 size_t novaq_linear_cross_entropy_workspace(int64_t N, int64_t D, int64_t V, int x_dtype,
                                             int w_dtype) {
-  if (N <= 0 || N >= INT - 1024 || !plain_float(x_dtype) ||
-      check_table(w_dtype, nullptr, V, D) != NOVAQ_OK)
+  if (N <= 0 || !plain_float(x_dtype) || check_table(w_dtype, nullptr, V, D) != NOVAQ_OK ||
+      check_loss_sizes(N, V, D) != NOVAQ_OK)
     return 256;
   return vocab_loss_workspace(N, D, V, x_dtype, w_dtype, false);
 }
 
 size_t novaq_linear_cross_entropy_backward_workspace(int64_t N, int64_t D, int64_t V, int x_dtype,
                                                      int w_dtype) {
-  if (N <= 0 || N >= INT - 1024 || !plain_float(x_dtype) ||
-      check_table(w_dtype, nullptr, V, D) != NOVAQ_OK)
+  if (N <= 0 || !plain_float(x_dtype) || check_table(w_dtype, nullptr, V, D) != NOVAQ_OK ||
+      check_loss_sizes(N, V, D) != NOVAQ_OK)
     return 256;
   return vocab_loss_workspace(N, D, V, x_dtype, w_dtype, true);
 }

@@ -1031,6 +1031,8 @@ int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, boo
   // (256 rows of P within 31 bits of bytes, whatever N)
   if (backward) most = std::min(most, ((int64_t)1 << 26) / std::max<int64_t>(N, 32));
   if (copy_w) most = std::min(most, ((int64_t)1 << 26) / dp);
+  // (a launch's threads stay below 2^32: fewer than 2^24 tiles of 128 x 128, each 256)
+  most = std::min(most, (((int64_t)1 << 24) - 1) / ((N + 127) / 128) * 128);
   most = std::max<int64_t>(most / 256 * 256, std::min<int64_t>(vr, 1024));
   if (most >= vr) return vr;
   auto cost = [&](int64_t rows) {
@@ -1258,8 +1260,9 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
     // (one workgroup, that sums the losses too, for up to 16 rows; for the 37 of 1024 x
     // 50000 23.5 us a call, with a launch for the sum 20.0)
     alone = N <= 16;
-    hipLaunchKernelGGL(loss_join_kernel, dim3(alone ? 1u : (unsigned)((N + 15) / 16)), dim3(1024), 0,
-                       st, stats, p.vtiles, N, targets, tl, lse, each,
+    hipLaunchKernelGGL(loss_join_kernel,
+                       dim3(alone ? 1u : (unsigned)std::min<int64_t>((N + 15) / 16, 1 << 18)),
+                       dim3(1024), 0, st, stats, p.vtiles, N, targets, tl, lse, each,
                        reduction == NOVAQ_REDUCE_MEAN, scal, out);
     rc = check_launch();
   }
