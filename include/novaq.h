@@ -432,7 +432,8 @@ size_t novaq_embedding_backward_workspace(int64_t N, int64_t V, int64_t D);
  * without a token are not touched (a table shared with the output layer).  grad
  * (N, D) and grad_table in F32, F16 or BF16.  Sums are fp32 in an order that
  * depends on the ids alone, so results repeat bit for bit; one rounding to
- * grad_table's type.  Ids outside 0 .. V - 1 add nothing.  N, V below 2^31.
+ * grad_table's type.  Ids outside 0 .. V - 1 add nothing.  N below 2^30, V
+ * below 2^31 - 1.
  * workspace: novaq_embedding_backward_workspace() bytes, 16-byte aligned, not
  * used after the call's kernels complete. */
 int novaq_embedding_backward(const void *grad, int grad_dtype, const void *ids, int id_bits,

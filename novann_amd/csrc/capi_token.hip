@@ -19,6 +19,9 @@ bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(
 bool plain_float(int dt) { return dt == F32 || dt == F16 || dt == BF16; }
 bool any_weight(int dt) { return dt >= F32 && dt <= E2M1; }
 constexpr int64_t INT = 0x7FFFFFFF;
+// The embedding's gradient: 64 threads for 16 sorted tokens, fewer than 2^32 in a
+// launch, and positions (with a block's and a wave's more) in 31 bits.
+constexpr int64_t MOST_TOKENS = (int64_t)1 << 30;
 
 // A (V, D) table: its type and whether it may have a scale, its sizes (256 fp32
 // rows stay within a buffer's 2 GiB).
@@ -122,7 +125,7 @@ int novaq_embedding(const void* ids, int id_bits, int64_t N, const void* table, 
 }
 
 size_t novaq_embedding_backward_workspace(int64_t N, int64_t V, int64_t D) {
-  if (N <= 0 || N >= INT - 1024 || V <= 0 || V >= INT || D <= 0 || D > (1 << 20)) return 0;
+  if (N <= 0 || N >= MOST_TOKENS || V <= 0 || V >= INT || D <= 0 || D > (1 << 20)) return 0;
   return embedding_backward_workspace(N, V, D);
 }
 
@@ -134,7 +137,7 @@ int novaq_embedding_backward(const void* grad, int grad_dtype, const void* ids, 
   int rc = check_table(out_dtype, nullptr, V, D);
   if (rc != NOVAQ_OK) return rc;
   if (N < 0) return NOVAQ_EINVAL;
-  if (N >= INT - 1024) return NOVAQ_ENOTSUP;
+  if (N >= MOST_TOKENS) return NOVAQ_ENOTSUP;
   rc = check_ids(ids, id_bits);
   if (rc != NOVAQ_OK) return rc;
   if (!grad_table || (N > 0 && (!grad || !ids))) return NOVAQ_EINVAL;

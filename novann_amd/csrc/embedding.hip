@@ -465,15 +465,15 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(
 
 // The runs that span chunks: the chunk where one begins adds its tail and the
 // heads of the chunks after it.  Eight waves take every eighth head each; their
-// sums are added in the waves' order.
+// sums are added in the waves' order.  The launch's chunks start at chunk0.
 template <int OT, int VEC>
 __global__ __launch_bounds__(512) void embedding_join_kernel(
-    const uint32_t* __restrict__ keys, int N, int CHUNK, int64_t V, int64_t D, float factor,
-    int accumulate, const float* __restrict__ head, const float* __restrict__ tail,
+    const uint32_t* __restrict__ keys, int chunk0, int N, int CHUNK, int64_t V, int64_t D,
+    float factor, int accumulate, const float* __restrict__ head, const float* __restrict__ tail,
     uint8_t* __restrict__ out) {
   constexpr int OB = OT == F32 ? 4 : 2;
   __shared__ float part[8][64 * VEC];
-  const int chunk = blockIdx.x, lane = threadIdx.x & 63;
+  const int chunk = chunk0 + (int)blockIdx.x, lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int e0 = chunk * CHUNK, e1 = e0 + CHUNK;
   if (e1 >= N) return;
@@ -691,10 +691,15 @@ int sums(const EmbedPlan& p, const uint8_t* grad, const uint32_t* keys, const ui
     hipLaunchKernelGGL((embedding_sum_kernel<GT, OT, VEC, 16>), grid, dim3(256), 0, st, grad, keys,
                        pos, (int)N, V, D, factor, accumulate, head, tail, out);
   int rc = check_launch();
-  if (rc != NOVAQ_OK || p.chunks < 2) return rc;
-  hipLaunchKernelGGL((embedding_join_kernel<OT, VEC>), dim3((unsigned)p.chunks, cols), dim3(512),
-                     0, st, keys, (int)N, p.chunk, V, D, factor, accumulate, head, tail, out);
-  return check_launch();
+  // (a launch's threads stay below 2^32)
+  constexpr int64_t most = (int64_t)1 << 22;
+  for (int64_t c0 = 0; c0 < p.chunks && p.chunks > 1 && rc == NOVAQ_OK; c0 += most) {
+    hipLaunchKernelGGL((embedding_join_kernel<OT, VEC>),
+                       dim3((unsigned)std::min(most, p.chunks - c0), cols), dim3(512), 0, st, keys,
+                       (int)c0, (int)N, p.chunk, V, D, factor, accumulate, head, tail, out);
+    rc = check_launch();
+  }
+  return rc;
 }
 
 template <int GT, int OT>

@@ -31,3 +31,21 @@ def test_loss_of_more_logits_than_one_launch():
     assert np.abs(host(each)[at] - want).max() <= 2 * e
     del x, each, lse
     torch.cuda.empty_cache()
+
+
+def test_embedding_gradient_of_more_tokens_than_one_launch():
+    """Sums of 2^27 tokens join 2^23 parts, 512 threads each; gradients of 0 and 1, whose
+    sums fp32 holds exactly in any order."""
+    N, V = (1 << 27) + 5, 700
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(2)
+    ids = torch.randint(0, V, (N,), generator=gen, device="cuda", dtype=torch.int32)
+    ids[-3:] = V - 1
+    g = torch.randint(0, 2, (N, 1), generator=gen, device="cuda").to(torch.bfloat16)
+    got = F.embedding_backward(g, ids, (V, 1))
+    want = torch.zeros(V, dtype=torch.float64, device="cuda")
+    for k in range(0, N, 1 << 24):
+        want += torch.bincount(ids[k:k + (1 << 24)], g[k:k + (1 << 24), 0].double(), V)
+    assert torch.equal(got[:, 0].double(), want)
+    del ids, g
+    torch.cuda.empty_cache()

@@ -26,3 +26,16 @@ def test_the_largest_have_a_workspace(N, D, V):
     lib = _lib.load()
     assert lib.novaq_linear_cross_entropy_workspace(N, D, V, 2, 2) > 256
     assert lib.novaq_linear_cross_entropy_backward_workspace(N, D, V, 2, 2) > 256
+
+
+def test_embedding_backward():
+    lib = _lib.load()
+
+    def call(N):
+        return lib.novaq_embedding_backward(FAKE, 0, FAKE, 64, N, 50, 8, 1.0, 0, FAKE, 0, FAKE,
+                                            1 << 62, None)
+
+    assert call(1 << 30) == _lib.ENOTSUP
+    assert call((1 << 31) - 1025) == _lib.ENOTSUP
+    assert lib.novaq_embedding_backward_workspace(1 << 30, 50, 8) == 0
+    assert lib.novaq_embedding_backward_workspace((1 << 30) - 1, 50, 8) > 1 << 32
