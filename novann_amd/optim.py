@@ -174,9 +174,9 @@ def _type_codes(tensors, what: str) -> list:
     return codes
 
 
-def _clip(grads, outs, max_norm: float, eps: float) -> torch.Tensor:
-    """The C call on contiguous device tensors; outs: where the clipped ones go,
-    or None."""
+def _clip(grads, at, outs, max_norm: float, eps: float) -> torch.Tensor:
+    """The C call on contiguous device tensors; at: their addresses; outs: where the
+    clipped ones go, or None."""
     n = len(grads)
     dev = grads[0].device if n else _device()
     # the rows of novaq_gradient: address, address, count, the two types (an array
@@ -184,7 +184,7 @@ def _clip(grads, outs, max_norm: float, eps: float) -> torch.Tensor:
     types = _type_codes(grads, "gradients")
     counts = list(map(_numel, grads))
     table = array("q", bytes(32 * n))
-    table[0::4] = at = array("q", list(map(_data_ptr, grads)))
+    table[0::4] = at = array("q", at)
     table[2::4] = array("q", counts)
     if outs is not None:
         if outs is not grads and list(map(_numel, outs)) != counts:
@@ -215,9 +215,6 @@ def _elements(g):
 def _distinct(grads) -> list:
     """The gradients, one whose elements an earlier one names left out: it would
     count twice, and be scaled twice in place."""
-    if set(map(type, grads)) == {torch.Tensor} and \
-            len(set(map(_data_ptr, grads))) == len(grads):
-        return grads
     kept, seen = [], set()
     for g in grads:
         if isinstance(g, (torch.Tensor, np.ndarray)) and math.prod(g.shape) > 0:
@@ -229,20 +226,22 @@ def _distinct(grads) -> list:
     return kept
 
 
-def _gradients(items) -> list:
+def _gradients(items):
     """The gradients among tensors, arrays and parameters, torch's own among them
     (those with one; one that is named twice, as a shared weight's may be, counts
-    once)."""
+    once), and the addresses of a list of tensors alone, else None."""
     items = list(items)
     if set(map(type, items)) == {torch.Tensor}:
-        return _distinct(items)
+        at = list(map(_data_ptr, items))
+        return (items, at) if len(set(at)) == len(at) else (_distinct(items), None)
     found = [p if isinstance(p, (torch.Tensor, np.ndarray))
              and not isinstance(p, torch.nn.Parameter) else p.grad for p in items]
-    return _distinct([g for g in found if g is not None])
+    return _distinct([g for g in found if g is not None]), None
 
 
-def _uploaded(grads) -> list:
-    """The gradients as contiguous tensors, arrays on the device."""
+def _uploaded(grads, at):
+    """The gradients as contiguous tensors, arrays on the device, and their
+    addresses."""
     def upload(g):
         if isinstance(g, np.ndarray):
             if g.dtype not in (np.float32, np.float64, np.float16):
@@ -250,16 +249,17 @@ def _uploaded(grads) -> list:
             return torch.from_numpy(np.ascontiguousarray(g)).to(_device())
         return g.contiguous()
 
-    if set(map(type, grads)) == {torch.Tensor} and all(map(_contiguous, grads)):
-        return grads
-    return [upload(g) for g in grads]
+    if at is None or not all(map(_contiguous, grads)):
+        grads = [upload(g) for g in grads]
+        at = list(map(_data_ptr, grads))
+    return grads, at
 
 
 def grad_norm(gradients: Iterable) -> torch.Tensor:
     """The 2-norm over all elements of all gradients (device tensors, numpy
     arrays, or parameters, whose ``grad`` counts), a 0-d fp32 device tensor.
     Squares are summed in fp64; one gradient named twice counts once."""
-    return _clip(_uploaded(_gradients(gradients)), None, 0.0, 0.0)
+    return _clip(*_uploaded(*_gradients(gradients)), None, 0.0, 0.0)
 
 
 def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
@@ -280,16 +280,18 @@ def clip_grad_norm(gradients: Iterable, max_norm: float, *, eps: float = 1e-6,
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0.0 or not eps >= 0.0:
         raise ValueError(f"max_norm and eps must not be negative, got {max_norm} and {eps}")
-    found = _gradients(gradients)
-    grads = _uploaded(found)
+    found, at = _gradients(gradients)
+    grads, at = _uploaded(found, at)
     if out is not None:
         outs = list(out)
         if len(outs) != len(grads):
             raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
         if not all(map(_contiguous, outs)):
             raise ValueError("every out must be contiguous")
-        return _clip(grads, outs, max_norm, eps)
-    norm = _clip(grads, grads, max_norm, eps)
+        return _clip(grads, at, outs, max_norm, eps)
+    norm = _clip(grads, at, grads, max_norm, eps)
+    if grads is found:
+        return norm
     for g, d in zip(found, grads):
         if isinstance(g, np.ndarray):
             g[...] = d.cpu().numpy()
