@@ -509,8 +509,10 @@ size_t novaq_clip_grad_norm_workspace(int64_t count);
  * and out = g * min(1, max_norm / (norm + eps)) for each gradient that has an out:
  * the factor in fp64, rounded to fp32 for one fp32 multiply where the gradient is
  * not F64, the product rounded to out's type.  *norm is rounded to fp32 (infinite
- * past its range).  The list is host memory, read before the call returns.  A NaN norm makes every output NaN; an infinite one
- * makes finite gradients 0.
+ * past its range).  The list is host memory, read before the call returns (past 128
+ * rows its check takes 48 bytes of host memory a row, NOVAQ_ESCRATCH if there are
+ * none).  A NaN norm makes every output NaN; an infinite one makes finite gradients
+ * 0.
  * Stands for the clipping inside SGD.step (novann/optim/sgd.py:37-82), for any
  * optimizer. */
 int novaq_clip_grad_norm(const novaq_gradient *list, int64_t count, double max_norm, double eps,

@@ -1023,7 +1023,8 @@ int logit_splits(int64_t N, int64_t V, int64_t D, double* us) {
 
 // The rows of a piece (a multiple of 256): at most 128 MiB of P (and of the
 // table's 16-bit copy), so that what one product writes the next ones find in
-// the 256 MB cache; among the sizes that divide the vocabulary into about that
+// the 256 MB cache, but 1024 rows where the vocabulary has them (P of more than
+// 65536 tokens is then larger: 2304 bytes a token); among the sizes that divide the vocabulary into about that
 // many pieces, the one whose products take the least time by the model above.
 int64_t loss_piece(int64_t N, int64_t D, int64_t dp, int64_t V, bool copy_w, bool backward) {
   const int64_t vr = (V + 255) / 256 * 256;
@@ -1084,9 +1085,14 @@ LossPlan loss_plan(int64_t N, int64_t D, int64_t V, int x_dtype, int w_dtype, bo
     const int E = 128 / dtype_bits(w_dtype), nt = stream_tiles(N);
     // a small table's few workgroups take their stages one after another, each the
     // longer the more fragments it copies: 0.54 us for one tile of tokens with E4M3
-    // codes, 1.6 for four, 2.9 with E2M1 ones (the split logits trade the join for a
-    // copy of the table: 2 us less than the model's; 103 tokens of 2560, 1280 classes
-    // E4M3: 44 us so, 21 split; 1 token: 18.9 so)
+    // codes, 1.6 for four, 2.9 with E2M1 ones; the split logits have a copy of the
+    // table in place of a join, taken as 2 us less than the model's.  GPU time of a
+    // call so and split: 103 tokens of 2560, 1280 classes E4M3 43.9 and 19.9 us; 37 of
+    // 4096, 5000 E2M1 39.4 and 34.1; 1 of 4096, 5000 E4M3 23.8 and 33.6; 16 of 4096,
+    // 2000 E2M1 22.0 and 23.0.  Of 108 shapes (1 to 128 tokens of 1024 to 8192, 512 to
+    // 5000 classes, E4M3, E2M1, bf16) the rule takes the faster side for 83 and loses
+    // at most 11 us on the others (64 of 2560, 1280 classes E2M1: 28.9 us, split 18.4;
+    // 128 of 1024, 1000 classes E4M3: 23.8 and 16.3).
     const int64_t stages = (D + 8 * E - 1) / (8 * E);
     if (p.lsplits > 1 && (double)stages * (0.2 + 0.17 * (E / 8) * nt) > logits_us - 2.0)
       p.stream = false;
@@ -1257,8 +1263,8 @@ int forward(const LossPlan& p, const void* x, int x_dtype, int64_t N, int64_t D,
   float* out = reduction == NOVAQ_REDUCE_NONE ? nullptr : loss;
   bool alone = false;
   if (p.lsplits == 1) {
-    // (one workgroup, that sums the losses too, for up to 16 rows; for the 37 of 1024 x
-    // 50000 23.5 us a call, with a launch for the sum 20.0)
+    // (one workgroup, that sums the losses too, for up to 16 rows; the 37 of 1024 x
+    // 50000 take 23.5 us a call so, with a workgroup for 16 rows each 20.0)
     alone = N <= 16;
     hipLaunchKernelGGL(loss_join_kernel,
                        dim3(alone ? 1u : (unsigned)std::min<int64_t>((N + 15) / 16, 1 << 18)),
