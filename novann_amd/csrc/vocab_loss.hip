@@ -863,7 +863,7 @@ __global__ __launch_bounds__(256) void loss_sums_store_kernel(const float* __res
                                                             const float* __restrict__ fx,
                                                             void* __restrict__ out) {
   __shared__ float4 part[SHARE ? 3 * 64 : 1];
-  const float s = w_scale ? *w_scale : 1.0f, all = scal[0] * s * inv_pscale;
+  const float scale = w_scale ? *w_scale : 1.0f, all = scal[0] * scale * inv_pscale;
   const int64_t per = dp / 4, total = N * per;
   constexpr int STEP = SHARE ? 4 : 1, UNITS = 256 / STEP;
   const int from = SHARE ? threadIdx.x >> 6 : 0, unit = SHARE ? threadIdx.x & 63 : threadIdx.x;
@@ -890,7 +890,7 @@ __global__ __launch_bounds__(256) void loss_sums_store_kernel(const float* __res
     }
     if (from > 0 || q0 + unit >= total || c >= D) continue;
     const bool none = targets && targets[n] == T_NONE;
-    const float a = fx ? fx[n] * s * inv_pscale : all;
+    const float a = fx ? fx[n] * scale * inv_pscale : all;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = none ? 0.0f : rounded(v[i] * a);
     const int64_t e = n * D + c;
