@@ -327,16 +327,10 @@ def prepare(case, seed):
         s["w"], s["g"] = w, g.to(TORCH[case["gdtype"]])
         if case["bits"] == 8:
             s["s"] = _pack(m, v, seed)
-            states = [(s["s"]["m"], 1), (s["s"]["me"], BLOCK), (s["s"]["v"], 1),
-                      (s["s"]["ve"], BLOCK)]
         else:
             s["m"], s["v"] = m, v
-            states = [(m, 1), (v, 1)]
         if op == "blocks":
             s["codes"] = _codes(case, w)
-        # (as a program holds them: lists of tensors, which are the buffers' parts)
-        s["weights"], s["grads"] = _parts(s["w"], shapes), _parts(s["g"], shapes)
-        s["states"] = list(zip(*(_parts(f, shapes, unit) for f, unit in states)))
     return s
 
 
@@ -379,11 +373,18 @@ def _own(s):
         y, kept = F.block_linear(s["x"], w, s["bias"], out_dtype=case["xdtype"], extras=True)
         gx, gw, gb = F.block_linear_backward(s["g"], kept, w, grad_dtype=case["gdtype"])
         return {"out": y, "grad_input": gx, "grad_weight": gw, "grad_bias": gb.view(-1)}
-    weights = s["weights"]
+    shapes = _shapes(case)
+    if case["bits"] == 8:
+        names = [("m", 1), ("me", BLOCK), ("v", 1), ("ve", BLOCK)]
+        states = [optim.State8(*parts) for parts in zip(
+            *(_parts(s["s"][k], shapes, unit) for k, unit in names))]
+    else:
+        states = list(zip(_parts(s["m"], shapes), _parts(s["v"], shapes)))
+    weights = _parts(s["w"], shapes)
     if case["op"] == "blocks":
         weights = [_quantized(w, *c) for w, c in zip(weights, zip(*(
             s["codes"][k] for k in ("q", "e", "qt", "et"))))]
-    optim.adamw_step(weights, s["grads"], s["states"], step=s["t"], seed=s["t"], **ADAM)
+    optim.adamw_step(weights, _parts(s["g"], shapes), states, step=s["t"], seed=s["t"], **ADAM)
     out = {"w": s["w"]}
     if case["bits"] == 8:
         out["m"], out["v"] = optim.State8(*(s["s"][k] for k in ("m", "me", "v", "ve"))).decode(
