@@ -368,7 +368,7 @@ class AdamW:
         for i, p in enumerate(self.params):
             if p.grad is None:
                 continue
-            if _is_f64(p):
+            if self._w[i].dtype == torch.float64:  # (its states' type, whatever .data is now)
                 self._step_f64(i)
                 continue
             data = getattr(p, "data", None)
@@ -415,7 +415,7 @@ class AdamW:
 
     def _step_f64(self, i: int) -> None:
         p, w = self.params[i], self._w[i]
-        w.copy_(torch.from_numpy(np.ascontiguousarray(p.data).reshape(w.shape)))
+        w.copy_(torch.from_numpy(np.ascontiguousarray(p.data, dtype=np.float64).reshape(w.shape)))
         hp = self._hp(0 if getattr(p, "name", None) in ("gamma", "beta") else 1)
         g, g32 = _dev_grad64(p.grad, w.device)
         if g.numel() != w.numel():

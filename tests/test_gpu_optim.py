@@ -184,3 +184,19 @@ def test_batchnorm_parameters_as_constructed():
     assert bn.gamma.data.dtype == bn.beta.data.dtype == np.float64
     assert np.array_equal(bn.gamma.data.view(np.uint64), ref["g"][0].view(np.uint64))
     assert np.array_equal(bn.beta.data.view(np.uint64), ref["b"][0].view(np.uint64))
+
+
+@pytest.mark.parametrize("first,later", [(np.float32, np.float64), (np.float64, np.float32)])
+def test_arrays_set_to_another_type(first, later):
+    """.data set to an array of another float type steps in the type of its states."""
+    rng = np.random.default_rng(11)
+    p = Parameters(rng.standard_normal((3, 40)).astype(first))
+    opt = AdamW([p], lr=0.01, weight_decay=0.1)
+    step = OR.adamw_step if first == np.float32 else OR.adamw_step_f64
+    m = v = np.zeros((3, 40), first)
+    for t in (1, 2):
+        p.data = rng.standard_normal((3, 40)).astype(later)
+        p.grad = rng.standard_normal((3, 40)).astype(np.float32)
+        w, m, v = step(p.data.astype(first), p.grad, m, v, t, 0.01, wd=0.1)
+        opt.step()
+        assert p.data.dtype == later and np.array_equal(p.data, w.astype(later))

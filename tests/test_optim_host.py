@@ -1,0 +1,33 @@
+"""AdamW's host side (tests/optim_host.py): which tensors its calls are given, in which order."""
+import numpy as np
+import pytest
+
+from novann_amd import optim
+from novann_amd.module import Parameters
+from oracle import optim_ref as OR
+from tests.optim_host import library  # noqa: F401  (a fixture)
+
+HP = dict(lr=0.01, weight_decay=0.1)
+
+
+def reference(w, g, m, v, t):
+    step = OR.adamw_step if w.dtype == np.float32 else OR.adamw_step_f64
+    return step(w, g, m, v, t, 0.01, 0.9, 0.999, 1e-8, 0.1)
+
+
+@pytest.mark.parametrize("first,later", [(np.float32, np.float64), (np.float64, np.float32)])
+def test_an_array_of_another_type_steps_in_the_states_type(library, first, later):
+    """.data is an attribute that a program may set: the step's type is the one that its
+    states have, and an array of another is converted, both ways."""
+    rng = np.random.default_rng(1)
+    p = Parameters(rng.standard_normal((3, 40)).astype(first))
+    opt = optim.AdamW([p], **HP)
+    library.owned = {t.data_ptr(): t.numel() * t.element_size()
+                     for t in (*opt._w, *opt.m_t, *opt.v_t)}
+    m = v = np.zeros((3, 40), first)
+    for t in (1, 2):
+        w = p.data = rng.standard_normal((3, 40)).astype(later)
+        p.grad = rng.standard_normal((3, 40)).astype(np.float32)
+        want, m, v = reference(w.astype(first), p.grad, m, v, t)
+        opt.step()
+        assert p.data is w and w.dtype == later and np.array_equal(w, want.astype(later))
