@@ -230,7 +230,7 @@ def _step(weights, masters, grads, states, decay, hp, seed: int, scales) -> None
             else:
                 for i, p in zip(which, at):
                     table[column + _ROW * i] = p
-    dev = masters[0].get_device()
+    dev = _get_device(masters[0])
     if dev < 0 or set(map(_get_device, everything)) != {dev}:
         raise ValueError("AdamW: parameters, gradients and states must be CUDA (HIP) device "
                          f"tensors on one device, got {set(map(_get_device, everything))} (-1: "
