@@ -250,17 +250,19 @@ def _step(weights, masters, grads, states, decay, hp, seed: int, scales) -> None
             w.amax, w.scale = st[0:1], st[1:2]
 
 
-def _scales(w) -> Optional[torch.Tensor]:
-    """Two adjacent floats for a per-tensor weight's amax and scale: its own where they are
-    adjacent, so that who reads them goes on with the new ones."""
+def _scales(w, master) -> Optional[torch.Tensor]:
+    """Two adjacent floats on the master's device for a per-tensor weight's amax and scale: its
+    own where they are adjacent there, so that who reads them goes on with the new ones (a
+    product moves a scale that lies elsewhere, the step writes where it says)."""
     if not isinstance(w, QuantizedParameters):
         return None
     a, s = w.amax, w.scale
     if isinstance(a, torch.Tensor) and a.dtype == s.dtype == torch.float32 and \
+            _get_device(a) == _get_device(s) == _get_device(master) and \
             s.data_ptr() == a.data_ptr() + 4 and a.untyped_storage().data_ptr() == \
             s.untyped_storage().data_ptr():
         return a.as_strided((2,), (1,))
-    return torch.empty(2, dtype=torch.float32, device=s.device)
+    return torch.empty(2, dtype=torch.float32, device=master.device)
 
 
 def adamw_step(weights: Iterable, grads: Iterable, states: Iterable, *, lr: float, step: int,
@@ -303,7 +305,7 @@ def adamw_step(weights: Iterable, grads: Iterable, states: Iterable, *, lr: floa
     if not all(map(_contiguous, grads)):
         grads = [g.contiguous() for g in grads]
     _step(weights, masters, grads, states, flags, hp, step if seed is None else seed,
-          [None] * len(weights) if masters is weights else [_scales(w) for w in weights])
+          [None] * len(weights) if masters is weights else list(map(_scales, weights, masters)))
 
 
 class AdamW:
@@ -340,8 +342,8 @@ class AdamW:
                        if state_dtype == "8bit" and w.dtype == torch.float32
                        else (torch.zeros_like(w), torch.zeros_like(w)) for w in self._w]
         self._amax_scale: List[Optional[torch.Tensor]] = [
-            torch.empty(2, dtype=torch.float32, device=dev)
-            if isinstance(p, QuantizedParameters) else None for p in self.params]
+            torch.empty(2, dtype=torch.float32, device=w.device)
+            if isinstance(p, QuantizedParameters) else None for p, w in zip(self.params, self._w)]
         self.m_t = [None if isinstance(s, State8) else s[0] for s in self.states]
         self.v_t = [None if isinstance(s, State8) else s[1] for s in self.states]
 

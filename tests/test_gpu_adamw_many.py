@@ -444,6 +444,22 @@ def test_refusals():
         s.decode("e4m3")
 
 
+def test_a_weight_whose_scale_is_on_the_host():
+    """The products move such a scale to the device; so does the step, which writes it."""
+    rng = np.random.default_rng(12)
+    w = (rng.standard_normal((30, 40)) * 0.05).astype(np.float32)
+    a, b = (QuantizedParameters.from_float(w, "e4m3", keep_master=True) for _ in range(2))
+    pair = torch.cat([b.amax, b.scale]).cpu()
+    b.amax, b.scale = pair[:1], pair[1:]
+    before, g = pair.clone(), torch.randn(30, 40, device="cuda")
+    for p in (a, b):
+        optim.adamw_step([p], [g], [tuple(torch.zeros(30, 40, device="cuda") for _ in range(2))],
+                         lr=0.1, step=1)
+    assert torch.equal(a.master, b.master) and torch.equal(a.scale, b.scale) and b.scale.is_cuda
+    assert torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8))
+    assert torch.equal(pair, before)
+
+
 def test_captured_and_on_another_stream():
     """A captured step replayed beside eager ones: the same states and bits."""
     rng = np.random.default_rng(10)

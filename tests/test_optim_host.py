@@ -1,9 +1,10 @@
 """AdamW's host side (tests/optim_host.py): which tensors its calls are given, in which order."""
 import numpy as np
 import pytest
+import torch
 
 from novann_amd import optim
-from novann_amd.module import Parameters
+from novann_amd.module import Parameters, QuantizedParameters
 from oracle import optim_ref as OR
 from tests.optim_host import library  # noqa: F401  (a fixture)
 
@@ -31,3 +32,17 @@ def test_an_array_of_another_type_steps_in_the_states_type(library, first, later
         want, m, v = reference(w.astype(first), p.grad, m, v, t)
         opt.step()
         assert p.data is w and w.dtype == later and np.array_equal(w, want.astype(later))
+
+
+def test_a_scale_elsewhere_is_not_written(monkeypatch):
+    """A per-tensor weight whose amax and scale lie side by side on another device than its
+    master: the step has two floats of its own beside the master."""
+    st, elsewhere, master = torch.ones(2), torch.ones(2), torch.zeros(4)
+    place = {st.data_ptr(): 0, elsewhere.data_ptr(): -1, master.data_ptr(): 0}
+    monkeypatch.setattr(optim, "_get_device", lambda t: place[t.data_ptr() & ~7])
+    for pair, own in ((st, True), (elsewhere, False)):
+        w = QuantizedParameters(torch.zeros(4, dtype=torch.uint8), (4,), "e4m3", pair[1:], pair[:1],
+                                master=master)
+        got = optim._scales(w, master)
+        assert got.numel() == 2 and got.device == master.device
+        assert (got.data_ptr() == pair.data_ptr()) == own
