@@ -308,6 +308,44 @@ def adamw_step(weights: Iterable, grads: Iterable, states: Iterable, *, lr: floa
           [None] * len(weights) if masters is weights else list(map(_scales, weights, masters)))
 
 
+def _span(a):
+    """Where the elements of an array (-1) or of a contiguous device tensor (its device's
+    index) lie: (place, first byte, end)."""
+    if isinstance(a, torch.Tensor):
+        at = a.data_ptr()
+        return _get_device(a), at, at + a.numel() * a.element_size()
+    at = a.__array_interface__["data"][0]
+    if a.flags.c_contiguous or a.size == 0:
+        return -1, at, at + a.nbytes
+    reach = [(n - 1) * s for n, s in zip(a.shape, a.strides)]
+    return (-1, at + sum(r for r in reach if r < 0),
+            at + sum(r for r in reach if r > 0) + a.itemsize)
+
+
+def _turns(spans) -> list:
+    """For each span 0, or one more than the last turn of the earlier ones that it shares bytes
+    with: the spans of one turn are apart."""
+    turns = [0] * len(spans)
+    group, place, end = [], None, 0
+
+    def number(group):
+        group.sort()
+        for k, i in enumerate(group):
+            for j in group[:k]:
+                if spans[i][1] < spans[j][2] and spans[j][1] < spans[i][2]:
+                    turns[i] = max(turns[i], turns[j] + 1)
+
+    # (groups of spans that reach into one another, from first bytes in order)
+    for i in sorted((i for i, s in enumerate(spans) if s[1] < s[2]), key=spans.__getitem__):
+        if spans[i][0] != place or spans[i][1] >= end:
+            number(group)
+            group, place, end = [], spans[i][0], 0
+        group.append(i)
+        end = max(end, spans[i][2])
+    number(group)
+    return turns
+
+
 class AdamW:
     """AdamW with decoupled weight decay (adamw.py:6-69).
 
@@ -363,25 +401,23 @@ class AdamW:
     def step(self) -> None:
         """One optimization step (adamw.py:41-65)."""
         self.t += 1
-        # parameters of one memory (a shared weight named twice) step one after another, in
-        # their order: the k-th of one memory is in the k-th call
-        calls: List[List[int]] = []
-        seen = {}
+        listed = []
         for i, p in enumerate(self.params):
             if p.grad is None:
                 continue
             if self._w[i].dtype == torch.float64:  # (its states' type, whatever .data is now)
                 self._step_f64(i)
-                continue
-            data = getattr(p, "data", None)
-            at = ("host", data.__array_interface__["data"][0]) if isinstance(
-                data, np.ndarray) else (self._w[i].device, self._w[i].data_ptr())
-            k = seen[at] = seen.get(at, -1) + 1
-            if k == len(calls):
-                calls.append([])
-            calls[k].append(i)
-        for call in calls:
-            self._step_call(call)
+            else:
+                listed.append(i)
+        # parameters that share memory (a weight named twice, views of one buffer) step one after
+        # another, in their order: an array's bytes are its own, its device copy is not
+        spans = []
+        for i in listed:
+            data = getattr(self.params[i], "data", None)
+            spans.append(_span(data if isinstance(data, np.ndarray) else self._w[i]))
+        turns = _turns(spans)
+        for turn in range(max(turns, default=-1) + 1):
+            self._step_call([i for i, k in zip(listed, turns) if k == turn])
 
     def _step_call(self, call: List[int]) -> None:
         for i in call:

@@ -376,6 +376,22 @@ def test_shared_parameters_step_once_for_each_name():
     assert torch.equal(buf, y)
 
 
+def test_arrays_that_overlap_step_one_after_another():
+    """Views of one host array, the second from what the first has left."""
+    rng = np.random.default_rng(13)
+    base = rng.standard_normal(150).astype(np.float32)
+    want = base.copy()
+    ps = [Parameters(base[:100]), Parameters(base[50:]), Parameters(base[1:])]
+    opt = optim.AdamW(ps, lr=0.1, weight_decay=0.02)
+    states = [(np.zeros(p.shape, np.float32),) * 2 for p in ps]
+    for t in (1, 2):
+        for k, (p, part) in enumerate(zip(ps, (want[:100], want[50:], want[1:]))):
+            p.grad = rng.standard_normal(p.shape).astype(np.float32)
+            part[...], *states[k] = OR.adamw_step(part.copy(), p.grad, *states[k], t, 0.1, wd=0.02)
+        opt.step()
+        assert np.array_equal(base, want)
+
+
 def test_class_with_8_bit_states():
     """The class's steps are the list's, seeded by its count."""
     rng = np.random.default_rng(11)

@@ -46,3 +46,50 @@ def test_a_scale_elsewhere_is_not_written(monkeypatch):
         got = optim._scales(w, master)
         assert got.numel() == 2 and got.device == master.device
         assert (got.data_ptr() == pair.data_ptr()) == own
+
+
+def views(kind):
+    """(the buffer, parts of it that share elements, others among them that do not)."""
+    base = np.random.default_rng(2).standard_normal(600).astype(np.float32)
+    return base, {
+        "ends": [base[:100], base[400:500], base[50:150], base[120:220]],
+        "shifted by one": [base, base[1:]],
+        "one inside another": [base[100:200], base[:300], base[120:130]],
+        "columns and rows": [base.reshape(20, 30)[:, :7], base.reshape(20, 30)[3], base[590:]],
+        "backwards": [base[300::-1], base[290:320]],
+        "the same twice": [base[:50], base[50:100], base[:50]],
+    }[kind]
+
+
+@pytest.mark.parametrize("kind", ["ends", "shifted by one", "one inside another",
+                                  "columns and rows", "backwards", "the same twice"])
+def test_overlapping_arrays_step_one_after_another(library, kind):
+    """As the reference steps them: each from what the one before it has left."""
+    base, parts = views(kind)
+    want = base.copy()
+
+    def in_copy(a):
+        at = a.__array_interface__["data"][0] - base.__array_interface__["data"][0]
+        return np.ndarray(a.shape, a.dtype, want.data, at, a.strides)
+
+    ps = [Parameters(a) for a in parts]
+    opt = optim.AdamW(ps, **HP)
+    rng = np.random.default_rng(3)
+    states = [(np.zeros(a.shape, np.float32),) * 2 for a in parts]
+    for t in (1, 2):
+        for k, p in enumerate(ps):
+            p.grad = rng.standard_normal(p.shape).astype(np.float32)
+            w = in_copy(parts[k])
+            w[...], *states[k] = reference(w.copy(), p.grad, *states[k], t)
+        opt.step()
+        assert np.array_equal(base, want)
+
+
+def test_arrays_side_by_side_are_one_call(library):
+    base = np.ones(300, np.float32)
+    ps = [Parameters(base[100 * i:100 * i + 100]) for i in (2, 0, 1)] + [
+        Parameters(np.ones(0, np.float32)) for _ in range(2)]
+    for p in ps:
+        p.grad = np.ones(p.shape, np.float32)
+    optim.AdamW(ps, **HP).step()
+    assert [count for count, _ in library.calls] == [5]
