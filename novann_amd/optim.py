@@ -192,9 +192,10 @@ _F32, _U8, _E4M3 = {torch.float32: 0}, {torch.uint8: 0}, {torch.float8_e4m3fn: 0
 _STATES, _STATES8 = ((2, _F32), (3, _F32)), ((2, _E4M3), (4, _U8), (3, _U8), (5, _U8))
 
 
-def _step(weights, masters, grads, states, decay, hp, seed: int, scales) -> None:
-    """The C call for lists of at least one.  masters: what is stepped; decay: a list or
-    None; scales: for each weight where a per-tensor one's amax and scale go, or None."""
+def _rows(weights, masters, grads, states, decay, scales) -> array:
+    """The rows of novaq_adamw_tensor for lists of at least one, once everything that they
+    name is looked at.  masters: what is stepped; decay: a list or None; scales: for each
+    weight where a per-tensor one's amax and scale go, or None."""
     counts = list(map(_numel, masters))
     sizes = list(map(len, states))
     if sizes.count(2) + sizes.count(4) != len(sizes):
@@ -240,14 +241,20 @@ def _step(weights, masters, grads, states, decay, hp, seed: int, scales) -> None
     for i, w in enumerate(weights):
         if isinstance(w, (QuantizedParameters, BlockQuantizedParameters)):
             _stored(table, _ROW * i, w, counts[i], scales[i], dev)
-    check(quant.on_device(masters[0].device, _lib.load().novaq_adamw_many,
-                          table.buffer_info()[0], len(masters), ctypes.byref(hp), _key(seed)),
-          "adamw step")
-    for w, st in zip(weights, scales):
-        if st is not None:
-            # the codes and scale the products read now follow the master (the next step
-            # rewrites st after this step's readers, in stream order)
-            w.amax, w.scale = st[0:1], st[1:2]
+    return table
+
+
+def _launch(table: array, weights, scales, dev, hp, seed: int) -> int:
+    """The C call's status; nothing was launched where it is NOVAQ_EINVAL."""
+    rc = quant.on_device(dev, _lib.load().novaq_adamw_many, table.buffer_info()[0],
+                         len(table) // _ROW, ctypes.byref(hp), _key(seed))
+    if rc == _lib.OK:
+        for w, st in zip(weights, scales):
+            if st is not None:
+                # the codes and scale the products read now follow the master (the next step
+                # rewrites st after this step's readers, in stream order)
+                w.amax, w.scale = st[0:1], st[1:2]
+    return rc
 
 
 def _scales(w, master) -> Optional[torch.Tensor]:
@@ -304,8 +311,10 @@ def adamw_step(weights: Iterable, grads: Iterable, states: Iterable, *, lr: floa
         masters = [_master(w) for w in weights]
     if not all(map(_contiguous, grads)):
         grads = [g.contiguous() for g in grads]
-    _step(weights, masters, grads, states, flags, hp, step if seed is None else seed,
-          [None] * len(weights) if masters is weights else list(map(_scales, weights, masters)))
+    scales = [None] * len(weights) if masters is weights else list(map(_scales, weights, masters))
+    table = _rows(weights, masters, grads, states, flags, scales)
+    check(_launch(table, weights, scales, masters[0].device, hp, step if seed is None else seed),
+          "adamw step")
 
 
 def _span(a):
@@ -322,27 +331,31 @@ def _span(a):
             at + sum(r for r in reach if r > 0) + a.itemsize)
 
 
-def _turns(spans) -> list:
-    """For each span 0, or one more than the last turn of the earlier ones that it shares bytes
-    with: the spans of one turn are apart."""
-    turns = [0] * len(spans)
+def _turns(count: int, spans) -> list:
+    """For each of so many parameters 0, or one more than the last turn of the earlier ones
+    whose memory it shares.  spans: (parameter, place, first byte, end, whether the step writes
+    there); what is only read may be shared."""
+    spans = sorted((s for s in spans if s[2] < s[3]), key=lambda s: s[1:3])
+    before = {}  # parameter -> the earlier ones that it waits for
     group, place, end = [], None, 0
 
-    def number(group):
-        group.sort()
-        for k, i in enumerate(group):
-            for j in group[:k]:
-                if spans[i][1] < spans[j][2] and spans[j][1] < spans[i][2]:
-                    turns[i] = max(turns[i], turns[j] + 1)
+    def share(group):
+        for k, a in enumerate(group):
+            for b in group[:k]:
+                if a[0] != b[0] and (a[4] or b[4]) and a[2] < b[3] and b[2] < a[3]:
+                    before.setdefault(max(a[0], b[0]), []).append(min(a[0], b[0]))
 
     # (groups of spans that reach into one another, from first bytes in order)
-    for i in sorted((i for i, s in enumerate(spans) if s[1] < s[2]), key=spans.__getitem__):
-        if spans[i][0] != place or spans[i][1] >= end:
-            number(group)
-            group, place, end = [], spans[i][0], 0
-        group.append(i)
-        end = max(end, spans[i][2])
-    number(group)
+    for s in spans:
+        if s[1] != place or s[2] >= end:
+            share(group)
+            group, place, end = [], s[1], 0
+        group.append(s)
+        end = max(end, s[3])
+    share(group)
+    turns = [0] * count
+    for i in sorted(before):
+        turns[i] = 1 + max(turns[j] for j in before[i])
     return turns
 
 
@@ -395,69 +408,93 @@ class AdamW:
             g = torch.nn.functional.pad(g.reshape(p.shape), (0, 1))
         return g.contiguous().reshape(w.shape)
 
-    def _hp(self, decay: int) -> "_lib.AdamW":
-        return _lib.AdamW(self.lr, self.b1, self.b2, self.eps, self.wd, self.t, decay)
+    def _hp(self, decay: int, t: int) -> "_lib.AdamW":
+        return _lib.AdamW(self.lr, self.b1, self.b2, self.eps, self.wd, t, decay)
 
     def step(self) -> None:
-        """One optimization step (adamw.py:41-65)."""
-        self.t += 1
-        listed = []
+        """One optimization step (adamw.py:41-65).  All gradients, states and codes are looked
+        at before anything is launched: a step that is refused changes nothing."""
+        t = self.t + 1
+        wide, listed, grads = [], [], {}
         for i, p in enumerate(self.params):
             if p.grad is None:
                 continue
             if self._w[i].dtype == torch.float64:  # (its states' type, whatever .data is now)
-                self._step_f64(i)
+                wide.append((i, *self._grad64(i)))
             else:
                 listed.append(i)
+                grads[i] = self._grad(p, self._w[i])
         # parameters that share memory (a weight named twice, views of one buffer) step one after
         # another, in their order: an array's bytes are its own, its device copy is not
         spans = []
-        for i in listed:
+        for k, i in enumerate(listed):
             data = getattr(self.params[i], "data", None)
-            spans.append(_span(data if isinstance(data, np.ndarray) else self._w[i]))
-        turns = _turns(spans)
-        for turn in range(max(turns, default=-1) + 1):
-            self._step_call([i for i, k in zip(listed, turns) if k == turn])
+            spans.append((k, *_span(data if isinstance(data, np.ndarray) else self._w[i]), True))
+        calls = {}
+        for turn, i in sorted(zip(_turns(len(listed), spans), listed)):
+            calls.setdefault((turn, self._w[i].device), []).append(i)
+        tables = [self._rows(call, grads) for call in calls.values()]
+        for call, table in zip(calls.values(), tables):
+            self._step_call(call, table, grads, t)
+            self.t = t
+        for i, g, g32 in wide:
+            self._step_f64(i, g, g32, t)
+            self.t = t
+        self.t = t
 
-    def _step_call(self, call: List[int]) -> None:
-        for i in call:
-            data = getattr(self.params[i], "data", None)
-            if isinstance(data, np.ndarray):
-                # the caller may have changed .data since the last step
-                self._w[i].copy_(torch.from_numpy(np.ascontiguousarray(data).reshape(
-                    self._w[i].shape).astype(np.float32, copy=False)))
-        ps, ws = [self.params[i] for i in call], [self._w[i] for i in call]
-        grads = [self._grad(p, w) for p, w in zip(ps, ws)]
-        decay = [getattr(p, "name", None) not in ("gamma", "beta") for p in ps]
-        states = [self.states[i] for i in call]
-        scales = [self._amax_scale[i] for i in call]
-        by_device = {}
-        for k, w in enumerate(ws):
-            by_device.setdefault(w.device, []).append(k)
+    def _rows(self, call: List[int], grads) -> array:
+        ps = [self.params[i] for i in call]
+        return _rows(ps, [self._w[i] for i in call], [grads[i] for i in call],
+                     [self.states[i] for i in call],
+                     [getattr(p, "name", None) not in ("gamma", "beta") for p in ps],
+                     [self._amax_scale[i] for i in call])
 
-        def run(ks):
-            part, m, g, s, d, a = ([x[k] for k in ks] for x in (ps, ws, grads, states, decay, scales))
-            _step(part, m, g, s, d, self._hp(1), self.t, a)
+    def _launch(self, call: List[int], table: array, t: int) -> int:
+        return _launch(table, [self.params[i] for i in call], [self._amax_scale[i] for i in call],
+                       self._w[call[0]].device, self._hp(1, t), t)
 
-        for ks in by_device.values():
-            try:
-                run(ks)
-            except ValueError:
-                # (nothing was launched) parameters that overlap step one after another; what
-                # else is wrong shows again
-                for k in ks:
-                    run([k])
-        for p, w in zip(ps, ws):
-            if isinstance(getattr(p, "data", None), np.ndarray):
-                p.data[...] = w.cpu().numpy().reshape(p.data.shape)
-
-    def _step_f64(self, i: int) -> None:
+    def _memory(self, k: int, i: int, g: torch.Tensor):
+        """The spans of parameter i of a call, its k-th."""
         p, w = self.params[i], self._w[i]
-        w.copy_(torch.from_numpy(np.ascontiguousarray(p.data, dtype=np.float64).reshape(w.shape)))
-        hp = self._hp(0 if getattr(p, "name", None) in ("gamma", "beta") else 1)
-        g, g32 = _dev_grad64(p.grad, w.device)
+        written = [w, *self.states[i], self._amax_scale[i]]
+        written += [getattr(p, name, None) for name in ("codes", "exponents", "codes_t",
+                                                        "exponents_t")]
+        spans = [(k, *_span(x), True) for x in written if x is not None]
+        if g.data_ptr() != w.data_ptr():
+            spans.append((k, *_span(g), False))
+        return spans
+
+    def _step_call(self, call: List[int], table: array, grads, t: int) -> None:
+        arrays = [(p.data, self._w[i]) for i, p in ((i, self.params[i]) for i in call)
+                  if isinstance(getattr(p, "data", None), np.ndarray)]
+        for data, w in arrays:
+            # the caller may have changed .data since the last step
+            w.copy_(torch.from_numpy(np.ascontiguousarray(data).reshape(w.shape).astype(
+                np.float32, copy=False)))
+        rc = self._launch(call, table, t)
+        if rc == _lib.EINVAL:
+            # memory that parameters share otherwise (one's gradient another's weight): in turn too
+            turns = _turns(len(call), [s for k, i in enumerate(call)
+                                       for s in self._memory(k, i, grads[i])])
+            for turn in range(max(turns) + 1) if any(turns) else ():
+                part = [i for i, n in zip(call, turns) if n == turn]
+                rc = self._launch(part, self._rows(part, grads), t)
+                check(rc, "adamw step")
+        check(rc, "adamw step")
+        for data, w in arrays:
+            data[...] = w.cpu().numpy().reshape(data.shape)
+
+    def _grad64(self, i: int):
+        w = self._w[i]
+        g, g32 = _dev_grad64(self.params[i].grad, w.device)
         if g.numel() != w.numel():
             raise ValueError(f"AdamW: gradient of {g.numel()} values for a parameter of {w.numel()}")
+        return g, g32
+
+    def _step_f64(self, i: int, g: torch.Tensor, g32: bool, t: int) -> None:
+        p, w = self.params[i], self._w[i]
+        w.copy_(torch.from_numpy(np.ascontiguousarray(p.data, dtype=np.float64).reshape(w.shape)))
+        hp = self._hp(0 if getattr(p, "name", None) in ("gamma", "beta") else 1, t)
         check(quant.on_device(w.device, _lib.load().novaq_adamw_step_f64, w.data_ptr(), g.data_ptr(),
                               int(g32), self.m_t[i].data_ptr(), self.v_t[i].data_ptr(), w.numel(),
                               ctypes.byref(hp)), "adamw f64")

@@ -26,6 +26,12 @@ class Library:
         self.calls = []   # (tensors, key) of each step of many
         self.owned = {}   # address -> bytes, where a test gives them
 
+    def novaq_status_string(self, status):
+        return b"status %d" % status
+
+    def novaq_last_hip_error(self):
+        return 0
+
     def rows(self, table, count):
         return np.array(array(table, count * WORDS, np.int64)).reshape(count, WORDS)
 

@@ -392,6 +392,39 @@ def test_arrays_that_overlap_step_one_after_another():
         assert np.array_equal(base, want)
 
 
+def test_a_refused_step_of_the_class_changes_nothing():
+    """One weight's codes on the host: the others are not stepped, and the step is not counted;
+    once they are back the step is the first."""
+    rng = np.random.default_rng(14)
+    bad = BlockQuantizedParameters.from_float(np.ones((8, 16), np.float32), keep_master=True)
+    ps = [Parameters(dev(rng.standard_normal(50).astype(np.float32))), bad,
+          Parameters(rng.standard_normal(30).astype(np.float32)),
+          Parameters(rng.standard_normal(9)), Parameters(rng.standard_normal(9))]
+    for p in ps:
+        p.grad = rng.standard_normal(p.shape).astype(np.float32)
+    opt = optim.AdamW(ps, lr=0.1)
+    before = [np.array(host_of(p)) for p in ps]
+    codes, bad.codes = bad.codes, bad.codes.cpu()
+    with pytest.raises(ValueError):
+        opt.step()
+    bad.codes = codes
+    ps[4].grad = np.ones(8)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert opt.t == 0
+    for p, w, m in zip(ps, before, opt.m_t):
+        assert np.array_equal(host_of(p), w) and not m.any()
+    ps[4].grad = None
+    opt.step()
+    want = OR.adamw_step(before[0], ps[0].grad, 0 * before[0], 0 * before[0], 1, 0.1)[0]
+    assert opt.t == 1 and np.array_equal(host_of(ps[0]), want)
+
+
+def host_of(p):
+    x = p.master if isinstance(p, BlockQuantizedParameters) else p.data
+    return x if isinstance(x, np.ndarray) else x.cpu().numpy()
+
+
 def test_class_with_8_bit_states():
     """The class's steps are the list's, seeded by its count."""
     rng = np.random.default_rng(11)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from novann_amd import optim
-from novann_amd.module import Parameters, QuantizedParameters
+from novann_amd.module import BlockQuantizedParameters, Parameters, QuantizedParameters
 from oracle import optim_ref as OR
 from tests.optim_host import library  # noqa: F401  (a fixture)
 
@@ -93,3 +93,55 @@ def test_arrays_side_by_side_are_one_call(library):
         p.grad = np.ones(p.shape, np.float32)
     optim.AdamW(ps, **HP).step()
     assert [count for count, _ in library.calls] == [5]
+
+
+def block_weight():
+    """Its codes and exponents on the host, where no step can write them."""
+    return BlockQuantizedParameters(
+        torch.zeros(8, 128, dtype=torch.uint8).view(torch.float8_e4m3fn),
+        torch.zeros(1, 4, dtype=torch.uint8), (8, 16), master=torch.zeros(8, 16))
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_a_step_that_is_refused_changes_nothing(library, shared):
+    """One wrong parameter, in the first call or a later one: no other is stepped, and the step
+    is not counted."""
+    rng = np.random.default_rng(4)
+    base = rng.standard_normal(100).astype(np.float32)
+    wide = Parameters(rng.standard_normal(7))
+    bad = block_weight()
+    ps = [Parameters(base), wide, bad, Parameters(base if shared else base.copy())]
+    kept = [p.data.copy() for p in (ps[0], wide, ps[3])]
+    opt = optim.AdamW(ps, **HP)
+    for p in ps:
+        p.grad = rng.standard_normal(p.shape).astype(np.float32)
+    with pytest.raises(ValueError):
+        opt.step()
+    wide.grad = np.ones(8)
+    bad.grad = None
+    with pytest.raises(ValueError):
+        opt.step()
+    assert opt.t == 0 and not library.calls
+    for p, before in zip((ps[0], wide, ps[3]), kept):
+        assert np.array_equal(p.data, before)
+    assert not any(m.any() for m in opt.m_t)
+    wide.grad = np.ones(7)
+    want, m, _ = reference(base, ps[0].grad, 0 * base, 0 * base, 1)
+    opt.step()
+    assert opt.t == 1 and np.array_equal(opt.m_t[0].numpy(), m)
+    assert shared or np.array_equal(ps[0].data, want)
+
+
+def test_a_gradient_that_is_another_weight(library):
+    """The weight is stepped after the parameter whose gradient it was."""
+    rng = np.random.default_rng(5)
+    a, b, c = (torch.from_numpy(rng.standard_normal(60).astype(np.float32)) for _ in range(3))
+    ps = [Parameters(a), Parameters(b), Parameters(c)]
+    ps[0].grad, ps[1].grad, ps[2].grad = b, torch.ones(60), torch.ones(60)
+    zero = np.zeros(60, np.float32)
+    want = [reference(x.numpy().copy(), g.numpy().copy(), zero, zero, 1)[0]
+            for x, g in ((a, b), (b, torch.ones(60)), (c, torch.ones(60)))]
+    optim.AdamW(ps, **HP).step()
+    assert [count for count, _ in library.calls] == [2, 1]
+    for x, w in zip((a, b, c), want):
+        assert np.array_equal(x.numpy(), w)
