@@ -18,6 +18,7 @@ gradient (``novaq_adamw_step_f64``); any other numpy array steps in float32
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
 from array import array
 from operator import attrgetter
@@ -434,8 +435,10 @@ class AdamW:
         for turn, i in sorted(zip(_turns(len(listed), spans), listed)):
             calls.setdefault((turn, self._w[i].device), []).append(i)
         tables = [self._rows(call, grads) for call in calls.values()]
+        # (each call's random numbers are its own: seeds past any step count)
+        seeds = itertools.count(t, 1 << 32)
         for call, table in zip(calls.values(), tables):
-            self._step_call(call, table, grads, t)
+            self._step_call(call, table, grads, t, seeds)
             self.t = t
         for i, g, g32 in wide:
             self._step_f64(i, g, g32, t)
@@ -449,9 +452,9 @@ class AdamW:
                      [getattr(p, "name", None) not in ("gamma", "beta") for p in ps],
                      [self._amax_scale[i] for i in call])
 
-    def _launch(self, call: List[int], table: array, t: int) -> int:
+    def _launch(self, call: List[int], table: array, t: int, seed: int) -> int:
         return _launch(table, [self.params[i] for i in call], [self._amax_scale[i] for i in call],
-                       self._w[call[0]].device, self._hp(1, t), t)
+                       self._w[call[0]].device, self._hp(1, t), seed)
 
     def _memory(self, k: int, i: int, g: torch.Tensor):
         """The spans of parameter i of a call, its k-th."""
@@ -464,21 +467,22 @@ class AdamW:
             spans.append((k, *_span(g), False))
         return spans
 
-    def _step_call(self, call: List[int], table: array, grads, t: int) -> None:
+    def _step_call(self, call: List[int], table: array, grads, t: int, seeds) -> None:
         arrays = [(p.data, self._w[i]) for i, p in ((i, self.params[i]) for i in call)
                   if isinstance(getattr(p, "data", None), np.ndarray)]
         for data, w in arrays:
             # the caller may have changed .data since the last step
             w.copy_(torch.from_numpy(np.ascontiguousarray(data).reshape(w.shape).astype(
                 np.float32, copy=False)))
-        rc = self._launch(call, table, t)
+        seed = next(seeds)
+        rc = self._launch(call, table, t, seed)
         if rc == _lib.EINVAL:
             # memory that parameters share otherwise (one's gradient another's weight): in turn too
             turns = _turns(len(call), [s for k, i in enumerate(call)
                                        for s in self._memory(k, i, grads[i])])
             for turn in range(max(turns) + 1) if any(turns) else ():
                 part = [i for i, n in zip(call, turns) if n == turn]
-                rc = self._launch(part, self._rows(part, grads), t)
+                rc = self._launch(part, self._rows(part, grads), t, seed if turn == 0 else next(seeds))
                 check(rc, "adamw step")
         check(rc, "adamw step")
         for data, w in arrays:

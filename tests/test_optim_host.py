@@ -145,3 +145,22 @@ def test_a_gradient_that_is_another_weight(library):
     assert [count for count, _ in library.calls] == [2, 1]
     for x, w in zip((a, b, c), want):
         assert np.array_equal(x.numpy(), w)
+
+
+def test_each_call_has_random_numbers_of_its_own(library):
+    """States in 8 bits of parameters that take turns: every call counts its elements from the
+    list's first, so no two calls may have one key, in a step or in the next ones."""
+    base = np.ones(200, np.float32)
+    w = torch.ones(64)
+    ps = [Parameters(base), Parameters(base[100:]), Parameters(base[150:]), Parameters(w),
+          Parameters(torch.ones(64))]
+    opt = optim.AdamW(ps, state_dtype="8bit", **HP)
+    for p in ps:
+        p.grad = torch.ones(p.shape)
+    ps[4].grad = w  # (its turn is after w's)
+    for _ in range(3):
+        opt.step()
+    keys = [key for _, key in library.calls]
+    assert len(keys) >= 9 and len(set(keys)) == len(keys)
+    # the first call's is the step's own
+    assert library.calls[0][1] == optim._key(1)
