@@ -21,6 +21,7 @@ import ctypes
 import itertools
 import math
 from array import array
+from collections.abc import Sequence
 from operator import attrgetter
 from typing import Iterable, List, NamedTuple, Optional
 
@@ -360,6 +361,26 @@ def _turns(count: int, spans) -> list:
     return turns
 
 
+class _States(Sequence):
+    """An AdamW's states, each (m_t[i], v_t[i]) or a State8, as a list that writes through."""
+
+    def __init__(self, opt) -> None:
+        self._opt = opt
+
+    def __len__(self) -> int:
+        return len(self._opt.m_t)
+
+    def __getitem__(self, i):
+        if isinstance(i, slice):
+            return [self[k] for k in range(*i.indices(len(self)))]
+        m, v = self._opt.m_t[i], self._opt.v_t[i]
+        return self._opt._state8[i] if m is None and v is None else (m, v)
+
+    def __setitem__(self, i: int, state) -> None:
+        pair, codes = (state, None) if len(state) == 2 else ((None, None), State8(*state))
+        (self._opt.m_t[i], self._opt.v_t[i]), self._opt._state8[i] = pair, codes
+
+
 class AdamW:
     """AdamW with decoupled weight decay (adamw.py:6-69).
 
@@ -388,16 +409,28 @@ class AdamW:
                 if p.data.dtype != torch.float32 or not p.data.is_contiguous():
                     raise TypeError("AdamW: device parameters must be contiguous float32")
                 self._w.append(p.data)
-        # (m_t[i], v_t[i]) are the moments of parameter i, both None where states[i] has them
-        # in 8 bits
-        self.states = [State8.zeros(w.numel(), w.device)
-                       if state_dtype == "8bit" and w.dtype == torch.float32
-                       else (torch.zeros_like(w), torch.zeros_like(w)) for w in self._w]
+        self._state8 = [State8.zeros(w.numel(), w.device)
+                        if state_dtype == "8bit" and w.dtype == torch.float32 else None
+                        for w in self._w]
+        # the moments that the next step reads, None where they are in 8 bits
+        self.m_t, self.v_t = ([torch.zeros_like(w) if s is None else None
+                               for w, s in zip(self._w, self._state8)] for _ in range(2))
         self._amax_scale: List[Optional[torch.Tensor]] = [
             torch.empty(2, dtype=torch.float32, device=w.device)
             if isinstance(p, QuantizedParameters) else None for p, w in zip(self.params, self._w)]
-        self.m_t = [None if isinstance(s, State8) else s[0] for s in self.states]
-        self.v_t = [None if isinstance(s, State8) else s[1] for s in self.states]
+
+    @property
+    def states(self) -> _States:
+        """Each parameter's (m_t[i], v_t[i]), or its State8."""
+        return _States(self)
+
+    @states.setter
+    def states(self, states) -> None:
+        states = list(states)
+        if len(states) != len(self.params):
+            raise ValueError(f"{len(states)} states for {len(self.params)} parameters")
+        for i, state in enumerate(states):
+            self.states[i] = state
 
     def _grad(self, p, w: torch.Tensor) -> torch.Tensor:
         """A parameter's gradient as the step reads it."""
@@ -493,6 +526,11 @@ class AdamW:
         g, g32 = _dev_grad64(self.params[i].grad, w.device)
         if g.numel() != w.numel():
             raise ValueError(f"AdamW: gradient of {g.numel()} values for a parameter of {w.numel()}")
+        for s in (self.m_t[i], self.v_t[i]):
+            if s.dtype != torch.float64 or s.numel() != w.numel() or not s.is_contiguous() or \
+                    _get_device(s) != _get_device(w):
+                raise ValueError("AdamW: a float64 parameter's states are contiguous float64 tensors "
+                                 "of as many elements, beside it")
         return g, g32
 
     def _step_f64(self, i: int, g: torch.Tensor, g32: bool, t: int) -> None:

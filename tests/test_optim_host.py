@@ -164,3 +164,56 @@ def test_each_call_has_random_numbers_of_its_own(library):
     assert len(keys) >= 9 and len(set(keys)) == len(keys)
     # the first call's is the step's own
     assert library.calls[0][1] == optim._key(1)
+
+
+def test_the_moments_that_are_set_are_the_ones_that_step(library):
+    """m_t and v_t are the optimizer's state: what a program puts there, as it does when it goes
+    on from a checkpoint, is what the next step reads."""
+    rng = np.random.default_rng(6)
+    ps = [Parameters(rng.standard_normal(20).astype(np.float32)),
+          Parameters(rng.standard_normal(20))]
+    opt = optim.AdamW(ps, **HP)
+    assert type(opt.m_t) is type(opt.v_t) is list
+    for way in range(3):
+        m, v = ([abs(rng.standard_normal(20)).astype(p.data.dtype) for p in ps] for _ in range(2))
+        new = [[torch.from_numpy(a.copy()) for a in x] for x in (m, v)]
+        if way == 0:
+            opt.m_t, opt.v_t = new
+        elif way == 1:
+            for i in range(2):
+                opt.m_t[i], opt.v_t[i] = new[0][i], new[1][i]
+        else:
+            opt.states = list(zip(*new))
+        assert all(opt.states[i][0] is opt.m_t[i] is new[0][i] for i in range(2))
+        want = []
+        for p, a, b in zip(ps, m, v):
+            p.grad = rng.standard_normal(20).astype(np.float32)
+            want.append(reference(p.data.copy(), p.grad, a, b, way + 1))
+        opt.step()
+        for i, (p, (w, a, b)) in enumerate(zip(ps, want)):
+            assert np.array_equal(p.data, w)
+            assert np.array_equal(opt.m_t[i].numpy(), a) and np.array_equal(opt.v_t[i].numpy(), b)
+    opt.m_t[1] = torch.zeros(20)  # (float32 beside a float64 parameter)
+    with pytest.raises(ValueError):
+        opt.step()
+    opt.m_t[1] = torch.zeros(20, dtype=torch.float64)
+    opt.m_t[0] = torch.zeros(19)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert opt.t == 3
+
+
+def test_states_in_8_bits_are_set_as_a_whole(library):
+    p = Parameters(torch.zeros(300))
+    p.grad = torch.ones(300)
+    opt = optim.AdamW([p], state_dtype="8bit", **HP)
+    assert opt.m_t == opt.v_t == [None] and isinstance(opt.states[0], optim.State8)
+    new = optim.State8.zeros(300)
+    opt.states[0] = tuple(new)
+    assert opt.states[0] == new and opt.states[-1:] == [new]
+    opt.step()
+    with pytest.raises(ValueError):
+        opt.states = []
+    opt.states = [(torch.zeros(300), torch.zeros(300))]
+    opt.step()
+    assert opt.m_t[0].any()
