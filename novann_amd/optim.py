@@ -83,7 +83,9 @@ class State8(NamedTuple):
     @classmethod
     def zeros(cls, n: int, device=None) -> "State8":
         dev, blocks = device or _device(), -(-n // quant.BLOCK)
-        codes, exponents = (torch.zeros(2, k, dtype=torch.uint8, device=dev) for k in (n, blocks))
+        # (rows of whole 16 bytes: a step whose tensors are aligned takes four elements at a time)
+        codes, exponents = (torch.zeros(2, -(-k // 16) * 16, dtype=torch.uint8, device=dev)[:, :k]
+                            for k in (n, blocks))
         return cls(codes[0].view(torch.float8_e4m3fn), exponents[0], codes[1], exponents[1])
 
     def check(self, what: str = "state") -> None:

@@ -217,3 +217,13 @@ def test_states_in_8_bits_are_set_as_a_whole(library):
     opt.states = [(torch.zeros(300), torch.zeros(300))]
     opt.step()
     assert opt.m_t[0].any()
+
+
+@pytest.mark.parametrize("n", [0, 1, 126, 127, 129, 1000, 2049])
+def test_new_states_are_aligned(n):
+    """All four on 16 bytes, whatever the size: one tensor that is not makes its whole step go
+    an element at a time."""
+    s = optim.State8.zeros(n, torch.device("cpu"))
+    for t, k in zip(s, (n, -(-n // 128)) * 2):
+        assert t.numel() == k and t.is_contiguous() and t.data_ptr() % 16 == 0
+        assert not t.view(torch.uint8).any()
