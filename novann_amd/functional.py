@@ -1091,6 +1091,8 @@ def layer_norm_backward(grad, input, weight, mean, rstd):
     R = x.numel() // D
     w = _row_arg(weight, D, "weight")
     m, r = _row_arg(mean, R, "mean"), _row_arg(rstd, R, "rstd")
+    if x.dim() == 1 and m is not None and r is not None:
+        m, r = m.reshape(()), r.reshape(())  # (an array of no dimensions is uploaded with one)
     if m is None or r is None or m.shape != x.shape[:-1] or r.shape != x.shape[:-1]:
         raise ValueError(f"mean and rstd do not match input {tuple(x.shape)}")
     at = x.get_device()

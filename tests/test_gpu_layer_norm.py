@@ -188,6 +188,18 @@ def test_shapes_and_kinds():
     assert gx.shape == (0, 100) and not gw.any() and not gb.any()
 
 
+def test_one_row_as_an_array():
+    """An array of one dimension there and back: the row's own gradients."""
+    x, w, b = data(np.random.default_rng(9), 1, 100, "f32")
+    g = torch.randn(1, 100, device="cuda")
+    h = [t.cpu().numpy() for t in (x[0], w, b, g[0])]
+    y, mean, rstd = F.layer_norm(h[0], h[1], h[2], extras=True)
+    want = F.layer_norm(x, w, b, extras=True)
+    got = F.layer_norm_backward(h[3], h[0], h[1], mean, rstd)
+    for a, c in zip((y, *got), (want[0], *F.layer_norm_backward(g, x, w, *want[1:]))):
+        assert isinstance(a, np.ndarray) and np.array_equal(a, c.cpu().numpy().reshape(100))
+
+
 def test_captured_and_on_another_stream():
     x, w, b = data(np.random.default_rng(8), 300, 784, "bf16")
     g = torch.randn(300, 784, device="cuda").bfloat16()
