@@ -529,6 +529,16 @@ bool fits_tiles(const novaq_adamw_tensor& t) {
          on(t.v, sa);
 }
 
+// Whether a per-tensor weight is stepped by the kernel of one tensor (optim.hip): the large one
+// of a call.  Its 2048 workgroups join their largest |w| in its amax once each, a list's one for
+// each run (E4M3 codes and fp32 gradients, the cast with it: 4096 x 4096 97 us so, 115 in the
+// list; 2048 x 2048 50 and 55; 1024 x 1024 24 both ways).  Several large ones take a launch or
+// two more each so (4 of 2048 x 2048 175 us, in the list 133; 4 of 4096 x 4096 410 and 413).
+bool steps_alone(const novaq_adamw_tensor& t, int64_t elements) {
+  return t.amax_scale && !t.m_exponents && t.grad_dtype == F32 && t.n >= (1 << 22) &&
+         t.n > elements / 2 && on(t.w, 16) && on(t.grad, 16) && on(t.m, 16) && on(t.v, 16);
+}
+
 }  // namespace
 
 int adamw_many_launch(const novaq_adamw_tensor* list, int64_t count, const novaq_adamw& hp,
@@ -566,10 +576,11 @@ int adamw_many_launch(const novaq_adamw_tensor* list, int64_t count, const novaq
   // Tiles that fill the card (8 weights of 4096 x 4096, fp32 states 741 us, in runs 824;
   // 8-bit states 471 and 514; 256 tiles 23.1 and 27.4, in 8 bits 16.5 and 23.2): a few take
   // longer than both launches (64 tiles 13.8 and 11.8, 8 tiles 13.9 and 9.0).
-  int64_t fitting = 0, bytes = 0;
+  int64_t fitting = 0, bytes = 0, elements = 0;
   for (int64_t i = 0; i < count; ++i) {
     const novaq_adamw_tensor& t = list[i];
     if (fits_tiles(t)) fitting += ((t.rows + 127) / 128) * ((t.cols + 127) / 128);
+    elements += t.n;
     bytes += t.n * (4 + (t.grad_dtype == F32 ? 4 : 2) + (t.m_exponents ? 2 : 8));
   }
   const bool in_tiles = fitting >= 256, past = bytes > (int64_t)1 << 28;
@@ -591,6 +602,7 @@ int adamw_many_launch(const novaq_adamw_tensor* list, int64_t count, const novaq
       auto* ve = static_cast<uint8_t*>(t.v_exponents);
       const uint32_t first = base;
       base += (uint32_t)((t.n + 127) / 128 * 128);
+      if (steps_alone(t, elements)) continue;
       if (t.codes && !t.amax_scale) {
         const TileRow r{t.w, t.grad, t.m, t.v, me, ve,
                         BlockOut{static_cast<uint8_t*>(t.codes), static_cast<uint8_t*>(t.exponents),
@@ -652,8 +664,13 @@ int adamw_many_launch(const novaq_adamw_tensor* list, int64_t count, const novaq
     for (int64_t i = from; i < at; ++i) {
       const novaq_adamw_tensor& t = list[i];
       if (!t.amax_scale) continue;
-      const int rc = cast_launch(t.w, F32, t.codes, t.q_dtype, t.n, 2, t.amax_scale,
-                                 t.amax_scale + 1, st);
+      int rc = NOVAQ_OK;
+      if (steps_alone(t, elements))
+        rc = adamw_launch(t.w, static_cast<const float*>(t.grad), static_cast<float*>(t.m),
+                          static_cast<float*>(t.v), t.n, hp.lr, hp.beta1, hp.beta2, hp.eps,
+                          hp.weight_decay, hp.step, t.decay, t.amax_scale, st);
+      if (rc == NOVAQ_OK)
+        rc = cast_launch(t.w, F32, t.codes, t.q_dtype, t.n, 2, t.amax_scale, t.amax_scale + 1, st);
       if (rc != NOVAQ_OK) return rc;
     }
   }

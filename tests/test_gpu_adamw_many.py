@@ -310,6 +310,29 @@ def test_weights_that_step_in_tiles(gdt, bits):
                 assert torch.equal(w.exponents_t, qt.exponents), (t, i)
 
 
+@pytest.mark.parametrize("qt", ["e4m3", "e5m2", "e2m1"])
+def test_a_large_per_tensor_weight(qt):
+    """One that is most of a call has a kernel of its own: the bits of a plain weight's step, the
+    codes and scale of the stepped master, beside small ones and where it decays or not."""
+    big, n = (2048, 2049 if qt != "e2m1" else 2050), 1000
+    for flags in ([True, False], [False, True]):
+        w = QuantizedParameters.from_float(torch.randn(big, device="cuda") * 0.05, qt,
+                                           keep_master=True)
+        small = torch.randn(n, device="cuda")
+        plain = [w.master.clone(), small.clone()]
+        grads = [torch.randn(big, device="cuda"), torch.randn(n, device="cuda")]
+        made = [torch.rand_like(t) * 1e-2 for t in (*grads, *grads)]
+        a, b = ([(t[0], t[2]), (t[1], t[3])] for t in ([x.clone() for x in made] for _ in range(2)))
+        for t in (1, 2):
+            optim.adamw_step([w, small], grads, a, step=t, decay=flags, **HP)
+            optim.adamw_step(plain, grads, b, step=t, decay=flags, **HP)
+            assert torch.equal(w.master, plain[0]) and torch.equal(small, plain[1])
+            assert all(torch.equal(x, y) for s, r in zip(a, b) for x, y in zip(s, r))
+            q = quant.quantize(w.master, qt)
+            assert torch.equal(w.codes.view(torch.uint8), q.data.view(torch.uint8))
+            assert torch.equal(w.scale, q.scale) and torch.equal(w.amax, q.amax)
+
+
 def test_the_class():
     """AdamW over parameters of every kind against the same steps one tensor at a time."""
     rng = np.random.default_rng(8)
