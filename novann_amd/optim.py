@@ -437,6 +437,9 @@ class AdamW:
     def _grad(self, p, w: torch.Tensor) -> torch.Tensor:
         """A parameter's gradient as the step reads it."""
         g = p.grad
+        if type(g) is torch.Tensor and g.dtype in _STEP_GRADS and g.shape == w.shape and \
+                _get_device(g) == _get_device(w) and g.is_contiguous():
+            return g
         if not (isinstance(g, torch.Tensor) and g.device == w.device and g.dtype in _STEP_GRADS):
             g = _dev_f32(g, w.device)
         if isinstance(p, QuantizedParameters) and p.stored_shape != p.shape:
@@ -460,19 +463,11 @@ class AdamW:
             else:
                 listed.append(i)
                 grads[i] = self._grad(p, self._w[i])
-        # parameters that share memory (a weight named twice, views of one buffer) step one after
-        # another, in their order: an array's bytes are its own, its device copy is not
-        spans = []
-        for k, i in enumerate(listed):
-            data = getattr(self.params[i], "data", None)
-            spans.append((k, *_span(data if isinstance(data, np.ndarray) else self._w[i]), True))
-        calls = {}
-        for turn, i in sorted(zip(_turns(len(listed), spans), listed)):
-            calls.setdefault((turn, self._w[i].device), []).append(i)
-        tables = [self._rows(call, grads) for call in calls.values()]
+        calls = self._calls(listed) if listed else []
+        tables = [self._rows(call, grads) for call in calls]
         # (each call's random numbers are its own: seeds past any step count)
         seeds = itertools.count(t, 1 << 32)
-        for call, table in zip(calls.values(), tables):
+        for call, table in zip(calls, tables):
             self._step_call(call, table, grads, t, seeds)
             self.t = t
         for i, g, g32 in wide:
@@ -480,10 +475,28 @@ class AdamW:
             self.t = t
         self.t = t
 
+    def _calls(self, listed: List[int]) -> List[List[int]]:
+        """The parameters by call.  Those that share memory (a weight named twice, views of one
+        buffer) step one after another, in their order: an array's bytes are its own, its device
+        copy is not.  (Device tensors that overlap but start apart are found by the C call.)"""
+        ws = [self._w[i] for i in listed]
+        arrays = [i for i in listed if isinstance(getattr(self.params[i], "data", None), np.ndarray)]
+        if len(arrays) < 2 and len(set(map(_data_ptr, ws))) == len(ws) == \
+                list(map(_get_device, ws)).count(_get_device(ws[0])):
+            return [listed]
+        arrays = set(arrays)
+        turns = _turns(len(listed), [
+            (k, *_span(self.params[i].data if i in arrays else w), True)
+            for k, (i, w) in enumerate(zip(listed, ws))])
+        calls = {}
+        for turn, i in sorted(zip(turns, listed)):
+            calls.setdefault((turn, self._w[i].device), []).append(i)
+        return list(calls.values())
+
     def _rows(self, call: List[int], grads) -> array:
-        ps = [self.params[i] for i in call]
+        ps, states = [self.params[i] for i in call], self.states
         return _rows(ps, [self._w[i] for i in call], [grads[i] for i in call],
-                     [self.states[i] for i in call],
+                     [states[i] for i in call],
                      [getattr(p, "name", None) not in ("gamma", "beta") for p in ps],
                      [self._amax_scale[i] for i in call])
 
