@@ -900,8 +900,9 @@ def block_linear(input, weight, bias=None, *, out_dtype: str = "f32", input_dtyp
 
     input (N, D_in): fp32, bf16 or f16 (quantized here, to ``input_dtype`` 'e4m3' or
     'e5m2', a scale for 128 columns of a row), or a quant.BlockQuantized (as ``layer_norm``
-    stores it); weight (D_out, D_in): BlockQuantizedParameters; bias: D_out values (fp32)
-    or None.  Returns (N, D_out) in ``out_dtype`` ('f32', 'bf16', 'f16'), rounded once from
+    stores it: the output then has the leading dimensions that its rows had there); weight
+    (D_out, D_in): BlockQuantizedParameters; bias: D_out values (fp32) or None.  Returns (N,
+    D_out) in ``out_dtype`` ('f32', 'bf16', 'f16'), rounded once from
     fp32 sums (each sum of 128 products within 2e-5 of the products' root of squares, the
     matrix core's own precision); ndarrays in -> ndarrays out (f32, f16).
 
@@ -923,7 +924,7 @@ def block_linear(input, weight, bias=None, *, out_dtype: str = "f32", input_dtyp
                              f"{weight.shape}")
         y = torch.empty((input.shape[0], D_out), dtype=store, device=input.data.device)
         _product(input, weight, b, y)
-        return y
+        return y if input.lead is None else y.view(*input.lead, D_out)
     x, xdt, was_numpy = _float_arg(input, "input")
     if x.dim() != 2:
         raise ValueError(f"block_linear expects a 2-D input, got shape {tuple(x.shape)}")
@@ -1031,8 +1032,8 @@ def layer_norm(input, weight=None, bias=None, *, eps: float = 1e-5,
 
     weight, bias: D values each (Parameters, tensors or arrays; None for 1 and 0).
     Returns input's shape in ``out_dtype`` ('f32', 'bf16', 'f16'; input's type by default),
-    rounded once; with 'e4m3' or 'e5m2' a quant.BlockQuantized of (rows, D), as
-    ``block_linear`` takes it.  ``extras=True`` returns (y, mean, rstd), both of input's
+    rounded once; with 'e4m3' or 'e5m2' a quant.BlockQuantized of (rows, D) that keeps the
+    leading dimensions, as ``block_linear`` takes it.  ``extras=True`` returns (y, mean, rstd), both of input's
     shape without the last dimension, for the backward; ndarrays in -> ndarrays out (f32,
     f16).  No counterpart in the reference, whose norms are over the batch."""
     x, xdt, was_numpy = _float_arg(input, "input")
@@ -1051,7 +1052,7 @@ def layer_norm(input, weight=None, bias=None, *, eps: float = 1e-5,
     if name in quant.BLOCK_DTYPES:
         y = torch.empty((R, quant.block_pitch(D)), dtype=quant.BLOCK_DTYPES[name], device=dev)
         e = torch.empty((R, quant.block_groups(D)), dtype=torch.uint8, device=dev)
-        q = quant.BlockQuantized(y, e, (R, D), name)
+        q = quant.BlockQuantized(y, e, (R, D), name, lead=None if x.dim() == 2 else tuple(shape[:-1]))
     else:
         y = torch.empty(shape, dtype=_out_dtype(name), device=dev)
     mean = rstd = None

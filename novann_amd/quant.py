@@ -13,6 +13,7 @@ at layer entry (novann/layers/linear/linear.py:81).
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -234,16 +235,20 @@ class BlockQuantized:
     uint8, one e for each 128 columns of a row (block_rows 1) or for 128 x 128 elements
     (block_rows 128), in rows of whole fours, the scale being 2^(e - 127).  transposed:
     the matrix is the transpose of the one it was made from (what a layer's backward
-    keeps of its input)."""
+    keeps of its input).  lead: the shape that the rows have in a tensor of other than two
+    dimensions (layer_norm's output), which a product's output has again; None: (rows,)."""
     data: torch.Tensor
     exponents: torch.Tensor
     shape: tuple
     dtype: str
     block_rows: int = 1
     transposed: bool = False
+    lead: Optional[tuple] = None
 
     def check(self, what: str = "blocks") -> int:
         """ValueError or TypeError unless the tensors hold that matrix; their device's index."""
+        if self.lead is not None and math.prod(self.lead) != self.shape[0]:
+            raise ValueError(f"{what}: rows {tuple(self.lead)} are not the matrix's {self.shape[0]}")
         return check_blocks(self.data, self.exponents, self.shape, self.dtype, self.block_rows,
                             what)
 

@@ -84,6 +84,18 @@ def test_serving(N):
     assert torch.equal(lin(norm(x)), y)
 
 
+@pytest.mark.parametrize("shape", [(300,), (2, 20, 300), (3, 1, 4, 300)])
+def test_serving_keeps_the_leading_dimensions(shape):
+    """The same rows as of the flattened input, in the input's shape."""
+    norm, lin = layers(300, 130)
+    norm.eval(), lin.eval()
+    x = torch.randn(shape, device="cuda")
+    y = lin(norm(x))
+    assert y.shape == (*shape[:-1], 130)
+    assert torch.equal(y.view(-1, 130), lin(norm(x.view(-1, 300))))
+    assert norm(x).shape == (x.numel() // 300, 300)
+
+
 def test_arrays():
     norm, lin = layers(70, 30)
     x = np.random.default_rng(0).standard_normal((6, 70))
