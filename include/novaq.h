@@ -566,7 +566,9 @@ int novaq_block_product(const void *x, int x_dtype, const void *x_exponents, int
 size_t novaq_block_linear_workspace(int64_t M, int64_t K, int64_t N);
 
 /* y (M, N) = Q(x) w^T + bias: x (M, K) in F32, F16 or BF16 quantized to blocks of its rows in
- * q_dtype, then novaq_block_product with w (N, K) in blocks of 128 x 128.  kept (K, M
+ * q_dtype, then novaq_block_product with w (N, K) in blocks of 128 x 128.  Q makes blocks as
+ * novaq_quantize_blocks does, but an infinity a NaN, its block's scale that of its other
+ * elements: a row with one is NaN, here and in the gradients.  kept (K, M
  * rounded up to 128) and kept_exponents, or both NULL: the transposed input in blocks of
  * its own, from the same read, for the backward.  M, K and N up to 2^22. */
 int novaq_block_linear(const void *x, int x_dtype, int64_t M, int64_t K, int q_dtype,
@@ -597,7 +599,7 @@ int novaq_block_linear_backward(const void *grad, int grad_dtype, int64_t M, int
  * in fp32, the deviations taken from the row's own mean; gamma, beta (D values, fp32) or
  * NULL for 1 and 0.  y in F32, F16 or BF16 (exponents NULL), rounded once, or in E4M3 or
  * E5M2 as blocks of 128 columns (codes (R, P) and exponents (R, G) as
- * novaq_quantize_blocks writes them with block_rows 1).  mean, rstd: R values each for the
+ * novaq_quantize_blocks writes them with block_rows 1, an infinity as a NaN).  mean, rstd: R values each for the
  * backward, or both NULL.  eps not negative.  D up to 2^20, R below 2^31.
  * No reference counterpart (the reference normalises over the batch). */
 int novaq_layer_norm(const void *x, int x_dtype, int64_t R, int64_t D, const float *gamma,

@@ -121,10 +121,11 @@ __device__ __forceinline__ float bq_scale(int e) { return u2f((uint32_t)e << 23)
 
 // max |v| as bits, a NaN counted as more than an infinity.
 __device__ __forceinline__ uint32_t bq_mag(float v) { return f2u(v) & 0x7FFFFFFFu; }
-// The same with NaNs passed over: blocks that hold one are looked at again.
-__device__ __forceinline__ uint32_t bq_mag_number(float v) {
+// The same with NaNs (and infinities, where they become NaNs) passed over: blocks that hold
+// one are looked at again.
+__device__ __forceinline__ uint32_t bq_mag_number(float v, bool inf_nan = false) {
   const uint32_t a = bq_mag(v);
-  return a > 0x7F800000u ? 0u : a;
+  return a > (inf_nan ? 0x7F7FFFFFu : 0x7F800000u) ? 0u : a;
 }
 
 // max over the 16 lanes of a row of lanes, in all of them.
@@ -139,19 +140,22 @@ __device__ __forceinline__ uint32_t bq_max16(uint32_t a) {
   return a;
 }
 
-// 4 codes of v * inv.  ODD: the block may hold an infinity or a NaN: this library's rule
+// 4 codes of v * inv.  ODD: the block may hold an infinity or a NaN: the casts' rule
 // saturates the first, and the second keeps its sign and has all other bits of its code
 // set, which the hardware's conversion does not do; in all others nothing exceeds the
-// largest code.
+// largest code.  inf_nan: an infinity becomes such a NaN too, what the layers' own operands
+// are made with: a gradient that has overflowed must not come out of a product finite.
 template <int DT, bool ODD>
-__device__ __forceinline__ uint32_t bq_encode4(float a, float b, float c, float d, float inv) {
+__device__ __forceinline__ uint32_t bq_encode4(float a, float b, float c, float d, float inv,
+                                               bool inf_nan = false) {
   a *= inv, b *= inv, c *= inv, d *= inv;
   uint32_t nan = 0;
   if constexpr (ODD) {
     auto bound = [&](float v, int at) {
       const float t = __builtin_amdgcn_fmed3f(v, -fmt_max(DT), fmt_max(DT));
-      nan |= v == v ? 0u : (0x7Fu | (f2u(v) >> 24 & 0x80u)) << at;
-      return v == v ? t : 0.0f;
+      const bool number = inf_nan ? fabsf(v) <= fmt_max(DT) : v == v;
+      nan |= number ? 0u : (0x7Fu | (f2u(v) >> 24 & 0x80u)) << at;
+      return number ? t : 0.0f;
     };
     a = bound(a, 0), b = bound(b, 8), c = bound(c, 16), d = bound(d, 24);
   }
@@ -190,16 +194,17 @@ __device__ __forceinline__ int bq_slot(int c, int chunk) {
 // + 3, columns 8 (t % 16) .. + 7 in v, zeros past the matrix (with 256 threads of 8 rows
 // the registers leave two waves a SIMD).  TILE: one exponent for the tile, else one for
 // each row (codes) and one for each column (codes_t).  ODD: the tile holds an infinity or
-// a NaN.  colsum (this tile row's partial sums, or null).  All threads come here.
+// a NaN; inf_nan as in bq_encode4.  colsum (this tile row's partial sums, or null).  All
+// threads come here.
 template <int DT, bool TILE, bool ODD>
 __device__ __forceinline__ void bq_tile_as(const float (&v)[BQ_R][8], int64_t R, int64_t C,
                                            int64_t rt, int64_t ct, const BlockOut& o,
-                                           float* colsum, BlockTileLds& lds) {
+                                           float* colsum, BlockTileLds& lds, bool inf_nan) {
   const int tid = threadIdx.x, rg = tid >> 4, cg = tid & 15, wave = tid >> 6;
   const int64_t r0 = rt * BQ + rg * BQ_R, c0 = ct * BQ + cg * 8;
   const int64_t groups = bq_groups(C), groups_t = bq_groups(R);
   const int64_t last = (C + 127) / 128 - 1, last_t = (R + 127) / 128 - 1;
-  auto mag = [](float f) { return ODD ? bq_mag_number(f) : bq_mag(f); };
+  auto mag = [&](float f) { return ODD ? bq_mag_number(f, inf_nan) : bq_mag(f); };
   int te = 0;
   if constexpr (TILE) {
     uint32_t m = 0;
@@ -227,8 +232,8 @@ __device__ __forceinline__ void bq_tile_as(const float (&v)[BQ_R][8], int64_t R,
         e = bq_exponent<DT>(bq_max16(m));
       }
       const float inv = bq_inverse(e);
-      const ti_u32x2 w{bq_encode4<DT, ODD>(v[i][0], v[i][1], v[i][2], v[i][3], inv),
-                       bq_encode4<DT, ODD>(v[i][4], v[i][5], v[i][6], v[i][7], inv)};
+      const ti_u32x2 w{bq_encode4<DT, ODD>(v[i][0], v[i][1], v[i][2], v[i][3], inv, inf_nan),
+                       bq_encode4<DT, ODD>(v[i][4], v[i][5], v[i][6], v[i][7], inv, inf_nan)};
       if (r0 + i < R) {
         *reinterpret_cast<ti_u32x2*>(to + i * bq_pitch(C)) = w;
         if (cg == 0 && (!TILE || (rg == 0 && i == 0))) {
@@ -279,7 +284,7 @@ __device__ __forceinline__ void bq_tile_as(const float (&v)[BQ_R][8], int64_t R,
     for (int j = 0; j < 8; ++j) {
       const float inv = bq_inverse(TILE ? te : (int)col[j]);
       *reinterpret_cast<uint32_t*>(lds.t + bq_slot(cg * 8 + j, rg >> 2) + (rg & 3) * 4) =
-          bq_encode4<DT, ODD>(v[0][j], v[1][j], v[2][j], v[3][j], inv);
+          bq_encode4<DT, ODD>(v[0][j], v[1][j], v[2][j], v[3][j], inv, inf_nan);
     }
   }
   if (!TILE && colsum) {
@@ -312,14 +317,16 @@ __device__ __forceinline__ void bq_tile_as(const float (&v)[BQ_R][8], int64_t R,
 template <int DT, bool TILE>
 __device__ __forceinline__ void bq_tile(const float (&v)[BQ_R][8], int64_t R, int64_t C, int64_t rt,
                                         int64_t ct, const BlockOut& o, float* colsum,
-                                        BlockTileLds& lds) {
+                                        BlockTileLds& lds, bool inf_nan = false) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < BQ_R; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, bq_mag(v[i][j]));
-  if (!__syncthreads_or(m >= 0x7F800000u)) bq_tile_as<DT, TILE, false>(v, R, C, rt, ct, o, colsum, lds);
-  else bq_tile_as<DT, TILE, true>(v, R, C, rt, ct, o, colsum, lds);
+  if (!__syncthreads_or(m >= 0x7F800000u))
+    bq_tile_as<DT, TILE, false>(v, R, C, rt, ct, o, colsum, lds, false);
+  else
+    bq_tile_as<DT, TILE, true>(v, R, C, rt, ct, o, colsum, lds, inf_nan);
 }
 
 // A thread's 4 x 8 part of tile (rt, ct) of x (R, C), zeros past it.

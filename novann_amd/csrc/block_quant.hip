@@ -17,7 +17,7 @@ namespace {
 template <int ST, int DT, bool TILE, bool VEC>
 __global__ __launch_bounds__(BQ_THREADS, 6) void block_tile_kernel(const void* __restrict__ x, int64_t R,
                                                          int64_t C, BlockOut o,
-                                                         float* __restrict__ sums) {
+                                                         float* __restrict__ sums, bool inf_nan) {
   __shared__ __attribute__((aligned(16))) BlockTileLds lds;
   const int64_t ctiles = (C + 127) / 128;
   const int64_t rt = blockIdx.x / ctiles, ct = blockIdx.x % ctiles;
@@ -27,14 +27,14 @@ __global__ __launch_bounds__(BQ_THREADS, 6) void block_tile_kernel(const void* _
   }
   float v[BQ_R][8];
   bq_load<ST, VEC>(x, R, C, rt, ct, v);
-  bq_tile<DT, TILE>(v, R, C, rt, ct, o, sums ? sums + rt * C : nullptr, lds);
+  bq_tile<DT, TILE>(v, R, C, rt, ct, o, sums ? sums + rt * C : nullptr, lds, inf_nan);
 }
 
 // The codes of rows alone: 16 lanes a block of 128 columns, 8 columns a lane.
 template <int ST, int DT, bool VEC>
 __global__ __launch_bounds__(256) void block_rows_kernel(const void* __restrict__ x, int64_t R,
                                                          int64_t C, uint8_t* __restrict__ codes,
-                                                         uint8_t* __restrict__ e) {
+                                                         uint8_t* __restrict__ e, bool inf_nan) {
   const int cg = threadIdx.x & 15;
   const int64_t blocks = (C + 127) / 128, groups = bq_groups(C), pitch = bq_pitch(C);
   const int64_t all = R * blocks, stride = (int64_t)gridDim.x * 16;
@@ -50,15 +50,15 @@ __global__ __launch_bounds__(256) void block_rows_kernel(const void* __restrict_
     if (odd) {
       m = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, bq_mag_number(v[j]));
+      for (int j = 0; j < 8; ++j) m = max(m, bq_mag_number(v[j], inf_nan));
       m = bq_max16(m);
     }
     const int x_ = bq_exponent<DT>(m);
     const float inv = bq_inverse(x_);
     ti_u32x2 w;
     if (odd)
-      w = ti_u32x2{bq_encode4<DT, true>(v[0], v[1], v[2], v[3], inv),
-                   bq_encode4<DT, true>(v[4], v[5], v[6], v[7], inv)};
+      w = ti_u32x2{bq_encode4<DT, true>(v[0], v[1], v[2], v[3], inv, inf_nan),
+                   bq_encode4<DT, true>(v[4], v[5], v[6], v[7], inv, inf_nan)};
     else
       w = ti_u32x2{bq_encode4<DT, false>(v[0], v[1], v[2], v[3], inv),
                    bq_encode4<DT, false>(v[4], v[5], v[6], v[7], inv)};
@@ -140,7 +140,7 @@ size_t quantize_blocks_workspace(int64_t R, int64_t C) {
 
 int quantize_blocks_launch(const void* x, int x_dtype, int64_t R, int64_t C, int dtype,
                            int block_rows, void* codes, void* e, void* codes_t, void* et,
-                           float* colsum, void* workspace, hipStream_t st) {
+                           float* colsum, void* workspace, bool inf_nan, hipStream_t st) {
   const bool vec = C % 8 == 0;
   const BlockOut o{static_cast<uint8_t*>(codes), static_cast<uint8_t*>(e),
                    static_cast<uint8_t*>(codes_t), static_cast<uint8_t*>(et)};
@@ -153,7 +153,7 @@ int quantize_blocks_launch(const void* x, int x_dtype, int64_t R, int64_t C, int
           const int64_t groups = (R * ((C + 127) / 128) + 15) / 16;
           hipLaunchKernelGGL((block_rows_kernel<ST, DT, VEC>),
                              dim3((unsigned)std::min<int64_t>(groups, 1 << 16)), dim3(256), 0, st,
-                             x, R, C, o.codes, o.e);
+                             x, R, C, o.codes, o.e, inf_nan);
           return check_launch();
         }
         const int64_t rt = (R + 127) / 128, tiles = rt * ((C + 127) / 128);
@@ -163,10 +163,10 @@ int quantize_blocks_launch(const void* x, int x_dtype, int64_t R, int64_t C, int
         const unsigned orders = codes && codes_t && tiles <= 128 ? 2 : 1;
         if (block_rows == 1)
           hipLaunchKernelGGL((block_tile_kernel<ST, DT, false, VEC>), dim3((unsigned)tiles, orders),
-                             dim3(BQ_THREADS), 0, st, x, R, C, o, sums);
+                             dim3(BQ_THREADS), 0, st, x, R, C, o, sums, inf_nan);
         else
           hipLaunchKernelGGL((block_tile_kernel<ST, DT, true, VEC>), dim3((unsigned)tiles),
-                             dim3(BQ_THREADS), 0, st, x, R, C, o, nullptr);
+                             dim3(BQ_THREADS), 0, st, x, R, C, o, nullptr, inf_nan);
         const int rc = check_launch();
         if (rc != NOVAQ_OK || !sums || rt == 1) return rc;
         hipLaunchKernelGGL(block_colsum_kernel, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, st,

@@ -103,7 +103,7 @@ int novaq_quantize_blocks(const void* x, int x_dtype, int64_t R, int64_t C, int 
   if (colsum && R > 128 && (!workspace || workspace_bytes < quantize_blocks_workspace(R, C)))
     return NOVAQ_EINVAL;
   return quantize_blocks_launch(x, x_dtype, R, C, dtype, block_rows, codes, exponents, codes_t,
-                                exponents_t, colsum, workspace, st);
+                                exponents_t, colsum, workspace, false, st);
 }
 
 int novaq_dequantize_blocks(const void* codes, int dtype, const void* exponents, int64_t R,
@@ -169,13 +169,14 @@ int novaq_block_linear(const void* x, int x_dtype, int64_t M, int64_t K, int q_d
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (N == 0)
     return kept ? quantize_blocks_launch(x, x_dtype, M, K, q_dtype, 1, nullptr, nullptr, kept,
-                                         kept_exponents, nullptr, nullptr, st)
+                                         kept_exponents, nullptr, nullptr, true, st)
                 : NOVAQ_OK;
   const ForwardWs p(M, K, N);
   if (!w || !w_exponents || !y || !workspace || workspace_bytes < p.total) return NOVAQ_EINVAL;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int rq = quantize_blocks_launch(x, x_dtype, M, K, q_dtype, 1, ws + p.codes,
-                                        ws + p.exponents, kept, kept_exponents, nullptr, nullptr, st);
+                                        ws + p.exponents, kept, kept_exponents, nullptr, nullptr, true,
+                                        st);
   if (rq != NOVAQ_OK) return rq;
   return block_product_launch(ws + p.codes, q_dtype, ws + p.exponents, 1, M, K, w, w_dtype,
                               w_exponents, 128, N, bias, y, y_dtype, ws + p.product, st);
@@ -212,14 +213,14 @@ int novaq_block_linear_backward(const void* grad, int grad_dtype, int64_t M, int
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   rc = quantize_blocks_launch(grad, grad_dtype, M, N, gq_dtype, 1, grad_input ? ws + p.g : nullptr,
                               grad_input ? ws + p.ge : nullptr, grad_weight ? ws + p.gt : nullptr,
-                              grad_weight ? ws + p.gte : nullptr, grad_bias, ws + p.rest, st);
+                              grad_weight ? ws + p.gte : nullptr, grad_bias, ws + p.rest, true, st);
   if (rc == NOVAQ_OK && grad_input)
     rc = block_product_launch(ws + p.g, gq_dtype, ws + p.ge, 1, M, N, w_t, w_dtype, w_t_exponents,
                               128, K, nullptr, grad_input, grad_dtype, ws + p.rest, st);
   if (rc != NOVAQ_OK || !grad_weight) return rc;
   if (!kept) {
     rc = quantize_blocks_launch(x, x_dtype, M, K, xq_dtype, 1, nullptr, nullptr, ws + p.xt,
-                                ws + p.xte, nullptr, nullptr, st);
+                                ws + p.xte, nullptr, nullptr, true, st);
     if (rc != NOVAQ_OK) return rc;
     kept = ws + p.xt, kept_exponents = ws + p.xte;
   }

@@ -89,15 +89,15 @@ __device__ __forceinline__ void put8(void* y, uint8_t* e, int64_t row, int64_t c
     if (odd) {
       m = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = max(m, bq_mag_number(v[k]));
+      for (int k = 0; k < 8; ++k) m = max(m, bq_mag_number(v[k], true));
       m = bq_max16(m);
     }
     const int x = bq_exponent<OT>(m);
     const float inv = bq_inverse(x);
     ti_u32x2 w;
     if (odd)
-      w = ti_u32x2{bq_encode4<OT, true>(v[0], v[1], v[2], v[3], inv),
-                   bq_encode4<OT, true>(v[4], v[5], v[6], v[7], inv)};
+      w = ti_u32x2{bq_encode4<OT, true>(v[0], v[1], v[2], v[3], inv, true),
+                   bq_encode4<OT, true>(v[4], v[5], v[6], v[7], inv, true)};
     else
       w = ti_u32x2{bq_encode4<OT, false>(v[0], v[1], v[2], v[3], inv),
                    bq_encode4<OT, false>(v[4], v[5], v[6], v[7], inv)};

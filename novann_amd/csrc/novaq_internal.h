@@ -234,11 +234,13 @@ size_t clip_grad_norm_workspace(int64_t count);
 int clip_grad_norm_launch(const novaq_gradient* list, int64_t count, double max_norm, double eps,
                           float* norm, void* workspace, hipStream_t stream);
 
-// FP8 blocks and their products (novaq.h has the semantics).
+// FP8 blocks and their products (novaq.h has the semantics).  inf_nan: infinities become NaN
+// codes, as a layer makes its operands, and the scale is that of the other elements.
 size_t quantize_blocks_workspace(int64_t R, int64_t C);
 int quantize_blocks_launch(const void* x, int x_dtype, int64_t R, int64_t C, int dtype,
                            int block_rows, void* codes, void* exponents, void* codes_t,
-                           void* exponents_t, float* colsum, void* workspace, hipStream_t stream);
+                           void* exponents_t, float* colsum, void* workspace, bool inf_nan,
+                           hipStream_t stream);
 int dequantize_blocks_launch(const void* codes, int dtype, const void* exponents, int64_t R,
                              int64_t C, int block_rows, void* out, int out_dtype,
                              hipStream_t stream);

@@ -904,7 +904,9 @@ def block_linear(input, weight, bias=None, *, out_dtype: str = "f32", input_dtyp
     (D_out, D_in): BlockQuantizedParameters; bias: D_out values (fp32) or None.  Returns (N,
     D_out) in ``out_dtype`` ('f32', 'bf16', 'f16'), rounded once from
     fp32 sums (each sum of 128 products within 2e-5 of the products' root of squares, the
-    matrix core's own precision); ndarrays in -> ndarrays out (f32, f16).
+    matrix core's own precision); ndarrays in -> ndarrays out (f32, f16).  A row of input
+    with an infinity or a NaN is NaN (an infinity has no scale: quantized here it becomes a
+    NaN, where ``quant.quantize_blocks`` saturates).
 
     ``extras=True`` returns (y, kept): the input transposed in blocks of its own, one byte
     an element, made from the same read, which ``block_linear_backward`` takes in the
@@ -966,7 +968,8 @@ def block_linear_backward(grad, input, weight, bias: bool = True, *, grad_dtype:
     Q(input^T)^T with both in blocks of 128 rows, grad_bias = grad summed over its rows.
     input: the forward's, or what its ``extras`` kept.  ``grad_dtype`` 'e5m2' keeps
     gradients of a range that 'e4m3' would flush (2^-9 of a block's largest is its
-    smallest step).  ndarrays in -> ndarrays out (f32, f16)."""
+    smallest step).  Infinities and NaNs of grad and input are NaNs in all that they have a
+    part in.  ndarrays in -> ndarrays out (f32, f16)."""
     D_out, D_in = _block_weight(weight)
     g, gdt, was_numpy = _float_arg(grad, "grad")
     if g.dim() != 2 or g.shape[1] != D_out:
