@@ -22,6 +22,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "novaq_block_copies.h"
 #include "novaq_convert.h"
 #include "novaq_internal.h"
 
@@ -104,12 +105,6 @@ struct BlockTile {
   static constexpr int step = NTH / 8;       // rows from one copy to the next
   static_assert(R % 64 == 0 && (R * 8) % NTH == 0 && step % 16 == 0, "tile shape");
 
-  // byte offset of this lane's first copy from the tile's first row
-  __device__ static __forceinline__ uint32_t first(int64_t ld, int tid) {
-    const int r = tid / 8, c = (tid % 8) ^ ((r >> 1) & 7);
-    return (uint32_t)r * (uint32_t)ld + c * 16;
-  }
-
   // Fragment of 16 rows from w0 + 16 i: lane l holds row l % 16, chunks l / 16 and
   // l / 16 + 4 (an order of K of its own, the same in both operands).
   __device__ static __forceinline__ bg_i32x8 read(const uint8_t* lds, int w0, int i, int lane) {
@@ -150,11 +145,12 @@ struct BlockGemm {
     const int lane = bg_lane(), tid = wave * 64 + lane;
     const int wm = (wave % WGM) * WM, wn = (wave / WGM) * WN;
     const uint8_t *pa = oa.p + m0 * oa.ld, *pb = ob.p + n0 * ob.ld;
-    // (bytes of the tile's rows that the operand has: at most 256 rows of 4 MiB; in 32 bits,
-    // as a minimum of 64 is no scalar instruction, and a descriptor lies in scalar registers)
-    const uint32_t na = (uint32_t)min((int)oa.rows - (int)m0, BM) * (uint32_t)oa.ld;
-    const uint32_t nb = (uint32_t)min((int)ob.rows - (int)n0, BN) * (uint32_t)ob.ld;
-    const uint32_t va = A::first(oa.ld, tid), vb = B::first(ob.ld, tid);
+    // (in 32 bits, as a minimum of 64 is no scalar instruction, and a descriptor lies in scalar
+    // registers)
+    const uint32_t na = block_detail::code_bytes(oa.rows, m0, BM, oa.ld);
+    const uint32_t nb = block_detail::code_bytes(ob.rows, n0, BN, ob.ld);
+    const uint32_t va = block_detail::code_offset(oa.ld, tid);
+    const uint32_t vb = block_detail::code_offset(ob.ld, tid);
     const uint32_t sa = A::step * (uint32_t)oa.ld, sb = B::step * (uint32_t)ob.ld;
     // (a copy of exponents is of 64 rows of one operand; wave w has copies w, w + WAVES ..)
     const uint8_t* eb[ecopies];
@@ -164,11 +160,11 @@ struct BlockGemm {
     for (int c = 0; c < ecopies; ++c) {
       const int r = min(wave + c * WAVES, esets - 1) * 64;
       const BlockOp& o = r < BM ? oa : ob;
-      const int first = r < BM ? (int)m0 + r : (int)n0 + r - BM, row = first >> o.shift;
-      const int erows = ((int)(o.rows - 1) >> o.shift) + 1;
-      eb[c] = o.e + row * o.lde;
-      en[c] = max(min(erows - row, 64), 0) * (int)o.lde;
-      ev[c] = (uint32_t)(((first + lane) >> o.shift) - row) * (uint32_t)o.lde;
+      const int first = r < BM ? (int)m0 + r : (int)n0 + r - BM;
+      const auto set = block_detail::exponent_set(o.rows, o.lde, o.shift, first, lane);
+      eb[c] = o.e + set.from;
+      en[c] = set.bytes;
+      ev[c] = set.offset;
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -179,10 +175,10 @@ struct BlockGemm {
     uint8_t* const elds = lds + 2 * stage;
     bg_u32x4 ra, rb;  // the descriptors of the stage that is copied next
     auto aim_a = [&](int kb) {
-      ra = bg_buffer(pa + (uint32_t)kb * BG_K, kb < kb1 ? na - (uint32_t)kb * BG_K : 0u);
+      ra = bg_buffer(pa + (uint32_t)kb * BG_K, block_detail::codes_left(na, kb, kb1));
     };
     auto aim_b = [&](int kb) {
-      rb = bg_buffer(pb + (uint32_t)kb * BG_K, kb < kb1 ? nb - (uint32_t)kb * BG_K : 0u);
+      rb = bg_buffer(pb + (uint32_t)kb * BG_K, block_detail::codes_left(nb, kb, kb1));
     };
     auto copy = [&](int i, int slot) {
       uint8_t* at = lds + slot * stage;
@@ -195,7 +191,7 @@ struct BlockGemm {
 #pragma unroll
       for (int c = 0; c < ecopies; ++c)
         if (esets % WAVES == 0 || wave + c * WAVES < esets)
-          bg_copy4(bg_buffer(eb[c] + (uint32_t)kb, kb < kb1 ? (uint32_t)max(en[c] - kb, 0) : 0u), ev[c],
+          bg_copy4(bg_buffer(eb[c] + (uint32_t)kb, block_detail::exponents_left(en[c], kb, kb1)), ev[c],
                    elds + ((kb >> 2) & 1) * elems + (wave + c * WAVES) * 256);
     };
     // (a byte each: dwords of four blocks, shifted where they are used, were 5% slower)
