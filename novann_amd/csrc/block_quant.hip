@@ -71,25 +71,14 @@ __global__ __launch_bounds__(256) void block_rows_kernel(const void* __restrict_
   }
 }
 
-// sums (n, C) added over n: 64 columns a workgroup, 16 waves of every 16th row (with 4 waves
-// and a row in flight each 64 x 4096 took 6.5 us, so 3.9).
+// sums (n, C) added over n.
 __global__ __launch_bounds__(1024) void block_colsum_kernel(const float* __restrict__ sums,
                                                             int64_t n, int64_t C,
                                                             float* __restrict__ out) {
   __shared__ float part[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  float s = 0.0f;
-  if (c < C) {
-#pragma unroll 4
-    for (int64_t i = wave; i < n; i += 16) s += sums[i * C + c];
-  }
-  part[wave][lane] = s;
-  __syncthreads();
-  if (wave != 0 || c >= C) return;
-#pragma unroll
-  for (int w = 1; w < 16; ++w) s += part[w][lane];
-  out[c] = s;
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float s = bq_join_rows(sums, n, C, c, part);
+  if (threadIdx.x < 64 && c < C) out[c] = s;
 }
 
 template <int DT, int OT>

@@ -361,23 +361,14 @@ __global__ __launch_bounds__(256) void norm_grad_columns_kernel(const NormGradAr
   a.sums[(int64_t)blockIdx.y * 2 * D + D + c] = b;
 }
 
-// The sums (n, 2, D) added over n: 64 columns a workgroup, 16 waves of every 16th row.
+// The sums (n, 2, D) added over n.
 __global__ __launch_bounds__(1024) void norm_join_kernel(const float* __restrict__ sums, int64_t n,
                                                          int64_t D, float* __restrict__ gw,
                                                          float* __restrict__ gb) {
   __shared__ float part[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  float s = 0.0f;
-  if (c < 2 * D) {
-#pragma unroll 4
-    for (int64_t i = wave; i < n; i += 16) s += sums[i * 2 * D + c];
-  }
-  part[wave][lane] = s;
-  __syncthreads();
-  if (wave != 0 || c >= 2 * D) return;
-#pragma unroll
-  for (int w = 1; w < 16; ++w) s += part[w][lane];
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float s = bq_join_rows(sums, n, 2 * D, c, part);
+  if (threadIdx.x >= 64 || c >= 2 * D) return;
   if (c < D) {
     if (gw) gw[c] = s;
   } else if (gb) {
