@@ -105,8 +105,9 @@ __device__ __forceinline__ int row_of(const T& rows, int count, uint32_t r) {
   return lo;
 }
 
-// FAST: the hardware's root and reciprocal (1 unit in the last place each) and constants
-// multiplied beforehand.  Such a step is within 2^-21 of itself, far below a rounding of w;
+// FAST: the hardware's root and reciprocal (1 unit in the last place each, 2^-23) and constants
+// multiplied beforehand (two, rounded once: 2^-24 each), with four products and sums rounded
+// once: such a step is within 10 * 2^-24 < 2^-20 of itself, far below a rounding of w;
 // correctly rounded ones are a third of the instructions that bound 8-bit states (336 M
 // elements with bf16 gradients 1182 us with them, 1024 with the hardware's).
 template <bool FAST>

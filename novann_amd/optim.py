@@ -1,19 +1,19 @@
 """AdamW with NovaNN's interface (novann/optim/adamw.py:6-69), on the GPU.
 
 Same constructor (parameters, lr, betas, weight_decay, epsilon), ``step`` and
-``zero_grad``; BatchNorm gamma / beta (by name) are not decayed, as there.
-Each step is the float32 update the reference computes on its float32 arrays,
-bit for bit (libnovaq ``novaq_adamw_step``).  ``QuantizedParameters`` step
-their fp32 ``master`` weights and re-quantize their codes and scale in the
-same call (``novaq_adamw_requantize``).  ``Parameters`` holding numpy arrays
-are uploaded at every step (so changes a caller makes to ``.data`` between
-steps count, as with the reference), stepped on the device and written back
-in place.  All of these step in one call over the list (``adamw_step``,
-libnovaq ``novaq_adamw_many``), with their states in fp32 or in 8 bits.
-float64 arrays (the BatchNorm gamma / beta, float64 in the reference too)
-keep float64 moments and step in float64 with numpy's promotion of a float32
-gradient (``novaq_adamw_step_f64``); any other numpy array steps in float32
-(the reference's float32 parameters).
+``zero_grad``; BatchNorm gamma / beta (by name) are not decayed, as there.  All
+parameters with a gradient step in one call over the list (``adamw_step``,
+libnovaq ``novaq_adamw_many``), those that share memory in calls one after
+another; their states are in fp32 or in 8 bits.  With fp32 states each element
+takes the float32 update the reference computes on its float32 arrays, bit for
+bit.  ``QuantizedParameters`` and ``BlockQuantizedParameters`` step their fp32
+``master`` weights, and their codes and scales are written again in the same
+call.  ``Parameters`` holding numpy arrays are uploaded at every step (so changes
+a caller makes to ``.data`` between steps count, as with the reference), stepped
+on the device and written back in place.  float64 arrays (the BatchNorm gamma /
+beta, float64 in the reference too) keep float64 moments and step in float64 with
+numpy's promotion of a float32 gradient (``novaq_adamw_step_f64``); any other
+numpy array steps in float32 (the reference's float32 parameters).
 """
 from __future__ import annotations
 
