@@ -458,6 +458,7 @@ class AdamW:
         for i, p in enumerate(self.params):
             if p.grad is None:
                 continue
+            self._array(i)
             if self._w[i].dtype == torch.float64:  # (its states' type, whatever .data is now)
                 wide.append((i, *self._grad64(i)))
             else:
@@ -535,6 +536,17 @@ class AdamW:
         check(rc, "adamw step")
         for data, w in arrays:
             data[...] = w.cpu().numpy().reshape(data.shape)
+
+    def _array(self, i: int) -> None:
+        """A parameter's .data, where it is an array: the step reads and writes it."""
+        data, w = getattr(self.params[i], "data", None), self._w[i]
+        if isinstance(data, np.ndarray):
+            if data.size != w.numel():
+                raise ValueError(f"AdamW: an array of {data.size} values for a parameter of {w.numel()}")
+            if not data.flags.writeable:
+                raise ValueError("AdamW: a parameter's array is read-only")
+        elif w.dtype == torch.float64:
+            raise TypeError("AdamW: a float64 parameter is a numpy array")
 
     def _grad64(self, i: int):
         w = self._w[i]

@@ -132,6 +132,20 @@ def test_a_step_that_is_refused_changes_nothing(library, shared):
     assert shared or np.array_equal(ps[0].data, want)
 
 
+def test_an_array_that_does_not_fit_is_refused_before_the_step(library):
+    """Set to another size, to a read-only array, or (float64) to a tensor, the last of three."""
+    for made, bad in ((np.float32, np.ones(5, np.float32)), (np.float64, np.ones(5)),
+                      (np.float32, np.broadcast_to(np.float32(1), 6)), (np.float64, torch.ones(6))):
+        ps = [Parameters(np.ones(8, np.float32)), Parameters(np.ones(8)), Parameters(np.ones(6, made))]
+        opt = optim.AdamW(ps, **HP)
+        for p in ps:
+            p.grad = np.ones(p.shape, np.float32)
+        ps[2].data = bad
+        with pytest.raises((ValueError, TypeError)):
+            opt.step()
+        assert opt.t == 0 and (ps[0].data == 1).all() and (ps[1].data == 1).all()
+
+
 def test_a_gradient_that_is_another_weight(library):
     """The weight is stepped after the parameter whose gradient it was."""
     rng = np.random.default_rng(5)
