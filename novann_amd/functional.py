@@ -902,11 +902,16 @@ def block_linear(input, weight, bias=None, *, out_dtype: str = "f32", input_dtyp
     'e5m2', a scale for 128 columns of a row), or a quant.BlockQuantized (as ``layer_norm``
     stores it: the output then has the leading dimensions that its rows had there); weight
     (D_out, D_in): BlockQuantizedParameters; bias: D_out values (fp32) or None.  Returns (N,
-    D_out) in ``out_dtype`` ('f32', 'bf16', 'f16'), rounded once from
-    fp32 sums (each sum of 128 products within 2e-5 of the products' root of squares, the
-    matrix core's own precision); ndarrays in -> ndarrays out (f32, f16).  A row of input
-    with an infinity or a NaN is NaN (an infinity has no scale: quantized here it becomes a
-    NaN, where ``quant.quantize_blocks`` saturates).
+    D_out) in ``out_dtype`` ('f32', 'bf16', 'f16'), rounded once; ndarrays in -> ndarrays out
+    (f32, f16).  A row of input with an infinity or a NaN is NaN (an infinity has no scale:
+    quantized here it becomes a NaN, where ``quant.quantize_blocks`` saturates).
+
+    Precision: the matrix core adds 8 products of neighbouring columns at a time and cuts each
+    off 2^-13 below the largest of them; all other sums are fp32's.  Against sums in 64 bits
+    an output is 1.5e-5 of the outputs' norm off, 7e-5 where columns differ by 2^8 in both
+    operands, fp32 ones too.  fp32 sums of the same values, at a tenth of the rate:
+    ``linear(quant.dequantize_blocks(q, 'bf16'), weight.dequantize())`` of the input's blocks
+    q, whose every value is one of bf16's.
 
     ``extras=True`` returns (y, kept): the input transposed in blocks of its own, one byte
     an element, made from the same read, which ``block_linear_backward`` takes in the
