@@ -601,8 +601,9 @@ int novaq_block_linear_backward(const void *grad, int grad_dtype, int64_t M, int
  * in fp32, the deviations taken from the row's own mean; gamma, beta (D values, fp32) or
  * NULL for 1 and 0.  y in F32, F16 or BF16 (exponents NULL), rounded once, or in E4M3 or
  * E5M2 as blocks of 128 columns (codes (R, P) and exponents (R, G) as
- * novaq_quantize_blocks writes them with block_rows 1, an infinity as a NaN).  mean, rstd: R values each for the
- * backward, or both NULL.  eps not negative.  D up to 2^20, R below 2^31.
+ * novaq_quantize_blocks writes them with block_rows 1, but an infinity as a NaN).  mean,
+ * rstd: R values each for the backward, or both NULL.  eps not negative.  D up to 2^20, R
+ * below 2^31.
  * No reference counterpart (the reference normalises over the batch). */
 int novaq_layer_norm(const void *x, int x_dtype, int64_t R, int64_t D, const float *gamma,
                      const float *beta, float eps, void *y, int y_dtype, void *exponents,

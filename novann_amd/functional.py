@@ -1041,9 +1041,9 @@ def layer_norm(input, weight=None, bias=None, *, eps: float = 1e-5,
     weight, bias: D values each (Parameters, tensors or arrays; None for 1 and 0).
     Returns input's shape in ``out_dtype`` ('f32', 'bf16', 'f16'; input's type by default),
     rounded once; with 'e4m3' or 'e5m2' a quant.BlockQuantized of (rows, D) that keeps the
-    leading dimensions, as ``block_linear`` takes it.  ``extras=True`` returns (y, mean, rstd), both of input's
-    shape without the last dimension, for the backward; ndarrays in -> ndarrays out (f32,
-    f16).  No counterpart in the reference, whose norms are over the batch."""
+    leading dimensions, as ``block_linear`` takes it.  ``extras=True`` returns (y, mean,
+    rstd), both of input's shape without the last dimension, for the backward; ndarrays in ->
+    ndarrays out (f32, f16).  No counterpart in the reference, whose norms are over the batch."""
     x, xdt, was_numpy = _float_arg(input, "input")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm is over the last dimension, got shape {tuple(x.shape)}")
@@ -1060,7 +1060,8 @@ def layer_norm(input, weight=None, bias=None, *, eps: float = 1e-5,
     if name in quant.BLOCK_DTYPES:
         y = torch.empty((R, quant.block_pitch(D)), dtype=quant.BLOCK_DTYPES[name], device=dev)
         e = torch.empty((R, quant.block_groups(D)), dtype=torch.uint8, device=dev)
-        q = quant.BlockQuantized(y, e, (R, D), name, lead=None if x.dim() == 2 else tuple(shape[:-1]))
+        q = quant.BlockQuantized(y, e, (R, D), name,
+                                 lead=None if x.dim() == 2 else tuple(shape[:-1]))
     else:
         y = torch.empty(shape, dtype=_out_dtype(name), device=dev)
     mean = rstd = None
